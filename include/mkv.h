@@ -11,6 +11,9 @@
  *       partials merged by log-sum-exp)
  *   K3  paged / contiguous causal prefill attention on MFMA
  *   K4  block-table gather (shared device functions + a standalone kernel)
+ *   K7  attention of trees of drafted tokens over the paged cache
+ *   K8  token log probabilities, entropy and top alternatives
+ *   K9  pages: copies, compaction of accepted rows, forks / growth / freeing
  *
  * Conventions
  *   - Every pointer is a device pointer unless stated otherwise.  The library
@@ -548,6 +551,91 @@ int mkv_linear_supported(int64_t rows, int n, int k, int act, int norm, int dtyp
 int mkv_linear(void* out, const void* x, int64_t x_row_stride, const void* w,
                const void* norm_weight, float eps, const void* residual, int64_t rows, int n,
                int k, int act, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A speculative decode step (no counterpart in the reference): attention of
+ * trees of drafted tokens, log probabilities, and the cache's pages.
+ *
+ * mkv_paged_tree: sequence s has n_s = cu_seqlens_q[s+1] - cu_seqlens_q[s]
+ * drafted tokens, rows of q (total_q, num_heads, head_dim), whose K and V are
+ * in the cache already: context_lens[s] counts them, and drafted token j sits at
+ * position context_lens[s] - n_s + j.  Row i of the sequence sees every position
+ * ahead of the drafted ones and drafted token j where
+ * tree_mask[(cu_seqlens_q[s] + i) * mask_stride + j] is not 0 (j < mask_cols).
+ * Softmax attention over what a row sees, scaled by sm_scale; a row that sees
+ * nothing gives zeros.  Positions in absent (-1) blocks are not seen.  mask_cols
+ * is the most drafted tokens of a sequence: rows past it give zeros.  Rows of q
+ * behind the last sequence are not written.
+ * fp32, bf16 and fp16 caches with q of that type; FP8 (per tensor, or per token
+ * and head) and INT8 (per token and head) caches with a bf16 or fp16 q.  Head
+ * sizes and groups as mkv_paged_decode; out has q's type and layout.  Sums and
+ * the softmax are fp32; 16-bit P holds 16 bits or more over bf16 caches and 11
+ * over the others.
+ */
+size_t mkv_paged_tree_workspace_size(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim,
+                                     int block_size, int max_blocks, int mask_cols, int kv_dtype);
+int mkv_paged_tree(void* out, const void* q, int q_dtype, const void* k_cache, const void* v_cache, int kv_dtype,
+                   int64_t num_blocks, const float* k_scale, const float* v_scale, int kv_scale_mode,
+                   const int32_t* block_tables, int64_t bt_stride, int max_blocks, const void* context_lens,
+                   int context_lens_dtype, const int32_t* cu_seqlens_q, const uint8_t* tree_mask, int64_t mask_stride,
+                   int mask_cols, int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim,
+                   int block_size, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* mkv_token_logprobs: for each row of logits (rows, vocab; fp32, bf16 or fp16,
+ * any alignment of an element, row stride row_stride): logprobs[row, i] = log
+ * softmax(logits)[ids[row, i]] (0 for an id below 0, NaN for one past the
+ * vocabulary), entropy[row] = -sum p log p, and the top (<= 64, <= vocab) largest
+ * logits' indices and log probabilities, larger first and the lower index first
+ * among equals (NaN counts as largest, the zeros as equal).  A row with a NaN or
+ * +inf, or with -inf alone, has NaN log probabilities, as log_softmax does.
+ * Outputs contiguous; all arithmetic fp32. */
+size_t mkv_token_logprobs_workspace_size(int64_t rows, int vocab, int top);
+int mkv_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, const void* logits,
+                       int64_t row_stride, int dtype, int64_t rows, int vocab, const void* ids, int64_t ids_stride,
+                       int num_ids, int ids_dtype, int top, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages.  tensors: a HOST array of num_tensors device pointers, pools (or
+ * per-token scale tensors) of num_pages pages of block_size token rows each;
+ * row_bytes: a HOST array of each tensor's bytes a token row (a multiple of 4;
+ * 16-byte accesses where rows and bases are multiples of 16).  The tensors do
+ * not overlap.
+ *
+ * mkv_copy_pages: page src[i] to page dst[i] of every tensor.  Pairs that name a
+ * page outside the pool are skipped.  No page may be the destination of two
+ * pairs, or the destination of one and the source of another.
+ *
+ * mkv_compact_slots: in every tensor, token row prefix_lens[b] + accepted[b, j] of
+ * sequence b moves to row prefix_lens[b] + j, as if all of a sequence's rows were
+ * read before any is written.  Entries below 0, and rows outside the block table
+ * or the pool, are skipped.  num_accepted <= 2048.  Sequences do not share the
+ * pages of these rows.
+ *
+ * mkv_assign_pages: one step of the page table.  Row i (of rows <= 1024) holds
+ * held[i] pages, block_tables[i, 0 .. held[i]), for seq_lens[i] tokens; ref_counts
+ * counts the rows (and other holders) of each page.  Row i goes on with the
+ * sequence that row parents[i] held before the call (its own where parents[i] ==
+ * i, none and length 0 where it is below 0): a row that stays keeps its pages, one
+ * that changes lets go of them and shares the pages that hold its parent's
+ * tokens.  Where a part-filled last page has other holders then, every row but the
+ * first of those for which it is the last gets a copy of its filled rows in a
+ * fresh page (the first too, if the page has holders besides).  Then the row grows
+ * to pages for tokens[i] tokens (NULL: no growth).  Fresh pages are the
+ * lowest-numbered with a count of 0 after all letting go, in row order, a copy
+ * first; a row whose pages do not fit what is left (or the table) is refused
+ * (granted[i] 0): it ends without pages, or as it was if it stayed.  A parent of
+ * rows or more is refused.  Table entries past a row's pages become 0. */
+int mkv_copy_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,
+                   int block_size, const void* src, const void* dst, int index_dtype, int64_t pairs, void* stream);
+int mkv_compact_slots(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,
+                      int block_size, const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                      const void* prefix_lens, int prefix_dtype, const void* accepted, int accepted_dtype,
+                      int64_t accepted_stride, int batch, int num_accepted, void* stream);
+size_t mkv_assign_pages_workspace_size(int rows, int max_blocks);
+int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,
+                     int block_size, int32_t* block_tables, int64_t bt_stride, int max_blocks, int64_t* seq_lens,
+                     int32_t* held, int32_t* ref_counts, const void* parents, int parents_dtype, const void* tokens,
+                     int tokens_dtype, uint8_t* granted, int rows, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 /* ------------------------------------------------------------------------
  * Measurement helper (no counterpart in the reference; for benchmarks).

@@ -1,0 +1,483 @@
+// Operations on the pages of the paged KV cache, over every layer's pools in
+// one launch: whole-page copies, the compaction of accepted drafted tokens,
+// and the page table's step (rows that fork, grow or are freed).
+//
+// All are moves of bytes and table entries: HBM bound where pages are copied
+// (each byte read once and written once), latency bound in the table step.
+// The pools' addresses travel in the kernel arguments (a scalar load each),
+// so a program's 2 x layers tensors need no device-side pointer table.
+#include "mkv_device.hpp"
+
+namespace mkv {
+namespace {
+
+constexpr int kMaxTensors = 64;  // a launch's pools: 1 KB of kernel arguments
+
+struct Pools {
+  char* base[kMaxTensors];
+  int64_t row_bytes[kMaxTensors];  // bytes of one token's row
+};
+
+// A workgroup copies kCopyBytes: four 16-byte loads a thread in flight ahead
+// of their stores.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;
+constexpr int64_t kCopyBytes = (int64_t)kCopyThreads * kCopyUnroll * 16;
+
+// bytes from s to d, both 4-byte aligned (16 with rows that are multiples of
+// it): the chunk [lo, lo + kCopyBytes) of them.
+MKV_DEV void copy_chunk(char* __restrict__ d, const char* __restrict__ s, int64_t lo, int64_t bytes, bool wide) {
+  const int64_t hi = min(lo + kCopyBytes, bytes);
+  if (wide) {
+    u32x4 v[kCopyUnroll];
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; ++j) {
+      const int64_t o = lo + 16 * (j * kCopyThreads + (int)threadIdx.x);
+      if (o < hi) v[j] = ld16_stream(s + o);
+    }
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; ++j) {
+      const int64_t o = lo + 16 * (j * kCopyThreads + (int)threadIdx.x);
+      if (o < hi) __builtin_nontemporal_store(v[j], reinterpret_cast<u32x4*>(d + o));
+    }
+  } else {
+    for (int64_t o = lo + 4 * (int)threadIdx.x; o < hi; o += 4 * kCopyThreads)
+      *reinterpret_cast<uint32_t*>(d + o) = *reinterpret_cast<const uint32_t*>(s + o);
+  }
+}
+
+// Page src[i] of every pool to page dst[i].  blockIdx.x: (tensor, chunk of a
+// page), blockIdx.y strides over the pairs.
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(Pools p, int block_size, int chunks, int64_t num_pages,
+                                                                 const void* __restrict__ src,
+                                                                 const void* __restrict__ dst, int i64, int64_t pairs) {
+  const int t = blockIdx.x / chunks;
+  const int64_t lo = (int64_t)(blockIdx.x % chunks) * kCopyBytes;
+  const int64_t bytes = p.row_bytes[t] * block_size;
+  if (lo >= bytes) return;
+  const bool wide = bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
+  for (int64_t i = blockIdx.y; i < pairs; i += gridDim.y) {
+    const int64_t a = load_index(src, i, i64), b = load_index(dst, i, i64);
+    if (a < 0 || a >= num_pages || b < 0 || b >= num_pages || a == b) continue;
+    copy_chunk(p.base[t] + b * bytes, p.base[t] + a * bytes, lo, bytes, wide);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Compaction: row prefix + accepted[b, j] of sequence b moves to prefix + j.
+// A workgroup takes one sequence, one pool and a slice of the rows' columns
+// and holds all of the sequence's rows of that slice in registers before it
+// writes any, so rows may overlap in any order.
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 256;
+constexpr int kMoveItems = 8;                             // 16-byte items a thread holds
+constexpr int kMaxMoves = kMoveThreads * kMoveItems;      // accepted offsets a sequence
+constexpr int kMoveLdsRows = kMaxMoves;
+
+template <typename T>
+MKV_DEV void move_rows(char* base, const int64_t* src, const int64_t* dst, int n, int64_t row_bytes, int col0, int cols) {
+  T v[kMoveItems];
+#pragma unroll
+  for (int j = 0; j < kMoveItems; ++j) {
+    const int it = j * kMoveThreads + (int)threadIdx.x;
+    const int e = it / cols;
+    if (e < n && src[e] >= 0)
+      v[j] = *reinterpret_cast<const T*>(base + src[e] * row_bytes + (int64_t)(col0 + it % cols) * sizeof(T));
+  }
+  // every row of the slice has been read before any is written
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kMoveItems; ++j) {
+    const int it = j * kMoveThreads + (int)threadIdx.x;
+    const int e = it / cols;
+    if (e < n && src[e] >= 0)
+      *reinterpret_cast<T*>(base + dst[e] * row_bytes + (int64_t)(col0 + it % cols) * sizeof(T)) = v[j];
+  }
+}
+
+__global__ __launch_bounds__(kMoveThreads) void compact_slots_kernel(Pools p, PagedIndex idx,
+                                                                     const void* __restrict__ prefix, int prefix_i64,
+                                                                     const void* __restrict__ accepted, int acc_i64,
+                                                                     int64_t acc_stride, int n, int slices) {
+  extern __shared__ int64_t slots[];  // [n] sources (-1: nothing to move), [n] destinations
+  const int t = blockIdx.x / slices, slice = blockIdx.x % slices, b = blockIdx.y;
+  const int64_t row_bytes = p.row_bytes[t];
+  const bool wide = row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
+  const int units = (int)(row_bytes / (wide ? 16 : 4));
+  const int cols = max(1, kMaxMoves / n);
+  if ((int64_t)slice * cols >= units) return;
+  const int64_t P = load_index(prefix, b, prefix_i64);
+  for (int j = threadIdx.x; j < n; j += kMoveThreads) {
+    const int64_t a = load_index(accepted, b * acc_stride + j, acc_i64);
+    int64_t s = -1, d = -1;
+    if (P >= 0 && a >= 0 && a != j && a < ((int64_t)1 << 40)) {
+      const int64_t mask = ((int64_t)1 << idx.bs_log2) - 1;
+      const int64_t ps = idx.physical_block(b, (P + a) >> idx.bs_log2), pd = idx.physical_block(b, (P + j) >> idx.bs_log2);
+      if (ps >= 0 && pd >= 0) {
+        s = (ps << idx.bs_log2) + ((P + a) & mask);
+        d = (pd << idx.bs_log2) + ((P + j) & mask);
+      }
+    }
+    slots[j] = s;
+    slots[n + j] = d;
+  }
+  __syncthreads();
+  const int col0 = slice * cols, take = min(cols, units - col0);
+  if (wide)
+    move_rows<u32x4>(p.base[t], slots, slots + n, n, row_bytes, col0, take);
+  else
+    move_rows<uint32_t>(p.base[t], slots, slots + n, n, row_bytes, col0, take);
+}
+
+// ---------------------------------------------------------------------------
+// The page table's step, one workgroup.  Whole numbers throughout: reference
+// counts change by atomic additions, whose order does not matter, and fresh
+// pages are the lowest-numbered free ones in row order, so the result is one
+// only.  A second kernel copies the part-filled pages that it lists.
+// ---------------------------------------------------------------------------
+constexpr int kMaxRows = 1024;
+constexpr int kAssignThreads = 1024;
+constexpr int kScanPer = 16;  // reference counts a thread looks at in one sweep
+
+struct AssignArgs {
+  int32_t* tables;
+  int64_t bt_stride;
+  int max_blocks;
+  int64_t* seq_lens;
+  int32_t* held;
+  int32_t* refs;
+  int64_t num_pages;
+  int bs_log2;
+  const void* parents;
+  const void* tokens;
+  int parents_i64, tokens_i64;
+  uint8_t* granted;
+  int rows;
+  int32_t* new_tables;  // workspace: (rows, max_blocks)
+  int32_t* spare;       // workspace: rows * max_blocks fresh pages at most
+  int32_t* copies;      // workspace: (rows, 3) source page, fresh page, live rows (0: none)
+};
+
+MKV_DEV int wave_sum(int v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// exclusive sum of v over the workgroup's threads in order; total in every thread
+MKV_DEV int block_scan(int v, int* lds, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kAssignThreads / 64; ++w) {
+    const int c = lds[w];
+    if (w < wave) before += c;
+    total += c;
+  }
+  return before + x - v;
+}
+MKV_DEV void ref_add(const AssignArgs& a, int page, int by) {
+  if (page >= 0 && page < a.num_pages)
+    __hip_atomic_fetch_add(a.refs + page, by, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MKV_DEV int ref_get(const AssignArgs& a, int64_t page) {
+  return __hip_atomic_load(a.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs a) {
+  __shared__ int s_src[kMaxRows], s_keep[kMaxRows], s_held[kMaxRows], s_at[kMaxRows], s_last[kMaxRows], s_start[kMaxRows],
+      s_grow[kMaxRows];
+  __shared__ uint8_t s_copy[kMaxRows], s_drop[kMaxRows];
+  __shared__ int s_scan[kAssignThreads / 64];
+  const int tid = threadIdx.x, R = a.rows, W = a.max_blocks;
+  const int64_t bs = (int64_t)1 << a.bs_log2;
+  // a thread a row
+  int64_t new_len = 0;
+  int want = 0, fill = 0;
+  bool valid = false, stays = false, gone = false, fits = false;
+  if (tid < R) {
+    const int64_t parent = load_index(a.parents, tid, a.parents_i64);
+    valid = parent < R;
+    gone = parent < 0;
+    stays = parent == tid || !valid;
+    const int src = gone || !valid ? tid : (int)parent;
+    const int old_held = min(max(a.held[tid], 0), W);
+    const int64_t len = a.seq_lens[src];
+    new_len = gone ? 0 : max(len, (int64_t)0);
+    const int64_t need = (new_len + bs - 1) >> a.bs_log2;
+    const int keep = gone ? 0 : stays ? old_held : (int)min(need, (int64_t)min(max(a.held[src], 0), W));
+    const int64_t tok = a.tokens ? load_index(a.tokens, tid, a.tokens_i64) : 0;
+    const int64_t w = tok <= 0 ? 0 : (tok + bs - 1) >> a.bs_log2;
+    fits = valid && w <= W;
+    want = fits ? (int)w : 0;
+    const int64_t at = new_len >> a.bs_log2;
+    fill = at < keep ? (int)(new_len & (bs - 1)) : 0;
+    s_src[tid] = src;
+    s_keep[tid] = keep;
+    s_held[tid] = old_held;
+    s_at[tid] = (int)min(at, (int64_t)W);
+    // rows without a part-filled page: numbers that no other row shares
+    s_last[tid] = fill ? a.tables[(int64_t)src * a.bt_stride + at] : -1 - tid;
+    if (s_last[tid] < 0 || s_last[tid] >= a.num_pages) {
+      s_last[tid] = -1 - tid;
+      fill = 0;
+    }
+    s_drop[tid] = stays;  // (for now: rows whose counts stay as they are)
+  }
+  __syncthreads();
+  // the rows' new tables so far, and the counts of what is taken and let go
+  for (int i = tid; i < R * W; i += kAssignThreads) {
+    const int r = i / W, w = i - r * W;
+    const int page = w < s_keep[r] ? a.tables[(int64_t)s_src[r] * a.bt_stride + w] : 0;
+    a.new_tables[i] = page;
+    if (!s_drop[r]) {
+      if (w < s_keep[r]) ref_add(a, page, 1);
+      if (w < s_held[r]) ref_add(a, a.tables[(int64_t)r * a.bt_stride + w], -1);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  // a part-filled page that others hold too is copied by all but its first row
+  int need = 0;
+  bool copy = false;
+  if (tid < R) {
+    if (fill) {
+      const int page = s_last[tid];
+      int alike = 0;
+      bool first = true;
+      for (int r = 0; r < R; ++r)
+        if (s_last[r] == page) {
+          ++alike;
+          first &= r >= tid;
+        }
+      const int count = ref_get(a, page);
+      copy = count > 1 && !(first && count == alike);
+    }
+    const int grow = max(want - s_keep[tid], 0);
+    need = fits ? (int)copy + grow : 0;
+    s_grow[tid] = grow;
+  }
+  int total;
+  const int start = block_scan(need, s_scan, total);
+  // the lowest-numbered free pages, as many as are asked for
+  int found = 0;
+  for (int64_t p0 = 0; p0 < a.num_pages && found < total; p0 += kAssignThreads * kScanPer) {
+    uint32_t free_bits = 0;
+#pragma unroll
+    for (int j = 0; j < kScanPer; ++j) {
+      const int64_t p = p0 + (int64_t)tid * kScanPer + j;
+      if (p < a.num_pages && ref_get(a, p) == 0) free_bits |= 1u << j;
+    }
+    int here;
+    int at = found + block_scan(__popc(free_bits), s_scan, here);
+    while (free_bits && at < total) {
+      const int j = __ffs(free_bits) - 1;
+      free_bits &= free_bits - 1;
+      a.spare[at++] = (int)(p0 + (int64_t)tid * kScanPer + j);
+    }
+    found += here;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid < R) {
+    const bool ok = fits && (need == 0 || start + need <= found);
+    const bool drop = !ok && !stays;
+    copy = copy && ok;
+    const int grow = ok ? s_grow[tid] : 0;
+    s_start[tid] = start + (copy ? 1 : 0);
+    s_grow[tid] = grow;
+    s_copy[tid] = copy;
+    s_drop[tid] = drop;
+    int32_t* c = a.copies + 3 * tid;
+    c[2] = 0;
+    if (copy) {
+      const int fresh = a.spare[start];
+      c[0] = s_last[tid];
+      c[1] = fresh;
+      c[2] = fill;
+      ref_add(a, s_last[tid], -1);
+      ref_add(a, fresh, 1);
+      s_last[tid] = fresh;
+    }
+    a.granted[tid] = ok;
+    a.held[tid] = drop ? 0 : s_keep[tid] + grow;
+    // (every row's length was read before the first barrier)
+    a.seq_lens[tid] = drop ? 0 : new_len;
+  }
+  __syncthreads();
+  for (int i = tid; i < R * W; i += kAssignThreads) {
+    const int r = i / W, w = i - r * W;
+    int page = a.new_tables[i];
+    const int keep = s_keep[r];
+    if (s_drop[r]) {
+      if (w < keep) ref_add(a, page, -1);
+      page = 0;
+    } else if (w < keep) {
+      if (s_copy[r] && w == s_at[r]) page = s_last[r];
+    } else if (w < keep + s_grow[r]) {
+      page = a.spare[s_start[r] + w - keep];
+      ref_add(a, page, 1);
+    }
+    a.tables[(int64_t)r * a.bt_stride + w] = page;
+  }
+}
+
+__global__ __launch_bounds__(kCopyThreads) void copy_listed_kernel(Pools p, int block_size, int chunks,
+                                                                  const int32_t* __restrict__ copies) {
+  const int t = blockIdx.x / chunks;
+  const int64_t lo = (int64_t)(blockIdx.x % chunks) * kCopyBytes;
+  const int32_t* c = copies + 3 * blockIdx.y;
+  const int64_t bytes = p.row_bytes[t] * c[2], page = p.row_bytes[t] * block_size;
+  if (lo >= bytes) return;
+  const bool wide = p.row_bytes[t] % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
+  copy_chunk(p.base[t] + c[1] * page, p.base[t] + c[0] * page, lo, bytes, wide);
+}
+
+int log2_exact(int64_t v) {
+  if (v <= 0 || (v & (v - 1))) return -1;
+  int l = 0;
+  while (((int64_t)1 << l) < v) ++l;
+  return l;
+}
+
+// The tensors from t0 on as a launch's pools; the largest row in bytes.
+int pools_at(const void* const* tensors, const int64_t* row_bytes, int num, int t0, Pools& p, int64_t& widest) {
+  const int n = num - t0 < kMaxTensors ? num - t0 : kMaxTensors;
+  widest = 0;
+  for (int t = 0; t < n; ++t) {
+    p.base[t] = reinterpret_cast<char*>(const_cast<void*>(tensors[t0 + t]));
+    p.row_bytes[t] = row_bytes[t0 + t];
+    widest = row_bytes[t0 + t] > widest ? row_bytes[t0 + t] : widest;
+  }
+  return n;
+}
+
+int check_pools(const void* const* tensors, const int64_t* row_bytes, int num, int64_t num_pages, int block_size) {
+  if (num < 0 || num_pages < 0 || num_pages > 0x7fffffff || block_size <= 0 || block_size > (1 << 20))
+    return MKV_ERR_BAD_SHAPE;
+  if (num && (!tensors || !row_bytes)) return MKV_ERR_NULL_POINTER;
+  for (int t = 0; t < num; ++t) {
+    if (!tensors[t]) return MKV_ERR_NULL_POINTER;
+    if (row_bytes[t] <= 0 || row_bytes[t] % 4 || row_bytes[t] > (1 << 24)) return MKV_ERR_BAD_SHAPE;
+    if (reinterpret_cast<uintptr_t>(tensors[t]) & 3) return MKV_ERR_MISALIGNED;
+  }
+  return MKV_OK;
+}
+
+bool index_ok(int dt) { return dt == MKV_INDEX_I32 || dt == MKV_INDEX_I64; }
+
+}  // namespace
+}  // namespace mkv
+
+using namespace mkv;
+
+extern "C" int mkv_copy_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,
+                              int block_size, const void* src, const void* dst, int index_dtype, int64_t pairs,
+                              void* stream) {
+  if (int st = check_pools(tensors, row_bytes, num_tensors, num_pages, block_size)) return st;
+  if (pairs < 0) return MKV_ERR_BAD_SHAPE;
+  if (!index_ok(index_dtype)) return MKV_ERR_UNSUPPORTED_DTYPE;
+  if (pairs == 0 || num_tensors == 0) return MKV_OK;
+  if (!src || !dst) return MKV_ERR_NULL_POINTER;
+  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
+    Pools p;
+    int64_t widest;
+    const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
+    const int64_t chunks = (widest * block_size + kCopyBytes - 1) / kCopyBytes;
+    if (chunks * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(chunks * n), (unsigned)(pairs < 65535 ? pairs : 65535)),
+                       dim3(kCopyThreads), 0, reinterpret_cast<hipStream_t>(stream), p, block_size, (int)chunks,
+                       num_pages, src, dst, (int)(index_dtype == MKV_INDEX_I64), pairs);
+    if (hipError_t e = hipGetLastError()) return (int)e;
+  }
+  return MKV_OK;
+}
+
+extern "C" int mkv_compact_slots(const void* const* tensors, const int64_t* row_bytes, int num_tensors,
+                                 int64_t num_pages, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                                 int max_blocks, const void* prefix_lens, int prefix_dtype, const void* accepted,
+                                 int accepted_dtype, int64_t accepted_stride, int batch, int num_accepted,
+                                 void* stream) {
+  if (int st = check_pools(tensors, row_bytes, num_tensors, num_pages, block_size)) return st;
+  if (batch < 0 || num_accepted < 0 || num_accepted > kMaxMoves || max_blocks < 0 || batch > 65535) return MKV_ERR_BAD_SHAPE;
+  if (!index_ok(prefix_dtype) || !index_ok(accepted_dtype)) return MKV_ERR_UNSUPPORTED_DTYPE;
+  const int bs_log2 = log2_exact(block_size);
+  if (bs_log2 < 0) return MKV_ERR_BAD_BLOCK_SIZE;
+  if (batch == 0 || num_accepted == 0 || num_tensors == 0) return MKV_OK;
+  if (!block_tables || !prefix_lens || !accepted) return MKV_ERR_NULL_POINTER;
+  if (bt_stride < max_blocks || accepted_stride < num_accepted) return MKV_ERR_BAD_STRIDE;
+  PagedIndex idx{block_tables, bt_stride, max_blocks, num_pages, bs_log2, 0};
+  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
+    Pools p;
+    int64_t widest;
+    const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
+    int64_t units = 0;  // (a narrow row of a 4-byte unit can have more units than a wide one)
+    for (int t = 0; t < n; ++t) {
+      const bool wide = p.row_bytes[t] % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
+      const int64_t u = p.row_bytes[t] / (wide ? 16 : 4);
+      units = u > units ? u : units;
+    }
+    const int cols = kMaxMoves / num_accepted > 1 ? kMaxMoves / num_accepted : 1;
+    const int64_t slices = (units + cols - 1) / cols;
+    if (slices * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL(compact_slots_kernel, dim3((unsigned)(slices * n), (unsigned)batch), dim3(kMoveThreads),
+                       (size_t)num_accepted * 16, reinterpret_cast<hipStream_t>(stream), p, idx, prefix_lens,
+                       (int)(prefix_dtype == MKV_INDEX_I64), accepted, (int)(accepted_dtype == MKV_INDEX_I64),
+                       accepted_stride, num_accepted, (int)slices);
+    if (hipError_t e = hipGetLastError()) return (int)e;
+  }
+  return MKV_OK;
+}
+
+extern "C" size_t mkv_assign_pages_workspace_size(int rows, int max_blocks) {
+  if (rows <= 0 || max_blocks < 0) return 0;
+  return ((size_t)rows * max_blocks * 2 + (size_t)rows * 4) * sizeof(int32_t);
+}
+
+extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors,
+                                int64_t num_pages, int block_size, int32_t* block_tables, int64_t bt_stride,
+                                int max_blocks, int64_t* seq_lens, int32_t* held, int32_t* ref_counts,
+                                const void* parents, int parents_dtype, const void* tokens, int tokens_dtype,
+                                uint8_t* granted, int rows, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = check_pools(tensors, row_bytes, num_tensors, num_pages, block_size)) return st;
+  if (rows < 0 || rows > kMaxRows || max_blocks < 0 || (int64_t)rows * max_blocks > (1 << 28)) return MKV_ERR_BAD_SHAPE;
+  if (!index_ok(parents_dtype) || (tokens && !index_ok(tokens_dtype))) return MKV_ERR_UNSUPPORTED_DTYPE;
+  const int bs_log2 = log2_exact(block_size);
+  if (bs_log2 < 0) return MKV_ERR_BAD_BLOCK_SIZE;
+  if (rows == 0) return MKV_OK;
+  if (!block_tables || !seq_lens || !held || !ref_counts || !parents || !granted || !workspace)
+    return MKV_ERR_NULL_POINTER;
+  if (bt_stride < max_blocks) return MKV_ERR_BAD_STRIDE;
+  if (workspace_bytes < mkv_assign_pages_workspace_size(rows, max_blocks)) return MKV_ERR_WORKSPACE_TOO_SMALL;
+  int32_t* ws = reinterpret_cast<int32_t*>(workspace);
+  const size_t cells = (size_t)rows * max_blocks;
+  // (a row asks for a copy and at most max_blocks pages: a row whose page is
+  // copied keeps at least that one)
+  AssignArgs a{block_tables, bt_stride, max_blocks, seq_lens, held, ref_counts, num_pages, bs_log2, parents, tokens,
+               (int)(parents_dtype == MKV_INDEX_I64), (int)(tokens_dtype == MKV_INDEX_I64), granted, rows, ws,
+               ws + cells, ws + 2 * cells};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(assign_pages_kernel, dim3(1), dim3(kAssignThreads), 0, s, a);
+  if (hipError_t e = hipGetLastError()) return (int)e;
+  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
+    Pools p;
+    int64_t widest;
+    const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
+    const int64_t chunks = (widest * block_size + kCopyBytes - 1) / kCopyBytes;
+    if (chunks * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL(copy_listed_kernel, dim3((unsigned)(chunks * n), (unsigned)rows), dim3(kCopyThreads), 0, s, p,
+                       block_size, (int)chunks, a.copies);
+    if (hipError_t e = hipGetLastError()) return (int)e;
+  }
+  return MKV_OK;
+}

@@ -12,15 +12,24 @@ with the reference engine's Python call signatures:
 * :func:`paged_attention_prefill_triton`, :func:`flash_attention_prefill` —
   causal prefill over the paged cache / over fresh contiguous K/V;
 * :func:`gather_kv` — block-table gather;
+* :func:`paged_attention_tree` — attention of trees of drafted tokens over
+  the paged cache (speculative decoding's verification step);
+* :func:`token_logprobs` — log probabilities of given tokens, entropy and
+  top alternatives;
+* :class:`CachePages`, :class:`PagePool` — page copies, compaction of accepted
+  drafted tokens, and page tables whose rows fork, grow and are freed on the
+  device;
 * :class:`Attention` and :mod:`mkv.context` — the layer and per-step
   metadata the runner drives.
 """
 from .attention import (DECODE_STREAM, DECODE_WORKGROUP, FP8_E4M3_MAX, Attention, calibrate_fp8_per_tensor,
                         flash_attention_prefill, gather_kv, paged_attention_decode,
                         paged_attention_decode_quantized, paged_attention_prefill_triton,
-                        store_kvcache, store_kvcache_fp8, store_kvcache_int8)
+                        paged_attention_tree, store_kvcache, store_kvcache_fp8, store_kvcache_int8)
 from .context import (Context, MixedAttentionSplit, current_context, get_context, reset_context,
                       set_context, split_mixed_decode_prefill_metadata, use_context_provider)
+from .logprobs import TokenLogprobs, token_logprobs
+from .pages import CachePages, PagePool
 
 __all__ = [
     "DECODE_STREAM", "DECODE_WORKGROUP", "FP8_E4M3_MAX", "Attention", "Context", "MixedAttentionSplit", "calibrate_fp8_per_tensor",
@@ -28,5 +37,6 @@ __all__ = [
     "paged_attention_decode_quantized", "paged_attention_prefill_triton", "reset_context",
     "set_context", "split_mixed_decode_prefill_metadata", "store_kvcache", "store_kvcache_fp8",
     "store_kvcache_int8",
+    "CachePages", "PagePool", "TokenLogprobs", "paged_attention_tree", "token_logprobs",
     "current_context", "use_context_provider",
 ]

@@ -89,6 +89,24 @@ SIGNATURES: dict[str, tuple] = {
     "mkv_gather_kv": (c_int, [
         c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int,
         c_int, c_int, c_int, c_int, c_void_p]),
+    "mkv_paged_tree_workspace_size": (c_size_t, [c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mkv_paged_tree": (c_int, [
+        c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int,
+        c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64,
+        c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "mkv_token_logprobs_workspace_size": (c_size_t, [c_int64, c_int, c_int]),
+    "mkv_token_logprobs": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_int64,
+        c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "mkv_copy_pages": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_int, c_int64,
+                               c_void_p]),
+    "mkv_compact_slots": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int,
+        c_int64, c_int, c_int, c_void_p]),
+    "mkv_assign_pages_workspace_size": (c_size_t, [c_int, c_int]),
+    "mkv_assign_pages": (c_int, [
+        c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+        c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "mkv_stream_read_probe_sink_words": (c_size_t, [c_int]),
     "mkv_stream_read_probe": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p]),
 }

@@ -17,6 +17,7 @@ paged_attention_decode_quantized attention.py:1213-1268 (fp8_per_tensor,
                                 fp8_per_token_head, int8_per_token_head)
 paged_attention_prefill_triton  attention.py:852-891 (+ FP8 KV keywords)
 flash_attention_prefill         attention.py:446-514
+paged_attention_tree            (none: trees of drafted tokens)
 Attention                       attention.py:1617-1807
 ==============================  =========================================
 
@@ -89,6 +90,15 @@ def _stream(dev: torch.device) -> int:
     object that torch.cuda.current_stream builds)."""
     return torch._C._cuda_getCurrentRawStream(
         dev.index if dev.index is not None else torch.cuda.current_device())
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """A launch on dev's current stream, from whichever device is current."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args)
 
 
 _side_streams: dict[int, torch.cuda.Stream] = {}
@@ -543,6 +553,95 @@ def flash_attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 # ---------------------------------------------------------------------------
+# K7: trees of drafted tokens
+# ---------------------------------------------------------------------------
+def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_tables: torch.Tensor, context_lens: torch.Tensor,
+                         cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor, scale: float,
+                         num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, *,
+                         k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                         kv_cache_dtype: str = "auto", out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over the paged cache (the
+    verification step of speculative decoding).
+
+    query: (total, num_heads, head_dim), the drafted tokens of every sequence one
+    after another (cu_seqlens_q, int32 (seqs + 1,)).  Their K and V are in the
+    cache: context_lens counts them, and a sequence's drafted token j sits at
+    position context_lens - n + j of its n.  tree_mask: bool or uint8 (total or
+    more, widest tree): row i sees the whole prefix ahead of the drafted tokens and
+    drafted token j of its sequence where tree_mask[i, j] (its ancestors and itself;
+    any mask goes).  A row that sees nothing gives zeros, and so do a sequence's
+    rows past the mask's width.  Rows behind the last sequence are not written.
+
+    fp32, bf16 and fp16 caches take a query of their type; the quantised ones
+    (kv_cache_dtype and scales as for paged_attention_prefill_triton) a bf16 or
+    fp16 query.  head_dim 128, or 64 with an even num_kv_heads.  out: written
+    instead of a new tensor (contiguous, like query)."""
+    dev = _require_gpu(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, tree_mask)
+    if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
+        raise ValueError(f"query must be (total, {num_heads}, {head_dim}); got {tuple(query.shape)}")
+    query = query.contiguous()
+    _check_cache(k_cache, v_cache, num_kv_heads, head_dim)
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} != the cache's {k_cache.shape[1]}")
+    if out is None:
+        out = torch.empty_like(query)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {query.dtype} tensor of {tuple(query.shape)} on {dev}")
+    per_token = kv_cache_dtype in PER_TOKEN_HEAD_MODES
+    quant = k_cache.dtype in (torch.float8_e4m3fn, torch.int8)
+    if per_token:
+        want = torch.int8 if kv_cache_dtype == "int8_per_token_head" else torch.float8_e4m3fn
+        if k_cache.dtype != want:
+            raise TypeError(f"{kv_cache_dtype} needs a {want} cache, got {k_cache.dtype}")
+        _check_token_scales(k_scale, v_scale, k_cache)
+    elif k_cache.dtype == torch.int8:
+        raise ValueError("an int8 cache needs kv_cache_dtype='int8_per_token_head' and its scales")
+    elif quant:
+        if kv_cache_dtype not in ("fp8_per_tensor", "auto") or k_scale is None or v_scale is None:
+            raise ValueError("an fp8 cache needs kv_cache_dtype='fp8_per_tensor' and k_scale/v_scale")
+    elif kv_cache_dtype != "auto":
+        raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} does not go with a {k_cache.dtype} cache")
+    if quant:
+        if query.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"a quantised cache takes a bfloat16 or float16 query, got {query.dtype}")
+        _require_gpu(query, k_scale, v_scale)
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or not (k_scale.numel() and v_scale.numel()):
+            raise TypeError("k_scale/v_scale must be float32 tensors")
+    elif query.dtype != k_cache.dtype:
+        raise TypeError(f"query {query.dtype} and cache {k_cache.dtype} must share a dtype")
+    bt = _block_table(block_tables)
+    cl = _ctx_lens(context_lens)
+    cu = cu_seqlens_q.to(torch.int32).contiguous()
+    total, num_seqs = query.shape[0], cl.numel()
+    if tree_mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"tree_mask must be bool or uint8, got {tree_mask.dtype}")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] < total:
+        raise ValueError(f"tree_mask must be ({total} or more, widest tree); got {tuple(tree_mask.shape)}")
+    if tree_mask.stride(1) != 1:
+        tree_mask = tree_mask.contiguous()
+    if cl.dim() != 1 or cu.numel() < num_seqs + 1 or bt.dim() != 2 or bt.shape[0] < num_seqs:
+        raise ValueError(f"cu_seqlens_q {tuple(cu.shape)} and block_tables {tuple(bt.shape)} must cover "
+                         f"{num_seqs} sequences")
+    if total == 0 or num_seqs == 0:
+        return out
+    kv_code = _dtype_code(k_cache, "k_cache")
+    sizes = (num_heads, num_kv_heads, head_dim, block_size)
+    nbytes = _lib.query("mkv_paged_tree_workspace_size", num_seqs, total, *sizes, bt.shape[1], tree_mask.shape[1],
+                        kv_code)
+    # (of the call's own: calls on several streams and captured graphs share none)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call_on(dev, "mkv_paged_tree", out.data_ptr(), query.data_ptr(), _dtype_code(query, "query"),
+             k_cache.data_ptr(), v_cache.data_ptr(), kv_code, k_cache.shape[0],
+             k_scale.data_ptr() if quant else None, v_scale.data_ptr() if quant else None,
+             _lib.SCALE_PER_TOKEN_HEAD if per_token else _lib.SCALE_PER_TENSOR,
+             bt.data_ptr(), bt.stride(0), bt.shape[1], cl.data_ptr(), _index_dtype(cl), cu.data_ptr(),
+             tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], num_seqs, total, *sizes, float(scale),
+             ws.data_ptr() if ws is not None else None, nbytes, _stream(dev))
+    return out
+
+
+# ---------------------------------------------------------------------------
 # K4: standalone gather
 # ---------------------------------------------------------------------------
 def gather_kv(cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -629,6 +728,14 @@ class Attention(nn.Module):
                                       scale, self.num_heads, self.num_kv_heads, self.head_dim,
                                       self.block_size, split_tokens=self.decode_split_tokens)
 
+    def _tree(self, q, context, cu_seqlens_q, scale):
+        quant = self._mode() != "auto"
+        return paged_attention_tree(
+            q, self.k_cache, self.v_cache, context.block_tables, context.context_lens, cu_seqlens_q,
+            context.tree_mask, scale, self.num_heads, self.num_kv_heads, self.head_dim, self.block_size,
+            k_scale=self.k_scale if quant else None, v_scale=self.v_scale if quant else None,
+            kv_cache_dtype=self.kv_cache_dtype)
+
     def _prefill(self, q, block_tables, context_lens, cu_seqlens_q, positions, scale):
         quant = self._mode() != "auto"
         return paged_attention_prefill_triton(
@@ -665,6 +772,12 @@ class Attention(nn.Module):
             cu_seqlens = context.cu_seqlens_q
             if cu_seqlens is None:
                 raise ValueError("cu_seqlens_q must be provided for varlen attention")
+            if getattr(context, "tree_mask", None) is not None:
+                # drafted tokens: each row sees the prefix and what its mask names
+                if context.context_lens is None or context.block_tables is None:
+                    raise ValueError("tree attention requires context_lens and block_tables")
+                o = self._tree(q, context, cu_seqlens, scale)
+                return o.reshape(o.shape[0], self.num_heads * self.head_dim)
             if context.is_full_prefill:
                 o = flash_attention_prefill(q, k, v, cu_seqlens, scale, self.num_heads,
                                             self.num_kv_heads, self.head_dim)

@@ -58,6 +58,10 @@ class Context:
     is_full_prefill: bool = False
     residual_slots: torch.Tensor | None = None
     residual_lens: torch.Tensor | None = None
+    # A verification step of speculative decoding (is_prefill, with
+    # cu_seqlens_q): which drafted tokens of its sequence each row sees, bool
+    # (tokens, widest tree).  The reference has no such step.
+    tree_mask: torch.Tensor | None = None
 
 
 def _as_list(values) -> list:
@@ -114,8 +118,9 @@ def reset_context() -> None:
 def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen_k=0,
                 slot_mapping=None, context_lens=None, block_tables=None, positions=None,
                 query_lens=None, is_decode=None, mixed_attention_split=None,
-                is_full_prefill=False, residual_slots=None, residual_lens=None) -> None:
-    """Reference: context.py:103-124 (same keyword names and defaults)."""
+                is_full_prefill=False, residual_slots=None, residual_lens=None, tree_mask=None) -> None:
+    """Reference: context.py:103-124 (same keyword names and defaults, and
+    tree_mask)."""
     global _context
     _context = Context(
         is_prefill=is_prefill, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
@@ -123,4 +128,4 @@ def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0
         context_lens=context_lens, block_tables=block_tables, positions=positions,
         query_lens=query_lens, is_decode=is_decode, mixed_attention_split=mixed_attention_split,
         is_full_prefill=is_full_prefill, residual_slots=residual_slots,
-        residual_lens=residual_lens)
+        residual_lens=residual_lens, tree_mask=tree_mask)
