@@ -66,17 +66,15 @@ struct TreeArgs {
   int q_dtype;
   float sm_scale;
   int max_splits;    // 1: no partial results
-  int target;        // workgroups that fill the GPU
+  int shares;        // the batch's keys over this many make a split
   int min_split;     // keys
-  int row_blocks;
   float* ws_o;       // partials: (seq, kv head, split, row cap, 128)
   float* ws_ml;      // (seq, kv head, split, row cap, 2)
   int row_cap;
 };
 
-// The share of a sequence that a split takes, the same for every sequence: the
-// batch's keys over the workgroups that fill the GPU, in whole tiles.  At most
-// max_splits for the longest.
+// The keys that a split takes, the same for every sequence: the batch's keys over
+// the plan's shares, in whole tiles, and at most max_splits for the longest.
 template <int UNIT>
 MKV_DEV int split_keys(const TreeArgs& a) {
   const int lane = threadIdx.x & 63;
@@ -93,8 +91,7 @@ MKV_DEV int split_keys(const TreeArgs& a) {
     sum += __shfl_xor(sum, o);
     longest = max(longest, __shfl_xor(longest, o));
   }
-  const float share = sum * (float)(a.num_kv_heads * a.row_blocks) / (float)a.target;
-  int len = (int)fminf(share, 1.0e9f);
+  int len = (int)fminf(sum / (float)a.shares, 1.0e9f) + 1;
   len = max(max(len, a.min_split), (longest + a.max_splits - 1) / a.max_splits);
   len = (len + UNIT - 1) / UNIT * UNIT;
   return uniform(len);
@@ -116,13 +113,50 @@ MKV_DEV float other_half(float x) {  // the value of lane ^ 32
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// LDS tiles: 256-byte key rows of 16-bit elements in 16-byte chunks, chunk c of
-// key at position c ^ swz(key).  swz is one-to-one on 16 keys (K operand reads:
-// 16 keys, one chunk) and moves four neighbouring keys to the four 64-byte
-// quarters of a row (transposed V reads: four keys, 32 dims), so both go without
-// bank conflicts.
-MKV_DEV int swz(int key) { return ((key & 3) << 2) | ((key >> 2) & 3); }
-MKV_DEV int tile_offset(int key, int chunk) { return key * 256 + ((chunk ^ swz(key)) << 4); }
+// The largest of three, NaN where one is (v_maximum3_f32).
+MKV_DEV float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
+// LDS tiles: a key's 128 cached elements as they are in the pool (256- or 128-byte
+// rows), its 16-byte chunk i at position i ^ swz(key).
+// 16-bit: swz is one-to-one on 16 keys (K operand reads: 16 keys, one chunk) and
+// moves four neighbouring keys to the four 64-byte quarters of a row (transposed
+// V reads: four keys, 32 dims).
+// 1-byte: two rows fill the 64 banks; swz is one-to-one on the 8 even (odd) keys
+// of 16, and the keys 4h .. 4h+3 and 8+4h .. 8+4h+3 of a transposed V read keep
+// their pairs of chunks apart.
+// Both read without bank conflicts.
+template <int EB>
+struct Tile {
+  static constexpr int kRow = kHeadDim * EB;
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kKeysPerDma = 1024 / kRow;  // a wave's 64 x 16 bytes
+  MKV_DEV static int swz(int key) {
+    if constexpr (EB == 2) return ((key & 3) << 2) | ((key >> 2) & 3);
+    return (key >> 1 & 4) | (key & 2) | (key >> 2 & 1);
+  }
+  MKV_DEV static int offset(int key, int chunk) { return key * kRow + ((chunk ^ swz(key)) << 4); }
+};
+
+template <int N>
+MKV_DEV void wait_vm() {  // all but the wave's last N vector memory operations are done
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 0xf70 | (N >> 4 << 14));
+  asm volatile("" ::: "memory");
+}
+// The wave's LDS reads and writes are done.
+MKV_DEV void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// The workgroup's waves meet, their LDS reads done; LDS DMA stays in flight.
+MKV_DEV void meet() {
+  wait_lds();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // Values that are not finite.  A drafted token that a row does not see weighs
 // P = 0 there, and 0 * inf or 0 * NaN would still reach the row's output: where a
@@ -205,25 +239,57 @@ MKV_DEV void zero_rows_past(const TreeArgs& a, const Work& w) {
   for (int64_t i = threadIdx.x; i < (q1 - first) * dims * size / 2; i += blockDim.x) o[i] = 0;
 }
 
+// 16 one-byte codes of the pool as exact fp16.
+template <int KV_DT>
+MKV_DEV f16x8 codes_to_f16(uint32_t lo, uint32_t hi) {
+  uint32_t w[4];
+  if constexpr (KV_DT == kKvI8PerToken) {
+    // 0x64xx is 1024 + xx in fp16: code + 128 in xx, then 1152 off
+    const uint32_t c[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = perm(0x64646464u, c[i >> 1], i & 1 ? 0x04030402u : 0x04010400u);
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) - off);
+    }
+  } else {
+    w[0] = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<false>(lo));
+    w[1] = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<true>(lo));
+    w[2] = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<false>(hi));
+    w[3] = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<true>(hi));
+  }
+  return __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
+}
+
+// The tile's pipeline.  K and V have one LDS buffer each: the DMA of the next
+// tile's K goes out once the products with K are done and lands under the softmax
+// and P V, the next V's once P V is done and lands under the next K Q^T.  With one
+// row group a wave reads only what it loaded itself and meets no barrier; with
+// more, a barrier stands on either side of each product.  One buffer (64 KB at
+// most) and at most 256 registers leave room for two workgroups a CU, whose
+// waves fill each other's waits and overlap MFMA with the softmax's VALU work.
 template <int KV_DT, int R, int KG, bool PAIR>
-__global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a) {
+MKV_DEV void tree_attention_body(const TreeArgs& a) {
   constexpr int CT = kOperand<KV_DT>;
   constexpr bool kTok = kPerTokenScale<KV_DT>;
-  constexpr int kThreads = 64 * R * KG;
+  constexpr int kWaves = R * KG, kThreads = 64 * kWaves;
   constexpr int TK = KG == 1 ? 64 : 32;   // keys a wave takes of a tile
   constexpr int NK = TK * KG;             // keys of a tile
   constexpr int NB = TK / 32;
   constexpr int kEb = DTypeInfo<KV_DT>::kBytes;
-  constexpr int kChunks = kHeadDim * kEb / 16;         // 16-byte chunks of a cached row
-  constexpr int kKeysPerLoad = kThreads / kChunks;     // keys of one load of the workgroup
-  constexpr int kLoads = NK / kKeysPerLoad;            // loads a thread, for K and for V each
-  static_assert(NK % kKeysPerLoad == 0 && kLoads >= 1, "a tile is whole loads");
-  constexpr int kJoinBytes = (KG - 1) * R * 64 * 66 * 4;
-  constexpr int kTileBytes = 2 * NK * 256;
-  __shared__ __align__(16) char lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
-  __shared__ float sc[kTok ? (PAIR ? 4 : 2) * NK : 1];  // K then V scales, for each head of a pair
-  char* const lds_k = lds;
-  char* const lds_v = lds + NK * 256;
+  using T = Tile<kEb>;
+  constexpr int kOwn = NK / kWaves;                     // keys a wave loads
+  constexpr int kDma = kOwn / T::kKeysPerDma;           // loads of K, and of V, a wave
+  constexpr int kSubs = kOwn > 16 ? kOwn / 16 : 1;      // 16-key sub-tiles (never across a block) they lie in
+  constexpr bool kShared = R > 1;
+  static_assert(kOwn % T::kKeysPerDma == 0 && kDma >= 1, "whole loads");
+  constexpr int kBuf = NK * T::kRow > 16384 ? NK * T::kRow : 16384;  // (the join's halves fit too)
+  __shared__ __align__(16) char lds_k[kBuf], lds_v[kBuf];
+  __shared__ float join_ml[KG > 1 ? 2 * R * 64 * 2 : 1];
+  __shared__ int pres[kShared ? 2 * (NK / 16) : 1];
+  constexpr int kHeads = PAIR ? 2 : 1;
+  constexpr int kScLoads = kTok ? 2 * kHeads * TK / 64 : 1;
+  __shared__ __align__(16) float sc_all[kTok ? kWaves * 2 * kHeads * TK : 4];  // a wave's own: [head][K, V][TK]
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int rg = wave % R, kg = wave / R;
@@ -234,9 +300,78 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
   if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
   if ((blockIdx.z > 0 && k0 >= w.ctx) || (int)blockIdx.y * 32 * R >= w.rows) return;
   const int kb0 = (int)k0, k1 = (int)min(k0 + len, (int64_t)w.ctx);
+  const int prefix = (int)min(w.prefix, (int64_t)0x7fffffff);
   const bool split = w.ctx > len;
 
-  // ---- q: this lane's row, dims 16 s + 8 h .. + 7 of step s ----
+  // ---- loads of tiles ----
+  const int64_t row_bytes = (int64_t)a.num_kv_heads * T::kRow;
+  const int64_t head_bytes = (int64_t)w.kvh * T::kRow;
+  const int own0 = wave * kOwn;  // first key of the tile that this wave loads
+  const int sub0 = own0 & ~15;
+  // lane's key and chunk of a load; loads of one sub-tile differ in the key's
+  // upper bits, which reach the swizzle's low bits
+  const int ld_key = lane / T::kChunks;
+  uint32_t voff[kDma > 4 ? 4 : kDma];
+  constexpr int kPerSub = kDma / kSubs;
+#pragma unroll
+  for (int i = 0; i < kPerSub; ++i) {
+    const int key = (own0 & 15) + i * T::kKeysPerDma + ld_key;
+    voff[i] = (uint32_t)(key * row_bytes) + 16 * ((lane % T::kChunks) ^ T::swz(key));
+  }
+  // block entries of the tile whose K is loaded next
+  int32_t slot[kSubs];
+  int32_t left[kSubs];  // rows of the sub-tile within the context and a present block
+  auto look_up = [&](int kb) {
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) {
+      const int t = kb + sub0 + 16 * u;
+      const int phys = t < k1 ? (int)a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
+      slot[u] = phys < 0 ? 0 : (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1));
+      left[u] = phys < 0 ? 0 : min(k1 - t, 16);
+    }
+  };
+  auto dma = [&](const char* pool, char* buf) {
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) {
+      // (rows past the last read zeros)
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(pool + slot[u] * row_bytes + head_bytes), (short)0,
+          left[u] > 0 ? (int)((left[u] - 1) * row_bytes + T::kRow) : 0, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < kPerSub; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(buf + (own0 + u * 16) * T::kRow + i * 1024), 16, voff[i], 0, 0, 0);
+    }
+  };
+  float sc_raw[kScLoads];
+  float* const sc = sc_all + (kTok ? wave * 2 * kHeads * TK : 0);
+  auto load_scales = [&](int kb) {
+    if constexpr (kTok) {
+#pragma unroll
+      for (int i = 0; i < kScLoads; ++i) {
+        const int at = lane + 64 * i, key = at % TK, which = at / TK;  // K head 0, V head 0, K head 1, V head 1
+        const int t = kb + kg * TK + key;
+        sc_raw[i] = 0.0f;
+        const int64_t phys = t < k1 ? a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
+        if (phys >= 0)
+          sc_raw[i] = ((which & 1) ? a.v_scale : a.k_scale)[((phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1))) *
+                                                               a.scale_heads + w.kvh * kHeads + (which >> 1)];
+      }
+    }
+  };
+  const bool any = kb0 < k1;
+  if (any) {
+    look_up(kb0);
+    load_scales(kb0);
+    if constexpr (kShared) {
+      if (lane == 0) pres[sub0 / 16] = left[0] > 0;
+    }
+    dma(a.k, lds_k);
+    dma(a.v, lds_v);
+  }
+
+  // ---- q: this lane's row; step s of the contraction takes dims 16 s + 8 h .. + 7
+  // (16-bit: chunk 2 s + h), or the lower or upper half of chunk 2 (s / 2) + h ----
   const int row = blockIdx.y * 32 * R + rg * 32 + c;
   const bool row_ok = row < w.rows;
   bool hi = false;
@@ -244,25 +379,14 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
   float score_mul = a.sm_scale * kLog2e;
   Op16<CT> qop[8];
   {
-    float x[8][8];
-    float top = 0.0f;
+    u32x4 raw[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       const bool mine = row_ok && (!PAIR || (s >> 2) == (int)hi);
-      const int d = 16 * (PAIR ? s & 3 : s) + 8 * h;
-      u32x4 v{0, 0, 0, 0};
-      if (mine) v = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (a.q_dtype == MKV_DTYPE_BF16) {
-          x[s][2 * j] = __uint_as_float(v[j] << 16);
-          x[s][2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
-        } else {
-          x[s][2 * j] = f16_bits_to_f32(v[j] & 0xffffu);
-          x[s][2 * j + 1] = f16_bits_to_f32(v[j] >> 16);
-        }
-        top = fmaxf(top, fmaxf(fabsf(x[s][2 * j]), fabsf(x[s][2 * j + 1])));
-      }
+      const int st = PAIR ? s & 3 : s;
+      const int d = kEb == 2 ? 16 * st + 8 * h : 16 * (2 * (st >> 1) + h) + 8 * (st & 1);
+      raw[s] = u32x4{0, 0, 0, 0};
+      if (mine) raw[s] = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);
     }
     // the loop keeps raw scores and wants score_mul > 0: a negative scale
     // moves its sign into q, a zero one makes q zero
@@ -271,9 +395,19 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
       f = score_mul < 0.0f ? -1.0f : 0.0f;
       score_mul = score_mul < 0.0f ? -score_mul : 1.0f;
     }
+    auto element = [&](int s, int j) {
+      const uint32_t x = raw[s][j >> 1];
+      if (a.q_dtype == MKV_DTYPE_BF16) return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
+      return f16_bits_to_f32(j & 1 ? x >> 16 : x & 0xffffu);
+    };
     if constexpr (CT == MKV_DTYPE_F16) {
       // a row's q times a power of two: a bf16 q in fp16 is exact but for
       // elements below 2^-24 of the row's largest
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(element(s, j)));
       top = fmaxf(top, other_half(top));
       if (top > 0.0f && top < __builtin_huge_valf()) {
         const int e = ilogbf(top);
@@ -286,216 +420,136 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (CT == MKV_DTYPE_BF16)
-          qop[s][j] = (__bf16)(x[s][j] * f);
+          qop[s][j] = (__bf16)(element(s, j) * f);
         else
-          qop[s][j] = (_Float16)(x[s][j] * f);
+          qop[s][j] = (_Float16)(element(s, j) * f);
       }
   }
   if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) score_mul *= load_uniform_f32(a.k_scale);
 
-  const int64_t row_bytes = (int64_t)a.num_kv_heads * kHeadDim * kEb;
-  const int64_t head_bytes = (int64_t)w.kvh * kHeadDim * kEb;
   const uint8_t* mask_row = a.mask + (w.q0 + (row_ok ? row / a.group : 0)) * a.mask_stride;
-
   f32x16 acc[4];
 #pragma unroll
   for (int b = 0; b < 4; ++b) acc[b] = f32x16{};
   float m_run = kNegBig, l_run = 0.0f;
 
-  // ---- staging: 16 keys never straddle a block ----
-  constexpr int kSubs = NK / 16;
-  u32x4 st_k[kLoads], st_v[kLoads];
-  const int ld_key = tid / kChunks, ld_ch = tid % kChunks;
-  uint32_t present = 0, present_next = 0;
-  constexpr int kScales = (PAIR ? 4 : 2) * NK, kScLoads = (kScales + kThreads - 1) / kThreads;
-  float st_sc[kScLoads];
-  auto load_tile = [&](int kb) {
-    present_next = 0;
-    int64_t slot[kSubs];
-#pragma unroll
-    for (int u = 0; u < kSubs; ++u) {
-      const int t = kb + 16 * u;
-      const int64_t phys = t < k1 ? a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
-      present_next |= phys >= 0 ? 1u << u : 0u;
-      slot[u] = phys < 0 ? -1 : (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1));
-    }
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int key = u * kKeysPerLoad + ld_key;
-      int64_t s = -1;
-#pragma unroll
-      for (int j = 0; j < kSubs; ++j)
-        if (key >> 4 == j) s = slot[j];
-      st_k[u] = st_v[u] = u32x4{0, 0, 0, 0};
-      if (s >= 0 && kb + key < k1) {
-        const int64_t o = (s + (key & 15)) * row_bytes + head_bytes + 16 * ld_ch;
-        st_k[u] = ld16(a.k + o);
-        st_v[u] = ld16(a.v + o);
-      }
-    }
-    if constexpr (kTok) {
-      constexpr int kHeads = PAIR ? 2 : 1;
-#pragma unroll
-      for (int i = 0; i < kScLoads; ++i) {
-        // K head 0, V head 0, K head 1, V head 1
-        const int key = (tid + i * kThreads) % NK, which = (tid + i * kThreads) / NK;
-        int64_t s = -1;
-#pragma unroll
-        for (int j = 0; j < kSubs; ++j)
-          if (key >> 4 == j) s = slot[j];
-        st_sc[i] = 0.0f;
-        if (which < 2 * kHeads && s >= 0 && kb + key < k1)
-          st_sc[i] = ((which & 1) ? a.v_scale : a.k_scale)[(s + (key & 15)) * a.scale_heads + w.kvh * kHeads + (which >> 1)];
-      }
-    }
-  };
-  auto convert = [&](u32x4 v, u32x4& lo, u32x4& hi16) {  // 16 codes -> 16 exact fp16
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t a0, a1;
-      if constexpr (KV_DT == kKvI8PerToken) {
-        a0 = __builtin_bit_cast(uint32_t, i8x2_to_f16x2<false>(v[j]));
-        a1 = __builtin_bit_cast(uint32_t, i8x2_to_f16x2<true>(v[j]));
-      } else {
-        a0 = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<false>(v[j]));
-        a1 = __builtin_bit_cast(uint32_t, fp8x2_to_f16x2<true>(v[j]));
-      }
-      if (j < 2) {
-        lo[2 * j] = a0;
-        lo[2 * j + 1] = a1;
-      } else {
-        hi16[2 * j - 4] = a0;
-        hi16[2 * j - 3] = a1;
-      }
-    }
-  };
-  auto store_tile = [&]() {
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int key = u * kKeysPerLoad + ld_key;
-      if constexpr (kEb == 2) {
-        *reinterpret_cast<u32x4*>(lds_k + tile_offset(key, ld_ch)) = st_k[u];
-        *reinterpret_cast<u32x4*>(lds_v + tile_offset(key, ld_ch)) = st_v[u];
-      } else {
-        u32x4 lo, hi16;
-        convert(st_k[u], lo, hi16);
-        *reinterpret_cast<u32x4*>(lds_k + tile_offset(key, 2 * ld_ch)) = lo;
-        *reinterpret_cast<u32x4*>(lds_k + tile_offset(key, 2 * ld_ch + 1)) = hi16;
-        convert(st_v[u], lo, hi16);
-        *reinterpret_cast<u32x4*>(lds_v + tile_offset(key, 2 * ld_ch)) = lo;
-        *reinterpret_cast<u32x4*>(lds_v + tile_offset(key, 2 * ld_ch + 1)) = hi16;
-      }
-    }
-    if constexpr (kTok) {
-#pragma unroll
-      for (int i = 0; i < kScLoads; ++i)
-        if (tid + i * kThreads < kScales) sc[tid + i * kThreads] = st_sc[i];
-    }
-  };
-
-  // transposed V reads: lane 4i + q of a 16-lane group reads key 4h + i at dims
-  // 16 (lane >> 4 & 1) + 4q of the block, and receives V[4h + 0..3][its dim]
-  const int vi = (lane & 15) >> 2, vq = lane & 3, vg = (lane >> 4) & 1;
-
-  if (kb0 < k1) load_tile(kb0);
-  for (int kb = kb0; kb < k1; kb += NK) {
-    __syncthreads();
-    store_tile();
-    present = present_next;
-    __syncthreads();
-    if (kb + NK < k1) load_tile(kb + NK);
-
-    const int key0 = kg * TK;  // this wave's keys of the tile
+  // transposed V reads: within a 16-lane group, lane d of the result holds dim d
+  // of keys 4h + 0..3 and 8 + 4h + 0..3 of 16.  16-bit: two reads, lane 4i + q
+  // reading key i (+ 4h, + 8) at dims 4q; 1-byte: lane 2i + q key i at dims 8q.
+  const int vg = (lane >> 4) & 1;
+  const int vi = kEb == 2 ? (lane & 15) >> 2 : (lane & 15) >> 1;
+  const int v_key = kEb == 2 ? 4 * h + vi : (vi & 3) + 4 * h + 2 * (vi & 4);
+  const int v_sub = kEb == 2 ? 8 * (lane & 1) : 8 * (lane & 1);
+  const int v_chunk = kEb == 2 ? 2 * vg + ((lane & 3) >> 1) : vg;
+  auto v_operand = [&](int nb, int half, int b) {
     typedef short i16x8 __attribute__((ext_vector_type(8)));
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-    auto v_operand = [&](int nb, int half, int b) {
-      const int key = key0 + 32 * nb + 16 * half + 4 * h + vi;
-      const int chunk = 4 * b + 2 * vg + (vq >> 1), sub = 8 * (vq & 1);
-      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + tile_offset(key, chunk) + sub));
-      const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + tile_offset(key + 8, chunk) + sub));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    const int key = kg * TK + 32 * nb + 16 * half + v_key;
+    if constexpr (kEb == 2) {
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + T::offset(key, 4 * b + v_chunk) + v_sub));
+      const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + T::offset(key + 8, 4 * b + v_chunk) + v_sub));
       const i16x8 vt = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
       return __builtin_bit_cast(Op16<CT>, vt);
-    };
-    // ---- what this lane's row sees of a tile that is not all prefix: element
+    } else {
+      const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_v + T::offset(key, 2 * b + v_chunk) + v_sub));
+      return codes_to_f16<KV_DT>((uint32_t)x[0], (uint32_t)x[1]);
+    }
+  };
+
+  for (int kb = kb0, turn = 0; kb < k1; kb += NK, turn ^= 1) {
+    wait_vm<kDma>();  // K is here, V may be on its way
+    if constexpr (kShared) meet();
+    const int key0 = kg * TK;  // this wave's keys of the tile
+    uint32_t present = 0;
+    if constexpr (kShared) {
+#pragma unroll
+      for (int u = 0; u < TK / 16; ++u) present |= uniform(pres[turn * (NK / 16) + key0 / 16 + u]) ? 1u << u : 0u;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u) present |= left[u] > 0 ? 1u << u : 0u;
+    }
+    if constexpr (kTok) {
+#pragma unroll
+      for (int i = 0; i < kScLoads; ++i) sc[lane + 64 * i] = sc_raw[i];
+    }
+    // ---- what this lane's row sees of keys that are not all prefix: element
     // e of key block nb is key 32 nb + 8 (e >> 2) + 4h + (e & 3) ----
-    const bool masked = kb + NK > min(w.prefix, (int64_t)k1) || present != (1u << kSubs) - 1;
+    const bool drafted = kb + key0 + TK > prefix;
+    const bool masked = drafted || kb + key0 + TK > k1 || present != (1u << TK / 16) - 1;
     uint32_t seen[NB] = {};
     if (masked) {
+      uint32_t few = 0;  // a mask narrower than a word
+      if (drafted && row_ok && a.mask_cols < 4)
+        for (int j = 0; j < a.mask_cols; ++j) few |= mask_row[j] ? 0xffu << 8 * j : 0u;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int kl = key0 + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
-          const int64_t j = kb + kl - w.prefix;
-          bool vis = kb + kl < k1 && ((present >> (kl >> 4)) & 1);
-          if (vis && j >= 0) vis = row_ok && j < a.mask_cols && mask_row[j] != 0;
-          seen[nb] |= vis ? 1u << e : 0u;
-        }
-      }
-      if (kb + NK > w.prefix) {
-        bool found = false;
-        for (int i = tid; i < NK * 16; i += kThreads) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(lds_v + 16 * i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) found |= not_finite2<CT>(v[j]);
-        }
-        if (__syncthreads_or(found)) {
-          for (int b = 0; b < 4; ++b) {
-            f32x16 marks = f32x16{};
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                Op16<CT> vt = v_operand(nb, half, b), sees;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float one = (seen[nb] >> (8 * half + j)) & 1 ? 1.0f : 0.0f;
-                  if constexpr (CT == MKV_DTYPE_BF16) {
-                    vt[j] = (__bf16)mark_of((float)vt[j]);
-                    sees[j] = (__bf16)one;
-                  } else {
-                    vt[j] = (_Float16)mark_of((float)vt[j]);
-                    sees[j] = (_Float16)one;
-                  }
-                }
-                marks = mfma32<CT>(vt, sees, marks);
-              }
-#pragma unroll
-            for (int bb = 0; bb < 4; ++bb)
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (bb == b && marks[e] > 0.0f) acc[bb][e] += marked_value(marks[e]);
+        for (int g = 0; g < 4; ++g) {
+          const int kl = 32 * nb + 8 * g + 4 * h, t = kb + key0 + kl;
+          const int j0 = t - prefix;  // the four keys' first column
+          uint32_t x = 0;
+          if (row_ok && j0 > -4 && j0 < a.mask_cols) {
+            const int at = a.mask_cols < 4 ? 0 : min(max(j0, 0), a.mask_cols - 4);
+            x = few;
+            if (a.mask_cols >= 4) __builtin_memcpy(&x, mask_row + at, 4);
+            x = j0 >= at ? x >> 8 * (j0 - at) : x << 8 * (at - j0);
           }
-          __syncthreads();
-          for (int i = tid; i < NK * 64; i += kThreads) {
-            uint32_t* v = reinterpret_cast<uint32_t*>(lds_v) + i;
-            constexpr uint32_t e = CT == MKV_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-            uint32_t x = *v;
-            if ((x & e) == e) x &= 0xffff0000u;
-            if (((x >> 16) & e) == e) x &= 0xffffu;
-            *v = x;
+          const bool here = (present >> (kl >> 4)) & 1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool vis = here && t + e < k1 && (j0 + e < 0 || (x >> 8 * e & 0xffu) != 0);
+            seen[nb] |= vis ? 1u << (4 * g + e) : 0u;
           }
-          __syncthreads();
         }
       }
     }
+
+    // ---- S^T = K Q^T ----
     f32x16 s[NB];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       s[nb] = f32x16{};
       const int key = key0 + 32 * nb + c;
+      if constexpr (kEb == 2) {
 #pragma unroll
-      for (int st = 0; st < 8; ++st) {
-        const u32x4 kw = *reinterpret_cast<const u32x4*>(lds_k + tile_offset(key, 2 * st + h));
-        s[nb] = mfma32<CT>(__builtin_bit_cast(Op16<CT>, kw), qop[st], s[nb]);
+        for (int st = 0; st < 8; ++st) {
+          const u32x4 kw = *reinterpret_cast<const u32x4*>(lds_k + T::offset(key, 2 * st + h));
+          s[nb] = mfma32<CT>(__builtin_bit_cast(Op16<CT>, kw), qop[st], s[nb]);
+        }
+      } else {
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          const u32x4 kw = *reinterpret_cast<const u32x4*>(lds_k + T::offset(key, 2 * st + h));
+          s[nb] = mfma32<CT>(codes_to_f16<KV_DT>(kw[0], kw[1]), qop[2 * st], s[nb]);
+          s[nb] = mfma32<CT>(codes_to_f16<KV_DT>(kw[2], kw[3]), qop[2 * st + 1], s[nb]);
+        }
       }
     }
-    const float* ks = sc + (PAIR && hi ? 2 * NK : 0) + key0;
+    __builtin_amdgcn_s_setprio(0);
+    // ---- the next tile's K, where this one's was ----
+    look_up(kb + NK);
+    load_scales(kb + NK);
+    if constexpr (kShared) {
+      if (lane == 0) pres[(turn ^ 1) * (NK / 16) + sub0 / 16] = left[0] > 0;
+    }
+    if constexpr (kShared) meet();
+    else wait_lds();
+    dma(a.k, lds_k);
+
+    // ---- softmax ----
+    const float* ks = sc + (PAIR && hi ? 2 * TK : 0);
     if constexpr (kTok) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[nb][e] *= ks[32 * nb + 8 * (e >> 2) + 4 * h + (e & 3)];
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(ks + 32 * nb + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nb][4 * g + e] *= x[e];
+        }
     }
     if (masked) {
 #pragma unroll
@@ -507,7 +561,7 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[nb][e]);
+      for (int e = 0; e < 16; e += 2) mx = max3(mx, s[nb][e], s[nb][e + 1]);
     mx = fmaxf(mx, other_half(mx));
     mx = fmaxf(mx * score_mul, kNegBig);
     const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
@@ -521,18 +575,90 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[b][e] *= alpha;
     }
-    float p[NB][16];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p[nb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][e], score_mul, -m_new));
-        l_run += p[nb][e];
-        if constexpr (kTok) {
-          p[nb][e] *= ks[NK + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3)];
-          if (masked) p[nb][e] = (seen[nb] >> e) & 1 ? p[nb][e] : 0.0f;
+      for (int g = 0; g < 4; ++g) {
+        f32x4 x;
+        if constexpr (kTok) x = *reinterpret_cast<const f32x4*>(ks + TK + 32 * nb + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = 4 * g + j;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][e], score_mul, -m_new));
+          l_run += p;
+          s[nb][e] = p;
+          if constexpr (kTok) {
+            s[nb][e] = p * x[j];
+            if (masked) s[nb][e] = (seen[nb] >> e) & 1 ? s[nb][e] : 0.0f;
+          }
         }
       }
+
+    // ---- O^T += V^T P^T ----
+    wait_vm<kDma>();  // V is here, the next K may be on its way
+    if constexpr (kShared) meet();
+    if (kShared ? kb + NK > prefix : drafted) {
+      bool found = false;
+      constexpr int kScan = kShared ? NK * T::kChunks / kThreads : TK * T::kChunks / 64;
+      for (int i = 0; i < kScan; ++i) {
+        const int at = kShared ? i * kThreads + tid : kg * TK * T::kChunks + i * 64 + lane;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(lds_v + 16 * at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kEb == 2) found |= not_finite2<CT>(v[j]);
+          // (e4m3: S.1111.111 alone)
+          else if constexpr (KV_DT != kKvI8PerToken)
+            found |= (((v[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+        }
+      }
+      if (kShared ? __syncthreads_or(found) : __builtin_amdgcn_ballot_w64(found) != 0) {
+        for (int b = 0; b < 4; ++b) {
+          f32x16 marks = f32x16{};
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              Op16<CT> vt = v_operand(nb, half, b), sees;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float one = !masked || ((seen[nb] >> (8 * half + j)) & 1) ? 1.0f : 0.0f;
+                if constexpr (CT == MKV_DTYPE_BF16) {
+                  vt[j] = (__bf16)mark_of((float)vt[j]);
+                  sees[j] = (__bf16)one;
+                } else {
+                  vt[j] = (_Float16)mark_of((float)vt[j]);
+                  sees[j] = (_Float16)one;
+                }
+              }
+              marks = mfma32<CT>(vt, sees, marks);
+            }
+#pragma unroll
+          for (int bb = 0; bb < 4; ++bb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (bb == b && marks[e] > 0.0f) acc[bb][e] += marked_value(marks[e]);
+        }
+        if constexpr (kShared) meet();
+        for (int i = 0; i < kScan * 4; ++i) {
+          const int at = kShared ? i * kThreads + tid : kg * TK * T::kChunks * 4 + i * 64 + lane;
+          uint32_t* v = reinterpret_cast<uint32_t*>(lds_v) + at;
+          uint32_t x = *v;
+          if constexpr (kEb == 2) {
+            constexpr uint32_t e = CT == MKV_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+            if ((x & e) == e) x &= 0xffff0000u;
+            if (((x >> 16) & e) == e) x &= 0xffffu;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if ((x >> 8 * j & 0x7fu) == 0x7fu) x &= ~(0xffu << 8 * j);
+          }
+          *v = x;
+        }
+        if constexpr (kShared) meet();
+        else wait_lds();
+      }
+    }
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -540,14 +666,23 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
         Op16<CT> ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float x = p[nb][8 * half + j];
-          if constexpr (CT == MKV_DTYPE_BF16) {
-            // bf16 holds P to 8 bits: a second term carries the rest, so that
-            // a row whose weight sits on few keys is as exact as decode's
-            ph[j] = (__bf16)x;
-            pl[j] = (__bf16)(x - (float)ph[j]);
-          } else {
-            ph[j] = (_Float16)x;
+          if constexpr (CT == MKV_DTYPE_BF16)
+            ph[j] = (__bf16)s[nb][8 * half + j];
+          else
+            ph[j] = (_Float16)s[nb][8 * half + j];
+        }
+        if constexpr (CT == MKV_DTYPE_BF16) {
+          // bf16 holds P to 8 bits: a second term carries the rest, so that a
+          // row whose weight sits on few keys is as exact as decode's.  p - hi is
+          // one dot product a value: hi_pair . (-1, 0) or (0, -1), + p
+          uint32_t lo_bits = 0x0000bf80u, hi_bits = 0xbf800000u;
+          asm volatile("" : "+s"(lo_bits), "+s"(hi_bits));
+          const bf16x2 neg_lo = __builtin_bit_cast(bf16x2, lo_bits), neg_hi = __builtin_bit_cast(bf16x2, hi_bits);
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const bf16x2 hp = {ph[j], ph[j + 1]};
+            pl[j] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_lo, s[nb][8 * half + j], false);
+            pl[j + 1] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_hi, s[nb][8 * half + j + 1], false);
           }
         }
 #pragma unroll
@@ -557,35 +692,45 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
           if constexpr (CT == MKV_DTYPE_BF16) acc[b] = mfma32<CT>(vt, pl, acc[b]);
         }
       }
+    __builtin_amdgcn_s_setprio(0);
+    // ---- the next tile's V, where this one's was ----
+    if constexpr (kShared) meet();
+    else wait_lds();
+    dma(a.v, lds_v);
   }
 
-  // ---- the key groups' results, joined in the first one's waves ----
+  // ---- the key groups' results, joined pairwise into the first one's ----
+  wait_vm<0>();
   if constexpr (KG > 1) {
-    __syncthreads();
-    float* part = reinterpret_cast<float*>(lds);
-    if (kg > 0) {
-      float* o = part + ((kg - 1) * R + rg) * 64 * 66;
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+    for (int step = KG / 2; step >= 1; step /= 2) {
+      meet();
+      if (kg >= step && kg < 2 * step) {
+        const int at = (kg - step) * R + rg;  // 0 or 1
+        float* o = reinterpret_cast<float*>(at ? lds_v : lds_k);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[(16 * b + e) * 64 + lane] = acc[b][e];
-      o[64 * 64 + lane] = m_run;
-      o[65 * 64 + lane] = l_run;
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[(16 * b + e) * 64 + lane] = acc[b][e];
+        join_ml[(at * 64 + lane) * 2] = m_run;
+        join_ml[(at * 64 + lane) * 2 + 1] = l_run;
+      }
+      meet();
+      if (kg < step) {
+        const int at = kg * R + rg;
+        const float* o = reinterpret_cast<const float*>(at ? lds_v : lds_k);
+        const float m = join_ml[(at * 64 + lane) * 2], l = join_ml[(at * 64 + lane) * 2 + 1];
+        const float m_new = fmaxf(m, m_run);
+        const float fa = __builtin_amdgcn_exp2f(m_run - m_new), fb = __builtin_amdgcn_exp2f(m - m_new);
+        m_run = m_new;
+        l_run = l_run * fa + l * fb;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[b][e] = acc[b][e] * fa + o[(16 * b + e) * 64 + lane] * fb;
+      }
     }
-    __syncthreads();
     if (kg > 0) return;
-    for (int g = 1; g < KG; ++g) {
-      const float* o = part + ((g - 1) * R + rg) * 64 * 66;
-      const float m = o[64 * 64 + lane], l = o[65 * 64 + lane];
-      const float m_new = fmaxf(m, m_run);
-      const float fa = __builtin_amdgcn_exp2f(m_run - m_new), fb = __builtin_amdgcn_exp2f(m - m_new);
-      m_run = m_new;
-      l_run = l_run * fa + l * fb;
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[b][e] = acc[b][e] * fa + o[(16 * b + e) * 64 + lane] * fb;
-    }
   }
   const float l = l_run + other_half(l_run);
   if (!row_ok) return;
@@ -617,6 +762,11 @@ __global__ __launch_bounds__(64 * R * KG) void tree_attention_kernel(TreeArgs a)
   }
 }
 
+template <int KV_DT, int R, int KG, bool PAIR>
+__global__ __launch_bounds__(64 * R * KG) __attribute__((amdgpu_waves_per_eu(2))) void tree_attention_kernel(TreeArgs a) {
+  tree_attention_body<KV_DT, R, KG, PAIR>(a);
+}
+
 // Rows of sequences in several splits: a wave a row, two dims a lane.
 constexpr int kJoinWaves = 4;
 template <int UNIT, bool FP8, bool PAIR>
@@ -629,17 +779,30 @@ __global__ __launch_bounds__(64 * kJoinWaves) void tree_join_kernel(TreeArgs a) 
   const int row = blockIdx.y * kJoinWaves + uniform(threadIdx.x >> 6);
   if (row >= w.rows) return;
   const int64_t at = (int64_t)blockIdx.x * a.max_splits * a.row_cap + row;
-  float m = kNegBig, l = 0.0f, x = 0.0f, y = 0.0f;
-  for (int z = 0; z < n; ++z) {
-    const int64_t i = at + (int64_t)z * a.row_cap;
-    const float mz = a.ws_ml[2 * i], lz = a.ws_ml[2 * i + 1];
-    const float* o = a.ws_o + i * kHeadDim + 2 * lane;
-    const float m_new = fmaxf(m, mz);
-    const float fa = __builtin_amdgcn_exp2f(m - m_new), fb = __builtin_amdgcn_exp2f(mz - m_new);
-    m = m_new;
-    l = l * fa + lz * fb;
-    x = x * fa + o[0] * fb;
-    y = y * fa + o[1] * fb;
+  // the largest maximum first (a lane a split), then the sums, eight splits'
+  // loads in flight
+  float m = kNegBig;
+  for (int z = lane; z < n; z += 64) m = fmaxf(m, a.ws_ml[2 * (at + (int64_t)z * a.row_cap)]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float l = 0.0f, x = 0.0f, y = 0.0f;
+  for (int z0 = 0; z0 < n; z0 += 8) {
+    f32x2 ml[8], o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = at + (int64_t)min(z0 + j, n - 1) * a.row_cap;
+      ml[j] = *reinterpret_cast<const f32x2*>(a.ws_ml + 2 * i);
+      o[j] = *reinterpret_cast<const f32x2*>(a.ws_o + i * kHeadDim + 2 * lane);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (z0 + j < n) {
+        const float f = __builtin_amdgcn_exp2f(ml[j][0] - m);
+        l += ml[j][1] * f;
+        x += o[j][0] * f;
+        y += o[j][1] * f;
+      }
+    }
   }
   float norm = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   if constexpr (FP8) norm *= load_uniform_f32(a.v_scale);
@@ -856,7 +1019,7 @@ struct Plan {
   int row_blocks;
   int row_cap;
   int unit;        // keys of a tile
-  int target;
+  int shares;
   int min_split;
   int max_splits;
 };
@@ -871,15 +1034,24 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   if (p.row_blocks < 1) p.row_blocks = 1;
   p.row_cap = p.row_blocks * 32 * p.row_groups;
   p.unit = p.row_groups == 1 ? 128 : 64;
-  p.target = p.row_groups == 8 ? 512 : 1024;
   p.min_split = 128;
-  const int64_t items = (int64_t)num_seqs * kernel_kv_heads * p.row_blocks;
-  // twice the even share: the longest sequences of a ragged batch
-  int64_t s = items > 0 ? 2 * (p.target + items - 1) / items : 1;
+  // Workgroups that run at once: two a CU of four waves, one of eight.  Where the
+  // sequences leave some free, their keys are dealt out so that all fit one round
+  // (a sequence's last split may be short: num_seqs shares are kept back); where
+  // they do not fit a round, in pieces of a quarter round; many sequences split
+  // only those of more than twice the mean.
+  const int64_t slots = p.row_groups == 8 ? 256 : 512;
+  const int64_t round = slots / ((int64_t)kernel_kv_heads * p.row_blocks) > 0 ? slots / ((int64_t)kernel_kv_heads * p.row_blocks) : 1;
+  int64_t shares;
+  if (num_seqs <= round)
+    shares = round - num_seqs > round / 4 ? round - num_seqs : round / 4;
+  else if (num_seqs < 4 * round)
+    shares = 4 * round - num_seqs > round ? 4 * round - num_seqs : round;
+  else
+    shares = num_seqs / 2;
+  p.shares = (int)(shares < 1 ? 1 : shares);
   const int64_t most = (capacity + p.min_split - 1) / p.min_split;
-  if (items >= 2 * p.target) s = 1;
-  if (s > most) s = most;
-  p.max_splits = (int)(s < 1 ? 1 : s);
+  p.max_splits = (int)(p.shares + 1 < most ? p.shares + 1 : most > 1 ? most : 1);
   return p;
 }
 
@@ -957,7 +1129,8 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
                               int64_t total_q, int num_heads, int num_kv_heads, int head_dim, int block_size,
                               float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (int st = check_tree(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols)) return st;
-  if (num_blocks < 0 || num_blocks > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+  // (token rows and, within 16 of them, bytes are counted in 32 bits)
+  if (num_blocks < 0 || num_blocks * block_size > 0x7fffffff || num_kv_heads > (1 << 16)) return MKV_ERR_BAD_SHAPE;
   if (num_seqs == 0 || total_q == 0) return MKV_OK;
   const bool code = kv_dtype == MKV_DTYPE_FP8E4M3 || kv_dtype == MKV_DTYPE_I8;
   const bool token = code && kv_scale_mode == MKV_SCALE_PER_TOKEN_HEAD;
@@ -1001,9 +1174,8 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
   a.q_dtype = q_dtype;
   a.sm_scale = sm_scale;
   a.max_splits = p.max_splits;
-  a.target = p.target;
+  a.shares = p.shares;
   a.min_split = p.min_split;
-  a.row_blocks = p.row_blocks;
   a.row_cap = p.row_cap;
   a.ws_o = reinterpret_cast<float*>(workspace);
   a.ws_ml = a.ws_o + (size_t)items * p.max_splits * p.row_cap * kHeadDim;
