@@ -73,6 +73,14 @@ struct TreeArgs {
   int row_cap;
 };
 
+// Element i of an int32 or int64 array, without a branch (so that loads of several
+// go out together).
+MKV_DEV int64_t load_len(const void* p, int i, int i64) {
+  const int32_t* x = reinterpret_cast<const int32_t*>(p);
+  const int32_t lo = x[(int64_t)i << i64], hi = x[((int64_t)i << i64) + i64];
+  return i64 ? (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo) : (int64_t)lo;
+}
+
 // The keys that a split takes, the same for every sequence: the batch's keys over
 // the plan's shares, in whole tiles, and at most max_splits for the longest.
 template <int UNIT>
@@ -81,10 +89,12 @@ MKV_DEV int split_keys(const TreeArgs& a) {
   const int64_t cap = (int64_t)a.idx.max_blocks << a.idx.bs_log2;
   float sum = 0.0f;  // (a rule of thumb's accuracy, the same in every wave)
   int longest = 0;
-  for (int s = lane; s < a.num_seqs; s += 64) {
-    const int64_t c = min(max(load_index(a.ctx, s, a.ctx_i64), (int64_t)0), cap);
-    sum += (float)c;
-    longest = max(longest, (int)c);
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const int64_t c = load_len(a.ctx, min(s, a.num_seqs - 1), a.ctx_i64);
+    const int n = s < a.num_seqs ? (int)min(max(c, (int64_t)0), cap) : 0;
+    sum += (float)n;
+    longest = max(longest, n);
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
@@ -165,13 +175,18 @@ MKV_DEV void meet() {
 // belong to.  Marks of up to 64 keys add up without mixing.
 constexpr float kMarkPos = 1.0f, kMarkNeg = 256.0f, kMarkNan = 32768.0f;
 MKV_DEV float mark_of(float x) {
-  return x != x ? kMarkNan : x == __builtin_huge_valf() ? kMarkPos : x == -__builtin_huge_valf() ? kMarkNeg : 0.0f;
+  float m = x == __builtin_huge_valf() ? kMarkPos : 0.0f;
+  m = x == -__builtin_huge_valf() ? kMarkNeg : m;
+  return x != x ? kMarkNan : m;
 }
-MKV_DEV float marked_value(float n) {  // n > 0
-  const bool nan = n >= kMarkNan;
-  n -= kMarkNan * floorf(n * (1.0f / kMarkNan));
-  const bool neg = n >= kMarkNeg, pos = n != kMarkNeg * floorf(n * (1.0f / kMarkNeg));
-  return nan || (neg && pos) ? __builtin_nanf("") : pos ? __builtin_huge_valf() : -__builtin_huge_valf();
+MKV_DEV float marked_value(float n) {  // 0 without marks
+  const float nans = floorf(n * (1.0f / kMarkNan));
+  n -= kMarkNan * nans;
+  const float negs = floorf(n * (1.0f / kMarkNeg));
+  n -= kMarkNeg * negs;
+  float v = n > 0.0f ? __builtin_huge_valf() : 0.0f;
+  v = negs > 0.0f ? v - __builtin_huge_valf() : v;  // (inf - inf: NaN)
+  return nans > 0.0f ? __builtin_nanf("") : v;
 }
 MKV_DEV bool not_finite(float x) { return !(fabsf(x) < __builtin_huge_valf()); }
 // two 16-bit elements: exponent bits all ones
@@ -199,7 +214,7 @@ MKV_DEV Work find_work(const TreeArgs& a, int item) {
   w.seq = item / a.num_kv_heads;
   const int64_t q0 = min(max((int64_t)a.cu[w.seq], (int64_t)0), a.total_q);
   const int64_t q1 = min(max((int64_t)a.cu[w.seq + 1], q0), a.total_q);
-  const int64_t c = max(load_index(a.ctx, w.seq, a.ctx_i64), (int64_t)0);
+  const int64_t c = max(load_len(a.ctx, w.seq, a.ctx_i64), (int64_t)0);
   w.q0 = q0;
   w.rows = (int)min(q1 - q0, (int64_t)a.mask_cols) * a.group;
   w.prefix = max(c - (q1 - q0), (int64_t)0);
@@ -286,7 +301,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   constexpr int kBuf = NK * T::kRow > 16384 ? NK * T::kRow : 16384;  // (the join's halves fit too)
   __shared__ __align__(16) char lds_k[kBuf], lds_v[kBuf];
   __shared__ float join_ml[KG > 1 ? 2 * R * 64 * 2 : 1];
-  __shared__ int pres[kShared ? 2 * (NK / 16) : 1];
+  __shared__ int slots[kShared ? 2 * (NK / 16) : 1];  // of each sub-tile, -1 absent, by the tile's parity
   constexpr int kHeads = PAIR ? 2 : 1;
   constexpr int kScLoads = kTok ? 2 * kHeads * TK / 64 : 1;
   __shared__ __align__(16) float sc_all[kTok ? kWaves * 2 * kHeads * TK : 4];  // a wave's own: [head][K, V][TK]
@@ -297,8 +312,10 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   const Work w = find_work(a, blockIdx.x);
   const int len = a.max_splits > 1 ? split_keys<NK>(a) : 0x7fffffff / NK * NK;
   const int64_t k0 = (int64_t)blockIdx.z * len;
-  if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
-  if ((blockIdx.z > 0 && k0 >= w.ctx) || (int)blockIdx.y * 32 * R >= w.rows) return;
+  if ((blockIdx.z > 0 && k0 >= w.ctx) || (int)blockIdx.y * 32 * R >= w.rows) {
+    if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
+    return;
+  }
   const int kb0 = (int)k0, k1 = (int)min(k0 + len, (int64_t)w.ctx);
   const int prefix = (int)min(w.prefix, (int64_t)0x7fffffff);
   const bool split = w.ctx > len;
@@ -318,16 +335,24 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     const int key = (own0 & 15) + i * T::kKeysPerDma + ld_key;
     voff[i] = (uint32_t)(key * row_bytes) + 16 * ((lane % T::kChunks) ^ T::swz(key));
   }
-  // block entries of the tile whose K is loaded next
-  int32_t slot[kSubs];
-  int32_t left[kSubs];  // rows of the sub-tile within the context and a present block
-  auto look_up = [&](int kb) {
+  // The tile whose K is loaded next: its sub-tiles' first token slots, and the
+  // rows of each that lie within the context in a present block.  The block
+  // entries come a tile ahead by a vector load (a scalar one would share its
+  // counter with the LDS reads), lane 0 the first sub-tile's, lane 32 the second's.
+  int32_t slot[kSubs], left[kSubs];
+  const int32_t* bt_row = a.idx.block_tables + (int64_t)w.seq * a.idx.bt_stride;
+  auto entry_load = [&](int kb) -> int32_t {
+    const int blk = (kb + sub0 + (kSubs > 1 ? 16 * h : 0)) >> a.idx.bs_log2;
+    return bt_row[min(blk, a.idx.max_blocks - 1)];
+  };
+  auto entry_use = [&](int kb, int32_t e) {
 #pragma unroll
     for (int u = 0; u < kSubs; ++u) {
       const int t = kb + sub0 + 16 * u;
-      const int phys = t < k1 ? (int)a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
-      slot[u] = phys < 0 ? 0 : (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1));
-      left[u] = phys < 0 ? 0 : min(k1 - t, 16);
+      const int phys = __builtin_amdgcn_readlane(e, 32 * u);
+      const bool ok = t < k1 && phys >= 0 && phys < (int)a.idx.num_blocks;
+      slot[u] = ok ? (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : 0;
+      left[u] = ok ? min(k1 - t, 16) : 0;
     }
   };
   auto dma = [&](const char* pool, char* buf) {
@@ -345,27 +370,34 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   };
   float sc_raw[kScLoads];
   float* const sc = sc_all + (kTok ? wave * 2 * kHeads * TK : 0);
-  auto load_scales = [&](int kb) {
+  auto load_scales = [&](int kb, int turn) {
     if constexpr (kTok) {
 #pragma unroll
       for (int i = 0; i < kScLoads; ++i) {
         const int at = lane + 64 * i, key = at % TK, which = at / TK;  // K head 0, V head 0, K head 1, V head 1
-        const int t = kb + kg * TK + key;
+        int sl;
+        if constexpr (kShared)
+          sl = slots[turn * (NK / 16) + (kg * TK + key) / 16];
+        else
+          sl = key < 16 ? (left[0] > 0 ? slot[0] : -1) : (left[kSubs - 1] > 0 ? slot[kSubs - 1] : -1);
         sc_raw[i] = 0.0f;
-        const int64_t phys = t < k1 ? a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
-        if (phys >= 0)
-          sc_raw[i] = ((which & 1) ? a.v_scale : a.k_scale)[((phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1))) *
-                                                               a.scale_heads + w.kvh * kHeads + (which >> 1)];
+        if (sl >= 0 && kb + kg * TK + key < k1)
+          sc_raw[i] = ((which & 1) ? a.v_scale : a.k_scale)[(int64_t)(sl + (key & 15)) * a.scale_heads + w.kvh * kHeads + (which >> 1)];
       }
     }
   };
   const bool any = kb0 < k1;
+  int32_t e_ahead = 0;
   if (any) {
-    look_up(kb0);
-    load_scales(kb0);
+    e_ahead = entry_load(kb0);
+    const int32_t e_next = entry_load(kb0 + NK);
+    entry_use(kb0, e_ahead);
+    e_ahead = e_next;
     if constexpr (kShared) {
-      if (lane == 0) pres[sub0 / 16] = left[0] > 0;
+      if (lane == 0) slots[sub0 / 16] = left[0] > 0 ? slot[0] : -1;
+      if constexpr (kTok) __syncthreads();
     }
+    load_scales(kb0, 0);
     dma(a.k, lds_k);
     dma(a.v, lds_v);
   }
@@ -385,45 +417,52 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       const bool mine = row_ok && (!PAIR || (s >> 2) == (int)hi);
       const int st = PAIR ? s & 3 : s;
       const int d = kEb == 2 ? 16 * st + 8 * h : 16 * (2 * (st >> 1) + h) + 8 * (st & 1);
-      raw[s] = u32x4{0, 0, 0, 0};
-      if (mine) raw[s] = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);
+      raw[s] = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);  // (within q for any row)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[s][j] = mine ? raw[s][j] : 0u;
     }
     // the loop keeps raw scores and wants score_mul > 0: a negative scale
     // moves its sign into q, a zero one makes q zero
-    float f = 1.0f;
+    uint32_t sign = 0u, keep = 0xffffffffu;
     if (!(score_mul > 0.0f) && score_mul == score_mul) {
-      f = score_mul < 0.0f ? -1.0f : 0.0f;
+      sign = score_mul < 0.0f ? 0x80008000u : 0u;
+      keep = score_mul < 0.0f ? keep : 0u;
       score_mul = score_mul < 0.0f ? -score_mul : 1.0f;
-    }
-    auto element = [&](int s, int j) {
-      const uint32_t x = raw[s][j >> 1];
-      if (a.q_dtype == MKV_DTYPE_BF16) return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
-      return f16_bits_to_f32(j & 1 ? x >> 16 : x & 0xffffu);
-    };
-    if constexpr (CT == MKV_DTYPE_F16) {
-      // a row's q times a power of two: a bf16 q in fp16 is exact but for
-      // elements below 2^-24 of the row's largest
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(element(s, j)));
-      top = fmaxf(top, other_half(top));
-      if (top > 0.0f && top < __builtin_huge_valf()) {
-        const int e = ilogbf(top);
-        f *= ldexpf(1.0f, 8 - e);
-        score_mul *= ldexpf(1.0f, e - 8);
-      }
     }
 #pragma unroll
     for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (CT == MKV_DTYPE_BF16)
-          qop[s][j] = (__bf16)(element(s, j) * f);
-        else
-          qop[s][j] = (_Float16)(element(s, j) * f);
+      for (int j = 0; j < 4; ++j) raw[s][j] = (raw[s][j] ^ sign) & keep;
+    if (kEb == 2 || a.q_dtype == MKV_DTYPE_F16) {  // q's type is the operands'
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(Op16<CT>, raw[s]);
+    } else {
+      // a bf16 q's row times a power of two: exact in fp16 but for elements
+      // below 2^-24 of the row's largest
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          top = max3(top, __uint_as_float(raw[s][j] << 16 & 0x7fffffffu), __uint_as_float(raw[s][j] & 0x7fff0000u));
+      top = fmaxf(top, other_half(top));
+      float f = 1.0f;
+      if (top > 0.0f && top < __builtin_huge_valf()) {
+        const int e = ilogbf(top);
+        f = ldexpf(1.0f, 8 - e);
+        score_mul *= ldexpf(1.0f, e - 8);
       }
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f16x2 x = {(_Float16)(__uint_as_float(raw[s][j] << 16) * f),
+                           (_Float16)(__uint_as_float(raw[s][j] & 0xffff0000u) * f)};
+          raw[s][j] = __builtin_bit_cast(uint32_t, x);
+        }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(Op16<CT>, raw[s]);
+    }
   }
   if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) score_mul *= load_uniform_f32(a.k_scale);
 
@@ -439,23 +478,41 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   const int vg = (lane >> 4) & 1;
   const int vi = kEb == 2 ? (lane & 15) >> 2 : (lane & 15) >> 1;
   const int v_key = kEb == 2 ? 4 * h + vi : (vi & 3) + 4 * h + 2 * (vi & 4);
-  const int v_sub = kEb == 2 ? 8 * (lane & 1) : 8 * (lane & 1);
   const int v_chunk = kEb == 2 ? 2 * vg + ((lane & 3) >> 1) : vg;
-  auto v_operand = [&](int nb, int half, int b) {
-    typedef short i16x8 __attribute__((ext_vector_type(8)));
+  // A swizzled chunk's offset is linear in the chunk under xor: chunk 2 st + h of
+  // K is base ^ st << 5, V's 32-dim block b is base ^ b << 6 (1-byte: << 5), and 8
+  // keys on (16-bit) flips one more bit; 16 and 32 keys on do not reach the swizzle.
+  const int k_base = T::offset(kg * TK + c, h);
+  const int v_base = T::offset(kg * TK + v_key, v_chunk) + 8 * (lane & 1);
+  struct VRaw {
+    uint32_t w[kEb == 2 ? 4 : 2];
+  };
+  auto v_read = [&](int nb, int half, int b) {
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-    const int key = kg * TK + 32 * nb + 16 * half + v_key;
+    char* const at = lds_v + (32 * nb + 16 * half) * T::kRow;
+    VRaw r;
     if constexpr (kEb == 2) {
-      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + T::offset(key, 4 * b + v_chunk) + v_sub));
-      const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_v + T::offset(key + 8, 4 * b + v_chunk) + v_sub));
-      const i16x8 vt = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-      return __builtin_bit_cast(Op16<CT>, vt);
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + (v_base ^ b << 6))));
+      const u32x2 up = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + (v_base ^ b << 6 ^ 32) + 8 * T::kRow)));
+      r.w[0] = lo[0];
+      r.w[1] = lo[1];
+      r.w[2] = up[0];
+      r.w[3] = up[1];
     } else {
-      const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(lds_v + T::offset(key, 2 * b + v_chunk) + v_sub));
-      return codes_to_f16<KV_DT>((uint32_t)x[0], (uint32_t)x[1]);
+      const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(at + (v_base ^ b << 5)));
+      r.w[0] = (uint32_t)x[0];
+      r.w[1] = (uint32_t)x[1];
     }
+    return r;
+  };
+  auto v_operand = [&](const VRaw& r) {
+    if constexpr (kEb == 2)
+      return __builtin_bit_cast(Op16<CT>, u32x4{r.w[0], r.w[1], r.w[2], r.w[3]});
+    else
+      return codes_to_f16<KV_DT>(r.w[0], r.w[1]);
   };
 
   for (int kb = kb0, turn = 0; kb < k1; kb += NK, turn ^= 1) {
@@ -465,7 +522,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     uint32_t present = 0;
     if constexpr (kShared) {
 #pragma unroll
-      for (int u = 0; u < TK / 16; ++u) present |= uniform(pres[turn * (NK / 16) + key0 / 16 + u]) ? 1u << u : 0u;
+      for (int u = 0; u < TK / 16; ++u) present |= uniform(slots[turn * (NK / 16) + key0 / 16 + u]) >= 0 ? 1u << u : 0u;
     } else {
 #pragma unroll
       for (int u = 0; u < kSubs; ++u) present |= left[u] > 0 ? 1u << u : 0u;
@@ -506,37 +563,47 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       }
     }
 
-    // ---- S^T = K Q^T ----
+    // ---- S^T = K Q^T, the operands of four steps read ahead of the four
+    // before (left to itself the compiler reads one and waits for it) ----
     f32x16 s[NB];
     __builtin_amdgcn_s_setprio(1);
+    {
+      constexpr int kReads = kEb == 2 ? 4 : 2;  // 16-byte reads of four steps
+      u32x4 kw[2][kReads];
+      auto read = [&](int i) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = f32x16{};
-      const int key = key0 + 32 * nb + c;
-      if constexpr (kEb == 2) {
-#pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          const u32x4 kw = *reinterpret_cast<const u32x4*>(lds_k + T::offset(key, 2 * st + h));
-          s[nb] = mfma32<CT>(__builtin_bit_cast(Op16<CT>, kw), qop[st], s[nb]);
+        for (int j = 0; j < kReads; ++j) {
+          const int st = (i & 1) * kReads + j;
+          kw[i & 1][j] = *reinterpret_cast<const u32x4*>(lds_k + (k_base ^ st << 5) + 32 * (i >> 1) * T::kRow);
         }
-      } else {
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      read(0);
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const u32x4 kw = *reinterpret_cast<const u32x4*>(lds_k + T::offset(key, 2 * st + h));
-          s[nb] = mfma32<CT>(codes_to_f16<KV_DT>(kw[0], kw[1]), qop[2 * st], s[nb]);
-          s[nb] = mfma32<CT>(codes_to_f16<KV_DT>(kw[2], kw[3]), qop[2 * st + 1], s[nb]);
+      for (int i = 0; i < 2 * NB; ++i) {
+        if (i + 1 < 2 * NB) read(i + 1);
+        if (!(i & 1)) s[i >> 1] = f32x16{};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int st = 4 * (i & 1) + j;
+          if constexpr (kEb == 2)
+            s[i >> 1] = mfma32<CT>(__builtin_bit_cast(Op16<CT>, kw[i & 1][j]), qop[st], s[i >> 1]);
+          else
+            s[i >> 1] = mfma32<CT>(codes_to_f16<KV_DT>(kw[i & 1][j >> 1][2 * (j & 1)], kw[i & 1][j >> 1][2 * (j & 1) + 1]), qop[st], s[i >> 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
     // ---- the next tile's K, where this one's was ----
-    look_up(kb + NK);
-    load_scales(kb + NK);
+    entry_use(kb + NK, e_ahead);
     if constexpr (kShared) {
-      if (lane == 0) pres[(turn ^ 1) * (NK / 16) + sub0 / 16] = left[0] > 0;
+      if (lane == 0) slots[(turn ^ 1) * (NK / 16) + sub0 / 16] = left[0] > 0 ? slot[0] : -1;
+      meet();
+    } else {
+      wait_lds();
     }
-    if constexpr (kShared) meet();
-    else wait_lds();
+    load_scales(kb + NK, turn ^ 1);
     dma(a.k, lds_k);
 
     // ---- softmax ----
@@ -612,13 +679,14 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
         }
       }
       if (kShared ? __syncthreads_or(found) : __builtin_amdgcn_ballot_w64(found) != 0) {
+#pragma unroll
         for (int b = 0; b < 4; ++b) {
           f32x16 marks = f32x16{};
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              Op16<CT> vt = v_operand(nb, half, b), sees;
+              Op16<CT> vt = v_operand(v_read(nb, half, b)), sees;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const float one = !masked || ((seen[nb] >> (8 * half + j)) & 1) ? 1.0f : 0.0f;
@@ -633,10 +701,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
               marks = mfma32<CT>(vt, sees, marks);
             }
 #pragma unroll
-          for (int bb = 0; bb < 4; ++bb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (bb == b && marks[e] > 0.0f) acc[bb][e] += marked_value(marks[e]);
+          for (int e = 0; e < 16; ++e) acc[b][e] += marked_value(marks[e]);
         }
         if constexpr (kShared) meet();
         for (int i = 0; i < kScan * 4; ++i) {
@@ -659,17 +724,26 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       }
     }
     __builtin_amdgcn_s_setprio(1);
+    {
+      VRaw vr[2][4];
+      auto read = [&](int i) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+        for (int b = 0; b < 4; ++b) vr[i & 1][b] = v_read(i >> 1, i & 1, b);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      read(0);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int i = 0; i < 2 * NB; ++i) {
+        if (i + 1 < 2 * NB) read(i + 1);
+        const f32x16& p = s[i >> 1];
+        const int half = i & 1;
         Op16<CT> ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if constexpr (CT == MKV_DTYPE_BF16)
-            ph[j] = (__bf16)s[nb][8 * half + j];
+            ph[j] = (__bf16)p[8 * half + j];
           else
-            ph[j] = (_Float16)s[nb][8 * half + j];
+            ph[j] = (_Float16)p[8 * half + j];
         }
         if constexpr (CT == MKV_DTYPE_BF16) {
           // bf16 holds P to 8 bits: a second term carries the rest, so that a
@@ -681,23 +755,28 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
             const bf16x2 hp = {ph[j], ph[j + 1]};
-            pl[j] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_lo, s[nb][8 * half + j], false);
-            pl[j + 1] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_hi, s[nb][8 * half + j + 1], false);
+            pl[j] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_lo, p[8 * half + j], false);
+            pl[j + 1] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_hi, p[8 * half + j + 1], false);
           }
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const Op16<CT> vt = v_operand(nb, half, b);
+          const Op16<CT> vt = v_operand(vr[i & 1][b]);
           acc[b] = mfma32<CT>(vt, ph, acc[b]);
           if constexpr (CT == MKV_DTYPE_BF16) acc[b] = mfma32<CT>(vt, pl, acc[b]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
     __builtin_amdgcn_s_setprio(0);
     // ---- the next tile's V, where this one's was ----
     if constexpr (kShared) meet();
     else wait_lds();
+    e_ahead = entry_load(kb + 2 * NK);
     dma(a.v, lds_v);
   }
+
+  if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
 
   // ---- the key groups' results, joined pairwise into the first one's ----
   wait_vm<0>();
@@ -950,7 +1029,7 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
           marks = __builtin_amdgcn_mfma_f32_32x32x2f32(mark_of(v_at(e, b)), (seen >> e) & 1 ? 1.0f : 0.0f, marks, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (marks[e] > 0.0f) acc[b][e] += marked_value(marks[e]);
+          acc[b][e] += marked_value(marks[e]);
       }
     }
   }
@@ -1034,7 +1113,6 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   if (p.row_blocks < 1) p.row_blocks = 1;
   p.row_cap = p.row_blocks * 32 * p.row_groups;
   p.unit = p.row_groups == 1 ? 128 : 64;
-  p.min_split = 128;
   // Workgroups that run at once: two a CU of four waves, one of eight.  Where the
   // sequences leave some free, their keys are dealt out so that all fit one round
   // (a sequence's last split may be short: num_seqs shares are kept back); where
@@ -1050,6 +1128,7 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   else
     shares = num_seqs / 2;
   p.shares = (int)(shares < 1 ? 1 : shares);
+  p.min_split = num_seqs * 4 <= round ? 128 : num_seqs * 2 <= round ? 256 : 1024;
   const int64_t most = (capacity + p.min_split - 1) / p.min_split;
   p.max_splits = (int)(p.shares + 1 < most ? p.shares + 1 : most > 1 ? most : 1);
   return p;
