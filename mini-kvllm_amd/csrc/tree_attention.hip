@@ -65,12 +65,13 @@ struct TreeArgs {
   int group;         // the kernel's query heads to a KV head
   int q_dtype;
   float sm_scale;
-  int max_splits;    // 1: no partial results
+  int splits;        // whether sequences may be split (else no partial results)
   int shares;        // the batch's keys over this many make a split
   int min_split;     // keys
-  float* ws_o;       // partials: (seq, kv head, split, row cap, 128)
-  float* ws_ml;      // (seq, kv head, split, row cap, 2)
+  float* ws_o;       // partials: (unit, kv head, row cap, 128)
+  float* ws_ml;      // (unit, kv head, row cap, 2)
   int row_cap;
+  int row_blocks;
 };
 
 // Element i of an int32 or int64 array, without a branch (so that loads of several
@@ -81,31 +82,75 @@ MKV_DEV int64_t load_len(const void* p, int i, int i64) {
   return i64 ? (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo) : (int64_t)lo;
 }
 
-// The keys that a split takes, the same for every sequence: the batch's keys over
-// the plan's shares, in whole tiles, and at most max_splits for the longest.
-template <int UNIT>
-MKV_DEV int split_keys(const TreeArgs& a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t cap = (int64_t)a.idx.max_blocks << a.idx.bs_log2;
-  float sum = 0.0f;  // (a rule of thumb's accuracy, the same in every wave)
-  int longest = 0;
-  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-    const int s = s0 + lane;
+// A unit is one split of one sequence; units go sequence by sequence.  Splits are
+// of `len` keys, the same for every sequence: the batch's keys over the plan's
+// shares, in whole tiles.  Every workgroup works this out for itself from the
+// context lengths (a lane a sequence), so that the units are numbered without
+// gaps: workgroups without work among the others would unbalance the CUs, which
+// the hardware fills in a fixed order.
+template <int TILE>
+struct Units {
+  const TreeArgs& a;
+  int len, total;
+  int before, n;  // this lane's sequence (of the 64 last looked at): its units, and those ahead of them
+
+  MKV_DEV int keys(int s0) const {
+    const int s = s0 + (threadIdx.x & 63);
     const int64_t c = load_len(a.ctx, min(s, a.num_seqs - 1), a.ctx_i64);
-    const int n = s < a.num_seqs ? (int)min(max(c, (int64_t)0), cap) : 0;
-    sum += (float)n;
-    longest = max(longest, n);
+    return s < a.num_seqs ? (int)min(max(c, (int64_t)0), (int64_t)a.idx.max_blocks << a.idx.bs_log2) : 0;
   }
+  // the units of sequences s0 .. s0 + 63, `base` ahead of them; their number
+  MKV_DEV int number(int s0, int k, int base) {
+    const int lane = threadIdx.x & 63;
+    n = s0 + lane < a.num_seqs ? max((k + len - 1) / len, 1) : 0;
+    int upto = n;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    sum += __shfl_xor(sum, o);
-    longest = max(longest, __shfl_xor(longest, o));
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o);
+      upto += lane >= o ? y : 0;
+    }
+    before = base + upto - n;
+    return uniform(__shfl(upto, 63));
   }
-  int len = (int)fminf(sum / (float)a.shares, 1.0e9f) + 1;
-  len = max(max(len, a.min_split), (longest + a.max_splits - 1) / a.max_splits);
-  len = (len + UNIT - 1) / UNIT * UNIT;
-  return uniform(len);
-}
+  MKV_DEV explicit Units(const TreeArgs& args) : a(args) {
+    const int k0 = keys(0);
+    float sum = (float)k0;  // (a rule of thumb's accuracy, the same in every wave)
+    for (int s0 = 64; s0 < a.num_seqs; s0 += 64) sum += (float)keys(s0);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    // (a little more than the even share: at most `shares` units beside the last
+    // one of each sequence, whatever the sum's rounding)
+    len = (int)fminf(sum * 1.0001f / (float)a.shares, 1.0e9f) + 1;
+    len = uniform((max(len, a.min_split) + TILE - 1) / TILE * TILE);
+    total = number(0, k0, 0);
+    for (int s0 = 64; s0 < a.num_seqs; s0 += 64) total += number(s0, keys(s0), total);
+  }
+  // the sequence of a unit, and its number within the sequence
+  MKV_DEV void of_unit(int unit, int& seq, int& z) {
+    seq = -1;
+    z = 0;
+    int base = 0;
+    for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+      if (a.num_seqs > 64) base += number(s0, keys(s0), base);
+      const uint64_t mine = __builtin_amdgcn_ballot_w64(unit >= before && unit < before + n);
+      if (mine) {
+        const int l = __builtin_ctzll(mine);
+        seq = s0 + l;
+        z = unit - uniform(__shfl(before, l));
+        return;
+      }
+    }
+  }
+  // a sequence's first unit, and their number
+  MKV_DEV void of_sequence(int seq, int& first, int& count) {
+    if (a.num_seqs > 64) {
+      int base = 0;
+      for (int s0 = 0; s0 <= seq; s0 += 64) base += number(s0, keys(s0), base);
+    }
+    first = uniform(__shfl(before, seq & 63));
+    count = uniform(__shfl(n, seq & 63));
+  }
+};
 
 template <int CT>
 using Op16 = typename std::conditional<CT == MKV_DTYPE_BF16, bf16x8, f16x8>::type;
@@ -208,10 +253,10 @@ struct Work {
   int ctx;          // keys, within the block table
 };
 
-MKV_DEV Work find_work(const TreeArgs& a, int item) {
+MKV_DEV Work find_work(const TreeArgs& a, int seq, int kvh) {
   Work w;
-  w.kvh = item % a.num_kv_heads;
-  w.seq = item / a.num_kv_heads;
+  w.kvh = kvh;
+  w.seq = seq;
   const int64_t q0 = min(max((int64_t)a.cu[w.seq], (int64_t)0), a.total_q);
   const int64_t q1 = min(max((int64_t)a.cu[w.seq + 1], q0), a.total_q);
   const int64_t c = max(load_len(a.ctx, w.seq, a.ctx_i64), (int64_t)0);
@@ -220,6 +265,34 @@ MKV_DEV Work find_work(const TreeArgs& a, int item) {
   w.prefix = max(c - (q1 - q0), (int64_t)0);
   w.ctx = (int)min(c, (int64_t)a.idx.max_blocks << a.idx.bs_log2);
   return w;
+}
+
+// A workgroup's place: row block, unit and KV head by its number (false: none).
+struct Place {
+  int rb, unit, kvh, seq, z, len;
+};
+template <int TILE>
+MKV_DEV bool find_place(const TreeArgs& a, Place& p) {
+  auto split = [&](int units) {
+    const int pairs = units * a.num_kv_heads;
+    p.rb = (int)blockIdx.x / pairs;
+    const int q = (int)blockIdx.x - p.rb * pairs;
+    p.unit = q / a.num_kv_heads;
+    p.kvh = q - p.unit * a.num_kv_heads;
+    return p.rb < a.row_blocks;
+  };
+  if (!a.splits) {
+    p.len = 0x7fffffff / TILE * TILE;
+    p.z = 0;
+    const bool ok = split(a.num_seqs);
+    p.seq = p.unit;
+    return ok;
+  }
+  Units<TILE> u(a);
+  p.len = u.len;
+  if (!split(u.total)) return false;
+  u.of_unit(p.unit, p.seq, p.z);
+  return p.seq >= 0;
 }
 
 // Element offset of row r (token r / group, head r % group) of the KV head in q
@@ -309,14 +382,16 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int rg = wave % R, kg = wave / R;
   const int c = lane & 31, h = lane >> 5;
-  const Work w = find_work(a, blockIdx.x);
-  const int len = a.max_splits > 1 ? split_keys<NK>(a) : 0x7fffffff / NK * NK;
-  const int64_t k0 = (int64_t)blockIdx.z * len;
-  if ((blockIdx.z > 0 && k0 >= w.ctx) || (int)blockIdx.y * 32 * R >= w.rows) {
-    if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
+  Place place;
+  if (!find_place<NK>(a, place)) return;
+  const int len = place.len;
+  const Work w = find_work(a, place.seq, place.kvh);
+  const bool zeroes = place.rb == 0 && place.z == 0 && w.kvh == 0;
+  if (place.rb * 32 * R >= w.rows) {
+    if (zeroes) zero_rows_past(a, w);
     return;
   }
-  const int kb0 = (int)k0, k1 = (int)min(k0 + len, (int64_t)w.ctx);
+  const int kb0 = place.z * len, k1 = (int)min((int64_t)kb0 + len, (int64_t)w.ctx);
   const int prefix = (int)min(w.prefix, (int64_t)0x7fffffff);
   const bool split = w.ctx > len;
 
@@ -404,7 +479,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
 
   // ---- q: this lane's row; step s of the contraction takes dims 16 s + 8 h .. + 7
   // (16-bit: chunk 2 s + h), or the lower or upper half of chunk 2 (s / 2) + h ----
-  const int row = blockIdx.y * 32 * R + rg * 32 + c;
+  const int row = place.rb * 32 * R + rg * 32 + c;
   const bool row_ok = row < w.rows;
   bool hi = false;
   const int64_t q_off = row_offset<PAIR>(a, w, row_ok ? row : 0, hi);
@@ -760,11 +835,10 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
           }
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const Op16<CT> vt = v_operand(vr[i & 1][b]);
-          acc[b] = mfma32<CT>(vt, ph, acc[b]);
-          if constexpr (CT == MKV_DTYPE_BF16) acc[b] = mfma32<CT>(vt, pl, acc[b]);
-        }
+        for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(vr[i & 1][b]), ph, acc[b]);
+        if constexpr (CT == MKV_DTYPE_BF16)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(vr[i & 1][b]), pl, acc[b]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -776,7 +850,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     dma(a.v, lds_v);
   }
 
-  if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
+  if (zeroes) zero_rows_past(a, w);
 
   // ---- the key groups' results, joined pairwise into the first one's ----
   wait_vm<0>();
@@ -814,7 +888,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   const float l = l_run + other_half(l_run);
   if (!row_ok) return;
   if (split) {
-    const int64_t at = ((int64_t)blockIdx.x * a.max_splits + blockIdx.z) * a.row_cap + row;
+    const int64_t at = ((int64_t)place.unit * a.num_kv_heads + w.kvh) * a.row_cap + row;
     float* o = a.ws_o + at * kHeadDim;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -850,18 +924,18 @@ __global__ __launch_bounds__(64 * R * KG) __attribute__((amdgpu_waves_per_eu(2))
 constexpr int kJoinWaves = 4;
 template <int UNIT, bool FP8, bool PAIR>
 __global__ __launch_bounds__(64 * kJoinWaves) void tree_join_kernel(TreeArgs a) {
-  const Work w = find_work(a, blockIdx.x);
-  const int len = split_keys<UNIT>(a);
-  const int n = (w.ctx + len - 1) / len;
+  const Work w = find_work(a, blockIdx.x / a.num_kv_heads, blockIdx.x % a.num_kv_heads);
+  int first, n;
+  Units<UNIT>(a).of_sequence(w.seq, first, n);
   if (n <= 1) return;
   const int lane = threadIdx.x & 63;
   const int row = blockIdx.y * kJoinWaves + uniform(threadIdx.x >> 6);
   if (row >= w.rows) return;
-  const int64_t at = (int64_t)blockIdx.x * a.max_splits * a.row_cap + row;
+  const int64_t at = ((int64_t)first * a.num_kv_heads + w.kvh) * a.row_cap + row, step = (int64_t)a.num_kv_heads * a.row_cap;
   // the largest maximum first (a lane a split), then the sums, eight splits'
   // loads in flight
   float m = kNegBig;
-  for (int z = lane; z < n; z += 64) m = fmaxf(m, a.ws_ml[2 * (at + (int64_t)z * a.row_cap)]);
+  for (int z = lane; z < n; z += 64) m = fmaxf(m, a.ws_ml[2 * (at + z * step)]);
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   float l = 0.0f, x = 0.0f, y = 0.0f;
@@ -869,7 +943,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void tree_join_kernel(TreeArgs a) 
     f32x2 ml[8], o[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int64_t i = at + (int64_t)min(z0 + j, n - 1) * a.row_cap;
+      const int64_t i = at + min(z0 + j, n - 1) * step;
       ml[j] = *reinterpret_cast<const f32x2*>(a.ws_ml + 2 * i);
       o[j] = *reinterpret_cast<const f32x2*>(a.ws_o + i * kHeadDim + 2 * lane);
     }
@@ -912,14 +986,15 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   __shared__ __align__(16) char lds[NK * kRow];
   const int tid = threadIdx.x, lane = tid & 63, kg = uniform(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const Work w = find_work(a, blockIdx.x);
-  const int len = a.max_splits > 1 ? split_keys<NK>(a) : 0x7fffffff / NK * NK;
-  const int64_t k0 = (int64_t)blockIdx.z * len;
-  if (blockIdx.y == 0 && blockIdx.z == 0 && w.kvh == 0) zero_rows_past(a, w);
-  if ((blockIdx.z > 0 && k0 >= w.ctx) || (int)blockIdx.y * 32 >= w.rows) return;
-  const int kb0 = (int)k0, k1 = (int)min(k0 + len, (int64_t)w.ctx);
+  Place place;
+  if (!find_place<NK>(a, place)) return;
+  const int len = place.len;
+  const Work w = find_work(a, place.seq, place.kvh);
+  if (place.rb == 0 && place.z == 0 && w.kvh == 0) zero_rows_past(a, w);
+  if (place.rb * 32 >= w.rows) return;
+  const int kb0 = place.z * len, k1 = (int)min((int64_t)kb0 + len, (int64_t)w.ctx);
   const bool split = w.ctx > len;
-  const int row = blockIdx.y * 32 + c;
+  const int row = place.rb * 32 + c;
   const bool row_ok = row < w.rows;
   bool hi = false;
   const int64_t q_off = row_offset<PAIR>(a, w, row_ok ? row : 0, hi);
@@ -1062,7 +1137,7 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   const float l = l_run + other_half(l_run);
   if (!row_ok) return;
   float norm = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-  const int64_t at = ((int64_t)blockIdx.x * a.max_splits + blockIdx.z) * a.row_cap + row;
+  const int64_t at = ((int64_t)place.unit * a.num_kv_heads + w.kvh) * a.row_cap + row;
   if (split && h == 0) {
     a.ws_ml[2 * at] = m_run;
     a.ws_ml[2 * at + 1] = l;
@@ -1100,7 +1175,8 @@ struct Plan {
   int unit;        // keys of a tile
   int shares;
   int min_split;
-  int max_splits;
+  bool splits;
+  int64_t units;   // at most
 };
 
 Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_group, int mask_cols, int64_t capacity,
@@ -1130,17 +1206,18 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   p.shares = (int)(shares < 1 ? 1 : shares);
   p.min_split = num_seqs * 4 <= round ? 128 : num_seqs * 2 <= round ? 256 : 1024;
   const int64_t most = (capacity + p.min_split - 1) / p.min_split;
-  p.max_splits = (int)(p.shares + 1 < most ? p.shares + 1 : most > 1 ? most : 1);
+  p.splits = most > 1;
+  p.units = !p.splits ? num_seqs : num_seqs + shares < num_seqs * most ? num_seqs + shares : num_seqs * most;
   return p;
 }
 
-size_t workspace_of(const Plan& p, int64_t items) {
-  return p.max_splits > 1 ? (size_t)items * p.max_splits * p.row_cap * (kHeadDim + 2) * sizeof(float) : 0;
+size_t workspace_of(const Plan& p, int kernel_kv_heads) {
+  return p.splits ? (size_t)p.units * kernel_kv_heads * p.row_cap * (kHeadDim + 2) * sizeof(float) : 0;
 }
 
 template <int KV_DT, bool PAIR>
 int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)p.row_blocks, (unsigned)p.max_splits);
+  const dim3 grid((unsigned)(p.units * a.num_kv_heads * p.row_blocks));
   if constexpr (KV_DT == MKV_DTYPE_F32) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_f32_kernel<PAIR>), grid, dim3(256), 0, s, a);
   } else {
@@ -1152,9 +1229,9 @@ int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
     }
   }
   if (hipError_t e = hipGetLastError()) return (int)e;
-  if (p.max_splits > 1) {
+  if (p.splits) {
     constexpr bool kFp8 = KV_DT == MKV_DTYPE_FP8E4M3;
-    const dim3 jgrid(grid.x, (unsigned)((p.row_cap + kJoinWaves - 1) / kJoinWaves));
+    const dim3 jgrid((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)((p.row_cap + kJoinWaves - 1) / kJoinWaves));
     if (p.unit == 128)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<128, kFp8, PAIR>), jgrid, dim3(64 * kJoinWaves), 0, s, a);
     else
@@ -1179,10 +1256,10 @@ int check_tree(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, i
 }
 
 Plan plan_of(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim, int block_size,
-             int max_blocks, int mask_cols, int kv_dtype, int64_t& items) {
+             int max_blocks, int mask_cols, int kv_dtype, int& kernel_kv_heads) {
   const int pair = head_dim == 64 ? 2 : 1;
   const int kv = num_kv_heads / pair, g = num_heads / num_kv_heads * pair;
-  items = (int64_t)num_seqs * kv;
+  kernel_kv_heads = kv;
   return make_plan(num_seqs, total_q, kv, g, mask_cols, (int64_t)max_blocks * block_size, kv_dtype == MKV_DTYPE_F32);
 }
 
@@ -1195,9 +1272,9 @@ extern "C" size_t mkv_paged_tree_workspace_size(int num_seqs, int64_t total_q, i
                                                 int head_dim, int block_size, int max_blocks, int mask_cols,
                                                 int kv_dtype) {
   if (check_tree(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols)) return 0;
-  int64_t items;
-  const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, items);
-  return workspace_of(p, items);
+  int kv;
+  const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, kv);
+  return workspace_of(p, kv);
 }
 
 extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void* k_cache, const void* v_cache,
@@ -1224,10 +1301,10 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
   if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
        reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace)) & 15u)
     return MKV_ERR_MISALIGNED;
-  int64_t items;
-  const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, items);
-  if (p.row_blocks > 65535 || p.max_splits > 65535) return MKV_ERR_BAD_SHAPE;
-  if (workspace_of(p, items) > workspace_bytes || (p.max_splits > 1 && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
+  int kv;
+  const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, kv);
+  if (p.units * kv * p.row_blocks > 0x7fffffff || p.row_cap / kJoinWaves > 65535) return MKV_ERR_BAD_SHAPE;
+  if (workspace_of(p, kv) > workspace_bytes || (p.splits && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
   const int pair = head_dim == 64 ? 2 : 1;
   TreeArgs a;
   a.out = out;
@@ -1252,12 +1329,13 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
   a.group = num_heads / num_kv_heads * pair;
   a.q_dtype = q_dtype;
   a.sm_scale = sm_scale;
-  a.max_splits = p.max_splits;
+  a.splits = p.splits;
   a.shares = p.shares;
   a.min_split = p.min_split;
   a.row_cap = p.row_cap;
+  a.row_blocks = p.row_blocks;
   a.ws_o = reinterpret_cast<float*>(workspace);
-  a.ws_ml = a.ws_o + (size_t)items * p.max_splits * p.row_cap * kHeadDim;
+  a.ws_ml = a.ws_o + (size_t)p.units * kv * p.row_cap * kHeadDim;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int fmt = token ? 0x100 | kv_dtype : kv_dtype;
 #define MKV_TREE(F) \
