@@ -65,53 +65,60 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(Pools p, int b
 
 // ---------------------------------------------------------------------------
 // Compaction: row prefix + accepted[b, j] of sequence b moves to prefix + j.
-// A workgroup takes one sequence, one pool and a slice of the rows' columns
-// and holds all of the sequence's rows of that slice in registers before it
-// writes any, so rows may overlap in any order.
+// A workgroup takes one sequence, a slice of the rows' columns and some of the
+// pools, and holds all of the sequence's rows of a pool's slice in registers
+// before it writes any, so rows may overlap in any order.  Several pools a
+// workgroup share the look-up of the rows, which is a chain of three memory round
+// trips (60 sequences, 56 pools: 29 us with one pool a workgroup).
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
 constexpr int kMoveItems = 8;                             // 16-byte items a thread holds
 constexpr int kMaxMoves = kMoveThreads * kMoveItems;      // accepted offsets a sequence
-constexpr int kMoveLdsRows = kMaxMoves;
+
+// Columns of a slice (a power of two) for rows of `units` items, n rows.
+__host__ MKV_DEV int slice_log2(int units, int n) {
+  int l = 0;
+  while ((1 << l) < units && (n << (l + 1)) <= kMaxMoves) ++l;
+  return l;
+}
 
 template <typename T>
-MKV_DEV void move_rows(char* base, const int64_t* src, const int64_t* dst, int n, int64_t row_bytes, int col0, int cols) {
+MKV_DEV void move_rows(char* base, const int64_t* src, const int64_t* dst, int n, int64_t row_bytes, int col0, int l2,
+                       int units) {
+  const int col = col0 + ((int)threadIdx.x & ((1 << l2) - 1));
+  const bool mine = col < units;
   T v[kMoveItems];
+  char* to[kMoveItems];
 #pragma unroll
   for (int j = 0; j < kMoveItems; ++j) {
-    const int it = j * kMoveThreads + (int)threadIdx.x;
-    const int e = it / cols;
-    if (e < n && src[e] >= 0)
-      v[j] = *reinterpret_cast<const T*>(base + src[e] * row_bytes + (int64_t)(col0 + it % cols) * sizeof(T));
+    const int e = (j * kMoveThreads + (int)threadIdx.x) >> l2;
+    to[j] = nullptr;
+    if (e < n && mine) {
+      const int64_t s = src[e];
+      if (s >= 0) {
+        to[j] = base + dst[e] * row_bytes + (int64_t)col * sizeof(T);
+        v[j] = *reinterpret_cast<const T*>(base + s * row_bytes + (int64_t)col * sizeof(T));
+      }
+    }
   }
   // every row of the slice has been read before any is written
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kMoveItems; ++j) {
-    const int it = j * kMoveThreads + (int)threadIdx.x;
-    const int e = it / cols;
-    if (e < n && src[e] >= 0)
-      *reinterpret_cast<T*>(base + dst[e] * row_bytes + (int64_t)(col0 + it % cols) * sizeof(T)) = v[j];
-  }
+  for (int j = 0; j < kMoveItems; ++j)
+    if (to[j]) *reinterpret_cast<T*>(to[j]) = v[j];
 }
 
-__global__ __launch_bounds__(kMoveThreads) void compact_slots_kernel(Pools p, PagedIndex idx,
-                                                                     const void* __restrict__ prefix, int prefix_i64,
-                                                                     const void* __restrict__ accepted, int acc_i64,
-                                                                     int64_t acc_stride, int n, int slices) {
+__global__ __launch_bounds__(kMoveThreads) __attribute__((amdgpu_waves_per_eu(5))) void compact_slots_kernel(
+    Pools p, int num, int per_group, PagedIndex idx, const void* __restrict__ prefix, int prefix_i64,
+    const void* __restrict__ accepted, int acc_i64, int64_t acc_stride, int n, int slices) {
   extern __shared__ int64_t slots[];  // [n] sources (-1: nothing to move), [n] destinations
-  const int t = blockIdx.x / slices, slice = blockIdx.x % slices, b = blockIdx.y;
-  const int64_t row_bytes = p.row_bytes[t];
-  const bool wide = row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
-  const int units = (int)(row_bytes / (wide ? 16 : 4));
-  const int cols = max(1, kMaxMoves / n);
-  if ((int64_t)slice * cols >= units) return;
+  const int group = blockIdx.x / slices, slice = blockIdx.x % slices, b = blockIdx.y;
   const int64_t P = load_index(prefix, b, prefix_i64);
   for (int j = threadIdx.x; j < n; j += kMoveThreads) {
     const int64_t a = load_index(accepted, b * acc_stride + j, acc_i64);
     int64_t s = -1, d = -1;
-    if (P >= 0 && a >= 0 && a != j && a < ((int64_t)1 << 40)) {
+    if (P >= 0 && P < ((int64_t)1 << 40) && a >= 0 && a != j && a < ((int64_t)1 << 40)) {
       const int64_t mask = ((int64_t)1 << idx.bs_log2) - 1;
       const int64_t ps = idx.physical_block(b, (P + a) >> idx.bs_log2), pd = idx.physical_block(b, (P + j) >> idx.bs_log2);
       if (ps >= 0 && pd >= 0) {
@@ -123,11 +130,17 @@ __global__ __launch_bounds__(kMoveThreads) void compact_slots_kernel(Pools p, Pa
     slots[n + j] = d;
   }
   __syncthreads();
-  const int col0 = slice * cols, take = min(cols, units - col0);
-  if (wide)
-    move_rows<u32x4>(p.base[t], slots, slots + n, n, row_bytes, col0, take);
-  else
-    move_rows<uint32_t>(p.base[t], slots, slots + n, n, row_bytes, col0, take);
+  for (int t = group * per_group; t < min(num, (group + 1) * per_group); ++t) {
+    const int64_t row_bytes = p.row_bytes[t];
+    const bool wide = row_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
+    const int units = (int)(row_bytes / (wide ? 16 : 4));
+    const int l2 = slice_log2(units, n);
+    if ((slice << l2) >= units) continue;
+    if (wide)
+      move_rows<u32x4>(p.base[t], slots, slots + n, n, row_bytes, slice << l2, l2, units);
+    else
+      move_rows<uint32_t>(p.base[t], slots, slots + n, n, row_bytes, slice << l2, l2, units);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -138,6 +151,7 @@ __global__ __launch_bounds__(kMoveThreads) void compact_slots_kernel(Pools p, Pa
 // ---------------------------------------------------------------------------
 constexpr int kMaxRows = 1024;
 constexpr int kAssignThreads = 1024;
+constexpr int kCells = 4;     // table entries a thread looks at at once
 constexpr int kScanPer = 16;  // reference counts a thread looks at in one sweep
 
 struct AssignArgs {
@@ -236,13 +250,23 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
   }
   __syncthreads();
   // the rows' new tables so far, and the counts of what is taken and let go
-  for (int i = tid; i < R * W; i += kAssignThreads) {
-    const int r = i / W, w = i - r * W;
-    const int page = w < s_keep[r] ? a.tables[(int64_t)s_src[r] * a.bt_stride + w] : 0;
-    a.new_tables[i] = page;
-    if (!s_drop[r]) {
-      if (w < s_keep[r]) ref_add(a, page, 1);
-      if (w < s_held[r]) ref_add(a, a.tables[(int64_t)r * a.bt_stride + w], -1);
+  // (kCells entries a thread at a time, their loads in one round trip)
+  for (int i0 = tid; i0 < R * W; i0 += kAssignThreads * kCells) {
+    int take[kCells], drop[kCells];
+#pragma unroll
+    for (int j = 0; j < kCells; ++j) {
+      const int i = i0 + j * kAssignThreads;
+      const int r = i < R * W ? i / W : 0, w = i < R * W ? i - r * W : W;
+      const bool keep = w < s_keep[r], held = w < s_held[r];
+      take[j] = keep ? a.tables[(int64_t)s_src[r] * a.bt_stride + w] : 0;
+      drop[j] = held && !s_drop[r] ? a.tables[(int64_t)r * a.bt_stride + w] : -1;
+      if (i < R * W) a.new_tables[i] = take[j];
+      if (!keep || s_drop[r]) take[j] = -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kCells; ++j) {
+      ref_add(a, take[j], 1);
+      ref_add(a, drop[j], -1);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -315,20 +339,37 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
     a.seq_lens[tid] = drop ? 0 : new_len;
   }
   __syncthreads();
-  for (int i = tid; i < R * W; i += kAssignThreads) {
-    const int r = i / W, w = i - r * W;
-    int page = a.new_tables[i];
-    const int keep = s_keep[r];
-    if (s_drop[r]) {
-      if (w < keep) ref_add(a, page, -1);
-      page = 0;
-    } else if (w < keep) {
-      if (s_copy[r] && w == s_at[r]) page = s_last[r];
-    } else if (w < keep + s_grow[r]) {
-      page = a.spare[s_start[r] + w - keep];
-      ref_add(a, page, 1);
+  for (int i0 = tid; i0 < R * W; i0 += kAssignThreads * kCells) {
+    int page[kCells], add[kCells], sub[kCells];
+#pragma unroll
+    for (int j = 0; j < kCells; ++j) {
+      const int i = i0 + j * kAssignThreads;
+      add[j] = sub[j] = -1;
+      page[j] = 0;
+      if (i < R * W) {
+        const int r = i / W, w = i - r * W, keep = s_keep[r];
+        if (w < keep)
+          page[j] = a.new_tables[i];
+        else if (!s_drop[r] && w < keep + s_grow[r])
+          page[j] = add[j] = a.spare[s_start[r] + w - keep];
+        if (s_drop[r]) {
+          if (w < keep) sub[j] = page[j];
+          page[j] = 0;
+        } else if (s_copy[r] && w == s_at[r]) {
+          page[j] = s_last[r];
+        }
+      }
     }
-    a.tables[(int64_t)r * a.bt_stride + w] = page;
+#pragma unroll
+    for (int j = 0; j < kCells; ++j) {
+      const int i = i0 + j * kAssignThreads;
+      ref_add(a, add[j], 1);
+      ref_add(a, sub[j], -1);
+      if (i < R * W) {
+        const int r = i / W;
+        a.tables[(int64_t)r * a.bt_stride + i - r * W] = page[j];
+      }
+    }
   }
 }
 
@@ -421,19 +462,22 @@ extern "C" int mkv_compact_slots(const void* const* tensors, const int64_t* row_
     Pools p;
     int64_t widest;
     const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
-    int64_t units = 0;  // (a narrow row of a 4-byte unit can have more units than a wide one)
+    int64_t slices = 1;
     for (int t = 0; t < n; ++t) {
       const bool wide = p.row_bytes[t] % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
-      const int64_t u = p.row_bytes[t] / (wide ? 16 : 4);
-      units = u > units ? u : units;
+      const int u = (int)(p.row_bytes[t] / (wide ? 16 : 4)), l2 = slice_log2(u, num_accepted);
+      const int64_t c = ((int64_t)u + (1 << l2) - 1) >> l2;
+      slices = c > slices ? c : slices;
     }
-    const int cols = kMaxMoves / num_accepted > 1 ? kMaxMoves / num_accepted : 1;
-    const int64_t slices = (units + cols - 1) / cols;
-    if (slices * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
-    hipLaunchKernelGGL(compact_slots_kernel, dim3((unsigned)(slices * n), (unsigned)batch), dim3(kMoveThreads),
-                       (size_t)num_accepted * 16, reinterpret_cast<hipStream_t>(stream), p, idx, prefix_lens,
-                       (int)(prefix_dtype == MKV_INDEX_I64), accepted, (int)(accepted_dtype == MKV_INDEX_I64),
-                       accepted_stride, num_accepted, (int)slices);
+    // pools a workgroup: one while that leaves CUs free, at most eight
+    int64_t per = (int64_t)n * slices * batch / 1024;
+    per = per < 1 ? 1 : per > 8 ? 8 : per;
+    const int64_t groups = (n + per - 1) / per;
+    if (slices * groups > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL(compact_slots_kernel, dim3((unsigned)(slices * groups), (unsigned)batch), dim3(kMoveThreads),
+                       (size_t)num_accepted * 16, reinterpret_cast<hipStream_t>(stream), p, n, (int)per, idx,
+                       prefix_lens, (int)(prefix_dtype == MKV_INDEX_I64), accepted,
+                       (int)(accepted_dtype == MKV_INDEX_I64), accepted_stride, num_accepted, (int)slices);
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
   return MKV_OK;

@@ -8,11 +8,14 @@
 // traffic.  Pass 1 gives a workgroup kChunk logits of one row (32 a thread, in
 // registers), so that a single row still spreads over many CUs, and leaves per
 // chunk (m, s, t), joined by the usual rescaling, and the maximum of each
-// thread's 32 logits.  Pass 2, one workgroup a row, joins the chunks and finds
-// the top k from those maxima: a value that at least k threads' maxima reach
-// bounds the k-th largest logit from below, so only the threads' logits that
-// reach it are read again (a few dozen of the vocabulary).  Selecting in pass 1
-// would cost its workgroups as many VALU cycles again as the whole softmax.
+// thread's 32 logits as a key in unsigned order (16 bits for 16-bit logits).
+// Pass 2, one workgroup a row, joins the chunks and finds the top k from those
+// maxima, held in registers: a value that at least k threads' maxima reach bounds
+// the k-th largest logit from below, so only the threads' logits that reach it
+// are read again (a few dozen of the vocabulary).  Selecting in pass 1 would cost
+// its workgroups as many VALU cycles again as the whole softmax.
+#include <type_traits>
+
 #include "mkv_device.hpp"
 
 namespace mkv {
@@ -40,19 +43,45 @@ struct LpArgs {
   float* top_logprobs; // (rows, top)
   int64_t* top_ids;    // (rows, top)
   float* stats;        // workspace: (rows, chunks, 4): m, s, t, unused
-  float* maxima;       // workspace: (rows, chunks, 256)
+  void* maxima;        // workspace: (rows, chunks, 256) keys, each row 16-byte aligned
 };
 
 // max that a NaN on either side wins (v_maximum3_f32)
 MKV_DEV float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// unsigned order of logits: NaN above +inf, the two zeros alike; 0 for none
+// Unsigned order of logits: NaN above +inf, the two zeros alike; 0 for none.  A
+// 16-bit logit's order is the upper half of it (fp16's by its own bits).
 MKV_DEV uint32_t order_of(float x) {
-  if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x == 0.0f ? 0.0f : x);
-  return u >> 31 ? ~u : u | 0x80000000u;
+  const uint32_t o = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 0xffffffffu : o;
+}
+MKV_DEV float value_of(uint32_t order) {
+  return __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order);  // (~0: a NaN)
 }
 MKV_DEV uint64_t key_of(float x, int i) { return (uint64_t)order_of(x) << 32 | (uint32_t)~i; }
+
+// Sums and maxima over the wave by DPP moves and lane swaps (no LDS round trips).
+template <class F>
+MKV_DEV float wave_all(float x, F f) {
+  // (x as it is rounded: a product fused into the first sum would differ from
+  // lane to lane)
+  asm volatile("" : "+v"(x));
+  x = f(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xf, 0xf, false)));
+  x = f(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4E, 0xf, 0xf, false)));
+  x = f(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x141, 0xf, 0xf, false)));
+  x = f(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x140, 0xf, 0xf, false)));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+MKV_DEV float wave_sum(float x) {
+  return wave_all(x, [](float a, float b) { return a + b; });
+}
+MKV_DEV float wave_max(float x) {
+  return wave_all(x, [](float a, float b) { return maximum(a, b); });
+}
 
 template <int DT>
 MKV_DEV float logit_at(const char* row, int64_t i) {
@@ -67,6 +96,14 @@ MKV_DEV float logit_at(const char* row, int64_t i) {
 // are read a logit at a time.
 template <int DT>
 struct Pieces {
+  using Key = typename std::conditional<DT == MKV_DTYPE_F32, uint32_t, uint16_t>::type;
+  // a logit's key: its order, for 16-bit logits in 16 bits
+  MKV_DEV static uint32_t key(float x) {
+    if constexpr (DT == MKV_DTYPE_F32) return order_of(x);
+    if constexpr (DT == MKV_DTYPE_BF16) return order_of(x) >> 16;
+    const uint32_t u = f32_to_f16_bits(x == 0.0f ? 0.0f : x);  // (exact)
+    return x != x ? 0xffffu : (u & 0x8000u ? ~u : u | 0x8000u) & 0xffffu;
+  }
   static constexpr int kVec = DT == MKV_DTYPE_F32 ? 4 : 8;
   static constexpr int kNum = kPer / kVec;
   MKV_DEV static int shift(const char* row) {
@@ -133,10 +170,13 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_chunk_kernel(LpArgs a) {
   float own = x[0];
 #pragma unroll
   for (int i = 1; i < kPer; ++i) own = maximum(own, x[i]);
-  if (a.top) a.maxima[(r * a.chunks + chunk) * kLpThreads + tid] = own;
-  float m = own;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) m = maximum(m, __shfl_xor(m, o));
+  if (a.top) {
+    // (a thread without a logit of the row: 0)
+    const bool none = P::start(chunk, 0, tid, shift) >= a.vocab;
+    reinterpret_cast<typename P::Key*>(a.maxima)[(r * a.chunks + chunk) * kLpThreads + tid] =
+        (typename P::Key)(none ? 0u : P::key(own));
+  }
+  const float m = wave_max(own);
   // the wave's sums around its own maximum; a wave without a finite one has
   // none (all -inf), or NaN (a NaN or +inf among its logits)
   Stat w{m, 0.0f, 0.0f};
@@ -150,11 +190,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_chunk_kernel(LpArgs a) {
       w.t = __builtin_fmaf(e, d, w.t);
     }
   }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    w.s += __shfl_xor(w.s, o);
-    w.t += __shfl_xor(w.t, o);
-  }
+  w.s = wave_sum(w.s);
+  w.t = wave_sum(w.t);
   __shared__ Stat part[kLpThreads / 64];
   if ((tid & 63) == 0) part[tid >> 6] = w;
   __syncthreads();
@@ -168,51 +205,90 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_chunk_kernel(LpArgs a) {
   }
 }
 
-// number of threads' true bits, times weight: the sum of v over the workgroup
-MKV_DEV int block_count(int v, int* lds) {
+// The row's keys, 16 bytes a thread at a time: up to kHeld vectors in registers
+// (16-bit logits: vocabularies up to 262144; fp32: 131072), the rest from memory.
+template <int DT>
+struct Keys {
+  using P = Pieces<DT>;
+  static constexpr int kPerVec = 16 / sizeof(typename P::Key);
+  static constexpr int kHeld = DT == MKV_DTYPE_F32 ? 16 : 4;
+  const u32x4* src;
+  int vecs;
+  u32x4 held[kHeld];
+
+  MKV_DEV static uint32_t get(const u32x4& v, int e) {
+    if constexpr (DT == MKV_DTYPE_F32) return v[e];
+    return e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu;
+  }
+  MKV_DEV void load(const void* p, int num) {
+    src = reinterpret_cast<const u32x4*>(p);
+    vecs = num / kPerVec;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int n = 0;
+    for (int j = 0; j < kHeld; ++j) {
+      const int at = j * kLpThreads + (int)threadIdx.x;
+      held[j] = u32x4{0, 0, 0, 0};
+      if (at < vecs) held[j] = src[at];
+    }
+  }
+  // f(key, number of the share)
+  template <class F>
+  MKV_DEV void each(F f) const {
 #pragma unroll
-  for (int w = 0; w < kLpThreads / 64; ++w) n += lds[w];
-  return n;
-}
+    for (int j = 0; j < kHeld; ++j) {
+      if (j * kLpThreads >= vecs) break;
+#pragma unroll
+      for (int e = 0; e < kPerVec; ++e) f(get(held[j], e), (j * kLpThreads + (int)threadIdx.x) * kPerVec + e);
+    }
+    for (int at = kHeld * kLpThreads + (int)threadIdx.x; at - (int)threadIdx.x < vecs; at += kLpThreads) {
+      const u32x4 v = at < vecs ? src[at] : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < kPerVec; ++e) f(get(v, e), at * kPerVec + e);
+    }
+  }
+};
 
 template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   using P = Pieces<DT>;
-  __shared__ Stat parts[kLpThreads / 64];
-  __shared__ int counts[kLpThreads / 64];
+  constexpr int kWaves = kLpThreads / 64;
+  __shared__ uint32_t counts[2][kWaves];
   __shared__ uint64_t cand[kMaxCand];
   __shared__ int subs[kMaxSub];
-  __shared__ int fill;
-  const int tid = threadIdx.x;
+  __shared__ int fill[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
   const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * (16 / P::kVec);
-  // the given tokens' logits go out first
+  // the given tokens' logits and the keys go out first
   float given = 0.0f;
   int64_t id = -1;
   if (tid < a.num_ids) {
     id = load_index(a.ids, r * a.ids_stride + tid, a.ids_i64);
     if (id >= 0 && id < a.vocab) given = logit_at<DT>(row, id);
   }
-  Stat st{-__builtin_huge_valf(), 0.0f, 0.0f};
-  for (int c = tid; c < a.chunks; c += kLpThreads) {
-    const u32x4 v = ld16(a.stats + (r * a.chunks + c) * 4);
-    st = join(st, Stat{__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2])});
+  const int shares = a.chunks * kLpThreads;
+  Keys<DT> keys;
+  if (a.top) keys.load(reinterpret_cast<const typename P::Key*>(a.maxima) + r * shares, shares);
+  if (tid < 2) fill[tid] = 0;
+  // the chunks' sums, in every wave: a lane a chunk
+  float m = -__builtin_huge_valf(), s = 0.0f, t = 0.0f;
+  for (int c0 = 0; c0 < a.chunks; c0 += 64) {
+    Stat st{-__builtin_huge_valf(), 0.0f, 0.0f};
+    if (c0 + lane < a.chunks) {
+      const u32x4 v = ld16(a.stats + (r * a.chunks + c0 + lane) * 4);
+      st = Stat{__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2])};
+    }
+    const float top = maximum(m, wave_max(st.m));
+    // equal maxima need no factor (and equal infinities have no difference)
+    const float d = st.m == top ? 0.0f : st.m - top, f = expf(d);
+    const float d0 = m == top ? 0.0f : m - top, f0 = expf(d0);
+    const float tn = wave_sum(f > 0.0f ? f * (st.t + st.s * d) : 0.0f);
+    t = (f0 > 0.0f ? f0 * (t + s * d0) : 0.0f) + tn;
+    s = s * f0 + wave_sum(st.s * f);
+    m = top;
   }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) st = join(st, Stat{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.t, o)});
-  if ((tid & 63) == 0) parts[tid >> 6] = st;
-  __syncthreads();
-  st = parts[0];
-#pragma unroll
-  for (int w = 1; w < kLpThreads / 64; ++w) st = join(st, parts[w]);
-  const float m = st.m, log_s = logf(st.s);
-  if (tid == 0) a.entropy[r] = log_s - st.t / st.s;
+  if (m != m) s = t = m;
+  const float log_s = logf(s);
+  if (tid == 0) a.entropy[r] = log_s - t / s;
   for (int i = tid; i < a.num_ids; i += kLpThreads) {
     if (i >= kLpThreads) {
       id = load_index(a.ids, r * a.ids_stride + i, a.ids_i64);
@@ -222,99 +298,115 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   }
   if (a.top == 0) return;
 
-  // ---- a threshold that k to kMaxSub threads' maxima reach ----
+  // ---- a threshold that k to kMaxSub shares' maxima reach ----
   const int k = a.top;
   const int shift = P::shift(row);
-  const int subs_all = a.chunks * kLpThreads;
-  const float* maxima = a.maxima + r * subs_all;
-  // a thread of pass 1 without a logit of the row counts for nothing
-  auto sub_key = [&](int i) -> uint32_t {
-    const int64_t s = P::start(i / kLpThreads, 0, i % kLpThreads, shift);
-    return s >= a.vocab || s + P::kVec <= 0 ? 0u : order_of(maxima[i]);
+  int turn = 0;
+  // the workgroup's sum of a count that each wave has in a scalar
+  auto all = [&](uint32_t wave_count) -> int {
+    if (lane == 0) counts[turn][wave] = wave_count;
+    __syncthreads();
+    uint32_t n = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n += counts[turn][w];
+    turn ^= 1;  // (the other half is free again: everyone has passed a barrier since)
+    return (int)n;
   };
-  // (from 1, which every share with a logit reaches, to above the largest)
-  uint32_t lo = 1, hi = 0xffffffffu;
-  auto reach = [&](uint32_t t) {
-    int n = 0;
-    for (int i = tid; i < subs_all; i += kLpThreads) n += sub_key(i) >= t;
-    return block_count(n, counts);
+  auto reach = [&](uint32_t least) -> int {
+    uint32_t n = 0;
+    keys.each([&](uint32_t key, int) { n += __popcll(__builtin_amdgcn_ballot_w64(key >= least)); });
+    return all(n);
   };
+  // the largest key, and the least that is a thread's largest (so that every
+  // thread with a share reaches it)
+  uint32_t own = 0;
+  keys.each([&](uint32_t key, int) { own = max(own, key); });
+  uint32_t hi = own, lo = own ? own : 0xffffffffu;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
+  }
+  if (lane == 0) {
+    subs[wave] = (int)hi;
+    subs[kWaves + wave] = (int)lo;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    hi = max(hi, (uint32_t)subs[w]);
+    lo = min(lo, (uint32_t)subs[kWaves + w]);
+  }
   int n_sub = reach(lo);
-  bool ties = false;
+  if (n_sub < k) {  // (few threads have a share)
+    lo = 1;
+    n_sub = reach(lo);
+  }
   if (n_sub > kMaxSub) {
-    int n_hi = reach(hi);
-    if (n_hi >= k) {  // (k NaNs or more)
+    const int n_hi = reach(hi);
+    if (n_hi >= k) {
       lo = hi;
       n_sub = n_hi;
-    } else {
-      // reach(lo) > kMaxSub, reach(hi) < k
-      while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const int n = reach(mid);
-        if (n >= k) {
-          lo = mid;
-          n_sub = n;
-          if (n <= kMaxSub) break;
-        } else {
-          hi = mid;
-        }
+    }
+    // reach(lo) > kMaxSub, reach(hi) < k
+    while (n_sub > kMaxSub && hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int n = reach(mid);
+      if (n >= k) {
+        lo = mid;
+        n_sub = n;
+      } else {
+        hi = mid;
       }
     }
-    ties = n_sub > kMaxSub;  // many shares with the same largest logit, lo
   }
-  // ---- the logits that reach it: with ties those above it, then the first
-  // that equal it, in the order of their places ----
-  const uint32_t from = ties && lo != 0xffffffffu ? lo + 1 : ties ? 0xffffffffu : lo;
-  if (tid == 0) fill = 0;
-  __syncthreads();
-  const bool above = !(ties && lo == 0xffffffffu);
-  if (above) {
-    for (int i = tid; i < subs_all; i += kLpThreads)
-      if (sub_key(i) >= from) {
-        const int at = atomicAdd(&fill, 1);
-        if (at < kMaxSub) subs[at] = i;
+  // many shares with one largest logit, lo: the logits above it, then the first
+  // that equal it, in the order of their places
+  const bool ties = n_sub > kMaxSub;
+  const uint32_t from = ties ? lo + 1 : lo;  // (32-bit keys: 0 past the last)
+  if (from) {
+    keys.each([&](uint32_t key, int share) {
+      if (key >= from) {
+        const int at = atomicAdd(&fill[0], 1);
+        if (at < kMaxSub) subs[at] = share;
       }
+    });
   }
   __syncthreads();
-  const int num_sub = above ? min(fill, kMaxSub) : 0;
-  __syncthreads();
-  if (tid == 0) fill = 0;
-  __syncthreads();
+  const int num_sub = min(fill[0], kMaxSub);
   for (int w = tid; w < num_sub * P::kNum; w += kLpThreads) {
     const int i = subs[w / P::kNum];
-    const int64_t s = P::start(i / kLpThreads, w % P::kNum, i % kLpThreads, shift);
+    const int64_t at = P::start(i / kLpThreads, w % P::kNum, i % kLpThreads, shift);
     float x[P::kVec];
-    P::load(row, s, a.vocab, x);
+    P::load(row, at, a.vocab, x);
 #pragma unroll
     for (int e = 0; e < P::kVec; ++e)
-      if (s + e >= 0 && s + e < a.vocab && order_of(x[e]) >= from) {
-        const int at = atomicAdd(&fill, 1);
-        if (at < kMaxCand) cand[at] = key_of(x[e], (int)(s + e));
+      if (at + e >= 0 && at + e < a.vocab && P::key(x[e]) >= from) {
+        const int c = atomicAdd(&fill[1], 1);
+        if (c < kMaxCand) cand[c] = key_of(x[e], (int)(at + e));
       }
   }
   __syncthreads();
-  int n = min(fill, kMaxCand);
+  int n = min(fill[1], kMaxCand);
   if (ties) {
-    // fewer than k may lie above: the first that equal lo, piece by piece
+    // fewer than k may lie above
     int have = n;
     for (int64_t base = 0; base < a.vocab && have < k; base += kLpThreads) {
       const int64_t i = base + tid;
       const float x = i < a.vocab ? logit_at<DT>(row, i) : 0.0f;
-      const bool hit = i < a.vocab && order_of(x) == lo;
+      const bool hit = i < a.vocab && P::key(x) == lo;
       const uint64_t ball = __builtin_amdgcn_ballot_w64(hit);
-      const int lane = tid & 63;
-      int before = __popcll(ball & ((1ull << lane) - 1));
+      if (lane == 0) counts[turn][wave] = (uint32_t)__popcll(ball);
       __syncthreads();
-      if (lane == 0) counts[tid >> 6] = __popcll(ball);
-      __syncthreads();
-      int all = 0;
+      int before = __popcll(ball & ((1ull << lane) - 1)), found = 0;
 #pragma unroll
-      for (int w = 0; w < kLpThreads / 64; ++w) {
-        if (w < (tid >> 6)) before += counts[w];
-        all += counts[w];
+      for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += (int)counts[turn][w];
+        found += (int)counts[turn][w];
       }
+      turn ^= 1;
       if (hit && have + before < k) cand[have + before] = key_of(x, (int)i);
-      have += min(all, k - have);
+      have += min(found, k - have);
     }
     n = max(n, have);
     __syncthreads();
@@ -322,15 +414,16 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   // ---- fewer candidates, by their (unlike) keys ----
   uint64_t least = 0;
   if (n > kLpThreads) {
-    uint64_t low = 0, high = ~0ull;  // low is reached by k or more, high by fewer
+    uint64_t low = 0, high = ~0ull;  // k or more reach low
     while (high - low > 1) {
       const uint64_t mid = low + (high - low) / 2;
-      int c = 0;
-      for (int i = tid; i < n; i += kLpThreads) c += cand[i] >= mid;
-      c = block_count(c, counts);
-      if (c >= k) {
+      uint32_t c = 0;
+      for (int i0 = 0; i0 < n; i0 += kLpThreads)
+        c += __popcll(__builtin_amdgcn_ballot_w64(i0 + tid < n && cand[i0 + tid] >= mid));
+      const int reached = all(c);
+      if (reached >= k) {
         low = mid;
-        if (c <= kLpThreads) break;
+        if (reached <= kLpThreads) break;
       } else {
         high = mid;
       }
@@ -344,9 +437,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += cand[j] > key;
     if (rank < k) {
-      const int at = (int)~(uint32_t)key;
-      a.top_ids[r * k + rank] = at;
-      a.top_logprobs[r * k + rank] = (logit_at<DT>(row, at) - m) - log_s;
+      a.top_ids[r * k + rank] = (int)~(uint32_t)key;
+      a.top_logprobs[r * k + rank] = (value_of((uint32_t)(key >> 32)) - m) - log_s;
     }
   }
 }
@@ -370,6 +462,7 @@ using namespace mkv;
 
 extern "C" size_t mkv_token_logprobs_workspace_size(int64_t rows, int vocab, int top) {
   if (rows <= 0 || vocab <= 0) return 0;
+  // (4 bytes a key: enough for every type)
   return (size_t)rows * chunks_of(vocab) * (4 + (top > 0 ? kLpThreads : 0)) * sizeof(float);
 }
 
