@@ -148,11 +148,17 @@ __global__ __launch_bounds__(kMoveThreads) __attribute__((amdgpu_waves_per_eu(5)
 // counts change by atomic additions, whose order does not matter, and fresh
 // pages are the lowest-numbered free ones in row order, so the result is one
 // only.  A second kernel copies the part-filled pages that it lists.
+//
+// Latency bound: a chain of memory round trips (parents; their lengths; the
+// tables; the counts' additions; the counts; the stores), so what the steps hand
+// on stays in LDS where it fits (tables of up to kLdsCells entries: 64 rows of 64
+// pages in 7 us, where rows and fresh pages through memory took 16).
 // ---------------------------------------------------------------------------
 constexpr int kMaxRows = 1024;
 constexpr int kAssignThreads = 1024;
 constexpr int kCells = 4;     // table entries a thread looks at at once
 constexpr int kScanPer = 16;  // reference counts a thread looks at in one sweep
+constexpr int kLdsCells = 8192;
 
 struct AssignArgs {
   int32_t* tables;
@@ -168,16 +174,11 @@ struct AssignArgs {
   int parents_i64, tokens_i64;
   uint8_t* granted;
   int rows;
-  int32_t* new_tables;  // workspace: (rows, max_blocks)
-  int32_t* spare;       // workspace: rows * max_blocks fresh pages at most
-  int32_t* copies;      // workspace: (rows, 3) source page, fresh page, live rows (0: none)
+  int32_t* new_tables;  // workspace: (rows, max_blocks), where they do not fit LDS
+  int32_t* spare;       // workspace: rows * max_blocks fresh pages at most, likewise
+  int32_t* copies;      // workspace: their number, then (source page, fresh page, live rows) each
 };
 
-MKV_DEV int wave_sum(int v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
 // exclusive sum of v over the workgroup's threads in order; total in every thread
 MKV_DEV int block_scan(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -207,45 +208,49 @@ MKV_DEV void ref_add(const AssignArgs& a, int page, int by) {
 MKV_DEV int ref_get(const AssignArgs& a, int64_t page) {
   return __hip_atomic_load(a.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// what this wave wrote is in memory (the workgroup's waves share the L1)
+MKV_DEV void written() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+template <bool LDS>
 __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs a) {
-  __shared__ int s_src[kMaxRows], s_keep[kMaxRows], s_held[kMaxRows], s_at[kMaxRows], s_last[kMaxRows], s_start[kMaxRows],
-      s_grow[kMaxRows];
+  __shared__ int s_src[kMaxRows], s_keep[kMaxRows], s_held[kMaxRows], s_at[kMaxRows], s_start[kMaxRows], s_grow[kMaxRows];
+  __shared__ __align__(16) int s_last[kMaxRows];
   __shared__ uint8_t s_copy[kMaxRows], s_drop[kMaxRows];
-  __shared__ int s_scan[kAssignThreads / 64];
+  __shared__ int s_scan[kAssignThreads / 64], s_listed;
+  __shared__ int lds_tables[LDS ? kLdsCells : 1], lds_spare[LDS ? kLdsCells : 1];
+  int* const fresh_tables = LDS ? lds_tables : a.new_tables;
+  int* const spare = LDS ? lds_spare : a.spare;
   const int tid = threadIdx.x, R = a.rows, W = a.max_blocks;
   const int64_t bs = (int64_t)1 << a.bs_log2;
   // a thread a row
   int64_t new_len = 0;
-  int want = 0, fill = 0;
+  int want = 0, fill = 0, at = 0;
   bool valid = false, stays = false, gone = false, fits = false;
+  if (tid == 0) s_listed = 0;
   if (tid < R) {
     const int64_t parent = load_index(a.parents, tid, a.parents_i64);
+    const int64_t tok = a.tokens ? load_index(a.tokens, tid, a.tokens_i64) : 0;
+    const int own_held = a.held[tid];
     valid = parent < R;
     gone = parent < 0;
     stays = parent == tid || !valid;
     const int src = gone || !valid ? tid : (int)parent;
-    const int old_held = min(max(a.held[tid], 0), W);
+    const int src_held = a.held[src];
     const int64_t len = a.seq_lens[src];
+    const int old_held = min(max(own_held, 0), W);
     new_len = gone ? 0 : max(len, (int64_t)0);
     const int64_t need = (new_len + bs - 1) >> a.bs_log2;
-    const int keep = gone ? 0 : stays ? old_held : (int)min(need, (int64_t)min(max(a.held[src], 0), W));
-    const int64_t tok = a.tokens ? load_index(a.tokens, tid, a.tokens_i64) : 0;
+    const int keep = gone ? 0 : stays ? old_held : (int)min(need, (int64_t)min(max(src_held, 0), W));
     const int64_t w = tok <= 0 ? 0 : (tok + bs - 1) >> a.bs_log2;
     fits = valid && w <= W;
     want = fits ? (int)w : 0;
-    const int64_t at = new_len >> a.bs_log2;
-    fill = at < keep ? (int)(new_len & (bs - 1)) : 0;
+    const int64_t last = new_len >> a.bs_log2;
+    fill = last < keep ? (int)(new_len & (bs - 1)) : 0;
+    at = (int)min(last, (int64_t)W);
     s_src[tid] = src;
     s_keep[tid] = keep;
     s_held[tid] = old_held;
-    s_at[tid] = (int)min(at, (int64_t)W);
-    // rows without a part-filled page: numbers that no other row shares
-    s_last[tid] = fill ? a.tables[(int64_t)src * a.bt_stride + at] : -1 - tid;
-    if (s_last[tid] < 0 || s_last[tid] >= a.num_pages) {
-      s_last[tid] = -1 - tid;
-      fill = 0;
-    }
+    s_at[tid] = at;
     s_drop[tid] = stays;  // (for now: rows whose counts stay as they are)
   }
   __syncthreads();
@@ -257,79 +262,100 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
     for (int j = 0; j < kCells; ++j) {
       const int i = i0 + j * kAssignThreads;
       const int r = i < R * W ? i / W : 0, w = i < R * W ? i - r * W : W;
-      const bool keep = w < s_keep[r], held = w < s_held[r];
-      take[j] = keep ? a.tables[(int64_t)s_src[r] * a.bt_stride + w] : 0;
-      drop[j] = held && !s_drop[r] ? a.tables[(int64_t)r * a.bt_stride + w] : -1;
-      if (i < R * W) a.new_tables[i] = take[j];
-      if (!keep || s_drop[r]) take[j] = -1;
+      take[j] = w < s_keep[r] ? a.tables[(int64_t)s_src[r] * a.bt_stride + w] : -1;
+      drop[j] = w < s_held[r] && !s_drop[r] ? a.tables[(int64_t)r * a.bt_stride + w] : -1;
     }
 #pragma unroll
     for (int j = 0; j < kCells; ++j) {
-      ref_add(a, take[j], 1);
+      const int i = i0 + j * kAssignThreads;
+      if (i < R * W) {
+        fresh_tables[i] = take[j];
+        if (!s_drop[i / W]) ref_add(a, take[j], 1);
+      }
       ref_add(a, drop[j], -1);
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  written();
   __syncthreads();
-  // a part-filled page that others hold too is copied by all but its first row
-  int need = 0;
+  // a part-filled page that others hold too is copied by all but its first row;
+  // rows without one have numbers that no other row shares
+  int page = -1 - tid;
+  if (tid < R && fill) {
+    page = fresh_tables[tid * W + at];
+    if (page < 0 || page >= a.num_pages) {
+      page = -1 - tid;
+      fill = 0;
+    }
+  }
+  s_last[tid] = page;
+  // (the counts: this row's page, and this thread's of the first sweep below)
+  const int count = fill ? ref_get(a, page) : 0;
+  uint32_t free_bits = 0;
+  auto sweep = [&](int64_t p0) {
+    free_bits = 0;
+#pragma unroll
+    for (int j = 0; j < kScanPer; ++j) {
+      const int64_t p = p0 + (int64_t)tid * kScanPer + j;
+      if (p < a.num_pages && ref_get(a, p) == 0) free_bits |= 1u << j;
+    }
+  };
+  sweep(0);
+  __syncthreads();
+  int need = 0, grow = 0;
   bool copy = false;
   if (tid < R) {
-    if (fill) {
-      const int page = s_last[tid];
-      int alike = 0;
-      bool first = true;
-      for (int r = 0; r < R; ++r)
-        if (s_last[r] == page) {
-          ++alike;
-          first &= r >= tid;
+    if (fill && count > 1) {
+      int alike = 0, ahead = 0;
+      for (int r0 = 0; r0 < R; r0 += 16) {  // (past the rows: numbers of their own)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(s_last + r0 + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            alike += (int)v[e] == page;
+            ahead += (int)v[e] == page && r0 + j + e < tid;
+          }
         }
-      const int count = ref_get(a, page);
-      copy = count > 1 && !(first && count == alike);
+      }
+      copy = ahead > 0 || count != alike;
     }
-    const int grow = max(want - s_keep[tid], 0);
+    grow = max(want - s_keep[tid], 0);
     need = fits ? (int)copy + grow : 0;
-    s_grow[tid] = grow;
   }
   int total;
   const int start = block_scan(need, s_scan, total);
   // the lowest-numbered free pages, as many as are asked for
   int found = 0;
   for (int64_t p0 = 0; p0 < a.num_pages && found < total; p0 += kAssignThreads * kScanPer) {
-    uint32_t free_bits = 0;
-#pragma unroll
-    for (int j = 0; j < kScanPer; ++j) {
-      const int64_t p = p0 + (int64_t)tid * kScanPer + j;
-      if (p < a.num_pages && ref_get(a, p) == 0) free_bits |= 1u << j;
-    }
+    if (p0) sweep(p0);
     int here;
-    int at = found + block_scan(__popc(free_bits), s_scan, here);
-    while (free_bits && at < total) {
+    int to = found + block_scan(__popc(free_bits), s_scan, here);
+    while (free_bits && to < total) {
       const int j = __ffs(free_bits) - 1;
       free_bits &= free_bits - 1;
-      a.spare[at++] = (int)(p0 + (int64_t)tid * kScanPer + j);
+      spare[to++] = (int)(p0 + (int64_t)tid * kScanPer + j);
     }
     found += here;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (!LDS) written();
   __syncthreads();
   if (tid < R) {
     const bool ok = fits && (need == 0 || start + need <= found);
     const bool drop = !ok && !stays;
     copy = copy && ok;
-    const int grow = ok ? s_grow[tid] : 0;
+    grow = ok ? grow : 0;
     s_start[tid] = start + (copy ? 1 : 0);
     s_grow[tid] = grow;
     s_copy[tid] = copy;
     s_drop[tid] = drop;
-    int32_t* c = a.copies + 3 * tid;
-    c[2] = 0;
     if (copy) {
-      const int fresh = a.spare[start];
-      c[0] = s_last[tid];
+      // (any order: the copies are apart)
+      int32_t* c = a.copies + 1 + 3 * atomicAdd(&s_listed, 1);
+      const int fresh = spare[start];
+      c[0] = page;
       c[1] = fresh;
       c[2] = fill;
-      ref_add(a, s_last[tid], -1);
+      ref_add(a, page, -1);
       ref_add(a, fresh, 1);
       s_last[tid] = fresh;
     }
@@ -339,24 +365,25 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
     a.seq_lens[tid] = drop ? 0 : new_len;
   }
   __syncthreads();
+  if (tid == 0) a.copies[0] = s_listed;
   for (int i0 = tid; i0 < R * W; i0 += kAssignThreads * kCells) {
-    int page[kCells], add[kCells], sub[kCells];
+    int entry[kCells], add[kCells], sub[kCells];
 #pragma unroll
     for (int j = 0; j < kCells; ++j) {
       const int i = i0 + j * kAssignThreads;
       add[j] = sub[j] = -1;
-      page[j] = 0;
+      entry[j] = 0;
       if (i < R * W) {
         const int r = i / W, w = i - r * W, keep = s_keep[r];
         if (w < keep)
-          page[j] = a.new_tables[i];
+          entry[j] = fresh_tables[i];
         else if (!s_drop[r] && w < keep + s_grow[r])
-          page[j] = add[j] = a.spare[s_start[r] + w - keep];
+          entry[j] = add[j] = spare[s_start[r] + w - keep];
         if (s_drop[r]) {
-          if (w < keep) sub[j] = page[j];
-          page[j] = 0;
+          if (w < keep) sub[j] = entry[j];
+          entry[j] = 0;
         } else if (s_copy[r] && w == s_at[r]) {
-          page[j] = s_last[r];
+          entry[j] = s_last[r];
         }
       }
     }
@@ -367,21 +394,26 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
       ref_add(a, sub[j], -1);
       if (i < R * W) {
         const int r = i / W;
-        a.tables[(int64_t)r * a.bt_stride + i - r * W] = page[j];
+        a.tables[(int64_t)r * a.bt_stride + i - r * W] = entry[j];
       }
     }
   }
 }
 
+// The listed copies, blockIdx.y strides over them.
+constexpr int kCopyRows = 16;
 __global__ __launch_bounds__(kCopyThreads) void copy_listed_kernel(Pools p, int block_size, int chunks,
                                                                   const int32_t* __restrict__ copies) {
+  const int n = copies[0];
   const int t = blockIdx.x / chunks;
   const int64_t lo = (int64_t)(blockIdx.x % chunks) * kCopyBytes;
-  const int32_t* c = copies + 3 * blockIdx.y;
-  const int64_t bytes = p.row_bytes[t] * c[2], page = p.row_bytes[t] * block_size;
-  if (lo >= bytes) return;
+  const int64_t page = p.row_bytes[t] * block_size;
   const bool wide = p.row_bytes[t] % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
-  copy_chunk(p.base[t] + c[1] * page, p.base[t] + c[0] * page, lo, bytes, wide);
+  for (int i = blockIdx.y; i < n; i += gridDim.y) {
+    const int32_t* c = copies + 1 + 3 * i;
+    const int64_t bytes = p.row_bytes[t] * c[2];
+    if (lo < bytes) copy_chunk(p.base[t] + c[1] * page, p.base[t] + c[0] * page, lo, bytes, wide);
+  }
 }
 
 int log2_exact(int64_t v) {
@@ -485,7 +517,8 @@ extern "C" int mkv_compact_slots(const void* const* tensors, const int64_t* row_
 
 extern "C" size_t mkv_assign_pages_workspace_size(int rows, int max_blocks) {
   if (rows <= 0 || max_blocks < 0) return 0;
-  return ((size_t)rows * max_blocks * 2 + (size_t)rows * 4) * sizeof(int32_t);
+  const size_t cells = (size_t)rows * max_blocks;
+  return ((cells > kLdsCells ? cells * 2 : 0) + (size_t)rows * 3 + 1) * sizeof(int32_t);
 }
 
 extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors,
@@ -509,9 +542,12 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
   // copied keeps at least that one)
   AssignArgs a{block_tables, bt_stride, max_blocks, seq_lens, held, ref_counts, num_pages, bs_log2, parents, tokens,
                (int)(parents_dtype == MKV_INDEX_I64), (int)(tokens_dtype == MKV_INDEX_I64), granted, rows, ws,
-               ws + cells, ws + 2 * cells};
+               ws + cells, cells > kLdsCells ? ws + 2 * cells : ws};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(assign_pages_kernel, dim3(1), dim3(kAssignThreads), 0, s, a);
+  if (cells > kLdsCells)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(assign_pages_kernel<false>), dim3(1), dim3(kAssignThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(assign_pages_kernel<true>), dim3(1), dim3(kAssignThreads), 0, s, a);
   if (hipError_t e = hipGetLastError()) return (int)e;
   for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
     Pools p;
@@ -519,7 +555,7 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
     const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
     const int64_t chunks = (widest * block_size + kCopyBytes - 1) / kCopyBytes;
     if (chunks * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
-    hipLaunchKernelGGL(copy_listed_kernel, dim3((unsigned)(chunks * n), (unsigned)rows), dim3(kCopyThreads), 0, s, p,
+    hipLaunchKernelGGL(copy_listed_kernel, dim3((unsigned)(chunks * n), (unsigned)(rows < kCopyRows ? rows : kCopyRows)), dim3(kCopyThreads), 0, s, p,
                        block_size, (int)chunks, a.copies);
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
