@@ -270,9 +270,13 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
       const int i = i0 + j * kAssignThreads;
       if (i < R * W) {
         fresh_tables[i] = take[j];
-        if (!s_drop[i / W]) ref_add(a, take[j], 1);
+        // (a page let go and taken again in the same place counts as before:
+        // most of a beam's)
+        if (!s_drop[i / W] && take[j] != drop[j]) {
+          ref_add(a, take[j], 1);
+          ref_add(a, drop[j], -1);
+        }
       }
-      ref_add(a, drop[j], -1);
     }
   }
   written();
@@ -291,12 +295,19 @@ __global__ __launch_bounds__(kAssignThreads) void assign_pages_kernel(AssignArgs
   // (the counts: this row's page, and this thread's of the first sweep below)
   const int count = fill ? ref_get(a, page) : 0;
   uint32_t free_bits = 0;
+  constexpr int kAgent = 16;  // sc1: coherent with the other CUs and with this one's atomics
+  const __amdgpu_buffer_rsrc_t refs =
+      __builtin_amdgcn_make_buffer_rsrc(a.refs, (short)0, (int)(a.num_pages * 4), 0x00020000);
   auto sweep = [&](int64_t p0) {
+    // (16 bytes at a time, past the L1: the additions went past it; what lies
+    // behind the last count reads 0 and is masked)
     free_bits = 0;
+    const int64_t first = p0 + (int64_t)tid * kScanPer;
 #pragma unroll
-    for (int j = 0; j < kScanPer; ++j) {
-      const int64_t p = p0 + (int64_t)tid * kScanPer + j;
-      if (p < a.num_pages && ref_get(a, p) == 0) free_bits |= 1u << j;
+    for (int j = 0; j < kScanPer; j += 4) {
+      const u32x4 c = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(refs, (int)((first + j) * 4), 0, kAgent));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) free_bits |= c[e] == 0 && first + j + e < a.num_pages ? 1u << (j + e) : 0u;
     }
   };
   sweep(0);
@@ -527,7 +538,7 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
                                 const void* parents, int parents_dtype, const void* tokens, int tokens_dtype,
                                 uint8_t* granted, int rows, void* workspace, size_t workspace_bytes, void* stream) {
   if (int st = check_pools(tensors, row_bytes, num_tensors, num_pages, block_size)) return st;
-  if (rows < 0 || rows > kMaxRows || max_blocks < 0 || (int64_t)rows * max_blocks > (1 << 28)) return MKV_ERR_BAD_SHAPE;
+  if (rows < 0 || rows > kMaxRows || num_pages > (1 << 28) || max_blocks < 0 || (int64_t)rows * max_blocks > (1 << 28)) return MKV_ERR_BAD_SHAPE;
   if (!index_ok(parents_dtype) || (tokens && !index_ok(tokens_dtype))) return MKV_ERR_UNSUPPORTED_DTYPE;
   const int bs_log2 = log2_exact(block_size);
   if (bs_log2 < 0) return MKV_ERR_BAD_BLOCK_SIZE;
