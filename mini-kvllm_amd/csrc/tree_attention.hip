@@ -82,6 +82,35 @@ MKV_DEV int64_t load_len(const void* p, int i, int i64) {
   return i64 ? (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo) : (int64_t)lo;
 }
 
+// Sums over the wave's lanes up to each (the last lane's is the whole), by DPP.
+template <typename X>
+MKV_DEV X wave_scan(X x) {
+  static_assert(sizeof(X) == 4, "");
+  auto add = [&](auto ctrl, auto rows) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    x += __builtin_bit_cast(X, y);
+  };
+  using All = std::integral_constant<int, 0xf>;
+  add(std::integral_constant<int, 0x111>{}, All{});  // row_shr 1, 2, 4, 8
+  add(std::integral_constant<int, 0x112>{}, All{});
+  add(std::integral_constant<int, 0x114>{}, All{});
+  add(std::integral_constant<int, 0x118>{}, All{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15, 31
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return x;
+}
+MKV_DEV float wave_sum(float x) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wave_scan(x)), 63));
+}
+
+// A workgroup's place: row block, unit, KV head and sequence with the split's
+// number and length, and the sequence's rows and context length as given.
+struct Place {
+  int rb, unit, kvh, seq, z, len;
+  int cu0, cu1;
+  int64_t ctx;
+};
+
 // A unit is one split of one sequence; units go sequence by sequence.  Splits are
 // of `len` keys, the same for every sequence: the batch's keys over the plan's
 // shares, in whole tiles.  Every workgroup works this out for itself from the
@@ -94,61 +123,66 @@ struct Units {
   int len, total;
   int before, n;  // this lane's sequence (of the 64 last looked at): its units, and those ahead of them
 
-  MKV_DEV int keys(int s0) const {
-    const int s = s0 + (threadIdx.x & 63);
-    const int64_t c = load_len(a.ctx, min(s, a.num_seqs - 1), a.ctx_i64);
-    return s < a.num_seqs ? (int)min(max(c, (int64_t)0), (int64_t)a.idx.max_blocks << a.idx.bs_log2) : 0;
+  int cu0, cu1;       // ... its rows in q, and the length of its context
+  int64_t ctx;
+
+  MKV_DEV int keys(int s0) {
+    const int s = s0 + (threadIdx.x & 63), i = min(s, a.num_seqs - 1);
+    ctx = load_len(a.ctx, i, a.ctx_i64);
+    cu0 = a.cu[i];
+    cu1 = a.cu[i + 1];
+    return s < a.num_seqs ? (int)min(max(ctx, (int64_t)0), (int64_t)a.idx.max_blocks << a.idx.bs_log2) : 0;
   }
   // the units of sequences s0 .. s0 + 63, `base` ahead of them; their number
   MKV_DEV int number(int s0, int k, int base) {
-    const int lane = threadIdx.x & 63;
-    n = s0 + lane < a.num_seqs ? max((k + len - 1) / len, 1) : 0;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o);
-      upto += lane >= o ? y : 0;
-    }
+    n = s0 + (int)(threadIdx.x & 63) < a.num_seqs ? max((k + len - 1) / len, 1) : 0;
+    const int upto = wave_scan(n);
     before = base + upto - n;
-    return uniform(__shfl(upto, 63));
+    return __builtin_amdgcn_readlane(upto, 63);
   }
   MKV_DEV explicit Units(const TreeArgs& args) : a(args) {
     const int k0 = keys(0);
-    float sum = (float)k0;  // (a rule of thumb's accuracy, the same in every wave)
-    for (int s0 = 64; s0 < a.num_seqs; s0 += 64) sum += (float)keys(s0);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    float sum = wave_sum((float)k0);  // (a rule of thumb's accuracy, the same in every wave)
+    for (int s0 = 64; s0 < a.num_seqs; s0 += 64) sum += wave_sum((float)keys(s0));
     // (a little more than the even share: at most `shares` units beside the last
     // one of each sequence, whatever the sum's rounding)
     len = (int)fminf(sum * 1.0001f / (float)a.shares, 1.0e9f) + 1;
     len = uniform((max(len, a.min_split) + TILE - 1) / TILE * TILE);
-    total = number(0, k0, 0);
+    total = number(0, a.num_seqs > 64 ? keys(0) : k0, 0);
     for (int s0 = 64; s0 < a.num_seqs; s0 += 64) total += number(s0, keys(s0), total);
   }
-  // the sequence of a unit, and its number within the sequence
-  MKV_DEV void of_unit(int unit, int& seq, int& z) {
-    seq = -1;
-    z = 0;
+  // a unit's sequence, its number within it, and what find_work() reads of it
+  MKV_DEV bool of_unit(int unit, Place& p) {
     int base = 0;
     for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
       if (a.num_seqs > 64) base += number(s0, keys(s0), base);
       const uint64_t mine = __builtin_amdgcn_ballot_w64(unit >= before && unit < before + n);
       if (mine) {
         const int l = __builtin_ctzll(mine);
-        seq = s0 + l;
-        z = unit - uniform(__shfl(before, l));
-        return;
+        p.seq = s0 + l;
+        p.z = unit - __builtin_amdgcn_readlane(before, l);
+        take(l, p);
+        return true;
       }
     }
+    return false;
   }
-  // a sequence's first unit, and their number
-  MKV_DEV void of_sequence(int seq, int& first, int& count) {
+  // a sequence's first unit, their number, and what find_work() reads of it
+  MKV_DEV int of_sequence(int seq, Place& p) {
     if (a.num_seqs > 64) {
       int base = 0;
       for (int s0 = 0; s0 <= seq; s0 += 64) base += number(s0, keys(s0), base);
     }
-    first = uniform(__shfl(before, seq & 63));
-    count = uniform(__shfl(n, seq & 63));
+    p.seq = seq;
+    p.unit = __builtin_amdgcn_readlane(before, seq & 63);
+    take(seq & 63, p);
+    return __builtin_amdgcn_readlane(n, seq & 63);
+  }
+  MKV_DEV void take(int l, Place& p) const {
+    p.cu0 = __builtin_amdgcn_readlane(cu0, l);
+    p.cu1 = __builtin_amdgcn_readlane(cu1, l);
+    p.ctx = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(ctx >> 32), l) << 32 |
+                      (uint32_t)__builtin_amdgcn_readlane((int)ctx, l));
   }
 };
 
@@ -253,13 +287,13 @@ struct Work {
   int ctx;          // keys, within the block table
 };
 
-MKV_DEV Work find_work(const TreeArgs& a, int seq, int kvh) {
+MKV_DEV Work find_work(const TreeArgs& a, const Place& p) {
   Work w;
-  w.kvh = kvh;
-  w.seq = seq;
-  const int64_t q0 = min(max((int64_t)a.cu[w.seq], (int64_t)0), a.total_q);
-  const int64_t q1 = min(max((int64_t)a.cu[w.seq + 1], q0), a.total_q);
-  const int64_t c = max(load_len(a.ctx, w.seq, a.ctx_i64), (int64_t)0);
+  w.kvh = p.kvh;
+  w.seq = p.seq;
+  const int64_t q0 = min(max((int64_t)p.cu0, (int64_t)0), a.total_q);
+  const int64_t q1 = min(max((int64_t)p.cu1, q0), a.total_q);
+  const int64_t c = max(p.ctx, (int64_t)0);
   w.q0 = q0;
   w.rows = (int)min(q1 - q0, (int64_t)a.mask_cols) * a.group;
   w.prefix = max(c - (q1 - q0), (int64_t)0);
@@ -267,10 +301,7 @@ MKV_DEV Work find_work(const TreeArgs& a, int seq, int kvh) {
   return w;
 }
 
-// A workgroup's place: row block, unit and KV head by its number (false: none).
-struct Place {
-  int rb, unit, kvh, seq, z, len;
-};
+// (false: a workgroup without work)
 template <int TILE>
 MKV_DEV bool find_place(const TreeArgs& a, Place& p) {
   auto split = [&](int units) {
@@ -285,14 +316,16 @@ MKV_DEV bool find_place(const TreeArgs& a, Place& p) {
     p.len = 0x7fffffff / TILE * TILE;
     p.z = 0;
     const bool ok = split(a.num_seqs);
-    p.seq = p.unit;
+    p.seq = min(p.unit, a.num_seqs - 1);
+    p.cu0 = a.cu[p.seq];
+    p.cu1 = a.cu[p.seq + 1];
+    p.ctx = load_len(a.ctx, p.seq, a.ctx_i64);
     return ok;
   }
   Units<TILE> u(a);
   p.len = u.len;
   if (!split(u.total)) return false;
-  u.of_unit(p.unit, p.seq, p.z);
-  return p.seq >= 0;
+  return u.of_unit(p.unit, p);
 }
 
 // Element offset of row r (token r / group, head r % group) of the KV head in q
@@ -349,19 +382,27 @@ MKV_DEV f16x8 codes_to_f16(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
 }
 
-// The tile's pipeline.  K and V have one LDS buffer each: the DMA of the next
-// tile's K goes out once the products with K are done and lands under the softmax
-// and P V, the next V's once P V is done and lands under the next K Q^T.  With one
-// row group a wave reads only what it loaded itself and meets no barrier; with
-// more, a barrier stands on either side of each product.  One buffer (64 KB at
-// most) and at most 256 registers leave room for two workgroups a CU, whose
-// waves fill each other's waits and overlap MFMA with the softmax's VALU work.
+// Keys a wave takes of a tile: two blocks of 32, whose products and softmax run
+// side by side; one with four key groups (16-bit tiles of 256 keys would not fit
+// twice in a CU's LDS, and short contexts end in the middle of so long a tile).
+template <int KV_DT, int R, int KG>
+constexpr int kTileKeys = KG == 4 ? 32 : 64;
+
+// The tile's pipeline.  K and V have one LDS buffer each.  A wave reads all of a
+// tile's K operands into registers, and the DMA of the next tile's K goes out
+// where they were, to land under the softmax and P V; likewise V's once its last
+// operands are read.  The second key block's K Q^T is issued among the first's
+// exponentials and the first's P V among the second's, so that MFMA and VALU work
+// of one wave overlap (two waves a SIMD alone reached little more than the sum of
+// the two: 2900 cycles for a tile's 1536 of MFMA and 1200 of VALU).  With one row
+// group a wave reads only what it loaded itself and meets no barrier.  One buffer
+// (64 KB at most) and at most 256 registers leave room for two workgroups a CU.
 template <int KV_DT, int R, int KG, bool PAIR>
 MKV_DEV void tree_attention_body(const TreeArgs& a) {
   constexpr int CT = kOperand<KV_DT>;
   constexpr bool kTok = kPerTokenScale<KV_DT>;
   constexpr int kWaves = R * KG, kThreads = 64 * kWaves;
-  constexpr int TK = KG == 1 ? 64 : 32;   // keys a wave takes of a tile
+  constexpr int TK = kTileKeys<KV_DT, R, KG>;  // keys a wave takes of a tile
   constexpr int NK = TK * KG;             // keys of a tile
   constexpr int NB = TK / 32;
   constexpr int kEb = DTypeInfo<KV_DT>::kBytes;
@@ -371,9 +412,10 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   constexpr int kSubs = kOwn > 16 ? kOwn / 16 : 1;      // 16-key sub-tiles (never across a block) they lie in
   constexpr bool kShared = R > 1;
   static_assert(kOwn % T::kKeysPerDma == 0 && kDma >= 1, "whole loads");
-  constexpr int kBuf = NK * T::kRow > 16384 ? NK * T::kRow : 16384;  // (the join's halves fit too)
+  constexpr int kSums = R * 4 * (KG - 1) * 4096;  // (what the key groups hand each other, over both)
+  constexpr int kBuf = NK * T::kRow > kSums / 2 ? NK * T::kRow : kSums / 2;
   __shared__ __align__(16) char lds_k[kBuf], lds_v[kBuf];
-  __shared__ float join_ml[KG > 1 ? 2 * R * 64 * 2 : 1];
+  __shared__ f32x2 join_ml[KG > 1 ? kWaves * 32 : 1];
   __shared__ int slots[kShared ? 2 * (NK / 16) : 1];  // of each sub-tile, -1 absent, by the tile's parity
   constexpr int kHeads = PAIR ? 2 : 1;
   constexpr int kScLoads = kTok ? 2 * kHeads * TK / 64 : 1;
@@ -385,7 +427,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   Place place;
   if (!find_place<NK>(a, place)) return;
   const int len = place.len;
-  const Work w = find_work(a, place.seq, place.kvh);
+  const Work w = find_work(a, place);
   const bool zeroes = place.rb == 0 && place.z == 0 && w.kvh == 0;
   if (place.rb * 32 * R >= w.rows) {
     if (zeroes) zero_rows_past(a, w);
@@ -403,8 +445,8 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   // lane's key and chunk of a load; loads of one sub-tile differ in the key's
   // upper bits, which reach the swizzle's low bits
   const int ld_key = lane / T::kChunks;
-  uint32_t voff[kDma > 4 ? 4 : kDma];
   constexpr int kPerSub = kDma / kSubs;
+  uint32_t voff[kPerSub];
 #pragma unroll
   for (int i = 0; i < kPerSub; ++i) {
     const int key = (own0 & 15) + i * T::kKeysPerDma + ld_key;
@@ -413,18 +455,18 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   // The tile whose K is loaded next: its sub-tiles' first token slots, and the
   // rows of each that lie within the context in a present block.  The block
   // entries come a tile ahead by a vector load (a scalar one would share its
-  // counter with the LDS reads), lane 0 the first sub-tile's, lane 32 the second's.
+  // counter with the LDS reads), a run of lanes a sub-tile.
   int32_t slot[kSubs], left[kSubs];
   const int32_t* bt_row = a.idx.block_tables + (int64_t)w.seq * a.idx.bt_stride;
   auto entry_load = [&](int kb) -> int32_t {
-    const int blk = (kb + sub0 + (kSubs > 1 ? 16 * h : 0)) >> a.idx.bs_log2;
+    const int blk = (kb + sub0 + 16 * (lane / (64 / kSubs))) >> a.idx.bs_log2;
     return bt_row[min(blk, a.idx.max_blocks - 1)];
   };
   auto entry_use = [&](int kb, int32_t e) {
 #pragma unroll
     for (int u = 0; u < kSubs; ++u) {
       const int t = kb + sub0 + 16 * u;
-      const int phys = __builtin_amdgcn_readlane(e, 32 * u);
+      const int phys = __builtin_amdgcn_readlane(e, 64 / kSubs * u);
       const bool ok = t < k1 && phys >= 0 && phys < (int)a.idx.num_blocks;
       slot[u] = ok ? (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : 0;
       left[u] = ok ? min(k1 - t, 16) : 0;
@@ -454,13 +496,31 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
         if constexpr (kShared)
           sl = slots[turn * (NK / 16) + (kg * TK + key) / 16];
         else
-          sl = key < 16 ? (left[0] > 0 ? slot[0] : -1) : (left[kSubs - 1] > 0 ? slot[kSubs - 1] : -1);
+        {
+          sl = -1;
+#pragma unroll
+          for (int u = 0; u < kSubs; ++u) sl = key >> 4 == u && left[u] > 0 ? slot[u] : sl;
+        }
         sc_raw[i] = 0.0f;
         if (sl >= 0 && kb + kg * TK + key < k1)
           sc_raw[i] = ((which & 1) ? a.v_scale : a.k_scale)[(int64_t)(sl + (key & 15)) * a.scale_heads + w.kvh * kHeads + (which >> 1)];
       }
     }
   };
+  // ---- q: this lane's row; step s of the contraction takes dims 16 s + 8 h .. + 7
+  // (16-bit: chunk 2 s + h), or the lower or upper half of chunk 2 (s / 2) + h ----
+  const int row = place.rb * 32 * R + rg * 32 + c;
+  const bool row_ok = row < w.rows;
+  bool hi = false;
+  const int64_t q_off = row_offset<PAIR>(a, w, row_ok ? row : 0, hi);
+  float score_mul = a.sm_scale * kLog2e;
+  u32x4 raw[8];  // (its loads go out ahead of the tiles')
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const int st = PAIR ? s & 3 : s;
+    const int d = kEb == 2 ? 16 * st + 8 * h : 16 * (2 * (st >> 1) + h) + 8 * (st & 1);
+    raw[s] = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);  // (within q for any row)
+  }
   const bool any = kb0 < k1;
   int32_t e_ahead = 0;
   if (any) {
@@ -469,7 +529,10 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     entry_use(kb0, e_ahead);
     e_ahead = e_next;
     if constexpr (kShared) {
-      if (lane == 0) slots[sub0 / 16] = left[0] > 0 ? slot[0] : -1;
+      if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) slots[sub0 / 16 + u] = left[u] > 0 ? slot[u] : -1;
+      }
       if constexpr (kTok) __syncthreads();
     }
     load_scales(kb0, 0);
@@ -477,25 +540,8 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     dma(a.v, lds_v);
   }
 
-  // ---- q: this lane's row; step s of the contraction takes dims 16 s + 8 h .. + 7
-  // (16-bit: chunk 2 s + h), or the lower or upper half of chunk 2 (s / 2) + h ----
-  const int row = place.rb * 32 * R + rg * 32 + c;
-  const bool row_ok = row < w.rows;
-  bool hi = false;
-  const int64_t q_off = row_offset<PAIR>(a, w, row_ok ? row : 0, hi);
-  float score_mul = a.sm_scale * kLog2e;
   Op16<CT> qop[8];
   {
-    u32x4 raw[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const bool mine = row_ok && (!PAIR || (s >> 2) == (int)hi);
-      const int st = PAIR ? s & 3 : s;
-      const int d = kEb == 2 ? 16 * st + 8 * h : 16 * (2 * (st >> 1) + h) + 8 * (st & 1);
-      raw[s] = ld16(reinterpret_cast<const uint16_t*>(a.q) + q_off + d);  // (within q for any row)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) raw[s][j] = mine ? raw[s][j] : 0u;
-    }
     // the loop keeps raw scores and wants score_mul > 0: a negative scale
     // moves its sign into q, a zero one makes q zero
     uint32_t sign = 0u, keep = 0xffffffffu;
@@ -505,9 +551,12 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       score_mul = score_mul < 0.0f ? -score_mul : 1.0f;
     }
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
+    for (int s = 0; s < 8; ++s) {
+      const bool mine = row_ok && (!PAIR || (s >> 2) == (int)hi);  // (a row past the last: zeros)
+      const uint32_t k = mine ? keep : 0u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) raw[s][j] = (raw[s][j] ^ sign) & keep;
+      for (int j = 0; j < 4; ++j) raw[s][j] = (raw[s][j] ^ sign) & k;
+    }
     if (kEb == 2 || a.q_dtype == MKV_DTYPE_F16) {  // q's type is the operands'
 #pragma unroll
       for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(Op16<CT>, raw[s]);
@@ -590,10 +639,147 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       return codes_to_f16<KV_DT>(r.w[0], r.w[1]);
   };
 
+  // ---- a tile's steps ----
+  constexpr int kReads = kEb == 2 ? 8 : 4;  // 16-byte reads of a key block's K
+  struct KOps {
+    u32x4 w[kReads];
+  };
+  struct VOps {
+    VRaw w[2][4];
+  };
+  auto k_read = [&](int nb, KOps& k) {
+#pragma unroll
+    for (int j = 0; j < kReads; ++j)
+      k.w[j] = *reinterpret_cast<const u32x4*>(lds_k + (k_base ^ j << 5) + 32 * nb * T::kRow);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto qk = [&](const KOps& k) {
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int st = 0; st < 8; ++st) {
+      if constexpr (kEb == 2)
+        s = mfma32<CT>(__builtin_bit_cast(Op16<CT>, k.w[st]), qop[st], s);
+      else
+        s = mfma32<CT>(codes_to_f16<KV_DT>(k.w[st >> 1][2 * (st & 1)], k.w[st >> 1][2 * (st & 1) + 1]), qop[st], s);
+    }
+    return s;
+  };
+  const float* const ks = sc + (PAIR && hi ? 2 * TK : 0) + 4 * h;
+  // scores of key block nb: K scales, -inf where the row does not see, and the
+  // running maximum (with what is already summed, and the pending P of the block
+  // before, brought to it)
+  auto s_max = [&](f32x16& s, int nb, bool masked, uint32_t see, f32x16& pending, auto has_pending) {
+    if constexpr (kTok) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(ks + 32 * nb + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * g + e] *= x[e];
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = (see >> e) & 1 ? s[e] : kNegInf;
+    }
+    float mx = max3(s[0], s[1], s[2]), my = max3(s[3], s[4], s[5]);
+#pragma unroll
+    for (int e = 6; e < 14; e += 4) {
+      mx = max3(mx, s[e], s[e + 1]);
+      my = max3(my, s[e + 2], s[e + 3]);
+    }
+    mx = max3(mx, s[14], s[15]);
+    mx = max3(mx, my, my);
+    mx = fmaxf(mx, other_half(mx));
+    mx = fmaxf(mx * score_mul, kNegBig);
+    const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
+    if (__builtin_amdgcn_ballot_w64(m_new != m_run)) {
+      // (before the first visible key there is nothing to rescale but marks)
+      const float alpha = m_run == kNegBig ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] *= alpha;
+      if constexpr (decltype(has_pending)::value) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pending[e] *= alpha;
+      }
+    }
+  };
+  auto s_exp = [&](f32x16& s, int nb, bool masked, uint32_t see) {
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+      if constexpr (kTok) x = *reinterpret_cast<const f32x4*>(ks + TK + 32 * nb + 8 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * g + j;
+        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], score_mul, -m_run));
+        sum[g & 1] += s[e];
+        if constexpr (kTok) {
+          s[e] *= x[j];
+          if (masked) s[e] = (see >> e) & 1 ? s[e] : 0.0f;
+        }
+      }
+    }
+    l_run += sum[0] + sum[1];
+  };
+  auto v_block = [&](int nb, VOps& v) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) v.w[half][b] = v_read(nb, half, b);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto pv = [&](const VOps& v, const f32x16& p) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      Op16<CT> ph, pl;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (CT == MKV_DTYPE_BF16)
+          ph[j] = (__bf16)p[8 * half + j];
+        else
+          ph[j] = (_Float16)p[8 * half + j];
+      }
+      if constexpr (CT == MKV_DTYPE_BF16) {
+        // bf16 holds P to 8 bits: a second term carries the rest, so that a
+        // row whose weight sits on few keys is as exact as decode's.  p - hi is
+        // one dot product a value: hi_pair . (-1, 0) or (0, -1), + p
+        uint32_t lo_bits = 0x0000bf80u, hi_bits = 0xbf800000u;
+        asm volatile("" : "+s"(lo_bits), "+s"(hi_bits));
+        const bf16x2 neg_lo = __builtin_bit_cast(bf16x2, lo_bits), neg_hi = __builtin_bit_cast(bf16x2, hi_bits);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const bf16x2 hp = {ph[j], ph[j + 1]};
+          pl[j] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_lo, p[8 * half + j], false);
+          pl[j + 1] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_hi, p[8 * half + j + 1], false);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(v.w[half][b]), ph, acc[b]);
+      if constexpr (CT == MKV_DTYPE_BF16) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(v.w[half][b]), pl, acc[b]);
+      }
+    }
+  };
+  // N MFMAs with V vector operations after each: what the scheduler is asked for
+  // where a key block's products stand beside the other's softmax
+  auto mix = [&](auto n_tag, auto v_tag) {
+#pragma unroll
+    for (int i = 0; i < decltype(n_tag)::value; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, decltype(v_tag)::value, 0);
+    }
+  };
+
   for (int kb = kb0, turn = 0; kb < k1; kb += NK, turn ^= 1) {
+    const int key0 = kg * TK;  // this wave's keys of the tile
     wait_vm<kDma>();  // K is here, V may be on its way
     if constexpr (kShared) meet();
-    const int key0 = kg * TK;  // this wave's keys of the tile
     uint32_t present = 0;
     if constexpr (kShared) {
 #pragma unroll
@@ -638,107 +824,27 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       }
     }
 
-    // ---- S^T = K Q^T, the operands of four steps read ahead of the four
-    // before (left to itself the compiler reads one and waits for it) ----
+
+    // ---- S^T = K Q^T of the first key block; all of K is read ----
+    KOps k_ops[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) k_read(nb, k_ops[nb]);
     f32x16 s[NB];
-    __builtin_amdgcn_s_setprio(1);
-    {
-      constexpr int kReads = kEb == 2 ? 4 : 2;  // 16-byte reads of four steps
-      u32x4 kw[2][kReads];
-      auto read = [&](int i) {
-#pragma unroll
-        for (int j = 0; j < kReads; ++j) {
-          const int st = (i & 1) * kReads + j;
-          kw[i & 1][j] = *reinterpret_cast<const u32x4*>(lds_k + (k_base ^ st << 5) + 32 * (i >> 1) * T::kRow);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      read(0);
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) {
-        if (i + 1 < 2 * NB) read(i + 1);
-        if (!(i & 1)) s[i >> 1] = f32x16{};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int st = 4 * (i & 1) + j;
-          if constexpr (kEb == 2)
-            s[i >> 1] = mfma32<CT>(__builtin_bit_cast(Op16<CT>, kw[i & 1][j]), qop[st], s[i >> 1]);
-          else
-            s[i >> 1] = mfma32<CT>(codes_to_f16<KV_DT>(kw[i & 1][j >> 1][2 * (j & 1)], kw[i & 1][j >> 1][2 * (j & 1) + 1]), qop[st], s[i >> 1]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    __builtin_amdgcn_s_setprio(0);
-    // ---- the next tile's K, where this one's was ----
+    s[0] = qk(k_ops[0]);
+    // ---- V is here; the next tile's K goes where this one's was ----
+    wait_vm<0>();
     entry_use(kb + NK, e_ahead);
     if constexpr (kShared) {
-      if (lane == 0) slots[(turn ^ 1) * (NK / 16) + sub0 / 16] = left[0] > 0 ? slot[0] : -1;
+      if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) slots[(turn ^ 1) * (NK / 16) + sub0 / 16 + u] = left[u] > 0 ? slot[u] : -1;
+      }
       meet();
     } else {
       wait_lds();
     }
     load_scales(kb + NK, turn ^ 1);
     dma(a.k, lds_k);
-
-    // ---- softmax ----
-    const float* ks = sc + (PAIR && hi ? 2 * TK : 0);
-    if constexpr (kTok) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(ks + 32 * nb + 8 * g + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nb][4 * g + e] *= x[e];
-        }
-    }
-    if (masked) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[nb][e] = (seen[nb] >> e) & 1 ? s[nb][e] : kNegInf;
-    }
-    float mx = kNegInf;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) mx = max3(mx, s[nb][e], s[nb][e + 1]);
-    mx = fmaxf(mx, other_half(mx));
-    mx = fmaxf(mx * score_mul, kNegBig);
-    const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
-    // (before the first visible key there is nothing to rescale but marks)
-    const float alpha = m_run == kNegBig ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-    m_run = m_new;
-    l_run *= alpha;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[b][e] *= alpha;
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 x;
-        if constexpr (kTok) x = *reinterpret_cast<const f32x4*>(ks + TK + 32 * nb + 8 * g + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = 4 * g + j;
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][e], score_mul, -m_new));
-          l_run += p;
-          s[nb][e] = p;
-          if constexpr (kTok) {
-            s[nb][e] = p * x[j];
-            if (masked) s[nb][e] = (seen[nb] >> e) & 1 ? s[nb][e] : 0.0f;
-          }
-        }
-      }
-
-    // ---- O^T += V^T P^T ----
-    wait_vm<kDma>();  // V is here, the next K may be on its way
-    if constexpr (kShared) meet();
     if (kShared ? kb + NK > prefix : drafted) {
       bool found = false;
       constexpr int kScan = kShared ? NK * T::kChunks / kThreads : TK * T::kChunks / 64;
@@ -798,118 +904,117 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
         else wait_lds();
       }
     }
-    __builtin_amdgcn_s_setprio(1);
-    {
-      VRaw vr[2][4];
-      auto read = [&](int i) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) vr[i & 1][b] = v_read(i >> 1, i & 1, b);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      read(0);
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) {
-        if (i + 1 < 2 * NB) read(i + 1);
-        const f32x16& p = s[i >> 1];
-        const int half = i & 1;
-        Op16<CT> ph, pl;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (CT == MKV_DTYPE_BF16)
-            ph[j] = (__bf16)p[8 * half + j];
-          else
-            ph[j] = (_Float16)p[8 * half + j];
-        }
-        if constexpr (CT == MKV_DTYPE_BF16) {
-          // bf16 holds P to 8 bits: a second term carries the rest, so that a
-          // row whose weight sits on few keys is as exact as decode's.  p - hi is
-          // one dot product a value: hi_pair . (-1, 0) or (0, -1), + p
-          uint32_t lo_bits = 0x0000bf80u, hi_bits = 0xbf800000u;
-          asm volatile("" : "+s"(lo_bits), "+s"(hi_bits));
-          const bf16x2 neg_lo = __builtin_bit_cast(bf16x2, lo_bits), neg_hi = __builtin_bit_cast(bf16x2, hi_bits);
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const bf16x2 hp = {ph[j], ph[j + 1]};
-            pl[j] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_lo, p[8 * half + j], false);
-            pl[j + 1] = (__bf16)__builtin_amdgcn_fdot2_f32_bf16(hp, neg_hi, p[8 * half + j + 1], false);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(vr[i & 1][b]), ph, acc[b]);
-        if constexpr (CT == MKV_DTYPE_BF16)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[b] = mfma32<CT>(v_operand(vr[i & 1][b]), pl, acc[b]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+
+    // ---- softmax and O^T += V^T P^T: the second block's K Q^T beside the first's
+    // exponentials, the first's P V beside the second's ----
+    VOps v_ops[NB];
+    s_max(s[0], 0, masked, seen[0], s[0], std::false_type{});
+    v_block(0, v_ops[0]);
+    if constexpr (NB == 2) {
+      s[1] = qk(k_ops[1]);
+      s_exp(s[0], 0, masked, seen[0]);
+      mix(std::integral_constant<int, 8>{}, std::integral_constant<int, kEb == 2 ? 6 : 10>{});
+      // (held here: the compiler would sink the exponentials to their use, behind
+      // the branches below and out of the MFMAs' shadow)
+      asm volatile("" : "+v"(s[0]), "+v"(l_run));
+      s_max(s[1], 1, masked, seen[NB - 1], s[0], std::true_type{});
+      v_block(1, v_ops[NB - 1]);
+      pv(v_ops[0], s[0]);
+      s_exp(s[1], 1, masked, seen[NB - 1]);
+      mix(std::integral_constant<int, CT == MKV_DTYPE_BF16 ? 16 : 8>{}, std::integral_constant<int, CT == MKV_DTYPE_BF16 ? 4 : 10>{});
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      s_exp(s[0], 0, masked, seen[0]);
     }
-    __builtin_amdgcn_s_setprio(0);
-    // ---- the next tile's V, where this one's was ----
+    // ---- all of V is read: the next tile's goes where it was ----
     if constexpr (kShared) meet();
     else wait_lds();
     e_ahead = entry_load(kb + 2 * NK);
     dma(a.v, lds_v);
+    pv(v_ops[NB - 1], s[NB - 1]);
   }
-
+  wait_vm<0>();
   if (zeroes) zero_rows_past(a, w);
 
-  // ---- the key groups' results, joined pairwise into the first one's ----
-  wait_vm<0>();
+  // ---- the key groups' results: each group sums its share of the dims ----
+  float l = l_run + other_half(l_run);
+  constexpr int kMine = 4 / KG;  // 32-dim blocks: kMine * kg ..
+  f32x16 res[kMine];
   if constexpr (KG > 1) {
+    if (h == 0) join_ml[wave * 32 + c] = f32x2{m_run, l};
+    meet();  // (all reads of the tiles are done, too)
+    float m = kNegBig;
+    f32x2 ml[KG];
 #pragma unroll
-    for (int step = KG / 2; step >= 1; step /= 2) {
-      meet();
-      if (kg >= step && kg < 2 * step) {
-        const int at = (kg - step) * R + rg;  // 0 or 1
-        float* o = reinterpret_cast<float*>(at ? lds_v : lds_k);
+    for (int g = 0; g < KG; ++g) {
+      ml[g] = join_ml[(g * R + rg) * 32 + c];
+      m = fmaxf(m, ml[g][0]);
+    }
+    const float f = __builtin_amdgcn_exp2f(m_run - m);
+    m_run = m;
+    l = 0.0f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+    for (int g = 0; g < KG; ++g) l += ml[g][1] * __builtin_amdgcn_exp2f(ml[g][0] - m);
+    // a 4 KB block to each group's summands from the others
+    auto at = [&](int to, int i, int from) {  // (from != to; i: the block of the group's)
+      const int n = ((to * kMine + i) * (KG - 1) + from - (from > to)) * R + rg;
+      return reinterpret_cast<u32x4*>((n < kBuf / 4096 ? lds_k : lds_v - kBuf) + n * 4096) + lane;
+    };
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[(16 * b + e) * 64 + lane] = acc[b][e];
-        join_ml[(at * 64 + lane) * 2] = m_run;
-        join_ml[(at * 64 + lane) * 2 + 1] = l_run;
-      }
-      meet();
-      if (kg < step) {
-        const int at = kg * R + rg;
-        const float* o = reinterpret_cast<const float*>(at ? lds_v : lds_k);
-        const float m = join_ml[(at * 64 + lane) * 2], l = join_ml[(at * 64 + lane) * 2 + 1];
-        const float m_new = fmaxf(m, m_run);
-        const float fa = __builtin_amdgcn_exp2f(m_run - m_new), fb = __builtin_amdgcn_exp2f(m - m_new);
-        m_run = m_new;
-        l_run = l_run * fa + l * fb;
+    for (int b = 0; b < 4; ++b) {
+      acc[b] *= f;
+      if (b / kMine != kg) {
+        u32x4* const o = at(b / kMine, b % kMine, kg);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[b][e] = acc[b][e] * fa + o[(16 * b + e) * 64 + lane] * fb;
+        for (int e = 0; e < 16; e += 4)
+          o[e * 16] = u32x4{__float_as_uint(acc[b][e]), __float_as_uint(acc[b][e + 1]), __float_as_uint(acc[b][e + 2]),
+                            __float_as_uint(acc[b][e + 3])};
       }
     }
-    if (kg > 0) return;
+    meet();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      f32x16 mine = acc[i];
+#pragma unroll
+      for (int g = 1; g < KG; ++g) mine = kg == g ? acc[g * kMine + i] : mine;
+      res[i] = f32x16{};
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {  // (in the groups' order for each)
+        if (g == kg) {
+          res[i] += mine;
+        } else {
+          const u32x4* const o = at(kg, i, g);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) res[i][e] += __uint_as_float(o[(e & 12) * 16][e & 3]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) res[i] = acc[i];
   }
-  const float l = l_run + other_half(l_run);
   if (!row_ok) return;
   if (split) {
     const int64_t at = ((int64_t)place.unit * a.num_kv_heads + w.kvh) * a.row_cap + row;
-    float* o = a.ws_o + at * kHeadDim;
+    float* o = a.ws_o + at * kHeadDim + 32 * kMine * kg + 4 * h;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int i = 0; i < kMine; ++i)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        st16(o + 32 * b + 2 * e + 4 * h, u32x4{__float_as_uint(acc[b][e]), __float_as_uint(acc[b][e + 1]),
-                                              __float_as_uint(acc[b][e + 2]), __float_as_uint(acc[b][e + 3])});
-    if (h == 0) {
-      a.ws_ml[2 * at] = m_run;
-      a.ws_ml[2 * at + 1] = l;
-    }
+        st16(o + 32 * i + 2 * e, u32x4{__float_as_uint(res[i][e]), __float_as_uint(res[i][e + 1]),
+                                       __float_as_uint(res[i][e + 2]), __float_as_uint(res[i][e + 3])});
+    if (h == 0 && kg == 0) *reinterpret_cast<f32x2*>(a.ws_ml + 2 * at) = f32x2{m_run, l};
     return;
   }
   float norm = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) norm *= load_uniform_f32(a.v_scale);
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
+  for (int i = 0; i < kMine; ++i) {
+    const int b = kMine * kg + i;
     if (PAIR && (b >> 1) != (int)hi) continue;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const float x[4] = {acc[b][e] * norm, acc[b][e + 1] * norm, acc[b][e + 2] * norm, acc[b][e + 3] * norm};
+      const float x[4] = {res[i][e] * norm, res[i][e + 1] * norm, res[i][e + 2] * norm, res[i][e + 3] * norm};
       store4(a.out, a.q_dtype, q_off + 32 * (PAIR ? b & 1 : b) + 2 * e + 4 * h, x);
     }
   }
@@ -920,61 +1025,108 @@ __global__ __launch_bounds__(64 * R * KG) __attribute__((amdgpu_waves_per_eu(2))
   tree_attention_body<KV_DT, R, KG, PAIR>(a);
 }
 
-// Rows of sequences in several splits: a wave a row, two dims a lane.
-constexpr int kJoinWaves = 4;
-template <int UNIT, bool FP8, bool PAIR>
-__global__ __launch_bounds__(64 * kJoinWaves) void tree_join_kernel(TreeArgs a) {
-  const Work w = find_work(a, blockIdx.x / a.num_kv_heads, blockIdx.x % a.num_kv_heads);
-  int first, n;
-  Units<UNIT>(a).of_sequence(w.seq, first, n);
+// Rows of sequences in several splits: half a wave two rows, four dims a lane.
+// Z waves of a workgroup share the splits of their rows.
+template <int Z>
+constexpr int kJoinRows = 16 / Z;  // a workgroup
+MKV_DEV float half_max(float x) {  // of the 32 lanes
+  auto get = [&](auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x = fmaxf(x, get(std::integral_constant<int, 0xB1>{}));   // lane ^ 1, ^ 2, then within 8, 16
+  x = fmaxf(x, get(std::integral_constant<int, 0x4E>{}));
+  x = fmaxf(x, get(std::integral_constant<int, 0x141>{}));
+  x = fmaxf(x, get(std::integral_constant<int, 0x140>{}));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int UNIT, int Z, bool FP8, bool PAIR>
+MKV_DEV void tree_join_body(const TreeArgs& a) {
+  constexpr int kAhead = 4;  // splits whose loads are in flight
+  Place place;
+  place.kvh = blockIdx.x % a.num_kv_heads;
+  const int n = Units<UNIT>(a).of_sequence(blockIdx.x / a.num_kv_heads, place);
   if (n <= 1) return;
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.y * kJoinWaves + uniform(threadIdx.x >> 6);
-  if (row >= w.rows) return;
-  const int64_t at = ((int64_t)first * a.num_kv_heads + w.kvh) * a.row_cap + row, step = (int64_t)a.num_kv_heads * a.row_cap;
-  // the largest maximum first (a lane a split), then the sums, eight splits'
-  // loads in flight
-  float m = kNegBig;
-  for (int z = lane; z < n; z += 64) m = fmaxf(m, a.ws_ml[2 * (at + z * step)]);
+  const Work w = find_work(a, place);
+  const int c = threadIdx.x & 31, wave = uniform(threadIdx.x >> 6);
+  const int row0 = blockIdx.y * kJoinRows<Z> + 2 * ((wave / Z) * 2 + (threadIdx.x >> 5 & 1));
+  if (blockIdx.y * kJoinRows<Z> >= w.rows || (Z == 1 && row0 >= w.rows)) return;
+  const bool one = row0 < w.rows, two = row0 + 1 < w.rows;
+  const int64_t at = ((int64_t)place.unit * a.num_kv_heads + w.kvh) * a.row_cap + (one ? row0 : 0),
+                step = (int64_t)a.num_kv_heads * a.row_cap;
+  const float* const ml = a.ws_ml + 2 * at;
+  const float* const o = a.ws_o + at * kHeadDim + 4 * c;
+  f32x2 x_ml[2][kAhead];
+  f32x4 x_o[2][kAhead];
+  auto load = [&](int z0) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  float l = 0.0f, x = 0.0f, y = 0.0f;
-  for (int z0 = 0; z0 < n; z0 += 8) {
-    f32x2 ml[8], o[8];
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = min(z0 + j, n - 1) * step;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t i = at + min(z0 + j, n - 1) * step;
-      ml[j] = *reinterpret_cast<const f32x2*>(a.ws_ml + 2 * i);
-      o[j] = *reinterpret_cast<const f32x2*>(a.ws_o + i * kHeadDim + 2 * lane);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (z0 + j < n) {
-        const float f = __builtin_amdgcn_exp2f(ml[j][0] - m);
-        l += ml[j][1] * f;
-        x += o[j][0] * f;
-        y += o[j][1] * f;
+      for (int r = 0; r < 2; ++r) {
+        x_ml[r][j] = *reinterpret_cast<const f32x2*>(ml + 2 * (i + (r && two)));
+        x_o[r][j] = *reinterpret_cast<const f32x4*>(o + (i + (r && two)) * kHeadDim);
       }
     }
+  };
+  load(wave % Z * kAhead);
+  float m[2] = {kNegBig, kNegBig}, l[2] = {0.0f, 0.0f};
+  f32x4 sum[2] = {};
+  for (int z = c; z < n; z += 32) {  // the largest maximum first, a lane a split
+    m[0] = fmaxf(m[0], ml[2 * z * step]);
+    m[1] = fmaxf(m[1], ml[2 * (z * step + two)]);
   }
-  float norm = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-  if constexpr (FP8) norm *= load_uniform_f32(a.v_scale);
-  bool hi = false;
-  int64_t off = row_offset<PAIR>(a, w, row, hi);
-  int d = 2 * lane;
-  if constexpr (PAIR) {
-    if ((d >= 64) != hi) return;
-    d &= 63;
+  m[0] = half_max(m[0]);
+  m[1] = half_max(m[1]);
+  for (int z0 = wave % Z * kAhead; z0 < n; z0 += Z * kAhead) {
+    if (z0 >= Z * kAhead) load(z0);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (z0 + j < n) {
+          const float f = __builtin_amdgcn_exp2f(x_ml[r][j][0] - m[r]);
+          l[r] += x_ml[r][j][1] * f;
+          sum[r] += x_o[r][j] * f;
+        }
+      }
   }
-  off += d;
-  if (a.q_dtype == MKV_DTYPE_F32) {
-    reinterpret_cast<float*>(a.out)[off] = x * norm;
-    reinterpret_cast<float*>(a.out)[off + 1] = y * norm;
-  } else {
-    const uint32_t b0 = a.q_dtype == MKV_DTYPE_BF16 ? f32_to_bf16_bits(x * norm) : f32_to_f16_bits(x * norm);
-    const uint32_t b1 = a.q_dtype == MKV_DTYPE_BF16 ? f32_to_bf16_bits(y * norm) : f32_to_f16_bits(y * norm);
-    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + off) = b0 | b1 << 16;
+  if constexpr (Z > 1) {
+    __shared__ f32x4 part[Z - 1][2][64];
+    __shared__ float part_l[Z - 1][2][64];
+    const int lane = threadIdx.x & 63;
+    if (wave > 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        part[wave - 1][r][lane] = sum[r];
+        part_l[wave - 1][r][lane] = l[r];
+      }
+    }
+    __syncthreads();
+    if (wave > 0 || !one) return;
+#pragma unroll
+    for (int z = 1; z < Z; ++z)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        sum[r] += part[z - 1][r][lane];
+        l[r] += part_l[z - 1][r][lane];
+      }
   }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if (r && !two) return;
+    float norm = l[r] > 0.0f ? 1.0f / l[r] : l[r] == 0.0f ? 0.0f : l[r];
+    if constexpr (FP8) norm *= load_uniform_f32(a.v_scale);
+    bool hi = false;
+    const int64_t off = row_offset<PAIR>(a, w, row0 + r, hi);
+    if (PAIR && (c >= 16) != hi) continue;
+    const float x[4] = {sum[r][0] * norm, sum[r][1] * norm, sum[r][2] * norm, sum[r][3] * norm};
+    store4(a.out, a.q_dtype, off + 4 * (PAIR ? c & 15 : c), x);
+  }
+}
+template <int UNIT, int Z, bool FP8, bool PAIR>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
+  tree_join_body<UNIT, Z, FP8, PAIR>(a);
 }
 
 // fp32 caches: products and sums in fp32 on the 32x32x2 fp32 MFMA, one row
@@ -989,7 +1141,7 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   Place place;
   if (!find_place<NK>(a, place)) return;
   const int len = place.len;
-  const Work w = find_work(a, place.seq, place.kvh);
+  const Work w = find_work(a, place);
   if (place.rb == 0 && place.z == 0 && w.kvh == 0) zero_rows_past(a, w);
   if (place.rb * 32 >= w.rows) return;
   const int kb0 = place.z * len, k1 = (int)min((int64_t)kb0 + len, (int64_t)w.ctx);
@@ -1184,17 +1336,17 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   Plan p;
   const int64_t toks = mask_cols < total_q ? mask_cols : total_q;
   const int64_t rows = toks * kernel_group;
-  p.row_groups = f32 || rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  p.row_groups = f32 || rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   p.row_blocks = (int)((rows + 32 * p.row_groups - 1) / (32 * p.row_groups));
   if (p.row_blocks < 1) p.row_blocks = 1;
   p.row_cap = p.row_blocks * 32 * p.row_groups;
-  p.unit = p.row_groups == 1 ? 128 : 64;
-  // Workgroups that run at once: two a CU of four waves, one of eight.  Where the
-  // sequences leave some free, their keys are dealt out so that all fit one round
-  // (a sequence's last split may be short: num_seqs shares are kept back); where
-  // they do not fit a round, in pieces of a quarter round; many sequences split
-  // only those of more than twice the mean.
-  const int64_t slots = p.row_groups == 8 ? 256 : 512;
+  p.unit = p.row_groups == 4 ? 64 : 128;
+  // Workgroups that run at once: two a CU.  Where the sequences leave some free,
+  // their keys are dealt out so that all fit one round (a sequence's last split may
+  // be short: num_seqs shares are kept back); where they do not fit a round, in
+  // pieces of a quarter round; many sequences split only those of more than twice
+  // the mean.
+  const int64_t slots = 512;
   const int64_t round = slots / ((int64_t)kernel_kv_heads * p.row_blocks) > 0 ? slots / ((int64_t)kernel_kv_heads * p.row_blocks) : 1;
   int64_t shares;
   if (num_seqs <= round)
@@ -1224,18 +1376,25 @@ int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
     switch (p.row_groups) {
       case 1: hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_kernel<KV_DT, 1, 4, PAIR>), grid, dim3(256), 0, s, a); break;
       case 2: hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_kernel<KV_DT, 2, 2, PAIR>), grid, dim3(256), 0, s, a); break;
-      case 4: hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_kernel<KV_DT, 4, 1, PAIR>), grid, dim3(256), 0, s, a); break;
-      default: hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_kernel<KV_DT, 8, 1, PAIR>), grid, dim3(512), 0, s, a); break;
+      default: hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_attention_kernel<KV_DT, 4, 1, PAIR>), grid, dim3(256), 0, s, a); break;
     }
   }
   if (hipError_t e = hipGetLastError()) return (int)e;
   if (p.splits) {
     constexpr bool kFp8 = KV_DT == MKV_DTYPE_FP8E4M3;
-    const dim3 jgrid((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)((p.row_cap + kJoinWaves - 1) / kJoinWaves));
+    // (few sequences in many splits each: the waves share them)
+    auto join = [&](auto unit, auto z) {
+      constexpr int kUnit = decltype(unit)::value, kZ = decltype(z)::value;
+      const dim3 jgrid((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)((p.row_cap + kJoinRows<kZ> - 1) / kJoinRows<kZ>));
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<kUnit, kZ, kFp8, PAIR>), jgrid, dim3(256), 0, s, a);
+    };
+    using I1 = std::integral_constant<int, 1>;
+    using I4 = std::integral_constant<int, 4>;
+    const bool many = p.units >= 8 * (int64_t)a.num_seqs && p.row_cap <= 4096;
     if (p.unit == 128)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<128, kFp8, PAIR>), jgrid, dim3(64 * kJoinWaves), 0, s, a);
+      many ? join(std::integral_constant<int, 128>{}, I4{}) : join(std::integral_constant<int, 128>{}, I1{});
     else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<64, kFp8, PAIR>), jgrid, dim3(64 * kJoinWaves), 0, s, a);
+      many ? join(std::integral_constant<int, 64>{}, I4{}) : join(std::integral_constant<int, 64>{}, I1{});
     return (int)hipGetLastError();
   }
   return MKV_OK;
@@ -1303,7 +1462,7 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
     return MKV_ERR_MISALIGNED;
   int kv;
   const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, kv);
-  if (p.units * kv * p.row_blocks > 0x7fffffff || p.row_cap / kJoinWaves > 65535) return MKV_ERR_BAD_SHAPE;
+  if (p.units * kv * p.row_blocks > 0x7fffffff || p.row_cap / kJoinRows<1> > 65535) return MKV_ERR_BAD_SHAPE;
   if (workspace_of(p, kv) > workspace_bytes || (p.splits && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
   const int pair = head_dim == 64 ? 2 : 1;
   TreeArgs a;
