@@ -612,7 +612,8 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         raise TypeError(f"query {query.dtype} and cache {k_cache.dtype} must share a dtype")
     bt = _block_table(block_tables)
     cl = _ctx_lens(context_lens)
-    cu = cu_seqlens_q.to(torch.int32).contiguous()
+    cu = cu_seqlens_q if cu_seqlens_q.dtype == torch.int32 else cu_seqlens_q.to(torch.int32)
+    cu = cu.contiguous()
     total, num_seqs = query.shape[0], cl.numel()
     if tree_mask.dtype not in (torch.bool, torch.uint8):
         raise TypeError(f"tree_mask must be bool or uint8, got {tree_mask.dtype}")

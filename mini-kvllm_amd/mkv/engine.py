@@ -44,6 +44,7 @@ from . import _lib
 from . import context as C
 from .attention import DECODE_STREAM, DECODE_WORKGROUP, Attention, _dtype_code, _stream
 from .decode_state import DecodeGraphs, DecodeMetadata
+from .logprobs import MAX_TOP, token_logprobs
 from .producer import qkv_norm_rope_append, qkv_norm_rope_append_decode
 
 _is_tracing = torch._C._is_tracing
@@ -72,6 +73,10 @@ class Request:
     num_cached: int = 0
     blocks: list[int] = field(default_factory=list)
     finished: bool = False
+    # alternatives to report with each generated token's log probability (None:
+    # neither), and what was reported: one TokenReport a generated token
+    logprobs: int | None = None
+    reports: list["TokenReport"] = field(default_factory=list)
 
     @property
     def num_generated(self) -> int:
@@ -83,6 +88,17 @@ class Request:
         tokens) are still to be computed; a decode step feeds exactly the last
         token."""
         return self.num_cached < len(self.tokens) - 1
+
+
+@dataclass(frozen=True)
+class TokenReport:
+    """A generated token's log probability, the entropy of the distribution
+    it was drawn from (in nats) and its likeliest tokens with their log
+    probabilities.  The distribution is the model's, at temperature 1."""
+
+    logprob: float
+    entropy: float
+    top: list[tuple[int, float]]
 
 
 @dataclass(frozen=True)
@@ -608,10 +624,16 @@ class Engine:
         self._pin_temp = torch.ones(self.max_rows, dtype=torch.float32).pin_memory()
 
     def add_request(self, prompt: list[int], max_tokens: int, ignore_eos: bool = True,
-                    temperature: float = 1.0) -> Request:
+                    temperature: float = 1.0, logprobs: int | None = None) -> Request:
+        """Queue a prompt.  ``logprobs``: report every generated token's log
+        probability and that many of its likeliest alternatives (0 to 64) in
+        ``Request.reports``."""
         if len(prompt) + max_tokens > self.max_blocks * self.bs:
             raise ValueError("prompt + max_tokens exceeds max_model_len")
-        req = Request(self._next_id, len(prompt), list(prompt), max_tokens, ignore_eos, temperature)
+        if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, self.model.cfg.vocab_size):
+            raise ValueError(f"logprobs {logprobs} outside 0..{min(MAX_TOP, self.model.cfg.vocab_size)}")
+        req = Request(self._next_id, len(prompt), list(prompt), max_tokens, ignore_eos, temperature,
+                      logprobs=logprobs)
         self._next_id += 1
         self.sched.add(req)
         return req
@@ -704,6 +726,19 @@ class Engine:
         self._loaded_lens = [len(r.tokens) for r in reqs]
         return tok
 
+    def _report(self, items: list[Scheduled], tok: torch.Tensor) -> None:
+        """The reports of a step's sampled tokens, for the requests that want
+        them: one pass over the logits that the tokens were drawn from."""
+        reqs = [s.req for s in items if s.samples]
+        if all(r.logprobs is None for r in reqs):
+            return
+        r = token_logprobs(self.last_logits, tok, max(r.logprobs or 0 for r in reqs))
+        logprob, entropy, top_lp, top_id = (x.tolist() for x in r)
+        for i, req in enumerate(reqs):
+            if req.logprobs is not None:
+                top = list(zip(top_id[i], top_lp[i]))[:req.logprobs]
+                req.reports.append(TokenReport(logprob[i], entropy[i], top))
+
     def step(self) -> list[Request]:
         items = self.sched.schedule()
         if not items:
@@ -715,6 +750,7 @@ class Engine:
         else:
             tok = self._run_mixed(items)
             self._rows = []  # decode rows must be reloaded before the next captured step
+        self._report(items, tok)
         sampled = tok.cpu().tolist()
         self.last_sampled = sampled
         dt = time.perf_counter() - t0

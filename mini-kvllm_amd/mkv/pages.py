@@ -46,23 +46,24 @@ class CachePages:
         self.num_blocks, self.block_size = shape
         if self.block_size & (self.block_size - 1):
             raise ValueError(f"block_size must be a power of two; got {self.block_size}")
-        spans = []
+        tokens = self.num_blocks * self.block_size
+        ptrs, rows = [], []
         for t in self.caches:
             if t.shape[:2] != shape:
                 raise ValueError(f"cache tensors of {tuple(t.shape[:2])} and {tuple(shape)} blocks and rows")
             if not t.is_contiguous():
                 raise ValueError("cache tensors must be contiguous")
-            nbytes = t.numel() * t.element_size()
-            if nbytes == 0 or nbytes // (self.num_blocks * self.block_size) % 4 or t.data_ptr() % 4:
+            ptr, row = t.data_ptr(), t.nbytes // tokens
+            if row == 0 or row % 4 or ptr % 4:
                 raise ValueError(f"a token's row must be a multiple of 4 bytes; got {tuple(t.shape)} {t.dtype}")
-            spans.append((t.data_ptr(), nbytes))
-        spans.sort()
-        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            ptrs.append(ptr)
+            rows.append(row)
+        spans = sorted(zip(ptrs, rows))
+        if any(a + n * tokens > b for (a, n), (b, _) in zip(spans, spans[1:])):
             raise ValueError("cache tensors overlap")
-        n = len(self.caches)
-        self._ptrs = (ctypes.c_void_p * n)(*(t.data_ptr() for t in self.caches))
-        self._rows = (ctypes.c_int64 * n)(*(t.numel() * t.element_size() // (self.num_blocks * self.block_size)
-                                            for t in self.caches))
+        n = len(ptrs)
+        self._ptrs = (ctypes.c_void_p * n)(*ptrs)
+        self._rows = (ctypes.c_int64 * n)(*rows)
         self._pools = (ctypes.addressof(self._ptrs), ctypes.addressof(self._rows), n, self.num_blocks, self.block_size)
 
     def copy(self, src: torch.Tensor | Sequence[int], dst: torch.Tensor | Sequence[int]) -> None:
