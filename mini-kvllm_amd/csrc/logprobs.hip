@@ -14,6 +14,12 @@
 // the k-th largest logit from below, so only the threads' logits that reach it
 // are read again (a few dozen of the vocabulary).  Selecting in pass 1 would cost
 // its workgroups as many VALU cycles again as the whole softmax.
+//
+// A vocabulary that one workgroup holds (up to 8185) takes one launch: a workgroup
+// a row, one wave where 2041 logits or fewer leave no work for four.  There the k-th
+// largest key is found by bisection over all of the row's keys, in registers
+// (4096 rows of 2000 bf16 logits, top 64: 23 us against 59 in two launches; 8 or 16 waves a row for
+// larger vocabularies were slower than two launches at any number of rows).
 #include <type_traits>
 
 #include "mkv_device.hpp"
@@ -106,6 +112,10 @@ struct Pieces {
   }
   static constexpr int kVec = DT == MKV_DTYPE_F32 ? 4 : 8;
   static constexpr int kNum = kPer / kVec;
+  template <int T>
+  MKV_DEV static int64_t start_of(int j, int tid, int shift) {  // one chunk, of T threads
+    return (j * T + tid) * kVec - shift;
+  }
   MKV_DEV static int shift(const char* row) {
     return (int)((reinterpret_cast<uintptr_t>(row) & 15) / (16 / kVec));
   }
@@ -443,10 +453,199 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   }
 }
 
+// Rows that a workgroup of W waves holds, PER logits a thread.
+template <int DT, int W, int PER>
+__global__ __launch_bounds__(64 * W) void logprobs_whole_kernel(LpArgs a) {
+  using P = Pieces<DT>;
+  constexpr int T = 64 * W, kPieces = PER / P::kVec;
+  __shared__ Stat part[W];
+  __shared__ uint32_t counts[2][W];
+  __shared__ uint64_t cand[kMaxTop];
+  __shared__ int places[kMaxTop], fill;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x;
+  const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * (16 / P::kVec);
+  const int shift = P::shift(row);
+  float given = 0.0f;
+  int64_t id = -1;
+  if (tid < a.num_ids) {
+    id = load_index(a.ids, r * a.ids_stride + tid, a.ids_i64);
+    if (id >= 0 && id < a.vocab) given = logit_at<DT>(row, id);
+  }
+  float x[PER];
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) P::load(row, P::template start_of<T>(j, tid, shift), a.vocab, x + j * P::kVec);
+  if (tid == 0) fill = 0;
+  float own = x[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) own = maximum(own, x[i]);
+  Stat w{wave_max(own), 0.0f, 0.0f};  // as in the first pass
+  if (w.m != -__builtin_huge_valf()) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float d = maximum(x[i] - w.m, -200.0f);
+      const float e = __builtin_amdgcn_exp2f(d * kLog2e);
+      w.s += e;
+      w.t = __builtin_fmaf(e, d, w.t);
+    }
+  }
+  w.s = wave_sum(w.s);
+  w.t = wave_sum(w.t);
+  if constexpr (W > 1) {
+    if (lane == 0) part[wave] = w;
+    __syncthreads();
+    w = part[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) w = join(w, part[i]);
+  }
+  const float m = w.m, s = m != m ? m : w.s, t = m != m ? m : w.t;
+  const float log_s = logf(s);
+  if (tid == 0) a.entropy[r] = log_s - t / s;
+  for (int i = tid; i < a.num_ids; i += T) {
+    if (i >= T) {
+      id = load_index(a.ids, r * a.ids_stride + i, a.ids_i64);
+      if (id >= 0 && id < a.vocab) given = logit_at<DT>(row, id);
+    }
+    a.logprobs[r * a.num_ids + i] = id < 0 ? 0.0f : id < a.vocab ? (given - m) - log_s : __builtin_nanf("");
+  }
+  if (a.top == 0) return;
+
+  const int k = a.top;
+  uint32_t key[PER], best = 0;  // (0: outside the row)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t at = P::template start_of<T>(i / P::kVec, tid, shift) + i % P::kVec;
+    key[i] = at >= 0 && at < a.vocab ? P::key(x[i]) : 0u;
+    best = max(best, key[i]);
+  }
+  int turn = 0;
+  auto total = [&](uint32_t n) -> int {  // over the waves
+    if constexpr (W > 1) {
+      if (lane == 0) counts[turn][wave] = n;
+      __syncthreads();
+      n = 0;
+#pragma unroll
+      for (int v = 0; v < W; ++v) n += counts[turn][v];
+      turn ^= 1;  // (the other half is free again: everyone has passed a barrier since)
+    }
+    return (int)n;
+  };
+  // the number of the workgroup's keys that reach `from`
+  auto reach = [&](uint32_t from) -> int {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      n += __popcll(__builtin_amdgcn_ballot_w64(key[i] >= from));
+      asm volatile("" : "+s"(n));  // (one ballot's registers at a time)
+    }
+    return total(n);
+  };
+  // The k-th largest key, lo: the k-th largest of a wave's best is at most that
+  // where the wave holds k.
+  uint32_t hi = best, least = best;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+    least = min(least, (uint32_t)__shfl_xor((int)least, o));
+  }
+  if constexpr (W > 1) {
+    __shared__ uint32_t tops[W], leasts[W];
+    if (lane == 0) {
+      tops[wave] = hi;
+      leasts[wave] = least;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      hi = max(hi, tops[v]);
+      least = max(least, leasts[v]);
+    }
+  }
+  uint32_t lo = max(least, 1u);
+  int reached = reach(lo);
+  if (reached > k) {
+    const int n = reach(hi);
+    if (n >= k) {
+      lo = hi;
+      reached = n;
+    }
+    while (reached > k && hi - lo > 1) {  // reached = those at lo or above; fewer than k at hi
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int n_mid = reach(mid);
+      if (n_mid >= k) {
+        lo = mid;
+        reached = n_mid;
+      } else {
+        hi = mid;
+      }
+    }
+  }
+  uint32_t above = 0, equal = 0;  // a bit a logit
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    above |= (uint32_t)(key[i] > lo) << i;
+    equal |= (uint32_t)(key[i] == lo) << i;
+  }
+  auto place = [&](int i) { return (int)P::template start_of<T>(i / P::kVec, tid, shift) + i % P::kVec; };
+  if (reached > k) {
+    // the first of the equal logits: those below place `end` (a thread's places
+    // rise with i)
+    auto below = [&](int end) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) n += min(max(end - place(j * P::kVec), 0), P::kVec);
+      return equal & (uint32_t)((1ull << n) - 1);
+    };
+    auto sum = [&](uint32_t bits) { return total((uint32_t)wave_sum((float)__popc(bits))); };
+    const int need = k - sum(above);
+    int begin = 0, end = a.vocab;  // fewer than need below begin, need or more below end
+    while (end - begin > 1) {
+      const int mid = begin + (end - begin) / 2;
+      const int n = sum(below(mid));
+      if (n >= need) end = mid;
+      else begin = mid;
+      if (n == need) break;
+    }
+    equal = below(end);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if ((above | equal) >> i & 1) {
+      const int at = atomicAdd(&fill, 1);
+      if (at < k) places[at] = place(i);
+    }
+  __syncthreads();
+  // a candidate's place is the number of larger ones (its logit comes from the row
+  // again: the logits' registers hold the keys since)
+  uint64_t mine = 0;
+  if (tid < k) cand[tid] = mine = key_of(logit_at<DT>(row, places[tid]), places[tid]);
+  __syncthreads();
+  if (tid < k) {
+    int rank = 0;
+    for (int j = 0; j < k; ++j) rank += cand[j] > mine;
+    a.top_ids[r * k + rank] = (int)~(uint32_t)mine;
+    a.top_logprobs[r * k + rank] = (value_of((uint32_t)(mine >> 32)) - m) - log_s;
+  }
+}
+
 int chunks_of(int vocab) { return (int)(((int64_t)vocab + 7 + kChunk - 1) / kChunk); }
 
 template <int DT>
 int launch_logprobs(const LpArgs& a, hipStream_t s) {
+  if (a.chunks == 1) {
+    const int64_t held = a.vocab + 7;  // (a row's start may leave 7 places empty)
+    auto whole = [&](auto w, auto per) {
+      constexpr int W = decltype(w)::value, kPerThread = decltype(per)::value;
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_whole_kernel<DT, W, kPerThread>), dim3((unsigned)a.rows), dim3(64 * W), 0, s, a);
+      return (int)hipGetLastError();
+    };
+    using I1 = std::integral_constant<int, 1>;
+    using I4 = std::integral_constant<int, 4>;
+    if (held <= 64 * 8) return whole(I1{}, std::integral_constant<int, 8>{});
+    if (held <= 64 * kPer) return whole(I1{}, std::integral_constant<int, kPer>{});
+    return whole(I4{}, std::integral_constant<int, kPer>{});
+  }
   const int64_t y = a.rows < 32768 ? a.rows : 32768;
   hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_chunk_kernel<DT>),
                      dim3(a.chunks, (unsigned)y, (unsigned)((a.rows + 32767) / 32768)), dim3(kLpThreads), 0, s, a);
@@ -462,6 +661,7 @@ using namespace mkv;
 
 extern "C" size_t mkv_token_logprobs_workspace_size(int64_t rows, int vocab, int top) {
   if (rows <= 0 || vocab <= 0) return 0;
+  if (chunks_of(vocab) == 1) return 256;  // (not used: one launch)
   // (4 bytes a key: enough for every type)
   return (size_t)rows * chunks_of(vocab) * (4 + (top > 0 ? kLpThreads : 0)) * sizeof(float);
 }
