@@ -1129,13 +1129,21 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
   tree_join_body<UNIT, Z, FP8, PAIR>(a);
 }
 
-// fp32 caches: products and sums in fp32 on the 32x32x2 fp32 MFMA, one row
-// group of 32 rows and four key groups.  Lane (c, h) supplies K[key c][64h + st]
-// and q[row c][64h + st] at step st, and for O^T its own keys' P again.
+// fp32 caches: products and sums in fp32 on the 32x32x2 fp32 MFMA, one row group
+// of 32 rows and four key groups, each of which loads its own 32 keys of a tile and
+// meets the others at the end alone.  Lane (c, h) supplies K[key c][64h + st] and
+// q[row c][64h + st] at step st, and for O^T its own keys' P again.  A tile's 128
+// MFMAs a wave (8192 cycles) and its 128 KB a CU take about as long as each other:
+// K and V have a buffer each, whose next tile goes out as soon as its last operands
+// are read, and one workgroup fills a CU's LDS (60 sequences of 300-800 keys with 16
+// drafted tokens, 8 KV heads: 102 us, 2.9 TB/s; with one buffer and four barriers a
+// tile 248 us).
+// LDS rows of 512 bytes, 16-byte chunk i at i ^ swz(key): one-to-one on 16 keys (K
+// operands), and keys 4 apart in the two halves of 256 bytes (V's).
 template <bool PAIR>
-__global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
-  constexpr int KG = 4, NK = 128, kRow = 528;  // 512-byte rows, 16 bytes apart in the banks
-  __shared__ __align__(16) char lds[NK * kRow];
+MKV_DEV void tree_attention_f32_body(const TreeArgs& a) {
+  constexpr int KG = 4, TK = 32, NK = TK * KG, kRow = 4 * kHeadDim, kDma = TK * kRow / 1024, kSubs = TK / 16;
+  __shared__ __align__(16) char lds_k[NK * kRow], lds_v[NK * kRow];
   const int tid = threadIdx.x, lane = tid & 63, kg = uniform(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
   Place place;
@@ -1145,6 +1153,7 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   if (place.rb == 0 && place.z == 0 && w.kvh == 0) zero_rows_past(a, w);
   if (place.rb * 32 >= w.rows) return;
   const int kb0 = place.z * len, k1 = (int)min((int64_t)kb0 + len, (int64_t)w.ctx);
+  const int prefix = (int)min(w.prefix, (int64_t)0x7fffffff);
   const bool split = w.ctx > len;
   const int row = place.rb * 32 + c;
   const bool row_ok = row < w.rows;
@@ -1154,114 +1163,162 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   float qv[64];
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
-    u32x4 v{0, 0, 0, 0};
-    if (row_ok && (!PAIR || h == (int)hi)) v = ld16(reinterpret_cast<const float*>(a.q) + q_off + (PAIR ? 0 : 64 * h) + i);
+    const u32x4 v = ld16(reinterpret_cast<const float*>(a.q) + q_off + (PAIR ? 0 : 64 * h) + i);  // (within q for any row)
 #pragma unroll
     for (int j = 0; j < 4; ++j) qv[i + j] = __uint_as_float(v[j]);
   }
-  const int64_t row_elems = (int64_t)a.num_kv_heads * kHeadDim;
+
+  // ---- loads of tiles, as above: two keys a load, a sub-tile of 16 keys never
+  // across a block ----
+  const int64_t row_bytes = (int64_t)a.num_kv_heads * kRow;
+  const int64_t head_bytes = (int64_t)w.kvh * kRow;
+  const int own0 = kg * TK;
+  auto swz = [](int key) { return (key & 3) | (key & 4) << 1 | (key & 8) >> 1; };
+  uint32_t voff[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) voff[i] = (uint32_t)((2 * i + h) * row_bytes) + 16 * (c ^ swz(2 * i + h));
+  int32_t slot[kSubs], left[kSubs];
+  const int32_t* bt_row = a.idx.block_tables + (int64_t)w.seq * a.idx.bt_stride;
+  auto entry_load = [&](int kb) -> int32_t {
+    const int blk = (kb + own0 + 16 * h) >> a.idx.bs_log2;
+    return bt_row[min(blk, a.idx.max_blocks - 1)];
+  };
+  auto entry_use = [&](int kb, int32_t e) {
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) {
+      const int t = kb + own0 + 16 * u;
+      const int phys = __builtin_amdgcn_readlane(e, 32 * u);
+      const bool ok = t < k1 && phys >= 0 && phys < (int)a.idx.num_blocks;
+      slot[u] = ok ? (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : 0;
+      left[u] = ok ? min(k1 - t, 16) : 0;
+    }
+  };
+  auto dma = [&](const char* pool, char* buf) {
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(pool + slot[u] * row_bytes + head_bytes), (short)0,
+          left[u] > 0 ? (int)((left[u] - 1) * row_bytes + kRow) : 0, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(buf + (own0 + u * 16) * kRow + i * 1024), 16, voff[i], 0, 0, 0);
+    }
+  };
+  int32_t e_ahead = 0;
+  if (kb0 < k1) {
+    e_ahead = entry_load(kb0);
+    const int32_t e_next = entry_load(kb0 + NK);
+    entry_use(kb0, e_ahead);
+    e_ahead = e_next;
+    dma(a.k, lds_k);
+    dma(a.v, lds_v);
+  }
+  const bool mine = row_ok && (!PAIR || h == (int)hi);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) qv[i] = mine ? qv[i] : 0.0f;
+
   const uint8_t* mask_row = a.mask + (w.q0 + (row_ok ? row / a.group : 0)) * a.mask_stride;
+  const int k_base = (own0 + c) * kRow + ((16 * h ^ swz(c)) << 4);
+  const int v_base = (own0 + 4 * h) * kRow + (((c >> 2) ^ 8 * h) << 4) + 4 * (c & 3);
   f32x16 acc[4];
 #pragma unroll
   for (int b = 0; b < 4; ++b) acc[b] = f32x16{};
   float m_run = kNegBig, l_run = 0.0f;
   for (int kb = kb0; kb < k1; kb += NK) {
+    wait_vm<kDma>();  // K is here, V may be on its way
     uint32_t present = 0;
-    int64_t slot[NK / 16];
 #pragma unroll
-    for (int u = 0; u < NK / 16; ++u) {
-      const int t = kb + 16 * u;
-      const int64_t phys = t < k1 ? a.idx.physical_block(w.seq, t >> a.idx.bs_log2) : -1;
-      present |= phys >= 0 ? 1u << u : 0u;
-      slot[u] = phys < 0 ? -1 : (phys << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1));
-    }
-    auto stage = [&](const char* pool) {
+    for (int u = 0; u < kSubs; ++u) present |= left[u] > 0 ? 1u << u : 0u;
+    const bool drafted = kb + own0 + TK > prefix;
+    uint32_t seen = 0xffffu;  // element e is key 8 (e >> 2) + 4h + (e & 3)
+    if (drafted || kb + own0 + TK > k1 || present != (1u << kSubs) - 1) {
 #pragma unroll
-      for (int u = 0; u < NK / 8; ++u) {  // 8 keys of 32 chunks a load
-        const int key = 8 * u + (tid >> 5);
-        u32x4 v{0, 0, 0, 0};
-        if (slot[u >> 1] >= 0 && kb + key < k1)
-          v = ld16(pool + ((slot[u >> 1] + (key & 15)) * row_elems + w.kvh * kHeadDim + 4 * (tid & 31)) * 4);
-        *reinterpret_cast<u32x4*>(lds + key * kRow + 16 * (tid & 31)) = v;
+      for (int e = 0; e < 16; ++e) {
+        const int kl = 8 * (e >> 2) + 4 * h + (e & 3), t = kb + own0 + kl, j = t - prefix;
+        bool vis = t < k1 && ((present >> (kl >> 4)) & 1);
+        if (vis && j >= 0) vis = row_ok && j < a.mask_cols && mask_row[j] != 0;
+        seen &= vis ? 0xffffu : ~(1u << e);
       }
-    };
-    __syncthreads();
-    stage(a.k);
-    __syncthreads();
-    f32x16 s = f32x16{};
-    const int key0 = 32 * kg;
-#pragma unroll
-    for (int i = 0; i < 64; i += 4) {
-      const u32x4 kw = *reinterpret_cast<const u32x4*>(lds + (key0 + c) * kRow + 256 * h + 4 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kw[j]), qv[i + j], s, 0, 0, 0);
     }
-    __syncthreads();
-    stage(a.v);
-    __syncthreads();
+    u32x4 kw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) kw[i] = *reinterpret_cast<const u32x4*>(lds_k + (k_base ^ i << 4));
+    f32x16 s = f32x16{}, s2 = f32x16{};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kw[i][j]), qv[4 * i + j], s, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kw[i][j + 1]), qv[4 * i + j + 1], s2, 0, 0, 0);
+      }
+    }
+    // ---- V is here; the next tile's K goes where this one's was ----
+    wait_vm<0>();
+    entry_use(kb + NK, e_ahead);
+    wait_lds();
+    dma(a.k, lds_k);
+    float v[4][16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        v[b][e] = *reinterpret_cast<const float*>(lds_v + (v_base ^ (8 * b ^ (e & 3) ^ (e & 4)) << 4) +
+                                                  (8 * (e >> 2) + (e & 3)) * kRow);
     float mx = kNegInf;
-    uint32_t seen = 0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int kl = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
-      const int64_t j = kb + kl - w.prefix;
-      bool vis = kb + kl < k1 && ((present >> (kl >> 4)) & 1);
-      if (vis && j >= 0) vis = row_ok && j < a.mask_cols && mask_row[j] != 0;
-      s[e] = vis ? s[e] * score_mul : kNegInf;
-      seen |= vis ? 1u << e : 0u;
+      s[e] = (seen >> e) & 1 ? (s[e] + s2[e]) * score_mul : kNegInf;
       mx = fmaxf(mx, s[e]);
     }
     mx = fmaxf(fmaxf(mx, other_half(mx)), kNegBig);
     const float m_new = fmaxf(mx, m_run);
-    const float alpha = m_run == kNegBig ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-    m_run = m_new;
-    l_run *= alpha;
+    if (__builtin_amdgcn_ballot_w64(m_new != m_run)) {
+      const float alpha = m_run == kNegBig ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[b][e] *= alpha;
-    float p[16];
+      for (int b = 0; b < 4; ++b) acc[b] *= alpha;
+    }
+    float p[16], sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(s[e] - m_new);
-      l_run += p[e];
+      p[e] = __builtin_amdgcn_exp2f(s[e] - m_run);
+      sum += p[e];
     }
-    auto v_at = [&](int e, int b) {
-      return *reinterpret_cast<const float*>(lds + (key0 + 8 * (e >> 2) + 4 * h + (e & 3)) * kRow + 4 * (32 * b + c));
-    };
-    bool found = false;
-    if (kb + key0 + 32 > w.prefix) {
-      for (int i = 0; i < 16; ++i) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(lds + (key0 + 2 * i + h) * kRow + 16 * c);
+    l_run += sum;
+    // ---- all of V is read: the next tile's goes where it was ----
+    wait_lds();
+    e_ahead = entry_load(kb + 2 * NK);
+    dma(a.v, lds_v);
+    if (drafted) {
+      bool found = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) found |= not_finite(__uint_as_float(v[j]));
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) found |= not_finite(v[b][e]);
+      if (__builtin_amdgcn_ballot_w64(found)) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          f32x16 marks = f32x16{};
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            marks = __builtin_amdgcn_mfma_f32_32x32x2f32(mark_of(v[b][e]), (seen >> e) & 1 ? 1.0f : 0.0f, marks, 0, 0, 0);
+            v[b][e] = not_finite(v[b][e]) ? 0.0f : v[b][e];
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[b][e] += marked_value(marks[e]);
+        }
       }
     }
-    const bool dirty = __builtin_amdgcn_ballot_w64(found) != 0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < 16; ++e)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float v = v_at(e, b);
-        if (dirty && not_finite(v)) v = 0.0f;
-        acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[e], acc[b], 0, 0, 0);
-      }
-    }
-    if (dirty) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        f32x16 marks = f32x16{};
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          marks = __builtin_amdgcn_mfma_f32_32x32x2f32(mark_of(v_at(e, b)), (seen >> e) & 1 ? 1.0f : 0.0f, marks, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          acc[b][e] += marked_value(marks[e]);
-      }
-    }
+      for (int b = 0; b < 4; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[b][e], p[e], acc[b], 0, 0, 0);
   }
+  wait_vm<0>();
   __syncthreads();
-  float* part = reinterpret_cast<float*>(lds);
+  float* part = reinterpret_cast<float*>(lds_k);
   static_assert((KG - 1) * 64 * 66 * 4 <= NK * kRow, "the join fits the tile");
   if (kg > 0) {
     float* o = part + (kg - 1) * 64 * 66;
@@ -1309,6 +1366,11 @@ __global__ __launch_bounds__(256) void tree_attention_f32_kernel(TreeArgs a) {
   }
 }
 
+template <bool PAIR>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void tree_attention_f32_kernel(TreeArgs a) {
+  tree_attention_f32_body<PAIR>(a);
+}
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -1341,12 +1403,12 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   if (p.row_blocks < 1) p.row_blocks = 1;
   p.row_cap = p.row_blocks * 32 * p.row_groups;
   p.unit = p.row_groups == 4 ? 64 : 128;
-  // Workgroups that run at once: two a CU.  Where the sequences leave some free,
-  // their keys are dealt out so that all fit one round (a sequence's last split may
-  // be short: num_seqs shares are kept back); where they do not fit a round, in
-  // pieces of a quarter round; many sequences split only those of more than twice
-  // the mean.
-  const int64_t slots = 512;
+  // Workgroups that run at once: two a CU (fp32: one).  Where the sequences leave
+  // some free, their keys are dealt out so that all fit one round (a sequence's last
+  // split may be short: num_seqs shares are kept back); where they do not fit a
+  // round, in pieces of a quarter round; many sequences split only those of more
+  // than twice the mean.
+  const int64_t slots = f32 ? 256 : 512;
   const int64_t round = slots / ((int64_t)kernel_kv_heads * p.row_blocks) > 0 ? slots / ((int64_t)kernel_kv_heads * p.row_blocks) : 1;
   int64_t shares;
   if (num_seqs <= round)
