@@ -10,15 +10,14 @@
 // chunk (m, s, t), joined by the usual rescaling, and the maximum of each
 // thread's 32 logits as a key in unsigned order (16 bits for 16-bit logits).
 // Pass 2, one workgroup a row, joins the chunks and finds the top k from those
-// maxima, held in registers: a value that at least k threads' maxima reach bounds
-// the k-th largest logit from below, so only the threads' logits that reach it
-// are read again (a few dozen of the vocabulary).  Selecting in pass 1 would cost
+// maxima, held in registers: a value that at least k of them reach bounds the k-th
+// largest logit from below, so only the threads' logits that reach it are read
+// again (a few dozen of the vocabulary).  Selecting in pass 1 would cost
 // its workgroups as many VALU cycles again as the whole softmax.
 //
 // A vocabulary that one workgroup holds (up to 8185) takes one launch: a workgroup
-// a row, one wave where 2041 logits or fewer leave no work for four.  There the k-th
-// largest key is found by bisection over all of the row's keys, in registers
-// (4096 rows of 2000 bf16 logits, top 64: 23 us against 59 in two launches; 8 or 16 waves a row for
+// a row, one wave where 2041 logits or fewer leave no work for four (4096 rows of 2000
+// bf16 logits, top 64: 19 us against 59 in two launches; 8 or 16 waves a row for
 // larger vocabularies were slower than two launches at any number of rows).
 #include <type_traits>
 
@@ -257,6 +256,57 @@ struct Keys {
   }
 };
 
+// Every thread's two keys, 2 W a lane, in every wave.
+template <int W>
+MKV_DEV void threads_bests(uint32_t a, uint32_t b, uint32_t (&bests)[2 * W]) {
+  if constexpr (W > 1) {
+    __shared__ uint32_t all[2][64 * W];
+    all[0][threadIdx.x] = a;
+    all[1][threadIdx.x] = b;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 2 * W; ++v) bests[v] = all[v / W][v % W * 64 + (threadIdx.x & 63)];
+  } else {
+    bests[0] = a;
+    bests[1] = b;
+  }
+}
+// Of these keys, one that k reach: the k-th largest or less, found a bit at a time
+// by each wave for itself, without a barrier; 0 where fewer than k are above 0.
+template <int BITS, int N>
+MKV_DEV uint32_t kth_best(const uint32_t (&bests)[N], int k) {
+  uint32_t least = 0;
+  for (int bit = BITS - 1; bit >= 0; --bit) {
+    const uint32_t mid = least | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int v = 0; v < N; ++v) n += __popcll(__builtin_amdgcn_ballot_w64(bests[v] >= mid));
+    if (n >= k) least = mid;
+    if (n == k) break;
+  }
+  return least;
+}
+// ... of the threads' keys, the larger of each thread's two where these are many
+// enough: k of 64 W leave few logits above the bound (1024 rows of 151936, top 20:
+// 70 us against 74; 4096 rows of 2000, top 64 the other way: 27 against 19).
+template <int BITS, int N>
+MKV_DEV uint32_t bound(const uint32_t (&bests)[N], int k) {
+  if (k > 32) return kth_best<BITS>(bests, k);
+  uint32_t larger[N / 2];
+#pragma unroll
+  for (int v = 0; v < N / 2; ++v) larger[v] = max(bests[v], bests[v + N / 2]);
+  return kth_best<BITS>(larger, k);
+}
+template <int N>
+MKV_DEV uint32_t largest(const uint32_t (&bests)[N]) {
+  uint32_t hi = 0;
+#pragma unroll
+  for (int v = 0; v < N; ++v) hi = max(hi, bests[v]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+  return hi;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   using P = Pieces<DT>;
@@ -327,32 +377,15 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
     keys.each([&](uint32_t key, int) { n += __popcll(__builtin_amdgcn_ballot_w64(key >= least)); });
     return all(n);
   };
-  // the largest key, and the least that is a thread's largest (so that every
-  // thread with a share reaches it)
-  uint32_t own = 0;
-  keys.each([&](uint32_t key, int) { own = max(own, key); });
-  uint32_t hi = own, lo = own ? own : 0xffffffffu;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
-  }
-  if (lane == 0) {
-    subs[wave] = (int)hi;
-    subs[kWaves + wave] = (int)lo;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    hi = max(hi, (uint32_t)subs[w]);
-    lo = min(lo, (uint32_t)subs[kWaves + w]);
-  }
+  // a bound of k shares, from the largest of the threads' even and odd ones
+  uint32_t own[2] = {0, 0};
+  keys.each([&](uint32_t key, int share) { own[share & 1] = max(own[share & 1], key); });
+  uint32_t bests[2 * kWaves];
+  threads_bests<kWaves>(own[0], own[1], bests);
+  uint32_t lo = max(bound<8 * sizeof(typename P::Key)>(bests, k), 1u);  // (0: few threads have a share)
   int n_sub = reach(lo);
-  if (n_sub < k) {  // (few threads have a share)
-    lo = 1;
-    n_sub = reach(lo);
-  }
   if (n_sub > kMaxSub) {
+    uint32_t hi = largest(bests);
     const int n_hi = reach(hi);
     if (n_hi >= k) {
       lo = hi;
@@ -454,14 +487,15 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
 }
 
 // Rows that a workgroup of W waves holds, PER logits a thread.
+constexpr int kFew = 256;  // candidates that are ranked against each other
 template <int DT, int W, int PER>
 __global__ __launch_bounds__(64 * W) void logprobs_whole_kernel(LpArgs a) {
   using P = Pieces<DT>;
   constexpr int T = 64 * W, kPieces = PER / P::kVec;
   __shared__ Stat part[W];
   __shared__ uint32_t counts[2][W];
-  __shared__ uint64_t cand[kMaxTop];
-  __shared__ int places[kMaxTop], fill;
+  __shared__ uint64_t cand[kFew];
+  __shared__ int fill;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
   const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * (16 / P::kVec);
@@ -511,12 +545,12 @@ __global__ __launch_bounds__(64 * W) void logprobs_whole_kernel(LpArgs a) {
   if (a.top == 0) return;
 
   const int k = a.top;
-  uint32_t key[PER], best = 0;  // (0: outside the row)
+  uint32_t key[PER], best[2] = {0, 0};  // (0: outside the row)
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int64_t at = P::template start_of<T>(i / P::kVec, tid, shift) + i % P::kVec;
     key[i] = at >= 0 && at < a.vocab ? P::key(x[i]) : 0u;
-    best = max(best, key[i]);
+    best[i >= PER / 2] = max(best[i >= PER / 2], key[i]);
   }
   int turn = 0;
   auto total = [&](uint32_t n) -> int {  // over the waves
@@ -540,92 +574,84 @@ __global__ __launch_bounds__(64 * W) void logprobs_whole_kernel(LpArgs a) {
     }
     return total(n);
   };
-  // The k-th largest key, lo: the k-th largest of a wave's best is at most that
-  // where the wave holds k.
-  uint32_t hi = best, least = best;
+  // ---- a bound that k logits reach, from the largest of the threads' halves ----
+  uint32_t bests[2 * W];
+  threads_bests<W>(best[0], best[1], bests);
+  uint32_t lo = max(bound<8 * sizeof(typename P::Key)>(bests, k), 1u);
+  uint32_t chosen = 0;  // a bit a logit
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
-    least = min(least, (uint32_t)__shfl_xor((int)least, o));
-  }
-  if constexpr (W > 1) {
-    __shared__ uint32_t tops[W], leasts[W];
-    if (lane == 0) {
-      tops[wave] = hi;
-      leasts[wave] = least;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < W; ++v) {
-      hi = max(hi, tops[v]);
-      least = max(least, leasts[v]);
-    }
-  }
-  uint32_t lo = max(least, 1u);
-  int reached = reach(lo);
-  if (reached > k) {
-    const int n = reach(hi);
-    if (n >= k) {
+  for (int i = 0; i < PER; ++i) chosen |= (uint32_t)(key[i] >= lo) << i;
+  auto sum = [&](uint32_t bits) { return total((uint32_t)wave_sum((float)__popc(bits))); };
+  int n = sum(chosen);
+  auto place = [&](int i) { return (int)P::template start_of<T>(i / P::kVec, tid, shift) + i % P::kVec; };
+  if (n > kFew) {
+    // ---- many (equal ones, or few threads with logits): exactly k, by the k-th
+    // largest of all keys, lo ----
+    uint32_t hi = largest(bests);
+    const int n_hi = reach(hi);
+    if (n_hi >= k) {
       lo = hi;
-      reached = n;
+      n = n_hi;
     }
-    while (reached > k && hi - lo > 1) {  // reached = those at lo or above; fewer than k at hi
+    while (n > k && hi - lo > 1) {  // n reach lo, fewer than k reach hi
       const uint32_t mid = lo + (hi - lo) / 2;
       const int n_mid = reach(mid);
       if (n_mid >= k) {
         lo = mid;
-        reached = n_mid;
+        n = n_mid;
       } else {
         hi = mid;
       }
     }
-  }
-  uint32_t above = 0, equal = 0;  // a bit a logit
+    uint32_t above = 0, equal = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    above |= (uint32_t)(key[i] > lo) << i;
-    equal |= (uint32_t)(key[i] == lo) << i;
-  }
-  auto place = [&](int i) { return (int)P::template start_of<T>(i / P::kVec, tid, shift) + i % P::kVec; };
-  if (reached > k) {
-    // the first of the equal logits: those below place `end` (a thread's places
-    // rise with i)
-    auto below = [&](int end) {
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) n += min(max(end - place(j * P::kVec), 0), P::kVec);
-      return equal & (uint32_t)((1ull << n) - 1);
-    };
-    auto sum = [&](uint32_t bits) { return total((uint32_t)wave_sum((float)__popc(bits))); };
-    const int need = k - sum(above);
-    int begin = 0, end = a.vocab;  // fewer than need below begin, need or more below end
-    while (end - begin > 1) {
-      const int mid = begin + (end - begin) / 2;
-      const int n = sum(below(mid));
-      if (n >= need) end = mid;
-      else begin = mid;
-      if (n == need) break;
+    for (int i = 0; i < PER; ++i) {
+      above |= (uint32_t)(key[i] > lo) << i;
+      equal |= (uint32_t)(key[i] == lo) << i;
     }
-    equal = below(end);
+    if (n > k) {
+      // the first of the equal logits: those below place `end` (a thread's places
+      // rise with i)
+      auto below = [&](int end) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) c += min(max(end - place(j * P::kVec), 0), P::kVec);
+        return equal & (uint32_t)((1ull << c) - 1);
+      };
+      const int need = k - sum(above);
+      int begin = 0, end = a.vocab;  // fewer than need below begin, need or more below end
+      while (end - begin > 1) {
+        const int mid = begin + (end - begin) / 2;
+        const int c = sum(below(mid));
+        if (c >= need) end = mid;
+        else begin = mid;
+        if (c == need) break;
+      }
+      equal = below(end);
+    }
+    chosen = above | equal;
+    n = k;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < PER; ++i)
-    if ((above | equal) >> i & 1) {
+    if (chosen >> i & 1) {
       const int at = atomicAdd(&fill, 1);
-      if (at < k) places[at] = place(i);
+      if (at < kFew) cand[at] = (uint64_t)place(i);
     }
   __syncthreads();
   // a candidate's place is the number of larger ones (its logit comes from the row
   // again: the logits' registers hold the keys since)
-  uint64_t mine = 0;
-  if (tid < k) cand[tid] = mine = key_of(logit_at<DT>(row, places[tid]), places[tid]);
+  for (int i = tid; i < n; i += T) cand[i] = key_of(logit_at<DT>(row, (int64_t)cand[i]), (int)cand[i]);
   __syncthreads();
-  if (tid < k) {
+  for (int i = tid; i < n; i += T) {
+    const uint64_t mine = cand[i];
     int rank = 0;
-    for (int j = 0; j < k; ++j) rank += cand[j] > mine;
-    a.top_ids[r * k + rank] = (int)~(uint32_t)mine;
-    a.top_logprobs[r * k + rank] = (value_of((uint32_t)(mine >> 32)) - m) - log_s;
+    for (int j = 0; j < n; ++j) rank += cand[j] > mine;
+    if (rank < k) {
+      a.top_ids[r * k + rank] = (int)~(uint32_t)mine;
+      a.top_logprobs[r * k + rank] = (value_of((uint32_t)(mine >> 32)) - m) - log_s;
+    }
   }
 }
 
