@@ -135,18 +135,18 @@ struct Units {
   }
   // the units of sequences s0 .. s0 + 63, `base` ahead of them; their number
   MKV_DEV int number(int s0, int k, int base) {
-    n = s0 + (int)(threadIdx.x & 63) < a.num_seqs ? max((k + len - 1) / len, 1) : 0;
+    n = s0 + (int)(threadIdx.x & 63) < a.num_seqs ? max((int)(((uint32_t)k + (uint32_t)len - 1) / (uint32_t)len), 1) : 0;
     const int upto = wave_scan(n);
     before = base + upto - n;
     return __builtin_amdgcn_readlane(upto, 63);
   }
   MKV_DEV explicit Units(const TreeArgs& args) : a(args) {
     const int k0 = keys(0);
-    float sum = wave_sum((float)k0);  // (a rule of thumb's accuracy, the same in every wave)
+    double sum = wave_sum((float)k0);  // (a rule of thumb's accuracy, the same in every wave)
     for (int s0 = 64; s0 < a.num_seqs; s0 += 64) sum += wave_sum((float)keys(s0));
     // (a little more than the even share: at most `shares` units beside the last
     // one of each sequence, whatever the sum's rounding)
-    len = (int)fminf(sum * 1.0001f / (float)a.shares, 1.0e9f) + 1;
+    len = (int)fminf((float)sum * 1.0001f / (float)a.shares, 1.0e9f) + 1;
     len = uniform((max(len, a.min_split) + TILE - 1) / TILE * TILE);
     total = number(0, a.num_seqs > 64 ? keys(0) : k0, 0);
     for (int s0 = 64; s0 < a.num_seqs; s0 += 64) total += number(s0, keys(s0), total);

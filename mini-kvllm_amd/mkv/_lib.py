@@ -8,6 +8,7 @@ operator raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
@@ -164,6 +165,12 @@ def call(name: str, *args) -> None:
     if status != 0:
         msg = load().mkv_status_string(status).decode()
         raise MkvError(name, status, msg)
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_size(name: str, *args) -> int:
+    """The value of a size entry point, which its arguments alone decide."""
+    return query(name, *args)
 
 
 def query(name: str, *args):

@@ -628,8 +628,8 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         return out
     kv_code = _dtype_code(k_cache, "k_cache")
     sizes = (num_heads, num_kv_heads, head_dim, block_size)
-    nbytes = _lib.query("mkv_paged_tree_workspace_size", num_seqs, total, *sizes, bt.shape[1], tree_mask.shape[1],
-                        kv_code)
+    nbytes = _lib.workspace_size("mkv_paged_tree_workspace_size", num_seqs, total, *sizes, bt.shape[1],
+                                 tree_mask.shape[1], kv_code)
     # (of the call's own: calls on several streams and captured graphs share none)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call_on(dev, "mkv_paged_tree", out.data_ptr(), query.data_ptr(), _dtype_code(query, "query"),

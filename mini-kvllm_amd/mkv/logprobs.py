@@ -61,7 +61,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top: int = 0) 
                         torch.empty(rows, top, dtype=torch.int64, device=dev))
     if rows == 0:
         return out
-    nbytes = _lib.query("mkv_token_logprobs_workspace_size", rows, vocab, top)
+    nbytes = _lib.workspace_size("mkv_token_logprobs_workspace_size", rows, vocab, top)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call_on(dev, "mkv_token_logprobs", out.logprobs.data_ptr(), out.entropy.data_ptr(),
              out.top_logprobs.data_ptr(), out.top_indices.data_ptr(), logits.data_ptr(),

@@ -174,7 +174,7 @@ class PagePool:
         parents = parents.contiguous()
         tokens = None if tokens is None else tokens.contiguous()
         granted = torch.empty(self.rows, dtype=torch.bool, device=self.device)
-        nbytes = _lib.query("mkv_assign_pages_workspace_size", self.rows, self.max_blocks)
+        nbytes = _lib.workspace_size("mkv_assign_pages_workspace_size", self.rows, self.max_blocks)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         stride = self.block_tables.stride(0) if self.rows > 1 else self.max_blocks
         _call_on(self.device, "mkv_assign_pages", *self.pages._pools, self.block_tables.data_ptr(), stride,
