@@ -1468,6 +1468,8 @@ int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
   return MKV_OK;
 }
 
+constexpr int64_t kMaxRows = 65535 * 16 - 255;
+
 int check_tree(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim, int block_size,
                int max_blocks, int mask_cols) {
   if (num_seqs < 0 || total_q < 0 || total_q > 0x7fffffff || num_heads <= 0 || num_kv_heads <= 0 || max_blocks < 0 ||
@@ -1479,6 +1481,8 @@ int check_tree(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, i
   if (log2_exact(block_size) < 4) return MKV_ERR_BAD_BLOCK_SIZE;
   if ((int64_t)num_seqs * num_kv_heads > 0x7fffffff || (int64_t)max_blocks * block_size > 0x7fff0000)
     return MKV_ERR_BAD_SHAPE;
+  // (a KV head's rows of a sequence: the join's grid)
+  if ((mask_cols < total_q ? mask_cols : total_q) * g * (head_dim == 64 ? 2 : 1) > kMaxRows) return MKV_ERR_BAD_SHAPE;
   return MKV_OK;
 }
 
@@ -1530,7 +1534,7 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
     return MKV_ERR_MISALIGNED;
   int kv;
   const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, kv);
-  if (p.units * kv * p.row_blocks > 0x7fffffff || p.row_cap / kJoinRows<1> > 65535) return MKV_ERR_BAD_SHAPE;
+  if (p.units * kv * p.row_blocks > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
   if (workspace_of(p, kv) > workspace_bytes || (p.splits && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
   const int pair = head_dim == 64 ? 2 : 1;
   TreeArgs a;
