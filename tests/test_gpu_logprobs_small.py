@@ -94,3 +94,18 @@ def test_not_finite_absent_and_outside(dev, vocab):
     many[:, 1::2] = vocab - 1
     got = mkv.token_logprobs(x[3:], many[3:], 0).logprobs
     assert torch.equal(got[:, 0::2], got[:, :1].expand(-1, 350)) and torch.equal(got[:, 1::2], got[:, 1:2].expand(-1, 350))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [257, 300, 505, 2041, 8185])
+def test_rows_of_one_value_or_two(dev, dtype, vocab):
+    """More equal logits than are ranked against each other, in every form."""
+    announce(f"logprobs, one value, vocabulary {vocab}, {dtype}")
+    x = torch.full((4, vocab), -1.5, device=dev, dtype=dtype)
+    x[1, ::2] = 3.0
+    x[2, 5:9] = 3.0
+    x[3] = -torch.inf
+    x[3, vocab - 70:] = 0.25
+    ids = torch.full((4, 1), vocab - 1, device=dev)
+    for top in (1, 3, 5, 64):
+        _check(x, ids, top)

@@ -245,3 +245,22 @@ def test_engine_reports_log_probabilities(dev, use_graphs):
             assert all(abs(float(x[i, j]) - lp) <= 1e-5 for j, lp in rep.top)
     assert [r.tokens[r.prompt_len:] for r in reqs] == plain, "reports change no token"
     assert [len(r.reports) for r in reqs] == [0 if n is None else 6 for n in wants]
+
+
+def test_engine_reports_survive_a_preemption(dev):
+    """A pool too small for all sequences: preempted requests start again from
+    their tokens, and keep one report a generated token."""
+    announce("engine: log probabilities with preemptions")
+    g = torch.Generator().manual_seed(22)
+    prompts = [torch.randint(0, CFG.vocab_size, (n,), generator=g).tolist() for n in (40, 44, 47, 30)]
+    model = E.Qwen3Model(CFG, dev, seed=5, block_size=BS)
+    eng = E.Engine(model, num_blocks=14, max_num_seqs=4, max_num_batched_tokens=64, max_model_len=256)
+    reqs = [eng.add_request(p, 24, logprobs=2) for p in prompts]
+    while not eng.sched.done():
+        eng.step()
+    assert eng.sched.num_preemptions > 0
+    for r in reqs:
+        assert r.num_generated == len(r.reports) == 24
+        for tok, rep in zip(r.tokens[r.prompt_len:], r.reports):
+            assert rep.logprob <= rep.top[0][1] and rep.top[0][1] >= rep.top[1][1] and rep.entropy >= -1e-4
+            assert tok != rep.top[0][0] or abs(rep.logprob - rep.top[0][1]) <= 1e-5
