@@ -264,3 +264,48 @@ def test_engine_reports_survive_a_preemption(dev):
         for tok, rep in zip(r.tokens[r.prompt_len:], r.reports):
             assert rep.logprob <= rep.top[0][1] and rep.top[0][1] >= rep.top[1][1] and rep.entropy >= -1e-4
             assert tok != rep.top[0][0] or abs(rep.logprob - rep.top[0][1]) <= 1e-5
+
+
+@pytest.mark.parametrize("kv", ["auto", "fp8_per_tensor", "fp8_per_token_head", "int8_per_token_head"])
+def test_a_chain_gives_the_chunked_prefill_s_logits(dev, kv):
+    """Two sequences' next tokens over each cache format, once as a chunk of a
+    prompt and once as a tree that is a chain: the same K and V are appended to the
+    same rows, and the logits agree to the roundings of bf16 activations (the bound
+    that the engine's logits meet against another attention)."""
+    announce(f"speculative: a chain against a prefill chunk, {kv} KV")
+    model = E.Qwen3Model(CFG, dev, seed=5, block_size=BS)
+    model.attach_kv_cache(12, kv)
+    g = torch.Generator().manual_seed(9)
+    lens, new = [40, 21], [9, 4]
+    tables = torch.tensor([[3, 7, 1, 5], [2, 9, 4, 0]], dtype=torch.int32)
+    toks = [torch.randint(0, CFG.vocab_size, (n + m,), generator=g) for n, m in zip(lens, new)]
+
+    def step(first, last, tree):
+        ids = torch.cat([x[a:b] for x, a, b in zip(toks, first, last)])
+        pos = torch.cat([torch.arange(a, b) for a, b in zip(first, last)])
+        row = torch.cat([torch.full((b - a,), r) for r, (a, b) in enumerate(zip(first, last))])
+        slots = (tables[row, pos // BS].long() * BS + pos % BS).to(dev)
+        sizes = [b - a for a, b in zip(first, last)]
+        cu = torch.tensor([0, sizes[0], sum(sizes)], dtype=torch.int32, device=dev)
+        mask = None
+        if tree:
+            mask = torch.ones(sum(sizes), max(sizes), dtype=torch.bool)
+            local = torch.cat([torch.arange(n) for n in sizes])
+            mask &= torch.arange(max(sizes))[None] <= local[:, None]
+            mask = mask.to(dev)
+        C.set_context(True, cu_seqlens_q=cu, max_seqlen_q=max(sizes), slot_mapping=slots,
+                      context_lens=torch.tensor(last, device=dev), block_tables=tables.to(dev), positions=pos.to(dev),
+                      tree_mask=mask)
+        try:
+            return model.logits(model(ids.to(dev), pos.to(dev), slots)).float()
+        finally:
+            C.reset_context()
+
+    step([0, 0], lens, False)
+    ends = [n + m for n, m in zip(lens, new)]
+    want = step(lens, ends, False)
+    got = step(lens, ends, True)
+    tol = 6e-2 + torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -14))) - 7)
+    diff = (got - want).abs()
+    print(f"max difference {float(diff.max()):.2e}, mean {float(diff.mean()):.2e}")
+    assert bool((diff <= tol).all()) and float(diff.mean()) <= 1e-2
