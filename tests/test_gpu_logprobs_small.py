@@ -109,3 +109,21 @@ def test_rows_of_one_value_or_two(dev, dtype, vocab):
     ids = torch.full((4, 1), vocab - 1, device=dev)
     for top in (1, 3, 5, 64):
         _check(x, ids, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [400, 2000, 8000, 50257])
+def test_the_largest_logits_side_by_side(dev, dtype, vocab):
+    """Rows whose largest logits lie in few threads' shares: sorted both ways, a
+    run of 300 larger ones (of one value or of many), and larger ones 8192 apart."""
+    announce(f"logprobs, large logits together, vocabulary {vocab}, {dtype}")
+    g = torch.Generator(device=dev).manual_seed(11)
+    x = torch.randn(6, vocab, generator=g, device=dev)
+    x[0], x[1] = x[0].sort().values, x[1].sort(descending=True).values
+    x[2, 40:340] += 12
+    x[3, vocab - 301:vocab - 1] = 9.0
+    x[4, ::8] += 12
+    x[5, torch.arange(0, vocab, 8192, device=dev)] += 20
+    x = x.to(dtype)
+    for top in (1, 20, 33, 64):
+        _check(x, torch.randint(vocab, (6, 2), generator=g, device=dev), top)
