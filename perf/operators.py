@@ -19,7 +19,6 @@ order, the page tables and every value.
 """
 from __future__ import annotations
 
-import functools
 import math
 import random
 import sys
@@ -239,9 +238,7 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------
 # One pass
 # ---------------------------------------------------------------------------
-@functools.cache
 def _mkv():
-    """The package, imported once, as a program does."""
     root = str(Path(__file__).resolve().parent.parent / "mini-kvllm_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
