@@ -569,8 +569,11 @@ int mkv_linear(void* out, const void* x, int64_t x_row_stride, const void* w,
  * fp32, bf16 and fp16 caches with q of that type; FP8 (per tensor, or per token
  * and head) and INT8 (per token and head) caches with a bf16 or fp16 q.  Head
  * sizes and groups as mkv_paged_decode; out has q's type and layout.  Sums and
- * the softmax are fp32; 16-bit P holds 16 bits or more over bf16 caches and 11
- * over the others.
+ * the softmax are fp32; P is rounded to two bf16 terms over bf16 caches and to fp16
+ * over the others (over those with V scales per token and head, P times the scale),
+ * in whatever range it and the scales lie: 2^-11 of each key's term, or 2^-32 of
+ * the row's largest term for terms 2^21 and more below it.  V scales per token and
+ * head below 2^-64 lose bits, ones above 2^101 may overflow.
  */
 size_t mkv_paged_tree_workspace_size(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim,
                                      int block_size, int max_blocks, int mask_cols, int kv_dtype);

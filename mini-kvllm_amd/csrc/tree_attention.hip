@@ -43,6 +43,24 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // nothing; any offset of the maximum cancels in the normalisation
 constexpr float kRescaleSlack = 8.0f;
 
+// Per-token-head V scales are folded into P ahead of its rounding to fp16, so it
+// is P times the scale that has to fit: the running maximum is that of score +
+// log2 |V scale| less kScaledLift, and the products' largest is 2^7 to 2^15 whatever
+// the scales are.  Products 2^21 below the largest are exact to fp16's half step,
+// lower ones to 2^-32 of the largest.  Scales below 2^kLeastScale count as that here
+// (a key may have none, and the normaliser's terms, P alone, stay below 2^79), ones
+// above 2^kMostScale as that (P stays within fp32's normal range).
+constexpr float kScaledLift = 7.0f, kLeastScale = -64.0f, kMostScale = 100.0f;
+MKV_DEV float scale_log2(float s) {  // (0, infinite and NaN scales: within the bounds)
+  return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(s)), kLeastScale), kMostScale);
+}
+// x 2^d, by halves: scales far apart bring factors below fp32's range to terms
+// above 1
+MKV_DEV float mul_exp2(float x, float d) {
+  const float f = __builtin_amdgcn_exp2f(0.5f * d);
+  return x * f * f;
+}
+
 struct TreeArgs {
   void* out;
   const void* q;
@@ -419,7 +437,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
   __shared__ int slots[kShared ? 2 * (NK / 16) : 1];  // of each sub-tile, -1 absent, by the tile's parity
   constexpr int kHeads = PAIR ? 2 : 1;
   constexpr int kScLoads = kTok ? 2 * kHeads * TK / 64 : 1;
-  __shared__ __align__(16) float sc_all[kTok ? kWaves * 2 * kHeads * TK : 4];  // a wave's own: [head][K, V][TK]
+  __shared__ __align__(16) float sc_all[kTok ? kWaves * 3 * kHeads * TK : 4];  // a wave's own: [head][K, V, log2 |V|][TK]
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int rg = wave % R, kg = wave / R;
@@ -486,7 +504,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     }
   };
   float sc_raw[kScLoads];
-  float* const sc = sc_all + (kTok ? wave * 2 * kHeads * TK : 0);
+  float* const sc = sc_all + (kTok ? wave * 3 * kHeads * TK : 0);
   auto load_scales = [&](int kb, int turn) {
     if constexpr (kTok) {
 #pragma unroll
@@ -664,7 +682,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     }
     return s;
   };
-  const float* const ks = sc + (PAIR && hi ? 2 * TK : 0) + 4 * h;
+  const float* const ks = sc + (PAIR && hi ? 3 * TK : 0) + 4 * h;
   // scores of key block nb: K scales, -inf where the row does not see, and the
   // running maximum (with what is already summed, and the pending P of the block
   // before, brought to it)
@@ -681,22 +699,40 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = (see >> e) & 1 ? s[e] : kNegInf;
     }
-    float mx = max3(s[0], s[1], s[2]), my = max3(s[3], s[4], s[5]);
+    float mx;
+    if constexpr (kTok) {
+      // of what P times its V scale comes to
+      mx = kNegInf;
 #pragma unroll
-    for (int e = 6; e < 14; e += 4) {
-      mx = max3(mx, s[e], s[e + 1]);
-      my = max3(my, s[e + 2], s[e + 3]);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(ks + 2 * TK + 32 * nb + 8 * g);
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = __builtin_fmaf(s[4 * g + j], score_mul, x[j]);
+        mx = max3(max3(mx, t[0], t[1]), t[2], t[3]);
+      }
+      mx = fmaxf(mx, other_half(mx));
+      mx = fmaxf(mx - kScaledLift, kNegBig);
+    } else {
+      float my = max3(s[3], s[4], s[5]);
+      mx = max3(s[0], s[1], s[2]);
+#pragma unroll
+      for (int e = 6; e < 14; e += 4) {
+        mx = max3(mx, s[e], s[e + 1]);
+        my = max3(my, s[e + 2], s[e + 3]);
+      }
+      mx = max3(mx, s[14], s[15]);
+      mx = max3(mx, my, my);
+      mx = fmaxf(mx, other_half(mx));
+      mx = fmaxf(mx * score_mul, kNegBig);
     }
-    mx = max3(mx, s[14], s[15]);
-    mx = max3(mx, my, my);
-    mx = fmaxf(mx, other_half(mx));
-    mx = fmaxf(mx * score_mul, kNegBig);
     const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
     if (__builtin_amdgcn_ballot_w64(m_new != m_run)) {
       // (before the first visible key there is nothing to rescale but marks)
       const float alpha = m_run == kNegBig ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      if constexpr (kTok) l_run = mul_exp2(l_run, m_run - m_new);
+      else l_run *= alpha;
       m_run = m_new;
-      l_run *= alpha;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -790,7 +826,11 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     }
     if constexpr (kTok) {
 #pragma unroll
-      for (int i = 0; i < kScLoads; ++i) sc[lane + 64 * i] = sc_raw[i];
+      for (int i = 0; i < kScLoads; ++i) {
+        const int at = lane + 64 * i, which = at / TK, to = at + (which >> 1) * TK;
+        sc[to] = sc_raw[i];
+        if (which & 1) sc[to + TK] = scale_log2(sc_raw[i]);
+      }
     }
     // ---- what this lane's row sees of keys that are not all prefix: element
     // e of key block nb is key 32 nb + 8 (e >> 2) + 4h + (e & 3) ----
@@ -954,7 +994,8 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
     m_run = m;
     l = 0.0f;
 #pragma unroll
-    for (int g = 0; g < KG; ++g) l += ml[g][1] * __builtin_amdgcn_exp2f(ml[g][0] - m);
+    for (int g = 0; g < KG; ++g)
+      l += kTok ? mul_exp2(ml[g][1], ml[g][0] - m) : ml[g][1] * __builtin_amdgcn_exp2f(ml[g][0] - m);
     // a 4 KB block to each group's summands from the others
     auto at = [&](int to, int i, int from) {  // (from != to; i: the block of the group's)
       const int n = ((to * kMine + i) * (KG - 1) + from - (from > to)) * R + rg;
@@ -1040,7 +1081,7 @@ MKV_DEV float half_max(float x) {  // of the 32 lanes
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-template <int UNIT, int Z, bool FP8, bool PAIR>
+template <int UNIT, int Z, int KV_DT, bool PAIR>
 MKV_DEV void tree_join_body(const TreeArgs& a) {
   constexpr int kAhead = 4;  // splits whose loads are in flight
   Place place;
@@ -1086,7 +1127,7 @@ MKV_DEV void tree_join_body(const TreeArgs& a) {
       for (int r = 0; r < 2; ++r) {
         if (z0 + j < n) {
           const float f = __builtin_amdgcn_exp2f(x_ml[r][j][0] - m[r]);
-          l[r] += x_ml[r][j][1] * f;
+          l[r] += kPerTokenScale<KV_DT> ? mul_exp2(x_ml[r][j][1], x_ml[r][j][0] - m[r]) : x_ml[r][j][1] * f;
           sum[r] += x_o[r][j] * f;
         }
       }
@@ -1116,7 +1157,7 @@ MKV_DEV void tree_join_body(const TreeArgs& a) {
   for (int r = 0; r < 2; ++r) {
     if (r && !two) return;
     float norm = l[r] > 0.0f ? 1.0f / l[r] : l[r] == 0.0f ? 0.0f : l[r];
-    if constexpr (FP8) norm *= load_uniform_f32(a.v_scale);
+    if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) norm *= load_uniform_f32(a.v_scale);
     bool hi = false;
     const int64_t off = row_offset<PAIR>(a, w, row0 + r, hi);
     if (PAIR && (c >= 16) != hi) continue;
@@ -1124,9 +1165,11 @@ MKV_DEV void tree_join_body(const TreeArgs& a) {
     store4(a.out, a.q_dtype, off + 4 * (PAIR ? c & 15 : c), x);
   }
 }
-template <int UNIT, int Z, bool FP8, bool PAIR>
+// (KV_DT: FP8 per tensor, FP8 per token and head for both formats with such
+// scales, fp32 for the rest)
+template <int UNIT, int Z, int KV_DT, bool PAIR>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a) {
-  tree_join_body<UNIT, Z, FP8, PAIR>(a);
+  tree_join_body<UNIT, Z, KV_DT, PAIR>(a);
 }
 
 // fp32 caches: products and sums in fp32 on the 32x32x2 fp32 MFMA, one row group
@@ -1449,12 +1492,12 @@ int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
   }
   if (hipError_t e = hipGetLastError()) return (int)e;
   if (p.splits) {
-    constexpr bool kFp8 = KV_DT == MKV_DTYPE_FP8E4M3;
+    constexpr int kFormat = kPerTokenScale<KV_DT> ? kKvFp8PerToken : KV_DT == MKV_DTYPE_FP8E4M3 ? KV_DT : MKV_DTYPE_F32;
     // (few sequences in many splits each: the waves share them)
     auto join = [&](auto unit, auto z) {
       constexpr int kUnit = decltype(unit)::value, kZ = decltype(z)::value;
       const dim3 jgrid((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)((p.row_cap + kJoinRows<kZ> - 1) / kJoinRows<kZ>));
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<kUnit, kZ, kFp8, PAIR>), jgrid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(tree_join_kernel<kUnit, kZ, kFormat, PAIR>), jgrid, dim3(256), 0, s, a);
     };
     using I1 = std::integral_constant<int, 1>;
     using I4 = std::integral_constant<int, 4>;
