@@ -560,8 +560,10 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
 
   Op16<CT> qop[8];
   {
-    // the loop keeps raw scores and wants score_mul > 0: a negative scale
-    // moves its sign into q, a zero one makes q zero
+    // the loop keeps raw scores and wants score_mul > 0: a negative scale (the
+    // softmax's times a per-tensor K scale) moves its sign into q, a zero one makes
+    // q zero
+    if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) score_mul *= load_uniform_f32(a.k_scale);
     uint32_t sign = 0u, keep = 0xffffffffu;
     if (!(score_mul > 0.0f) && score_mul == score_mul) {
       sign = score_mul < 0.0f ? 0x80008000u : 0u;
@@ -606,7 +608,6 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(Op16<CT>, raw[s]);
     }
   }
-  if constexpr (KV_DT == MKV_DTYPE_FP8E4M3) score_mul *= load_uniform_f32(a.k_scale);
 
   const uint8_t* mask_row = a.mask + (w.q0 + (row_ok ? row / a.group : 0)) * a.mask_stride;
   f32x16 acc[4];
