@@ -592,7 +592,9 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       top = fmaxf(top, other_half(top));
       float f = 1.0f;
       if (top > 0.0f && top < __builtin_huge_valf()) {
-        const int e = ilogbf(top);
+        // (rows below 2^-60 take that one's power, so that f and its inverse are in
+        // fp32's range; elements below 2^-82 lose bits)
+        const int e = max(ilogbf(top), -60);
         f = ldexpf(1.0f, 8 - e);
         score_mul *= ldexpf(1.0f, e - 8);
       }
