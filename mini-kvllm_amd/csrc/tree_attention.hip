@@ -38,19 +38,21 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr int kHeadDim = 128;
 constexpr float kNegBig = -1e30f;
 constexpr float kNegInf = -__builtin_huge_valf();
-// the running maximum moves only when a tile exceeds it by more than 2^8: P
-// stays within 2^8 (exact in range in bf16 and fp16) and most tiles rescale
-// nothing; any offset of the maximum cancels in the normalisation
+// the running maximum moves only when a tile exceeds it by more than 2^8, so that
+// most tiles rescale nothing; any offset of the maximum cancels in the normalisation
 constexpr float kRescaleSlack = 8.0f;
+// fp16 P: the maximum is offered less 7, so that a row's largest P is 2^7 to 2^15.  P
+// 2^21 below the largest is exact to fp16's half step, the rest to 2^-32 of the
+// largest (with the largest at 1, a context of 130,000 keys of 2^-26 beside one key
+// lost all of them, 2^-8 of the weight in all).
+constexpr float kHalfLift = 7.0f;
 
 // Per-token-head V scales are folded into P ahead of its rounding to fp16, so it
 // is P times the scale that has to fit: the running maximum is that of score +
-// log2 |V scale| less kScaledLift, and the products' largest is 2^7 to 2^15 whatever
-// the scales are.  Products 2^21 below the largest are exact to fp16's half step,
-// lower ones to 2^-32 of the largest.  Scales below 2^kLeastScale count as that here
+// log2 |V scale| (less kHalfLift).  Scales below 2^kLeastScale count as that here
 // (a key may have none, and the normaliser's terms, P alone, stay below 2^79), ones
 // above 2^kMostScale as that (P stays within fp32's normal range).
-constexpr float kScaledLift = 7.0f, kLeastScale = -64.0f, kMostScale = 100.0f;
+constexpr float kLeastScale = -64.0f, kMostScale = 100.0f;
 MKV_DEV float scale_log2(float s) {  // (0, infinite and NaN scales: within the bounds)
   return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(s)), kLeastScale), kMostScale);
 }
@@ -419,6 +421,7 @@ template <int KV_DT, int R, int KG, bool PAIR>
 MKV_DEV void tree_attention_body(const TreeArgs& a) {
   constexpr int CT = kOperand<KV_DT>;
   constexpr bool kTok = kPerTokenScale<KV_DT>;
+  constexpr float kLift = CT == MKV_DTYPE_F16 ? kHalfLift : 0.0f;
   constexpr int kWaves = R * KG, kThreads = 64 * kWaves;
   constexpr int TK = kTileKeys<KV_DT, R, KG>;  // keys a wave takes of a tile
   constexpr int NK = TK * KG;             // keys of a tile
@@ -715,7 +718,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
         mx = max3(max3(mx, t[0], t[1]), t[2], t[3]);
       }
       mx = fmaxf(mx, other_half(mx));
-      mx = fmaxf(mx - kScaledLift, kNegBig);
+      mx = fmaxf(mx - kLift, kNegBig);
     } else {
       float my = max3(s[3], s[4], s[5]);
       mx = max3(s[0], s[1], s[2]);
@@ -727,7 +730,7 @@ MKV_DEV void tree_attention_body(const TreeArgs& a) {
       mx = max3(mx, s[14], s[15]);
       mx = max3(mx, my, my);
       mx = fmaxf(mx, other_half(mx));
-      mx = fmaxf(mx * score_mul, kNegBig);
+      mx = fmaxf(__builtin_fmaf(mx, score_mul, -kLift), kNegBig);
     }
     const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
     if (__builtin_amdgcn_ballot_w64(m_new != m_run)) {
