@@ -571,8 +571,8 @@ MKV_DEV void prefill_mfma_body(const PrefillArgs& a) {
   // 1-byte caches, converted exactly while staging).
   // Per-token-head FP8 / INT8 caches: codes staged as exact fp16, scales
   // applied per key (K scale to the score, V scale to P, which stays one
-  // fp16 term: the running max is raised where a tile's V scales would take
-  // P * v_scale past the fp16 range, see the softmax below).
+  // fp16 term: the running max is moved so that P * v_scale lies in fp16's
+  // range, see the softmax below).
   constexpr bool kTokScale = kPerTokenScale<KV_DT>;
   constexpr int CT = (KV_DT == MKV_DTYPE_FP8E4M3 || kTokScale) ? MKV_DTYPE_F16 : KV_DT;
   constexpr int kEbG = DTypeInfo<KV_DT>::kBytes;  // cache element bytes
@@ -881,7 +881,7 @@ MKV_DEV void prefill_mfma_body(const PrefillArgs& a) {
       // the waves holding V scales (tid & 64; with head pairing one per KV
       // head) also store the tile's largest one
       if (tid < kScLoads && (tid & 64)) {
-        const float vm = wave_max_dpp(stg_sc);
+        const float vm = wave_max_dpp(fabsf(stg_sc));
         if (lane == 0) vmax_lds[2 * buf + (tid >> 7)] = vm;
       }
     }
@@ -1048,12 +1048,14 @@ MKV_DEV void prefill_mfma_body(const PrefillArgs& a) {
     // is the scaled max of the raw ones (rounding a product by a positive
     // constant is monotonic), and each P takes one FMA.
     float l_scaled[kRowTiles];
-    // Per-token-head V scales fold into P, which must stay below the fp16
-    // maximum: P <= 2^8 (the lazy rescale), so a tile whose largest V scale
-    // is 2^e times a fraction in [1/2, 1) with e > 7 lifts the max it offers
-    // the running max by e - 7 (log2 units), which keeps P * v_scale <= 2^15.
-    // Any offset of the running max cancels in the normalisation; with every
-    // V scale below 128 (FP8 amax < 57344, INT8 amax < 16256) it is 0.
+    // Per-token-head V scales fold into P, and the product has to lie in fp16's
+    // range: P <= 2^8 (the lazy rescale), so a tile whose largest V scale is 2^e
+    // times a fraction in [1/2, 1) offers the running max its own plus e - 7 (log2
+    // units), which keeps P * v_scale <= 2^15 and a tile's largest P times its
+    // largest V scale at 2^6 or more: products 2^20 below that are exact to
+    // fp16's half step, lower ones to 2^-31 of it.  Any offset of the running max
+    // cancels in the normalisation.  (Scales below 2^-40 count as that: a tile may
+    // have none, and P, whose sum is the normaliser, stays below 2^54.)
     // (The scale is the same in every lane: its exponent is taken from the
     // bits in scalar registers, e = biased exponent - 126, so the lift holds
     // no vector register through the softmax.)
@@ -1062,7 +1064,7 @@ MKV_DEV void prefill_mfma_body(const PrefillArgs& a) {
       float vm = vmax_lds[2 * buf];
       if constexpr (PAIR) vm = fmaxf(vm, vmax_lds[2 * buf + 1]);
       const int e = ((__builtin_amdgcn_readfirstlane(__float_as_int(vm)) >> 23) & 0xff) - 126;
-      v_lift = e > 7 ? (float)(e - 7) : 0.0f;
+      v_lift = (float)(max(e, -39) - 7);
     }
     // per-token-head K scales of this lane's keys 16kt + 4kg + r
     if constexpr (kTokScale) {
