@@ -669,7 +669,9 @@ MKV_DEV float q_operands(const DecodeArgs& a, float (&qf)[32], QOps<KV_DT>& qop,
     for (int i = 0; i < 32; ++i) qm = fmaxf(qm, fabsf(qf[i]));
     qm = wave_max(qm);
     if (qm > 0.0f && qm < __builtin_huge_valf()) {
-      const int e = ilogbf(qm);
+      // (from 2^-60 up: the factor and its inverse stay in fp32's range; elements
+      // below 2^-82 lose bits)
+      const int e = max(ilogbf(qm), -60);
       const float f = ldexpf(1.0f, 8 - e);
 #pragma unroll
       for (int i = 0; i < 32; ++i) qf[i] *= f;

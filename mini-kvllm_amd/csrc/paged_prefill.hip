@@ -943,7 +943,9 @@ MKV_DEV void prefill_mfma_body(const PrefillArgs& a) {
     // power-of-two normalisation so that q is exact and in range in fp16
     qmax = wave_max_dpp(qmax);
     if (qmax > 0.0f && qmax < __builtin_huge_valf()) {
-      const int e = ilogbf(qmax);
+      // (from 2^-60 up: the factor and its inverse stay in fp32's range; elements
+      // below 2^-82 lose bits)
+      const int e = max(ilogbf(qmax), -60);
       const float f = ldexpf(1.0f, 8 - e);
 #pragma unroll
       for (int rt = 0; rt < kRowTiles; ++rt)
