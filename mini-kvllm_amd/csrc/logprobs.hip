@@ -51,6 +51,14 @@ struct LpArgs {
   void* maxima;        // workspace: (rows, chunks, 256) keys, each row 16-byte aligned
 };
 
+// A workgroup a row: rows past a grid's first dimension (below 2^32 threads) go on in
+// the second.
+constexpr int64_t kGridRows = (int64_t)1 << 22;
+MKV_DEV int64_t row_of_grid() { return blockIdx.x + blockIdx.y * kGridRows; }
+inline dim3 grid_of_rows(int64_t rows) {
+  return dim3((unsigned)(rows < kGridRows ? rows : kGridRows), (unsigned)((rows + kGridRows - 1) / kGridRows));
+}
+
 // max that a NaN on either side wins (v_maximum3_f32)
 MKV_DEV float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
@@ -316,7 +324,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_row_kernel(LpArgs a) {
   __shared__ int subs[kMaxSub];
   __shared__ int fill[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
+  const int64_t r = row_of_grid();
+  if (r >= a.rows) return;
   const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * (16 / P::kVec);
   // the given tokens' logits and the keys go out first
   float given = 0.0f;
@@ -497,7 +506,8 @@ __global__ __launch_bounds__(64 * W) void logprobs_whole_kernel(LpArgs a) {
   __shared__ uint64_t cand[kFew];
   __shared__ int fill;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
+  const int64_t r = row_of_grid();
+  if (r >= a.rows) return;
   const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * (16 / P::kVec);
   const int shift = P::shift(row);
   float given = 0.0f;
@@ -663,7 +673,7 @@ int launch_logprobs(const LpArgs& a, hipStream_t s) {
     const int64_t held = a.vocab + 7;  // (a row's start may leave 7 places empty)
     auto whole = [&](auto w, auto per) {
       constexpr int W = decltype(w)::value, kPerThread = decltype(per)::value;
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_whole_kernel<DT, W, kPerThread>), dim3((unsigned)a.rows), dim3(64 * W), 0, s, a);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_whole_kernel<DT, W, kPerThread>), grid_of_rows(a.rows), dim3(64 * W), 0, s, a);
       return (int)hipGetLastError();
     };
     using I1 = std::integral_constant<int, 1>;
@@ -676,7 +686,7 @@ int launch_logprobs(const LpArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_chunk_kernel<DT>),
                      dim3(a.chunks, (unsigned)y, (unsigned)((a.rows + 32767) / 32768)), dim3(kLpThreads), 0, s, a);
   if (hipError_t e = hipGetLastError()) return (int)e;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_row_kernel<DT>), dim3((unsigned)a.rows), dim3(kLpThreads), 0, s, a);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(logprobs_row_kernel<DT>), grid_of_rows(a.rows), dim3(kLpThreads), 0, s, a);
   return (int)hipGetLastError();
 }
 
