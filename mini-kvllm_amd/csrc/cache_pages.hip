@@ -458,6 +458,17 @@ int check_pools(const void* const* tensors, const int64_t* row_bytes, int num, i
   return MKV_OK;
 }
 
+// A grid's first dimension in workgroups of 256 threads: below 2^32 threads.
+constexpr int64_t kMaxGrid = 0xffffff;
+
+// Whether a page's chunks of every tensor fit a launch's grid.
+bool copies_fit(const int64_t* row_bytes, int num, int block_size) {
+  int64_t widest = 0;
+  for (int t = 0; t < num; ++t) widest = row_bytes[t] > widest ? row_bytes[t] : widest;
+  const int n = num < kMaxTensors ? num : kMaxTensors;
+  return (widest * block_size + kCopyBytes - 1) / kCopyBytes * n <= kMaxGrid;
+}
+
 bool index_ok(int dt) { return dt == MKV_INDEX_I32 || dt == MKV_INDEX_I64; }
 
 }  // namespace
@@ -473,12 +484,12 @@ extern "C" int mkv_copy_pages(const void* const* tensors, const int64_t* row_byt
   if (!index_ok(index_dtype)) return MKV_ERR_UNSUPPORTED_DTYPE;
   if (pairs == 0 || num_tensors == 0) return MKV_OK;
   if (!src || !dst) return MKV_ERR_NULL_POINTER;
+  if (!copies_fit(row_bytes, num_tensors, block_size)) return MKV_ERR_BAD_SHAPE;
   for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
     Pools p;
     int64_t widest;
     const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
     const int64_t chunks = (widest * block_size + kCopyBytes - 1) / kCopyBytes;
-    if (chunks * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
     hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(chunks * n), (unsigned)(pairs < 65535 ? pairs : 65535)),
                        dim3(kCopyThreads), 0, reinterpret_cast<hipStream_t>(stream), p, block_size, (int)chunks,
                        num_pages, src, dst, (int)(index_dtype == MKV_INDEX_I64), pairs);
@@ -501,11 +512,12 @@ extern "C" int mkv_compact_slots(const void* const* tensors, const int64_t* row_
   if (!block_tables || !prefix_lens || !accepted) return MKV_ERR_NULL_POINTER;
   if (bt_stride < max_blocks || accepted_stride < num_accepted) return MKV_ERR_BAD_STRIDE;
   PagedIndex idx{block_tables, bt_stride, max_blocks, num_pages, bs_log2, 0};
-  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
-    Pools p;
-    int64_t widest;
-    const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
-    int64_t slices = 1;
+  Pools p;
+  int n;
+  int64_t widest, slices, per, groups;
+  auto plan = [&](int t0) {  // the launch for the tensors from t0 on
+    n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
+    slices = 1;
     for (int t = 0; t < n; ++t) {
       const bool wide = p.row_bytes[t] % 16 == 0 && (reinterpret_cast<uintptr_t>(p.base[t]) & 15) == 0;
       const int u = (int)(p.row_bytes[t] / (wide ? 16 : 4)), l2 = slice_log2(u, num_accepted);
@@ -513,10 +525,16 @@ extern "C" int mkv_compact_slots(const void* const* tensors, const int64_t* row_
       slices = c > slices ? c : slices;
     }
     // pools a workgroup: one while that leaves CUs free, at most eight
-    int64_t per = (int64_t)n * slices * batch / 1024;
+    per = (int64_t)n * slices * batch / 1024;
     per = per < 1 ? 1 : per > 8 ? 8 : per;
-    const int64_t groups = (n + per - 1) / per;
-    if (slices * groups > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+    groups = (n + per - 1) / per;
+    return slices * groups <= kMaxGrid;
+  };
+  // (every launch fits, or none runs)
+  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors)
+    if (!plan(t0)) return MKV_ERR_BAD_SHAPE;
+  for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
+    if (num_tensors > kMaxTensors) plan(t0);
     hipLaunchKernelGGL(compact_slots_kernel, dim3((unsigned)(slices * groups), (unsigned)batch), dim3(kMoveThreads),
                        (size_t)num_accepted * 16, reinterpret_cast<hipStream_t>(stream), p, n, (int)per, idx,
                        prefix_lens, (int)(prefix_dtype == MKV_INDEX_I64), accepted,
@@ -547,6 +565,8 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
     return MKV_ERR_NULL_POINTER;
   if (bt_stride < max_blocks) return MKV_ERR_BAD_STRIDE;
   if (workspace_bytes < mkv_assign_pages_workspace_size(rows, max_blocks)) return MKV_ERR_WORKSPACE_TOO_SMALL;
+  // (ahead of the table's step, which the copies complete)
+  if (!copies_fit(row_bytes, num_tensors, block_size)) return MKV_ERR_BAD_SHAPE;
   int32_t* ws = reinterpret_cast<int32_t*>(workspace);
   const size_t cells = (size_t)rows * max_blocks;
   // (a row asks for a copy and at most max_blocks pages: a row whose page is
@@ -565,7 +585,6 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
     int64_t widest;
     const int n = pools_at(tensors, row_bytes, num_tensors, t0, p, widest);
     const int64_t chunks = (widest * block_size + kCopyBytes - 1) / kCopyBytes;
-    if (chunks * n > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
     hipLaunchKernelGGL(copy_listed_kernel, dim3((unsigned)(chunks * n), (unsigned)(rows < kCopyRows ? rows : kCopyRows)), dim3(kCopyThreads), 0, s, p,
                        block_size, (int)chunks, a.copies);
     if (hipError_t e = hipGetLastError()) return (int)e;

@@ -1518,6 +1518,7 @@ int launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
 }
 
 constexpr int64_t kMaxRows = 65535 * 16 - 255;
+constexpr int64_t kMaxGrid = 0xffffff;  // workgroups of 256 threads: below 2^32 threads
 
 int check_tree(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim, int block_size,
                int max_blocks, int mask_cols) {
@@ -1583,7 +1584,7 @@ extern "C" int mkv_paged_tree(void* out, const void* q, int q_dtype, const void*
     return MKV_ERR_MISALIGNED;
   int kv;
   const Plan p = plan_of(num_seqs, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks, mask_cols, kv_dtype, kv);
-  if (p.units * kv * p.row_blocks > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
+  if (p.units * kv * p.row_blocks > kMaxGrid) return MKV_ERR_BAD_SHAPE;
   if (workspace_of(p, kv) > workspace_bytes || (p.splits && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
   const int pair = head_dim == 64 ? 2 : 1;
   TreeArgs a;
