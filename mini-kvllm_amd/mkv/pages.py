@@ -193,8 +193,9 @@ class PagePool:
 
     def fork(self, row: int, rows: Sequence[int]) -> torch.Tensor:
         """Let the given rows go on with row's sequence (see :meth:`assign`)."""
+        rows = list(rows)
         if not 0 <= row < self.rows or row in rows:
-            raise ValueError(f"row {row} must be one of 0..{self.rows - 1} and not among {list(rows)}")
+            raise ValueError(f"row {row} must be one of 0..{self.rows - 1} and not among {rows}")
         return self.assign(self._parents(rows, row))
 
     def free(self, rows: Sequence[int]) -> None:
