@@ -624,9 +624,12 @@ int mkv_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int
  * fresh page (the first too, if the page has holders besides).  Then the row grows
  * to pages for tokens[i] tokens (NULL: no growth).  Fresh pages are the
  * lowest-numbered with a count of 0 after all letting go, in row order, a copy
- * first; a row whose pages do not fit what is left (or the table) is refused
- * (granted[i] 0): it ends without pages, or as it was if it stayed.  A parent of
- * rows or more is refused.  Table entries past a row's pages become 0. */
+ * first; a row whose pages do not fit what the rows ahead of it asked for leaves is
+ * refused (granted[i] 0): it ends without pages, or as it was if it stayed.  What a
+ * refused row asked for counts as well: no row overtakes it, so that in a step where
+ * one is refused for want of pages, every row behind it that needs any is too (their
+ * requests fit once pages are let go, in the order of rows).  A row that does not fit
+ * the table, and a parent of rows or more, is refused and asks for nothing.  Table entries past a row's pages become 0. */
 int mkv_copy_pages(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,
                    int block_size, const void* src, const void* dst, int index_dtype, int64_t pairs, void* stream);
 int mkv_compact_slots(const void* const* tensors, const int64_t* row_bytes, int num_tensors, int64_t num_pages,

@@ -162,6 +162,8 @@ class PagePool:
         order.  Returns a bool (rows,) tensor: False for a row that was refused
         because the pool or the table has no room (it ends freed, or as it was if
         it went on with its own sequence), or because its parent is not a row.
+        Requests are served in row order: pages that a refused row asked for are
+        not handed to the rows behind it, which are refused too if they need any.
 
         parents, tokens: int32 or int64 (rows,).  seq_lens takes the parent's
         length (0 for a row without one: a new request's, set once its prompt is
