@@ -92,9 +92,10 @@ class Request:
 
 @dataclass(frozen=True)
 class TokenReport:
-    """A generated token's log probability, the entropy of the distribution
-    it was drawn from (in nats) and its likeliest tokens with their log
-    probabilities.  The distribution is the model's, at temperature 1."""
+    """A generated token's log probability, the entropy of the distribution (in
+    nats) and its likeliest tokens with their log probabilities.  All are of the
+    model's own distribution, that of its logits as they are: the request's
+    temperature, by which the token was drawn, is not in them."""
 
     logprob: float
     entropy: float
@@ -627,7 +628,7 @@ class Engine:
                     temperature: float = 1.0, logprobs: int | None = None) -> Request:
         """Queue a prompt.  ``logprobs``: report every generated token's log
         probability and that many of its likeliest alternatives (0 to 64) in
-        ``Request.reports``."""
+        ``Request.reports`` (at temperature 1, whatever the request's is)."""
         if len(prompt) + max_tokens > self.max_blocks * self.bs:
             raise ValueError("prompt + max_tokens exceeds max_model_len")
         if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, self.model.cfg.vocab_size):
