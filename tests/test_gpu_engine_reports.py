@@ -18,7 +18,7 @@ def test_reports_do_not_depend_on_the_temperature(dev, use_graphs):
     g = torch.Generator().manual_seed(23)
     prompts = [torch.randint(0, CFG.vocab_size, (n,), generator=g).tolist() for n in (9, 9, 40)]
     model = E.Qwen3Model(CFG, dev, seed=5, block_size=BS)
-    eng = E.Engine(model, num_blocks=96, max_num_seqs=3, max_num_batched_tokens=64, max_model_len=256,
+    eng = E.Engine(model, num_blocks=96, max_num_seqs=4, max_num_batched_tokens=64, max_model_len=256,
                    use_graphs=use_graphs)
     reqs = [eng.add_request(p, 5, temperature=t, logprobs=2) for p, t in zip(prompts, (4.0, 0.3, 2.5))]
     seen = 0
