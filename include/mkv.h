@@ -559,8 +559,10 @@ int mkv_linear(void* out, const void* x, int64_t x_row_stride, const void* w,
  * mkv_paged_tree: sequence s has n_s = cu_seqlens_q[s+1] - cu_seqlens_q[s]
  * drafted tokens, rows of q (total_q, num_heads, head_dim), whose K and V are
  * in the cache already: context_lens[s] counts them, and drafted token j sits at
- * position context_lens[s] - n_s + j.  Row i of the sequence sees every position
- * ahead of the drafted ones and drafted token j where
+ * position context_lens[s] - n_s + j (a context shorter than its tree has no
+ * prefix: token j at position j, those past the context in no cache and unseen).
+ * Row i of the sequence sees every position ahead of the drafted ones and drafted
+ * token j where
  * tree_mask[(cu_seqlens_q[s] + i) * mask_stride + j] is not 0 (j < mask_cols).
  * Softmax attention over what a row sees, scaled by sm_scale; a row that sees
  * nothing gives zeros.  Positions in absent (-1) blocks are not seen.  mask_cols

@@ -166,7 +166,8 @@ struct Units {
     for (int s0 = 64; s0 < a.num_seqs; s0 += 64) sum += wave_sum((float)keys(s0));
     // (a little more than the even share: at most `shares` units beside the last
     // one of each sequence, whatever the sum's rounding)
-    len = (int)fminf((float)sum * 1.0001f / (float)a.shares, 1.0e9f) + 1;
+    // (at most a block table's largest capacity, 0x7fff0000 keys: one unit then)
+    len = (int)fminf((float)sum * 1.0001f / (float)a.shares, 2147418112.0f) + 1;
     len = uniform((max(len, a.min_split) + TILE - 1) / TILE * TILE);
     total = number(0, a.num_seqs > 64 ? keys(0) : k0, 0);
     for (int s0 = 64; s0 < a.num_seqs; s0 += 64) total += number(s0, keys(s0), total);
