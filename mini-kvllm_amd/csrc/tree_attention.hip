@@ -1471,10 +1471,13 @@ Plan make_plan(int num_seqs, int64_t total_q, int kernel_kv_heads, int kernel_gr
   p.min_split = num_seqs * 4 <= round ? 128 : num_seqs * 2 <= round ? 256 : 1024;
   const int64_t most = (capacity + p.min_split - 1) / p.min_split;
   // Short block tables are not split at all: a second launch and the partial
-  // results cost more than the tiles one after another (one sequence, 8 KV heads,
-  // bf16: 16 rows of 700 keys 13.4 us against 17.6, of 1000 15.2 against 17.5; 64
-  // rows of 380 15.8 against 16.9, of 500 17.7 against 17.0; 128 rows of 250 16.5
-  // against 16.8, of 380 19.7 against 17.0; fp32 at 250 keys 21.1 against 19.3).
+  // results cost more than the tiles one after another where the host's calls follow
+  // each other (one sequence, 8 KV heads, bf16: 16 rows of 700 keys 13.4 us against
+  // 17.6, of 1000 15.2 against 17.5; 64 rows of 380 15.8 against 16.9, of 500 17.7
+  // against 17.0; 128 rows of 250 16.5 against 16.8, of 380 19.7 against 17.0; fp32 at
+  // 250 keys 21.1 against 19.3), and for many sequences anyhow (60 of 16 rows and
+  // 300-800 keys: bf16 30.4 against 33.2, FP8 20.4 against 23.5; one of 700 in a graph
+  // 13.1 against 12.1).  By the table's width: the contexts are on the device.
   const int64_t whole = f32 ? 128 : p.row_groups == 1 ? 1024 : p.row_groups == 2 ? 384 : 256;
   p.splits = most > 1 && capacity > whole;
   p.units = !p.splits ? num_seqs : num_seqs + shares < num_seqs * most ? num_seqs + shares : num_seqs * most;
