@@ -14,6 +14,7 @@
  *   K7  attention of trees of drafted tokens over the paged cache
  *   K8  token log probabilities, entropy and top alternatives
  *   K9  pages: copies, compaction of accepted rows, forks / growth / freeing
+ *   K10 verification of drafted tokens against the target's distribution
  *
  * Conventions
  *   - Every pointer is a device pointer unless stated otherwise.  The library
@@ -644,6 +645,38 @@ int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int n
                      int32_t* held, int32_t* ref_counts, const void* parents, int parents_dtype, const void* tokens,
                      int tokens_dtype, uint8_t* granted, int rows, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/* mkv_verify_drafts: the drafted tokens that the target's distribution accepts,
+ * from given random numbers, and the next token of each sequence.  Sequence s has
+ * the nodes cu_seqlens_q[s] .. cu_seqlens_q[s+1] of logits (total, vocab; fp32, bf16
+ * or fp16, any alignment of an element, row stride row_stride): node 0 is its last
+ * token, the others are drafted, node i a child of node parents[i] < i of the
+ * sequence (NULL: of i - 1) and token_ids[i].  Row i is the target's logits behind
+ * node i, and row i of draft_logits the draft's, from which the children's tokens
+ * were drawn (of dtype; rows without children are not read; NULL: the tokens were
+ * given without a distribution, as one that holds nothing else).  With
+ * p = softmax(logits / T), q = softmax(draft_logits / T), T = temperatures[s] (NULL:
+ * 1) the children of the node reached are looked at in their order: x is accepted if
+ * uniforms[x's row] q(x) < p(x), and its children are next; else p becomes
+ * max(0, p - q) over its sum.  accepted (num_seqs, max_nodes): the path's nodes,
+ * node 0 first, -1 behind; num_accepted: their number; next_tokens: argmax p / noise
+ * of what is left at the last of them, noise (num_seqs, vocab; row stride
+ * noise_stride) being exponential variates, the lowest index first among equals (of p
+ * itself where rounding leaves nothing).  acceptance (total): the chance of each node
+ * as the first of its siblings, min(1, p / q); 1 for node 0.
+ * T <= 1e-30 (0, say): greedy, the largest logit (the first of equals, a NaN largest)
+ * has all of p; so does a row with a NaN or +inf, or with -inf alone.  A draft row
+ * with one of these counts as absent.  Tokens outside the vocabulary and nodes whose
+ * parent is no earlier node are never accepted; nodes past max_nodes (<= 1024) are not
+ * looked at (acceptance 0); a sequence without nodes has num_accepted 0 and next token
+ * -1.  acceptance behind the last sequence is not written.  Sums are fp32. */
+size_t mkv_verify_drafts_workspace_size(int64_t total, int vocab, int num_seqs, int max_nodes, int has_draft);
+int mkv_verify_drafts(int64_t* accepted, int64_t* num_accepted, int64_t* next_tokens, float* acceptance,
+                      const void* logits, int64_t row_stride, const void* draft_logits, int64_t draft_stride, int dtype,
+                      int64_t total, int vocab, const void* token_ids, int ids_dtype, const void* parents,
+                      int parents_dtype, const int32_t* cu_seqlens_q, int num_seqs, int max_nodes,
+                      const float* uniforms, const float* noise, int64_t noise_stride, const float* temperatures,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Measurement helper (no counterpart in the reference; for benchmarks).

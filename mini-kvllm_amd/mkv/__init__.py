@@ -16,6 +16,8 @@ with the reference engine's Python call signatures:
   the paged cache (speculative decoding's verification step);
 * :func:`token_logprobs` — log probabilities of given tokens, entropy and
   top alternatives;
+* :func:`verify_drafts` — drafted tokens (chains, trees) accepted against the
+  target's distribution from given random numbers, and the next token;
 * :class:`CachePages`, :class:`PagePool` — page copies, compaction of accepted
   drafted tokens, and page tables whose rows fork, grow and are freed on the
   device;
@@ -30,6 +32,7 @@ from .context import (Context, MixedAttentionSplit, current_context, get_context
                       set_context, split_mixed_decode_prefill_metadata, use_context_provider)
 from .logprobs import TokenLogprobs, token_logprobs
 from .pages import CachePages, PagePool
+from .verify import VerifiedDrafts, verify_drafts
 
 __all__ = [
     "DECODE_STREAM", "DECODE_WORKGROUP", "FP8_E4M3_MAX", "Attention", "Context", "MixedAttentionSplit", "calibrate_fp8_per_tensor",
@@ -37,6 +40,7 @@ __all__ = [
     "paged_attention_decode_quantized", "paged_attention_prefill_triton", "reset_context",
     "set_context", "split_mixed_decode_prefill_metadata", "store_kvcache", "store_kvcache_fp8",
     "store_kvcache_int8",
-    "CachePages", "PagePool", "TokenLogprobs", "paged_attention_tree", "token_logprobs",
+    "CachePages", "PagePool", "TokenLogprobs", "VerifiedDrafts", "paged_attention_tree", "token_logprobs",
+    "verify_drafts",
     "current_context", "use_context_provider",
 ]

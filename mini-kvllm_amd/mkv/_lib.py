@@ -108,6 +108,11 @@ SIGNATURES: dict[str, tuple] = {
     "mkv_assign_pages": (c_int, [
         c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
         c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "mkv_verify_drafts_workspace_size": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
+    "mkv_verify_drafts": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_void_p,
+        c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_size_t,
+        c_void_p]),
     "mkv_stream_read_probe_sink_words": (c_size_t, [c_int]),
     "mkv_stream_read_probe": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p]),
 }
