@@ -14,6 +14,7 @@
  *   K7  attention of trees of drafted tokens over the paged cache
  *   K8  token log probabilities, entropy and top alternatives
  *   K9  pages: copies, compaction of accepted rows, forks / growth / freeing
+ *   K11 eviction by accumulated attention weight
  *   K10 verification of drafted tokens against the target's distribution
  *
  * Conventions
@@ -645,6 +646,34 @@ int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int n
                      int32_t* held, int32_t* ref_counts, const void* parents, int parents_dtype, const void* tokens,
                      int tokens_dtype, uint8_t* granted, int rows, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/* mkv_trim_pages: row i of a page table as mkv_assign_pages keeps it lets go of its
+ * pages past those of seq_lens[i] tokens: their counts fall by one, their entries
+ * become 0, held[i] falls (rows <= 1024; a row that holds no more than it needs is
+ * left alone). */
+int mkv_trim_pages(int32_t* block_tables, int64_t bt_stride, int max_blocks, const int64_t* seq_lens, int32_t* held,
+                   int32_t* ref_counts, int64_t num_pages, int block_size, int rows, void* stream);
+
+/* mkv_evict_tokens: every layer and KV head keeps budget tokens of each sequence of
+ * more than that: its first `sinks`, its last `recent` (sinks + recent <= budget) and,
+ * of the others, those with the largest weights (NaN above all, the earlier of equal
+ * ones), which are moved to its positions 0 .. budget - 1 in their order, by head.
+ * weights: a HOST array of num_layers device pointers, fp32 (num_pages, block_size,
+ * num_kv_heads) each; tensors: a HOST array of the num_tensors tensors whose rows move
+ * (the weights among them, if they shall), tensor t of layer layer_of[t], (num_pages,
+ * block_size, num_kv_heads, head_bytes[t] bytes), a multiple of 4 up to 2048 (HOST arrays);
+ * 16-byte accesses where head_bytes and base are multiples of 16.  The tensors do not
+ * overlap, and sequences share no page of the positions below budget.
+ * new_lens[b] = min(seq_lens[b], budget).  What lies at positions from budget on stays
+ * as it was; positions outside the block table or the pool are left out (their weights
+ * count as lowest). */
+size_t mkv_evict_tokens_workspace_size(int num_layers, int batch, int num_kv_heads, int block_size, int max_blocks,
+                                       int budget);
+int mkv_evict_tokens(const void* const* tensors, const int64_t* head_bytes, const int* layer_of, int num_tensors,
+                     const void* const* weights, int num_layers, int64_t num_pages, int block_size, int num_kv_heads,
+                     const int32_t* block_tables, int64_t bt_stride, int max_blocks, const void* seq_lens,
+                     int seq_lens_dtype, int batch, int budget, int sinks, int recent, int64_t* new_lens,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* mkv_verify_drafts: the drafted tokens that the target's distribution accepts,
  * from given random numbers, and the next token of each sequence.  Sequence s has

@@ -427,6 +427,25 @@ __global__ __launch_bounds__(kCopyThreads) void copy_listed_kernel(Pools p, int 
   }
 }
 
+// Rows let go of the pages past their tokens', a workgroup a row.
+__global__ __launch_bounds__(256) void trim_pages_kernel(int32_t* __restrict__ tables, int64_t bt_stride, int max_blocks,
+                                                        const int64_t* __restrict__ seq_lens, int32_t* held,
+                                                        int32_t* refs, int64_t num_pages, int bs_log2) {
+  const int r = blockIdx.x;
+  const int64_t len = max(seq_lens[r], (int64_t)0);
+  const int64_t need = (len + ((int64_t)1 << bs_log2) - 1) >> bs_log2;
+  const int has = min(max(held[r], 0), max_blocks);
+  __syncthreads();  // (every thread has read held[r])
+  if (need >= has) return;
+  int32_t* const row = tables + (int64_t)r * bt_stride;
+  for (int w = (int)need + threadIdx.x; w < has; w += 256) {
+    const int page = row[w];
+    if (page >= 0 && page < num_pages) __hip_atomic_fetch_add(refs + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    row[w] = 0;
+  }
+  if (threadIdx.x == 0) held[r] = (int)need;
+}
+
 int log2_exact(int64_t v) {
   if (v <= 0 || (v & (v - 1))) return -1;
   int l = 0;
@@ -590,4 +609,18 @@ extern "C" int mkv_assign_pages(const void* const* tensors, const int64_t* row_b
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
   return MKV_OK;
+}
+
+extern "C" int mkv_trim_pages(int32_t* block_tables, int64_t bt_stride, int max_blocks, const int64_t* seq_lens,
+                              int32_t* held, int32_t* ref_counts, int64_t num_pages, int block_size, int rows,
+                              void* stream) {
+  if (rows < 0 || rows > kMaxRows || num_pages < 0 || num_pages > 0x7fffffff || max_blocks < 0) return MKV_ERR_BAD_SHAPE;
+  const int bs_log2 = log2_exact(block_size);
+  if (bs_log2 < 0) return MKV_ERR_BAD_BLOCK_SIZE;
+  if (rows == 0) return MKV_OK;
+  if (!block_tables || !seq_lens || !held || !ref_counts) return MKV_ERR_NULL_POINTER;
+  if (bt_stride < max_blocks) return MKV_ERR_BAD_STRIDE;
+  hipLaunchKernelGGL(trim_pages_kernel, dim3((unsigned)rows), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
+                     block_tables, bt_stride, max_blocks, seq_lens, held, ref_counts, num_pages, bs_log2);
+  return (int)hipGetLastError();
 }

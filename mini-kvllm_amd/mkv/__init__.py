@@ -21,6 +21,8 @@ with the reference engine's Python call signatures:
 * :class:`CachePages`, :class:`PagePool` — page copies, compaction of accepted
   drafted tokens, and page tables whose rows fork, grow and are freed on the
   device;
+* :class:`CacheEviction` — tokens of little accumulated attention weight leave
+  the cache, by layer and KV head;
 * :class:`Attention` and :mod:`mkv.context` — the layer and per-step
   metadata the runner drives.
 """
@@ -30,6 +32,7 @@ from .attention import (DECODE_STREAM, DECODE_WORKGROUP, FP8_E4M3_MAX, Attention
                         paged_attention_tree, store_kvcache, store_kvcache_fp8, store_kvcache_int8)
 from .context import (Context, MixedAttentionSplit, current_context, get_context, reset_context,
                       set_context, split_mixed_decode_prefill_metadata, use_context_provider)
+from .eviction import CacheEviction
 from .logprobs import TokenLogprobs, token_logprobs
 from .pages import CachePages, PagePool
 from .verify import VerifiedDrafts, verify_drafts
@@ -40,7 +43,7 @@ __all__ = [
     "paged_attention_decode_quantized", "paged_attention_prefill_triton", "reset_context",
     "set_context", "split_mixed_decode_prefill_metadata", "store_kvcache", "store_kvcache_fp8",
     "store_kvcache_int8",
-    "CachePages", "PagePool", "TokenLogprobs", "VerifiedDrafts", "paged_attention_tree", "token_logprobs",
+    "CacheEviction", "CachePages", "PagePool", "TokenLogprobs", "VerifiedDrafts", "paged_attention_tree", "token_logprobs",
     "verify_drafts",
     "current_context", "use_context_provider",
 ]

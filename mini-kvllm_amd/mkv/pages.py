@@ -185,6 +185,15 @@ class PagePool:
                  granted.data_ptr(), self.rows, ws.data_ptr(), nbytes, _stream(self.device))
         return granted
 
+    def trim(self) -> None:
+        """Let every row go of its pages past those of seq_lens tokens (after an
+        eviction has shortened sequences, say).  On the device, in place; pages that
+        other rows hold too stay theirs."""
+        stride = self.block_tables.stride(0) if self.rows > 1 else self.max_blocks
+        _call_on(self.device, "mkv_trim_pages", self.block_tables.data_ptr(), stride, self.max_blocks,
+                 self.seq_lens.data_ptr(), self.held.data_ptr(), self.ref_counts.data_ptr(), self.pages.num_blocks,
+                 self.pages.block_size, self.rows, _stream(self.device))
+
     def _parents(self, rows: Sequence[int], parent: int) -> torch.Tensor:
         rows = list(rows)
         if not all(0 <= r < self.rows for r in rows) or len(set(rows)) != len(rows):

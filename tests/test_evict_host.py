@@ -1,0 +1,68 @@
+"""What the eviction and the page table's trim refuse, on the CPU: the wrappers'
+checks and the library's own (which return before any launch)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import mkv
+from mkv import _lib
+from test_step_operators_host import lib, p  # noqa: F401  (lib: a fixture)
+
+
+def evict(lib, **over):  # noqa: F811
+    n = 3
+    ptrs, layers = (ctypes.c_void_p * n)(p, p, p), (ctypes.c_int * n)(0, 0, 0)
+    a = dict(tensors=ctypes.addressof(ptrs), bytes=(ctypes.c_int64 * n)(256, 256, 4), layers=ctypes.addressof(layers), n=n,
+             weights=ctypes.addressof(ptrs), num_layers=1, pages=10, bs=16, heads=2, bt=p, stride=4, blocks=4, lens=p,
+             lens_dt=1, batch=2, budget=8, sinks=1, recent=2, new=p, ws=p, ws_bytes=1 << 20, stream=None)
+    assert set(over) <= set(a)
+    a.update(over)
+    if not isinstance(a["bytes"], (int, type(None))):
+        keep = a["bytes"]
+        a["bytes"] = ctypes.addressof(keep)
+    return lib.mkv_evict_tokens(*a.values())
+
+
+def test_evict_refusals(lib):  # noqa: F811
+    assert evict(lib, bs=24) == -6 and evict(lib, heads=0) == -2 and evict(lib, heads=1025) == -2
+    assert evict(lib, batch=70000) == -2 and evict(lib, budget=0) == -2 and evict(lib, sinks=-1) == -2
+    assert evict(lib, sinks=5, recent=4) == -2 and evict(lib, recent=2 ** 31 - 1) == -2
+    assert evict(lib, pages=1 << 28) == -2 and evict(lib, blocks=1 << 28, stride=1 << 28) == -2
+    for name in ("tensors", "bytes", "layers", "weights", "bt", "lens", "new", "ws"):
+        assert evict(lib, **{name: None}) == -1, name
+    assert evict(lib, stride=3) == -9 and evict(lib, lens_dt=4) == -3 and evict(lib, ws=p + 2) == -8
+    for size in (0, 6, 2052):
+        assert evict(lib, bytes=(ctypes.c_int64 * 3)(256, size, 4)) == -2
+    assert evict(lib, layers=ctypes.addressof((ctypes.c_int * 3)(0, 0, 1))) == -2
+    assert evict(lib, tensors=ctypes.addressof((ctypes.c_void_p * 3)(p, p + 2, p))) == -8
+    assert evict(lib, weights=ctypes.addressof((ctypes.c_void_p * 1)(None))) == -1
+    need = lib.mkv_evict_tokens_workspace_size(1, 2, 2, 16, 4, 8)
+    assert need == 2 * 2 * 8 * 4 and evict(lib, ws_bytes=need - 1) == -7
+    assert lib.mkv_evict_tokens_workspace_size(1, 2, 2, 16, 1024, 8) == 2 * 2 * (8 + 16384) * 4
+    assert evict(lib, batch=0) == 0 and evict(lib, num_layers=0, n=0) == 0
+    # (a grid past 2^32 threads)
+    assert evict(lib, batch=65535, heads=1024, ws_bytes=1 << 62) == -2
+
+
+def test_trim_refusals(lib):  # noqa: F811
+    def trim(bt=p, stride=4, blocks=4, lens=p, held=p, refs=p, pages=10, bs=16, rows=3):
+        return lib.mkv_trim_pages(bt, stride, blocks, lens, held, refs, pages, bs, rows, None)
+
+    assert trim(rows=1025) == -2 and trim(rows=-1) == -2 and trim(pages=1 << 31) == -2 and trim(bs=12) == -6
+    assert trim(stride=3) == -9 and trim(bt=None) == -1 and trim(lens=None) == -1 and trim(held=None) == -1
+    assert trim(refs=None) == -1 and trim(rows=0) == 0
+
+
+def test_the_wrapper_s_checks():
+    kv, w = torch.zeros(4, 16, 2, 8), torch.zeros(4, 16, 2)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        mkv.CacheEviction([kv], [kv.clone()], [w])
+    with pytest.raises(ValueError, match="every layer needs"):
+        mkv.CacheEviction([kv], [], [w])
+    with pytest.raises(ValueError, match="every layer needs"):
+        mkv.CacheEviction([], [], [])
+    with pytest.raises(ValueError, match="go together"):
+        mkv.CacheEviction([kv], [kv], [w], [w])
