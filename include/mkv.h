@@ -14,6 +14,7 @@
  *   K7  attention of trees of drafted tokens over the paged cache
  *   K8  token log probabilities, entropy and top alternatives
  *   K9  pages: copies, compaction of accepted rows, forks / growth / freeing
+ *   K12 attention weights accumulated beside the cache
  *   K11 eviction by accumulated attention weight
  *   K10 verification of drafted tokens against the target's distribution
  *
@@ -646,6 +647,37 @@ int mkv_assign_pages(const void* const* tensors, const int64_t* row_bytes, int n
                      int32_t* held, int32_t* ref_counts, const void* parents, int parents_dtype, const void* tokens,
                      int tokens_dtype, uint8_t* granted, int rows, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/* ------------------------------------------------------------------------
+ * What stays in the cache (no counterpart in the reference): attention weights
+ * accumulated beside it, eviction by them, and the verification of drafted tokens.
+ *
+ * mkv_paged_weights: weights, fp32 (num_blocks, block_size, num_kv_heads) in the
+ * pool's slot order, takes for every token t of a sequence's context and every KV
+ * head h
+ *
+ *   decay weights[slot(t), h] + sum_ij softmax_t(sm_scale q_ij . k_t)
+ *
+ * over the sequence's rows i of q (total_q, num_heads, head_dim) and the query heads
+ * j of h.  Sequence s has rows cu_seqlens_q[s] .. cu_seqlens_q[s+1] (NULL: row s
+ * alone, total_q = num_seqs), the last n_s tokens of its context: row i is at position
+ * context_lens[s] - n_s + i and sees the tokens up to there (one ahead of position 0
+ * none, and adds nothing).  The entries of those last n_s tokens, new to the cache,
+ * start from 0 whatever they hold; with decay 0 all do, and none is read.  Tokens past
+ * the block table and in absent (-1) blocks are not seen and have no entry; entries
+ * outside the contexts are left as they are.  Sequences that share pages must not be
+ * in one call.
+ * Cache formats, q types, scales (K's only) and groups as mkv_paged_tree; head_dim 64
+ * or 128 with any num_kv_heads; num_heads <= 8192.  Products are exact, their sums
+ * and the softmax fp32.  A row with a NaN score, or +inf, gives NaN to all it sees. */
+size_t mkv_paged_weights_workspace_size(int num_seqs, int64_t total_q, int num_heads, int num_kv_heads, int head_dim,
+                                        int block_size, int max_blocks, int kv_dtype, int one_row);
+int mkv_paged_weights(float* weights, float decay, const void* q, int q_dtype, const void* k_cache, int kv_dtype,
+                      int64_t num_blocks, const float* k_scale, int kv_scale_mode, const int32_t* block_tables,
+                      int64_t bt_stride, int max_blocks, const void* context_lens, int context_lens_dtype,
+                      const int32_t* cu_seqlens_q, int num_seqs, int64_t total_q, int num_heads, int num_kv_heads,
+                      int head_dim, int block_size, float sm_scale, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 /* mkv_trim_pages: row i of a page table as mkv_assign_pages keeps it lets go of its
  * pages past those of seq_lens[i] tokens: their counts fall by one, their entries

@@ -14,6 +14,8 @@ with the reference engine's Python call signatures:
 * :func:`gather_kv` — block-table gather;
 * :func:`paged_attention_tree` — attention of trees of drafted tokens over
   the paged cache (speculative decoding's verification step);
+* :func:`paged_attention_weights` — the attention weight that each cached token
+  receives, accumulated beside the cache (what an eviction goes by);
 * :func:`token_logprobs` — log probabilities of given tokens, entropy and
   top alternatives;
 * :func:`verify_drafts` — drafted tokens (chains, trees) accepted against the
@@ -29,7 +31,8 @@ with the reference engine's Python call signatures:
 from .attention import (DECODE_STREAM, DECODE_WORKGROUP, FP8_E4M3_MAX, Attention, calibrate_fp8_per_tensor,
                         flash_attention_prefill, gather_kv, paged_attention_decode,
                         paged_attention_decode_quantized, paged_attention_prefill_triton,
-                        paged_attention_tree, store_kvcache, store_kvcache_fp8, store_kvcache_int8)
+                        paged_attention_tree, paged_attention_weights, store_kvcache, store_kvcache_fp8,
+                        store_kvcache_int8)
 from .context import (Context, MixedAttentionSplit, current_context, get_context, reset_context,
                       set_context, split_mixed_decode_prefill_metadata, use_context_provider)
 from .eviction import CacheEviction
@@ -43,7 +46,8 @@ __all__ = [
     "paged_attention_decode_quantized", "paged_attention_prefill_triton", "reset_context",
     "set_context", "split_mixed_decode_prefill_metadata", "store_kvcache", "store_kvcache_fp8",
     "store_kvcache_int8",
-    "CacheEviction", "CachePages", "PagePool", "TokenLogprobs", "VerifiedDrafts", "paged_attention_tree", "token_logprobs",
+    "CacheEviction", "CachePages", "PagePool", "TokenLogprobs", "VerifiedDrafts", "paged_attention_tree",
+    "paged_attention_weights", "token_logprobs",
     "verify_drafts",
     "current_context", "use_context_provider",
 ]

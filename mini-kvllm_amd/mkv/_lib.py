@@ -108,6 +108,10 @@ SIGNATURES: dict[str, tuple] = {
     "mkv_assign_pages": (c_int, [
         c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
         c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "mkv_paged_weights_workspace_size": (c_size_t, [c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mkv_paged_weights": (c_int, [
+        c_void_p, c_float, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p,
+        c_int, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
     "mkv_trim_pages": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "mkv_evict_tokens_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "mkv_evict_tokens": (c_int, [

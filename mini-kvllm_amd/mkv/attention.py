@@ -18,6 +18,7 @@ paged_attention_decode_quantized attention.py:1213-1268 (fp8_per_tensor,
 paged_attention_prefill_triton  attention.py:852-891 (+ FP8 KV keywords)
 flash_attention_prefill         attention.py:446-514
 paged_attention_tree            (none: trees of drafted tokens)
+paged_attention_weights         (none: weights accumulated beside the cache)
 Attention                       attention.py:1617-1807
 ==============================  =========================================
 
@@ -640,6 +641,87 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
              tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], num_seqs, total, *sizes, float(scale),
              ws.data_ptr() if ws is not None else None, nbytes, _stream(dev))
     return out
+
+
+# ---------------------------------------------------------------------------
+# K12: attention weights beside the cache
+# ---------------------------------------------------------------------------
+def paged_attention_weights(query: torch.Tensor, k_cache: torch.Tensor, weights: torch.Tensor,
+                            block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                            num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, *,
+                            cu_seqlens_q: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                            kv_cache_dtype: str = "auto", decay: float = 1.0) -> torch.Tensor:
+    """Accumulate, beside the paged cache, the attention weight that each cached
+    token receives from a step's queries (what :class:`mkv.CacheEviction` goes by).
+
+    weights: fp32 (num_blocks, block_size, num_kv_heads), contiguous, in the cache's
+    slot order, changed in place and returned: every token of a sequence's context
+    gets decay times what it had plus the softmax weights that the sequence's rows
+    give it, summed over the rows and the query heads of its KV head.  query: (total,
+    num_heads, head_dim), rows of the last tokens of each context: one a sequence (a
+    decode step), or cu_seqlens_q (int32 (seqs + 1,)) of them (a chunk of a prompt, or
+    its last few queries), row i of n at position context_lens - n + i, seeing the
+    tokens up to there.  The tokens that these rows brought start from 0, whatever
+    their entries held; decay 0 starts every token of the contexts from 0.
+
+    The caches' formats, query types and scales are :func:`paged_attention_tree`'s
+    (K alone); head_dim 64 or 128.  Sequences of one call must not share pages.
+    Captured in a graph, a call accumulates anew at every replay."""
+    dev = _require_gpu(query, k_cache, weights, block_tables, context_lens,
+                       *(t for t in (cu_seqlens_q, k_scale) if t is not None))
+    if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
+        raise ValueError(f"query must be (total, {num_heads}, {head_dim}); got {tuple(query.shape)}")
+    _check_cache(k_cache, k_cache, num_kv_heads, head_dim)
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} != the cache's {k_cache.shape[1]}")
+    if weights.shape != k_cache.shape[:3] or weights.dtype != torch.float32 or not weights.is_contiguous():
+        raise ValueError(f"weights must be a contiguous float32 tensor of {tuple(k_cache.shape[:3])}; got "
+                         f"{weights.dtype} {tuple(weights.shape)}")
+    per_token = kv_cache_dtype in PER_TOKEN_HEAD_MODES
+    quant = k_cache.dtype in (torch.float8_e4m3fn, torch.int8)
+    if per_token:
+        want = torch.int8 if kv_cache_dtype == "int8_per_token_head" else torch.float8_e4m3fn
+        if k_cache.dtype != want:
+            raise TypeError(f"{kv_cache_dtype} needs a {want} cache, got {k_cache.dtype}")
+        _check_token_scales(k_scale, k_scale, k_cache)
+    elif k_cache.dtype == torch.int8:
+        raise ValueError("an int8 cache needs kv_cache_dtype='int8_per_token_head' and its scales")
+    elif quant:
+        if kv_cache_dtype not in ("fp8_per_tensor", "auto") or k_scale is None:
+            raise ValueError("an fp8 cache needs kv_cache_dtype='fp8_per_tensor' and k_scale")
+    elif kv_cache_dtype != "auto":
+        raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} does not go with a {k_cache.dtype} cache")
+    if quant:
+        if query.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"a quantised cache takes a bfloat16 or float16 query, got {query.dtype}")
+        if k_scale.dtype != torch.float32 or not k_scale.numel():
+            raise TypeError("k_scale must be a float32 tensor")
+    elif query.dtype != k_cache.dtype:
+        raise TypeError(f"query {query.dtype} and cache {k_cache.dtype} must share a dtype")
+    query = query.contiguous()
+    bt = _block_table(block_tables)
+    cl = _ctx_lens(context_lens)
+    total, num_seqs = query.shape[0], cl.numel()
+    cu = None if cu_seqlens_q is None else cu_seqlens_q.to(torch.int32).contiguous()
+    if cl.dim() != 1 or bt.dim() != 2 or bt.shape[0] < num_seqs or (total != num_seqs if cu is None else
+                                                                   cu.dim() != 1 or cu.numel() < num_seqs + 1):
+        raise ValueError(f"{total} rows, cu_seqlens_q {None if cu is None else tuple(cu.shape)} and block_tables "
+                         f"{tuple(bt.shape)} must fit {num_seqs} sequences (one row each without cu_seqlens_q)")
+    if num_seqs == 0 or bt.shape[1] == 0 or weights.numel() == 0:
+        return weights
+    kv_code = _dtype_code(k_cache, "k_cache")
+    sizes = (num_heads, num_kv_heads, head_dim, block_size)
+    nbytes = _lib.workspace_size("mkv_paged_weights_workspace_size", num_seqs, total, *sizes, bt.shape[1], kv_code,
+                                 int(cu is None))
+    # (of the call's own: calls on several streams and captured graphs share none)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call_on(dev, "mkv_paged_weights", weights.data_ptr(), float(decay), query.data_ptr(), _dtype_code(query, "query"),
+             k_cache.data_ptr(), kv_code, k_cache.shape[0], k_scale.data_ptr() if quant else None,
+             _lib.SCALE_PER_TOKEN_HEAD if per_token else _lib.SCALE_PER_TENSOR, bt.data_ptr(),
+             bt.stride(0) if num_seqs > 1 else bt.shape[1], bt.shape[1], cl.data_ptr(), _index_dtype(cl),
+             None if cu is None else cu.data_ptr(), num_seqs, total, *sizes, float(scale),
+             ws.data_ptr() if ws is not None else None, nbytes, _stream(dev))
+    return weights
 
 
 # ---------------------------------------------------------------------------

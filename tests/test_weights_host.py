@@ -1,0 +1,51 @@
+"""What the attention weights' operator refuses, on the CPU: the wrapper's checks
+and the library's own (which return before any launch)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import mkv
+from mkv import _lib
+from test_step_operators_host import lib, p  # noqa: F401  (lib: a fixture)
+
+
+def weights(lib, **over):  # noqa: F811
+    a = dict(w=p, decay=1.0, q=p, q_dt=_lib.DTYPE_BF16, k=p, kv_dt=_lib.DTYPE_BF16, blocks=8, ks=None, mode=0, bt=p,
+             bt_stride=4, max_blocks=4, ctx=p, ctx_dt=1, cu=p, seqs=2, total=16, hq=8, hkv=4, d=128, bs=16, scale=0.1,
+             ws=p, ws_bytes=1 << 20, stream=None)
+    assert set(over) <= set(a)
+    a.update(over)
+    return lib.mkv_paged_weights(*a.values())
+
+
+def test_refusals(lib):  # noqa: F811
+    assert weights(lib, d=96) == -4 and weights(lib, hq=9) == -5 and weights(lib, hq=68) == -5
+    assert weights(lib, bs=8) == -6 and weights(lib, bs=24) == -6
+    assert weights(lib, q_dt=_lib.DTYPE_F16) == -3 and weights(lib, kv_dt=_lib.DTYPE_I8) == -3
+    assert weights(lib, kv_dt=7) == -3 and weights(lib, mode=2) == -3 and weights(lib, ctx_dt=5) == -3
+    assert weights(lib, kv_dt=_lib.DTYPE_FP8E4M3, q_dt=_lib.DTYPE_F32) == -3
+    assert weights(lib, kv_dt=_lib.DTYPE_FP8E4M3) == -1
+    for name in ("w", "q", "k", "bt", "ctx"):
+        assert weights(lib, **{name: None}) == -1, name
+    assert weights(lib, bt_stride=3) == -9 and weights(lib, q=p + 8) == -8 and weights(lib, k=p + 2) == -8
+    assert weights(lib, w=p + 2) == -8 and weights(lib, ws=p + 8) == -8
+    assert weights(lib, seqs=-1) == -2 and weights(lib, total=-1) == -2 and weights(lib, blocks=1 << 30) == -2
+    assert weights(lib, max_blocks=1 << 28, bt_stride=1 << 28) == -2 and weights(lib, total=1 << 28) == -2
+    assert weights(lib, hq=16384, hkv=1024) == -2
+    # one row a sequence
+    assert weights(lib, cu=None) == -2 and weights(lib, cu=None, total=2, seqs=2, w=None) == -1
+    assert weights(lib, seqs=0) == 0 and weights(lib, max_blocks=0) == 0 and weights(lib, blocks=0) == 0
+    need = lib.mkv_paged_weights_workspace_size(2, 16, 8, 4, 128, 16, 4, _lib.DTYPE_BF16, 0)
+    assert need >= 16 * 8 * 4 and weights(lib, ws_bytes=need - 1) == -7
+    assert lib.mkv_paged_weights_workspace_size(2, 2, 8, 4, 128, 16, 4, _lib.DTYPE_BF16, 1) == 0
+    assert lib.mkv_paged_weights_workspace_size(2, 2, 8, 4, 128, 16, 4096, _lib.DTYPE_BF16, 1) > 0
+    # (a grid past 2^32 threads)
+    assert weights(lib, seqs=1 << 23, total=1 << 23, ws_bytes=1 << 62) == -2
+
+
+def test_the_wrapper_s_checks():
+    q, k, w = torch.zeros(2, 8, 128), torch.zeros(4, 16, 8, 128), torch.zeros(4, 16, 8)
+    bt, cl = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        mkv.paged_attention_weights(q, k, w, bt, cl, 0.1, 8, 8, 128, 16)
