@@ -28,6 +28,9 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// (lambdas whose arrays have to stay in registers)
+#define MKV_INLINE __attribute__((always_inline))
+
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr float kNegBig = -1e30f;
@@ -58,9 +61,10 @@ struct WeightArgs {
   float* ws_t;         // scores of split contexts
   f32x2* ws_ml;        // (sequence, KV head, unit, query): maximum and sum
   // chunks
-  int splits;          // of a row block's keys
-  f32x2* part_ml;      // (split, row): maximum and sum
-  float* lse;          // (row) log2 of the normaliser, +inf for a row that sees nothing
+  int shares;          // pieces of the normalisers' work, at most
+  f32x2* part_ml;      // (piece + block, KV head, row of the block): maximum and sum
+  float* lse;          // (row) log2 of the normaliser, +inf for a row that sees nothing;
+                       // rows by KV head, sequence, token and head of the group
 };
 
 template <int CT>
@@ -413,21 +417,47 @@ struct Rows {
 MKV_DEV void dma16(__amdgpu_buffer_rsrc_t r, char* lds, uint32_t voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
 }
-MKV_DEV void wait_all() {  // the wave's memory operations are done
+template <int N>
+MKV_DEV void wait_vm() {  // all but the wave's last N vector memory operations are done
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | 0xf70 | (N >> 4 << 14));
+  asm volatile("" ::: "memory");
+}
+// The workgroup's waves meet, their LDS operations done; loads stay in flight.
+MKV_DEV void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 MKV_DEV int div_group(const WeightArgs& a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.inv_group); }
 
-// Which of the sequences' parts (s has parts(s)) number `i` is, and its place in it;
-// false past the last.  Every wave works it out alike, a lane a sequence.
+template <class X>
+MKV_DEV X wave_sum(X x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+MKV_DEV int64_t lane64(int64_t x, int l) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)x, l));
+}
+// Which of the sequences' parts (sequence q has parts(q)) number i is: the sequence
+// and its place in it; false past the last.  Every wave works it out alike, a lane a
+// sequence, so that workgroups' numbers have no gaps.
+struct Place {
+  int seq, at, parts;
+  int first;  // number of the sequence's first part
+  Seq q;
+};
 template <class F>
-MKV_DEV bool find_part(int num_seqs, int i, int& seq, int& place, F parts) {
+MKV_DEV bool find_part(const WeightArgs& a, int i, Place& p, F parts) {
   const int lane = threadIdx.x & 63;
   int base = 0;
-  for (int s0 = 0; s0 < num_seqs; s0 += 64) {
-    const int n = s0 + lane < num_seqs ? parts(s0 + lane) : 0;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    const Seq q = seq_of(a, min(s0 + lane, a.num_seqs - 1));
+    const int n = s0 + lane < a.num_seqs ? parts(q) : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -438,8 +468,11 @@ MKV_DEV bool find_part(int num_seqs, int i, int& seq, int& place, F parts) {
     const uint64_t mine = __builtin_amdgcn_ballot_w64(i >= upto - n && i < upto);
     if (mine) {
       const int l = __builtin_ctzll(mine);
-      seq = s0 + l;
-      place = i - __builtin_amdgcn_readlane(upto - n, l);
+      p.seq = s0 + l;
+      p.parts = __builtin_amdgcn_readlane(n, l);
+      p.first = __builtin_amdgcn_readlane(upto, l) - p.parts;
+      p.at = i - p.first;
+      p.q = Seq{lane64(q.q0, l), lane64(q.n, l), lane64(q.first, l), __builtin_amdgcn_readlane(q.keys, l)};
       return true;
     }
     base = __builtin_amdgcn_readlane(upto, 63);
@@ -449,65 +482,147 @@ MKV_DEV bool find_part(int num_seqs, int i, int& seq, int& place, F parts) {
 
 template <int KV, int CT, int D>
 struct Formats {
-  static constexpr bool kF32 = KV == MKV_DTYPE_F32;
+  static constexpr bool kF32 = KV == MKV_DTYPE_F32, kCodes = DTypeInfo<KV>::kBytes == 1;
   static constexpr int kEb = DTypeInfo<KV>::kBytes;
   static constexpr int kQb = kF32 ? 4 : 2;
   static constexpr int kOps = kF32 ? D / 8 : D / 16;  // 16-byte operands of a lane's row of 32
   static constexpr int kBlocks = kF32 ? 1 : 2;        // blocks of 32 that a wave holds
 };
 
-// S = A B^T of two blocks of 32 rows, from their operands.
-template <bool F32, int CT, int N>
-MKV_DEV f32x16 product(const u32x4 (&A)[N], const u32x4 (&B)[N]) {
-  f32x16 s = f32x16{};
+// N MFMAs with V vector operations after each: what the scheduler is asked for where
+// products stand beside another block's exponentials.
+template <int N, int V>
+MKV_DEV void mix() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+  }
+}
+
+// S[b] = A B[b]^T of blocks of 32 rows, from their operands.
+template <bool F32, int CT, int NB, int N>
+MKV_DEV void products(const u32x4 (&A)[N], const u32x4 (&B)[NB][N], f32x16 (&S)[NB]) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b) S[b] = f32x16{};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(A[i][e]), __uint_as_float(B[i][e]), s, 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          S[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(A[i][e]), __uint_as_float(B[b][i][e]), S[b], 0, 0, 0);
     } else {
-      s = mfma32<CT>(A[i], B[i], s);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) S[b] = mfma32<CT>(A[i], B[b][i], S[b]);
     }
   }
-  return s;
 }
 
-constexpr int kStreamKeys = 128;  // a tile of K
+// A tile of K, a block of 32 at least for every group of waves that shares it out;
+// three tiles' room, so that loads have two tiles' time.
+template <int R>
+constexpr int kStreamKeys = R == 1 ? 128 : 64;
+constexpr int kMinPiece = 256;  // keys
+
+// The normalisers' work is (block of ROWS rows, its keys) after (block, its keys), in
+// the sequences' order, dealt out in even pieces: a piece may end one block and begin
+// the next (8 chunks of 512 rows over 1.5-4.6k keys, whole blocks in shares of their
+// own: 88 us).  Block b of a sequence costs what its last row sees, in keys x group,
+//   E(b) = first group + (b + 1) ROWS,   C(b) = E(0) + .. + E(b - 1),
+// whole numbers that doubles hold exactly.
+template <int ROWS, int TILE>
+struct Pieces {
+  const WeightArgs& a;
+  double total = 0.0;
+  int num;       // pieces
+  Seq own;       // of the lane's sequence (of the first 64)
+
+  MKV_DEV Seq lane_seq(int s0) const {
+    return s0 == 0 ? own : seq_of(a, min(s0 + (int)(threadIdx.x & 63), a.num_seqs - 1));
+  }
+  MKV_DEV int blocks(const Seq& q) const { return (int)((q.n * a.group + ROWS - 1) / ROWS); }
+  MKV_DEV double cost(const Seq& q, int b) const {  // C(b)
+    return (double)b * ((double)max(q.first, (int64_t)0) * a.group + 0.5 * ROWS * (b + 1));
+  }
+  MKV_DEV double start(int i) const { return i >= num ? total : floor(total * i / num); }
+  MKV_DEV explicit Pieces(const WeightArgs& args) : a(args) {
+    const int lane = threadIdx.x & 63;
+    own = seq_of(a, min(lane, a.num_seqs - 1));
+    for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+      const Seq q = lane_seq(s0);
+      total += wave_sum(s0 + lane < a.num_seqs ? cost(q, blocks(q)) : 0.0);
+    }
+    const double most = total / ((double)a.group * kMinPiece);
+    num = uniform(most < a.shares ? (int)most + 1 : a.shares);
+  }
+  // The sequence in which x lies (x < total): costs and blocks ahead of it.
+  MKV_DEV void find(double x, Seq& q, int& seq, double& base, int& base_blocks) const {
+    const int lane = threadIdx.x & 63;
+    base = 0.0;
+    base_blocks = 0;
+    for (int s0 = 0;; s0 += 64) {
+      const Seq s = lane_seq(s0);
+      const bool mine = s0 + lane < a.num_seqs;
+      const int n = mine ? blocks(s) : 0;
+      const double c = mine ? cost(s, n) : 0.0;
+      double upto = c;
+      int upto_n = n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(upto, o);
+        const int yn = __shfl_up(upto_n, o);
+        if (lane >= o) {
+          upto += y;
+          upto_n += yn;
+        }
+      }
+      upto += base;
+      const uint64_t here = __builtin_amdgcn_ballot_w64(mine && x < upto);
+      if (here || s0 + 64 >= a.num_seqs) {
+        const int l = here ? __builtin_ctzll(here) : 63;
+        seq = min(s0 + l, a.num_seqs - 1);
+        q = Seq{lane64(s.q0, l), lane64(s.n, l), lane64(s.first, l), __builtin_amdgcn_readlane(s.keys, l)};
+        base = __builtin_bit_cast(double, lane64(__builtin_bit_cast(int64_t, upto - c), l));
+        base_blocks += __builtin_amdgcn_readlane(upto_n - n, l);
+        return;
+      }
+      base = __builtin_bit_cast(double, lane64(__builtin_bit_cast(int64_t, upto), 63));
+      base_blocks += __builtin_amdgcn_readlane(upto_n, 63);
+    }
+  }
+  // The last block of the sequence that begins at y or ahead of it.
+  MKV_DEV int block_of(const Seq& q, double y) const {
+    int lo = 0, hi = blocks(q) - 1;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (cost(q, mid) <= y) lo = mid;
+      else hi = mid - 1;
+    }
+    return uniform(lo);
+  }
+  // The key at which a piece that begins (ends) y into a block does.
+  MKV_DEV int key_of(double y) const { return uniform((int)(y / a.group) / TILE * TILE); }
+};
 
 // The rows' normalisers.  R groups of waves hold different rows, 4 / R take different
-// keys of the same; blockIdx.y splits the keys further.
+// keys of the same.
 template <int KV, int CT, int D, int R>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weights_lse_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R == 1 ? 1 : 2))) void weights_lse_kernel(WeightArgs a) {
   using F = Formats<KV, CT, D>;
   using K = Rows<D * F::kEb>;
   constexpr int RB = D * F::kEb, KG = kWaves / R, NQ = F::kBlocks, kRows = 32 * NQ * R;
-  constexpr int kOwn = kStreamKeys / kWaves, kSubs = kOwn / 16, kDma = 16 * RB / 1024;
-  __shared__ __align__(16) char tile[2][kStreamKeys * RB];
-  __shared__ int there[2][kStreamKeys / 16];
-  __shared__ float scales[2][kStreamKeys];
+  constexpr int kStream = kStreamKeys<R>, kOwn = kStream / kWaves, kSubs = kOwn / 16, kDma = 16 * RB / 1024;
+  // (arrays by name: reads of one do not wait for the loads into another)
+  __shared__ __align__(16) char tile0[kStream * RB], tile1[kStream * RB], tile2[kStream * RB];
+  __shared__ __align__(16) float scales[3][F::kCodes ? kStream : 4];
   __shared__ f32x2 joined[KG > 1 ? kWaves : 1][32 * NQ];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int c = lane & 31, hf = lane >> 5, rg = wave % R, kg = wave / R;
-  const int h = blockIdx.x % a.num_kv_heads;
-  int seq, block;
-  if (!find_part(a.num_seqs, blockIdx.x / a.num_kv_heads, seq, block, [&](int s) {
-        const Seq q = seq_of(a, s);
-        return (int)((q.n * a.group + kRows - 1) / kRows);
-      }))
-    return;
-  seq = uniform(seq);
-  const Seq sq = seq_of(a, seq);
-  const int rows = (int)sq.n * a.group;
-  const int row0 = block * kRows + rg * 32 * NQ;  // this wave's first
-  // keys below limit(r) are seen by row r
-  auto limit = [&](int r) { return (int)min(max(sq.first + div_group(a, r) + 1, (int64_t)0), (int64_t)sq.keys); };
-  const int k_end = limit(min(block * kRows + kRows, rows) - 1);
-  // this split's share of them, whole tiles
-  const int share = ((k_end + a.splits - 1) / a.splits + kStreamKeys - 1) / kStreamKeys * kStreamKeys;
-  const int kb0 = (int)min((int64_t)blockIdx.y * share, (int64_t)k_end), k1 = (int)min((int64_t)kb0 + share, (int64_t)k_end);
-  const bool active = row0 < rows;
-  const int low = active ? limit(row0) : 0, high = active ? limit(min(row0 + 32 * NQ, rows) - 1) : 0;
+  const int h = blockIdx.x % a.num_kv_heads, piece = blockIdx.x / a.num_kv_heads;
+  const Pieces<kRows, kStream> work(a);
+  if (piece >= work.num) return;
   float mul = a.mul;
   if (a.scale_mode == 1) mul *= load_uniform_f32(a.k_scale);
   // the maximum is of raw scores and wants mul > 0: its sign goes into q (0: q is 0)
@@ -517,24 +632,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     keep = mul < 0.0f ? keep : 0u;
     mul = mul < 0.0f ? -mul : 1.0f;
   }
-  u32x4 q[NQ][F::kOps];
-  int lim[NQ];
-#pragma unroll
-  for (int b = 0; b < NQ; ++b) {
-    const int r = row0 + 32 * b + c;
-    const bool ok = r < rows;
-    const int tok = div_group(a, ok ? r : 0), j = (ok ? r : 0) - tok * a.group;
-    const char* p = a.q + ((sq.q0 + tok) * a.num_heads + h * a.group + j) * (int64_t)(D * F::kQb);
-    lim[b] = ok ? limit(r) : 0;
-#pragma unroll
-    for (int s = 0; s < F::kOps; ++s) {
-      const int d = F::kF32 ? 8 * s + 4 * hf : F::kEb == 2 ? 16 * s + 8 * hf : 16 * (2 * (s >> 1) + hf) + 8 * (s & 1);
-      q[b][s] = ok ? ld16(p + d * F::kQb) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[b][s][e] = (q[b][s][e] ^ sign) & keep;
-    }
-  }
-  // ---- loads of tiles: a wave 32 keys, sub-tiles of 16 never across a block ----
+  // ---- loads of tiles: a wave its share, sub-tiles of 16 keys never across a block ----
   const int64_t row_bytes = (int64_t)a.num_kv_heads * RB;
   uint32_t voff[kDma];
 #pragma unroll
@@ -542,45 +640,91 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     const int r = i * K::kPerDma + lane / K::kChunks;
     voff[i] = (uint32_t)(r * row_bytes) + 16 * ((lane % K::kChunks) ^ K::swz(r));
   }
-  float scale_next = 1.0f;
-  auto issue = [&](int kb, int to) {
+  const double end = work.start(piece + 1);
+  for (double x = work.start(piece); x < end;) {
+    Seq sq;
+    int seq, base_blocks;
+    double base;
+    work.find(x, sq, seq, base, base_blocks);
+    const int block = work.block_of(sq, x - base);
+    const double c0 = base + work.cost(sq, block), c1 = base + work.cost(sq, block + 1);
+    const bool whole = x <= c0 && end >= c1;
+    const int rows = (int)sq.n * a.group;
+    const int row0 = block * kRows + rg * 32 * NQ;  // this wave's first
+    // keys below limit(r) are seen by row r
+    auto limit = [&](int r) { return (int)min(max(sq.first + div_group(a, r) + 1, (int64_t)0), (int64_t)sq.keys); };
+    const int k_end = limit(min(block * kRows + kRows, rows) - 1);
+    const int kb0 = min(work.key_of(max(x - c0, 0.0)), k_end), k1 = end >= c1 ? k_end : min(work.key_of(end - c0), k_end);
+    x = c1;
+    const bool active = row0 < rows;
+    const int low = active ? limit(row0) : 0, high = active ? limit(min(row0 + 32 * NQ, rows) - 1) : 0;
+    u32x4 q[NQ][F::kOps];
+    int lim[NQ];
 #pragma unroll
-    for (int u = 0; u < kSubs; ++u) {
-      const int at = wave * kOwn + 16 * u, t = kb + at;
-      const int64_t phys = t < k1 ? a.idx.physical_block(seq, t >> a.idx.bs_log2) : -1;
-      const int64_t slot = (max(phys, (int64_t)0) << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1));
-      const int left = phys >= 0 ? min(k1 - t, 16) : 0;
-      // (rows past the last read zeros)
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(a.k + (phys >= 0 ? slot : 0) * row_bytes + (int64_t)h * RB), (short)0,
-          left > 0 ? (int)((left - 1) * row_bytes + RB) : 0, 0x00020000);
+    for (int b = 0; b < NQ; ++b) {
+      const int r = row0 + 32 * b + c;
+      const bool ok = r < rows;
+      const int tok = div_group(a, ok ? r : 0), j = (ok ? r : 0) - tok * a.group;
+      const char* p = a.q + ((sq.q0 + tok) * a.num_heads + h * a.group + j) * (int64_t)(D * F::kQb);
+      lim[b] = ok ? limit(r) : 0;
 #pragma unroll
-      for (int i = 0; i < kDma; ++i) dma16(r, &tile[to][at * RB + i * 1024], voff[i]);
-      if (lane == 0) there[to][at / 16] = left > 0;
+      for (int s = 0; s < F::kOps; ++s) {
+        const int d = F::kF32 ? 8 * s + 4 * hf : !F::kCodes ? 16 * s + 8 * hf : 16 * (2 * (s >> 1) + hf) + 8 * (s & 1);
+        q[b][s] = ld16(p + d * F::kQb);  // (within q for any row)
+      }
     }
-    if (a.scale_mode == 2 && tid < kStreamKeys) {
-      const int t = kb + tid, slot = t < k1 ? slot_of(a, seq, t) : -1;
-      scale_next = slot >= 0 ? a.k_scale[(int64_t)slot * a.num_kv_heads + h] : 0.0f;
-    }
-  };
-  float m[NQ], l[NQ];
+    // The tile's block entries, a lane a sub-tile, come a tile ahead of its loads.
+    auto entries = [&](int kb) -> int {
+      const int t = kb + 16 * (lane & (kStream / 16 - 1));
+      const int blk = min(t >> a.idx.bs_log2, a.idx.max_blocks - 1);
+      return a.idx.block_tables[(int64_t)seq * a.idx.bt_stride + blk];
+    };
+    // which sub-tiles are there, a bit each
+    auto presence = [&](int kb, int e) -> uint32_t {
+      const bool ok = kb + 16 * (lane & (kStream / 16 - 1)) < k1 && e >= 0 && e < a.idx.num_blocks;
+      return (uint32_t)__builtin_amdgcn_ballot_w64(ok) & ((1u << kStream / 16) - 1);
+    };
+    float scale_next[3] = {1.0f, 1.0f, 1.0f};
+    uint32_t there[3];
+    auto issue = [&](int kb, int e, auto nth) MKV_INLINE {
+      constexpr int to_tile = decltype(nth)::value;
+      char* const to = to_tile == 0 ? tile0 : to_tile == 1 ? tile1 : tile2;
+      there[to_tile] = presence(kb, e);
 #pragma unroll
-  for (int b = 0; b < NQ; ++b) {
-    m[b] = kNegBig;
-    l[b] = 0.0f;
-  }
-  if (kb0 < k1) issue(kb0, 0);
-  for (int kb = kb0, par = 0; kb < k1; kb += kStreamKeys, par ^= 1) {
-    if (a.scale_mode == 2 && tid < kStreamKeys) scales[par][tid] = scale_next;
-    wait_all();
-    __syncthreads();  // the tile is here, and everyone is done with the other one
-    if (kb + kStreamKeys < k1) issue(kb + kStreamKeys, par ^ 1);
-    for (int kbl = kg; kbl < kStreamKeys / 32; kbl += KG) {
-      const int key0 = kb + 32 * kbl;
-      if (key0 >= min(high, k1)) break;
-      u32x4 k[F::kOps];
-      const char* const at = tile[par] + 32 * kbl * RB;
-      if constexpr (F::kEb >= 2) {
+      for (int u = 0; u < kSubs; ++u) {
+        const int sub = wave * kSubs + u, t = kb + 16 * sub;
+        const bool ok = there[to_tile] >> sub & 1;
+        const int64_t slot = ok ? ((int64_t)__builtin_amdgcn_readlane(e, sub) << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : 0;
+        // (rows past the last read zeros)
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(a.k + slot * row_bytes + (int64_t)h * RB), (short)0,
+            ok ? (int)((min(k1 - t, 16) - 1) * row_bytes + RB) : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kDma; ++i) dma16(r, to + 16 * sub * RB + i * 1024, voff[i]);
+      }
+      if (F::kCodes && a.scale_mode == 2 && tid < kStream) {
+        const int t = kb + tid, slot = t < k1 ? slot_of(a, seq, t) : -1;
+        scale_next[to_tile] = slot >= 0 ? a.k_scale[(int64_t)slot * a.num_kv_heads + h] : 0.0f;
+      }
+    };
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      m[b] = kNegBig;
+      l[b] = 0.0f;
+    }
+    // The scores of 32 keys wait while the next block's products run, so that one
+    // wave's matrix and vector operations overlap.
+    f32x16 pend[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) pend[b] = kNegInf;  // (adds nothing)
+    int pend_key = -0x40000000;  // its first key
+    bool pend_lo = true, pend_up = true;
+    float pend_scale[F::kCodes ? 16 : 1];
+#pragma unroll
+    for (int e = 0; e < (F::kCodes ? 16 : 1); ++e) pend_scale[e] = 1.0f;
+    auto k_operand = [&](const char* at, u32x4 (&k)[F::kOps]) MKV_INLINE {
+      if constexpr (!F::kCodes) {
 #pragma unroll
         for (int s = 0; s < F::kOps; ++s) k[s] = *reinterpret_cast<const u32x4*>(at + K::offset(c, 2 * s + hf));
       } else {
@@ -591,25 +735,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           k[s + 1] = codes_to_16<KV, CT>(w[2], w[3]);
         }
       }
-      const bool lo_there = uniform(there[par][2 * kbl]) != 0, up_there = uniform(there[par][2 * kbl + 1]) != 0;
-      const bool masked = key0 + 32 > min(low, k1) || !lo_there || !up_there;
+    };
+    auto softmax = [&](auto masked) MKV_INLINE {  // of what waits
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
-        f32x16 s = product<F::kF32, CT>(k, q[b]);
-        if (a.scale_mode == 2) {
+        f32x16& s = pend[b];
+        if (F::kCodes && a.scale_mode == 2) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(&scales[par][32 * kbl + 8 * g + 4 * hf]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] *= x[e];
-          }
+          for (int e = 0; e < 16; ++e) s[e] *= pend_scale[F::kCodes ? e : 0];
         }
-        if (masked) {
-          const int lm = min(lim[b], k1) - key0 - 4 * hf;
+        if constexpr (decltype(masked)::value) {
+          const int lm = min(lim[b], k1) - pend_key - 4 * hf;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int kl = 8 * (e >> 2) + (e & 3);
-            s[e] = kl < lm && (e < 8 ? lo_there : up_there) ? s[e] : kNegInf;
+            s[e] = kl < lm && (e < 8 ? pend_lo : pend_up) ? s[e] : kNegInf;
           }
         }
         float mx = s[0];
@@ -618,10 +758,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         mx = fmaxf(mx, other_half(mx));
         mx = fmaxf(mx * mul, kNegBig);
         const float m_new = mx > m[b] + kRescaleSlack ? mx : m[b];
-        if (__builtin_amdgcn_ballot_w64(m_new != m[b])) {
-          l[b] *= __builtin_amdgcn_exp2f(m[b] - m_new);
-          m[b] = m_new;
-        }
+        l[b] *= __builtin_amdgcn_exp2f(m[b] - m_new);
+        m[b] = m_new;
         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
@@ -630,55 +768,159 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
         l[b] += sum0 + sum1;
       }
-    }
-  }
+    };
+    auto needs_mask = [&] { return pend_key + 32 > min(low, k1) || !pend_lo || !pend_up; };
+    auto attend = [&](const char* at, const float* sc, int key0, bool lo_there, bool up_there) MKV_INLINE {
+      u32x4 k[F::kOps];
+      k_operand(at, k);
+      f32x16 s[NQ];
+      if (needs_mask()) {
+        products<F::kF32, CT, NQ>(k, q, s);
+        softmax(std::true_type{});
+      } else {  // (one basic block: the products among the exponentials)
+        products<F::kF32, CT, NQ>(k, q, s);
+        softmax(std::false_type{});
+        mix<F::kF32 ? 64 : NQ * F::kOps, F::kF32 ? 2 : 8>();
+      }
 #pragma unroll
-  for (int b = 0; b < NQ; ++b) l[b] += other_half(l[b]);
-  if constexpr (KG > 1) {
-    if (hf == 0) {
+      for (int b = 0; b < NQ; ++b) pend[b] = s[b];
+      pend_key = key0;
+      pend_lo = lo_there;
+      pend_up = up_there;
+      if (F::kCodes && a.scale_mode == 2) {
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) joined[wave][32 * b + c] = f32x2{m[b], l[b]};
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(sc + 8 * g + 4 * hf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pend_scale[F::kCodes ? 4 * g + e : 0] = y[e];
+        }
+      }
+    };
+    int e_next = 0;
+    auto step = [&](int kb, auto nth) MKV_INLINE {
+      constexpr int n = decltype(nth)::value;
+      if (kb >= k1) return;
+      const char* const tile = n == 0 ? tile0 : n == 1 ? tile1 : tile2;
+      if (kb + kStream < k1)
+        wait_vm<kSubs * kDma>();  // (the next tile's loads may be on their way)
+      else
+        wait_vm<0>();
+      if (F::kCodes && a.scale_mode == 2 && tid < kStream) scales[n][tid] = scale_next[n];
+      meet();  // the tile is here, and everyone is done with the one before
+      if (kb + 2 * kStream < k1) {
+        const int e = e_next;
+        e_next = entries(kb + 3 * kStream);
+        issue(kb + 2 * kStream, e, std::integral_constant<int, (n + 2) % 3>{});
+      }
+#pragma unroll
+      for (int kbl0 = 0; kbl0 < kStream / 32; kbl0 += KG) {
+        const int kbl = kbl0 + kg, key0 = kb + 32 * kbl;
+        if (kbl >= kStream / 32 || key0 >= min(high, k1)) break;
+        attend(tile + 32 * kbl * RB, &scales[n][F::kCodes ? 32 * kbl : 0], key0, there[n] >> 2 * kbl & 1, there[n] >> (2 * kbl + 1) & 1);
+      }
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    meet();  // (everyone is done with the block before)
+    if (kb0 < k1) {
+      const int e0 = entries(kb0), e1 = entries(kb0 + kStream);
+      e_next = entries(kb0 + 2 * kStream);
+      issue(kb0, e0, I0{});
+      if (kb0 + kStream < k1) issue(kb0 + kStream, e1, I1{});
     }
-    __syncthreads();
-    if (kg > 0) return;
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int s = 0; s < F::kOps; ++s) {
+        const uint32_t k = row0 + 32 * b + c < rows ? keep : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[b][s][e] = (q[b][s][e] ^ sign) & k;
+      }
+    for (int kb = kb0; kb < k1; kb += 3 * kStream) {
+      step(kb, I0{});
+      step(kb + kStream, I1{});
+      step(kb + 2 * kStream, I2{});
+    }
+    softmax(std::true_type{});
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) l[b] += other_half(l[b]);
+    if constexpr (KG > 1) {
+      if (hf == 0) {
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) joined[wave][32 * b + c] = f32x2{m[b], l[b]};
+      }
+      meet();
+      if (kg > 0) continue;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        float top = m[b], sum = 0.0f;
+#pragma unroll
+        for (int g = 1; g < KG; ++g) top = fmaxf(top, joined[g * R + rg][32 * b + c][0]);
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          const f32x2 v = joined[g * R + rg][32 * b + c];
+          sum += v[1] * __builtin_amdgcn_exp2f(v[0] - top);
+        }
+        m[b] = top;
+        l[b] = sum;
+      }
+    }
+    if (hf) continue;
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
-      float top = m[b], sum = 0.0f;
-#pragma unroll
-      for (int g = 1; g < KG; ++g) top = fmaxf(top, joined[g * R + rg][32 * b + c][0]);
-#pragma unroll
-      for (int g = 0; g < KG; ++g) {
-        const f32x2 v = joined[g * R + rg][32 * b + c];
-        sum += v[1] * __builtin_amdgcn_exp2f(v[0] - top);
-      }
-      m[b] = top;
-      l[b] = sum;
+      const int r = row0 + 32 * b + c;
+      if (r >= rows) continue;
+      if (whole)
+        a.lse[(h * a.total_q + sq.q0) * a.group + r] = l[b] == 0.0f ? -kNegInf : m[b] + __builtin_amdgcn_logf(l[b]);
+      else  // (pieces and blocks rise together: their sum is a place of its own)
+        a.part_ml[((int64_t)(piece + base_blocks + block) * a.num_kv_heads + h) * kRows + r - block * kRows] = f32x2{m[b], l[b]};
     }
-  }
-  if (hf) return;
-#pragma unroll
-  for (int b = 0; b < NQ; ++b) {
-    const int r = row0 + 32 * b + c;
-    if (r >= rows) continue;
-    const int tok = div_group(a, r);
-    const int64_t at = (sq.q0 + tok) * a.num_heads + h * a.group + r - tok * a.group;
-    if (a.splits > 1)
-      a.part_ml[blockIdx.y * a.total_q * a.num_heads + at] = f32x2{m[b], l[b]};
-    else
-      a.lse[at] = l[b] == 0.0f ? -kNegInf : m[b] + __builtin_amdgcn_logf(l[b]);
   }
 }
 
+// Rows whose keys were in several pieces, a workgroup a block of them.
+template <int ROWS, int TILE>
 __global__ __launch_bounds__(kThreads) void weights_join_kernel(WeightArgs a) {
-  const int64_t n = a.total_q * a.num_heads, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n) return;
-  float m = kNegBig, l = 0.0f;
-  for (int z = 0; z < a.splits; ++z) m = fmaxf(m, a.part_ml[z * n + i][0]);
-  for (int z = 0; z < a.splits; ++z) {
-    const f32x2 v = a.part_ml[z * n + i];
-    l += v[1] * __builtin_amdgcn_exp2f(v[0] - m);
+  const int h = blockIdx.x % a.num_kv_heads, number = blockIdx.x / a.num_kv_heads;
+  const Pieces<ROWS, TILE> work(a);
+  Place p;
+  if (!find_part(a, number, p, [&](const Seq& q) { return work.blocks(q); })) return;
+  double base = 0.0;
+  for (int s0 = 0; s0 <= p.seq; s0 += 64) {
+    const Seq q = work.lane_seq(s0);
+    base += wave_sum(s0 + (int)(threadIdx.x & 63) < p.seq ? work.cost(q, work.blocks(q)) : 0.0);
   }
-  a.lse[i] = l == 0.0f ? -kNegInf : m + __builtin_amdgcn_logf(l);
+  const double c0 = base + work.cost(p.q, p.at), c1 = base + work.cost(p.q, p.at + 1);
+  // the pieces from `lo` to `hi` have a part of it
+  int lo = (int)(c0 / work.total * work.num), hi = (int)(c1 / work.total * work.num);
+  while (lo > 0 && work.start(lo) > c0) --lo;
+  while (lo + 1 < work.num && work.start(lo + 1) <= c0) ++lo;
+  hi = min(hi, work.num - 1);
+  while (hi + 1 < work.num && work.start(hi + 1) < c1) ++hi;
+  while (hi > lo && work.start(hi) >= c1) --hi;
+  const int n = hi - lo + 1;
+  if (n == 1) return;
+  const int rows = (int)p.q.n * a.group - p.at * ROWS;
+  const f32x2* part = a.part_ml + ((int64_t)(lo + number) * a.num_kv_heads + h) * ROWS;
+  const int64_t step = (int64_t)a.num_kv_heads * ROWS;
+  for (int r = threadIdx.x; r < min(rows, ROWS); r += kThreads) {
+    constexpr int kAhead = 8;
+    float m = kNegBig, l = 0.0f;
+    for (int z0 = 0; z0 < n; z0 += kAhead) {
+      f32x2 v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j] = part[min(z0 + j, n - 1) * step + r];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (z0 + j < n) {
+          const float top = fmaxf(m, v[j][0]);
+          l = l * __builtin_amdgcn_exp2f(m - top) + v[j][1] * __builtin_amdgcn_exp2f(v[j][0] - top);
+          m = top;
+        }
+    }
+    a.lse[(h * a.total_q + p.q.q0) * a.group + p.at * ROWS + r] = l == 0.0f ? -kNegInf : m + __builtin_amdgcn_logf(l);
+  }
 }
 
 // The keys' weights.
@@ -689,25 +931,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   using Q = Rows<RB>;
   constexpr int NK = F::kBlocks, kUnit = 32 * NK * kWaves, kTile = 16384 / RB;  // rows of q a tile: 32, 64 or 128
   constexpr int kDma = kTile / kWaves / Q::kPerDma;
-  __shared__ __align__(16) char tile[2][kTile * RB];
-  __shared__ __align__(16) float lse[2][kTile];
-  __shared__ __align__(16) int last[2][kTile];  // the position of a row: the last that it sees
+  constexpr int kNorms = kTile > 64 ? kTile / 64 : 1;  // loads of their normalisers
+  __shared__ __align__(16) char tile0[kTile * RB], tile1[kTile * RB], tile2[kTile * RB];
+  __shared__ __align__(16) float norm0[64 * kNorms], norm1[64 * kNorms], norm2[64 * kNorms];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, hf = lane >> 5;
   float mul0 = a.mul;
   if (a.scale_mode == 1) mul0 *= load_uniform_f32(a.k_scale);
   for (int64_t at = blockIdx.x;; at += gridDim.x) {
     const int h = (int)(at % a.num_kv_heads);
-    int seq, place;
+    Place place;
     if (at / a.num_kv_heads > 0x7fffffff ||
-        !find_part(a.num_seqs, (int)(at / a.num_kv_heads), seq, place, [&](int s) {
-          const Seq q = seq_of(a, s);
-          return (q.keys + kUnit - 1) / kUnit;
-        }))
+        !find_part(a, (int)(at / a.num_kv_heads), place, [&](const Seq& q) { return (q.keys + kUnit - 1) / kUnit; }))
       return;
-    seq = uniform(seq);
-    const Seq sq = seq_of(a, seq);
+    const int seq = place.seq;
+    const Seq sq = place.q;
     const int rows = (int)sq.n * a.group;
-    const int unit0 = place * kUnit, key0 = unit0 + wave * 32 * NK;  // this wave's first key
+    const int unit0 = place.at * kUnit, key0 = unit0 + wave * 32 * NK;  // this wave's first key
     // ---- this lane's keys ----
     u32x4 k[NK][F::kOps];
     float mul[NK], sum[NK];
@@ -730,12 +969,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       if (a.scale_mode == 2) mul[b] *= a.k_scale[(int64_t)max(slot[b], 0) * a.num_kv_heads + h];
       sum[b] = 0.0f;
     }
-    // ---- rows that see any of the unit's keys ----
-    const int64_t skip = max((int64_t)unit0 - sq.first, (int64_t)0) * a.group;
-    const int r_begin = (int)min(skip, (int64_t)rows) / kTile * kTile;
-    float lse_next = 0.0f;
-    int last_next = 0;
-    auto issue = [&](int r0, int to) {
+    // ---- key t is seen by the rows from (t - first) group on: those that see any of
+    // the unit's keys, and each lane's keys' first ----
+    auto first_row = [&](int t) {
+      return (int)min(max((int64_t)t - sq.first, (int64_t)0) * a.group, (int64_t)0x7fffffff);
+    };
+    const int r_begin = min(first_row(unit0), rows) / kTile * kTile;
+    const int none = first_row(key0), all = first_row(key0 + 32 * NK - 1);
+    int from[NK];
+#pragma unroll
+    for (int b = 0; b < NK; ++b) from[b] = first_row(key0 + 32 * b + c);
+    const int64_t norms = (h * a.total_q + sq.q0) * a.group;
+    auto issue = [&](int r0, auto nth) {
+      constexpr int n = decltype(nth)::value;
+      char* const to = n == 0 ? tile0 : n == 1 ? tile1 : tile2;
+      float* const to_norm = n == 0 ? norm0 : n == 1 ? norm1 : norm2;
       const int tok0 = div_group(a, r0), tok1 = div_group(a, min(r0 + kTile, rows) - 1);
       const int64_t head = (sq.q0 + tok0) * a.num_heads + h * a.group;  // tok0's first row
       const __amdgpu_buffer_rsrc_t r =
@@ -748,63 +996,79 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         const uint32_t off = (uint32_t)(((tok - tok0) * a.num_heads + row - tok * a.group) * RB) +
                              16 * ((lane % Q::kChunks) ^ Q::swz(in));
         // (rows past the last read zeros)
-        dma16(r, &tile[to][(wave * (kTile / kWaves) + i * Q::kPerDma) * RB], row < rows ? off : 0x7ffffff0u);
+        dma16(r, to + (wave * (kTile / kWaves) + i * Q::kPerDma) * RB, row < rows ? off : 0x7ffffff0u);
       }
-      if (tid < kTile) {
-        const int row = r0 + tid, tok = div_group(a, row);
-        lse_next = row < rows ? a.lse[(sq.q0 + tok) * a.num_heads + h * a.group + row - tok * a.group] : -kNegInf;
-        last_next = row < rows ? (int)min(max(sq.first + tok, (int64_t)-1), (int64_t)0x7fffffff) : -1;
+      // (every wave loads the same normalisers to the same place, and counts as many)
+      const __amdgpu_buffer_rsrc_t ln = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(a.lse + norms + r0), (short)0, min(rows - r0, kTile) * 4, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < kNorms; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ln, (__attribute__((address_space(3))) void*)(to_norm + 64 * i), 4,
+                                                 4 * lane + 256 * i, 0, 0, 0);
+    };
+    // 32 rows of q from row0 on against this wave's keys
+    auto attend = [&](const char* at, const float* norm_at, int row0, auto masked) {
+      u32x4 q[F::kOps];
+#pragma unroll
+      for (int s = 0; s < F::kOps; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + Q::offset(c, 2 * s + hf));
+      f32x4 norm[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) norm[g] = *reinterpret_cast<const f32x4*>(norm_at + 8 * g + 4 * hf);
+      f32x16 s[NK];
+      products<F::kF32, CT, NK>(q, k, s);
+#pragma unroll
+      for (int b = 0; b < NK; ++b) {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], mul[b], -norm[e >> 2][e & 3]));
+        if constexpr (decltype(masked)::value) {
+          const int lo = from[b] - row0 - 4 * hf, hi = rows - row0 - 4 * hf;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int r = 8 * (e >> 2) + (e & 3);
+            p[e] = r >= lo && r < hi ? p[e] : 0.0f;
+          }
+        }
+        float s0 = p[0], s1 = p[1];
+#pragma unroll
+        for (int e = 2; e < 16; e += 2) {
+          s0 += p[e];
+          s1 += p[e + 1];
+        }
+        sum[b] += s0 + s1;
       }
     };
-    __syncthreads();  // (everyone is done with the unit before)
-    if (r_begin < rows) issue(r_begin, 0);
-    for (int r0 = r_begin, par = 0; r0 < rows; r0 += kTile, par ^= 1) {
-      wait_all();
-      if (tid < kTile) {
-        lse[par][tid] = lse_next;
-        last[par][tid] = last_next;
-      }
-      __syncthreads();
-      if (r0 + kTile < rows) issue(r0 + kTile, par ^ 1);
+    auto step = [&](int r0, auto nth) {
+      constexpr int n = decltype(nth)::value;
+      if (r0 >= rows) return;
+      if (r0 + kTile < rows)
+        wait_vm<kDma + kNorms>();  // (the next tile's loads may be on their way)
+      else
+        wait_vm<0>();
+      meet();  // the tile is here, and everyone is done with the one before
+      if (r0 + 2 * kTile < rows) issue(r0 + 2 * kTile, std::integral_constant<int, (n + 2) % 3>{});
+#pragma unroll
       for (int rb = 0; rb < kTile / 32; ++rb) {
-        if (r0 + 32 * rb >= rows) break;
-        // (rows' positions rise: the block's first and last)
-        const int least = uniform(last[par][32 * rb]);
-        const int most = uniform(last[par][min(32 * rb + 31, rows - 1 - r0)]);
-        if (most < key0) continue;
-        u32x4 q[F::kOps];
-#pragma unroll
-        for (int s = 0; s < F::kOps; ++s)
-          q[s] = *reinterpret_cast<const u32x4*>(tile[par] + 32 * rb * RB + Q::offset(c, 2 * s + hf));
-        f32x4 norm[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) norm[g] = *reinterpret_cast<const f32x4*>(&lse[par][32 * rb + 8 * g + 4 * hf]);
-#pragma unroll
-        for (int b = 0; b < NK; ++b) {
-          const f32x16 s = product<F::kF32, CT>(q, k[b]);
-          float p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], mul[b], -norm[e >> 2][e & 3]));
-          // rows that end ahead of the block's last key, and those past the last row,
-          // whose normaliser makes their weight 0 unless the key is not finite
-          if (least < key0 + 32 * b + 31 || r0 + 32 * rb + 32 > rows) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              typedef int i32x4 __attribute__((ext_vector_type(4)));
-              const i32x4 end = *reinterpret_cast<const i32x4*>(&last[par][32 * rb + 8 * g + 4 * hf]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) p[4 * g + e] = end[e] >= key0 + 32 * b + c ? p[4 * g + e] : 0.0f;
-            }
-          }
-          float s0 = p[0], s1 = p[1];
-#pragma unroll
-          for (int e = 2; e < 16; e += 2) {
-            s0 += p[e];
-            s1 += p[e + 1];
-          }
-          sum[b] += s0 + s1;
-        }
+        const int row0 = r0 + 32 * rb;
+        if (row0 >= rows || row0 + 31 < none) continue;
+        const char* const at = (n == 0 ? tile0 : n == 1 ? tile1 : tile2) + 32 * rb * RB;
+        const float* const norm_at = (n == 0 ? norm0 : n == 1 ? norm1 : norm2) + 32 * rb;
+        if (row0 < all || row0 + 32 > rows)
+          attend(at, norm_at, row0, std::true_type{});
+        else
+          attend(at, norm_at, row0, std::false_type{});
       }
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    meet();  // (everyone is done with the unit before)
+    if (r_begin < rows) issue(r_begin, I0{});
+    if (r_begin + kTile < rows) issue(r_begin + kTile, I1{});
+    for (int r0 = r_begin; r0 < rows; r0 += 3 * kTile) {
+      step(r0, I0{});
+      step(r0 + kTile, I1{});
+      step(r0 + 2 * kTile, I2{});
     }
 #pragma unroll
     for (int b = 0; b < NK; ++b) {
@@ -829,8 +1093,8 @@ struct Plan {
   // decode
   int ni, unit, max_units, grid_units;
   // chunks
-  int row_groups, splits;
-  int64_t row_units;
+  int row_groups, rows, shares;  // rows: of a block
+  int64_t row_units;             // blocks at most
   int column_grid;
   size_t bytes;
 };
@@ -857,16 +1121,15 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
   }
   const int held = f32 ? 32 : 64;  // rows of a wave
   const int64_t rows = total_q * group, mean = rows / num_seqs;
-  p.row_groups = mean <= held ? 1 : mean <= 2 * held ? 2 : 4;
-  p.row_units = num_seqs + rows / (held * p.row_groups);
-  const int64_t blocks = p.row_units * kv_heads, tiles = (capacity + kStreamKeys - 1) / kStreamKeys;
-  int64_t splits = 1024 / blocks;
-  splits = splits > tiles ? tiles : splits;
-  p.splits = (int)(splits < 1 ? 1 : splits);
+  p.row_groups = mean <= held && !f32 ? 1 : mean <= 2 * held ? 2 : 4;
+  p.rows = held * p.row_groups;
+  p.row_units = num_seqs + rows / p.rows;
+  // pieces for two workgroups a CU, which run at once
+  p.shares = (int)(512 / kv_heads > 0 ? 512 / kv_heads : 1);
   const int unit = f32 ? 128 : 256;
   const int64_t units = (int64_t)num_seqs * ((capacity + unit - 1) / unit) * kv_heads;
   p.column_grid = (int)(units < 8192 ? units : 8192);
-  p.bytes = (size_t)total_q * heads * (4 + (p.splits > 1 ? 8 * (size_t)p.splits : 0));
+  p.bytes = (size_t)total_q * heads * 4 + (size_t)(p.row_units + p.shares) * kv_heads * p.rows * 8;
   p.bytes = (p.bytes + 15) / 16 * 16;
   return p;
 }
@@ -889,18 +1152,25 @@ int launch_weights(WeightArgs& a, const Plan& p, hipStream_t s) {
     }
     return (int)hipGetLastError();
   }
-  const dim3 grid((unsigned)(p.row_units * a.num_kv_heads), (unsigned)p.splits);
-  switch (p.row_groups) {
-    case 1: hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_lse_kernel<KV, CT, D, 1>), grid, dim3(kThreads), 0, s, a); break;
-    case 2: hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_lse_kernel<KV, CT, D, 2>), grid, dim3(kThreads), 0, s, a); break;
-    default: hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_lse_kernel<KV, CT, D, 4>), grid, dim3(kThreads), 0, s, a); break;
-  }
-  if (hipError_t e = hipGetLastError()) return (int)e;
-  if (p.splits > 1) {
-    hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((a.total_q * a.num_heads + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, s, a);
+  auto normalisers = [&](auto groups) {
+    constexpr int R = decltype(groups)::value, kRows = 32 * Formats<KV, CT, D>::kBlocks * R;
+    const dim3 grid((unsigned)(p.shares * a.num_kv_heads));
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_lse_kernel<KV, CT, D, R>), grid, dim3(kThreads), 0, s, a);
     if (hipError_t e = hipGetLastError()) return (int)e;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_join_kernel<kRows, kStreamKeys<R>>),
+                       dim3((unsigned)(p.row_units * a.num_kv_heads)), dim3(kThreads), 0, s, a);
+    return (int)hipGetLastError();
+  };
+  int st = 0;
+  if (p.row_groups == 4) {
+    st = normalisers(std::integral_constant<int, 4>{});
+  } else if (p.row_groups == 2) {
+    st = normalisers(std::integral_constant<int, 2>{});
+  } else {
+    if constexpr (KV != MKV_DTYPE_F32)  // (three of its tiles would not fit the LDS)
+      st = normalisers(std::integral_constant<int, 1>{});
   }
+  if (st) return st;
   hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_columns_kernel<KV, CT, D>), dim3((unsigned)p.column_grid), dim3(kThreads), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -997,9 +1267,9 @@ extern "C" int mkv_paged_weights(float* weights, float decay, const void* q, int
   a.max_units = p.max_units;
   a.ws_ml = reinterpret_cast<f32x2*>(workspace);
   a.ws_t = reinterpret_cast<float*>(a.ws_ml + (p.decode ? (size_t)num_seqs * num_kv_heads * p.max_units * 4 * p.ni : 0));
-  a.splits = p.splits;
+  a.shares = p.shares;
   a.part_ml = reinterpret_cast<f32x2*>(workspace);
-  a.lse = reinterpret_cast<float*>(a.part_ml + (!p.decode && p.splits > 1 ? (size_t)p.splits * total_q * num_heads : 0));
+  a.lse = reinterpret_cast<float*>(a.part_ml + (p.decode ? 0 : (size_t)(p.row_units + p.shares) * num_kv_heads * p.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool half = q_dtype == MKV_DTYPE_F16;
   switch (kv_dtype) {
