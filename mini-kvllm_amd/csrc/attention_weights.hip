@@ -175,15 +175,20 @@ template <int KV, int CT, int D>
 struct DecodeQ {
   static constexpr int kOps = KV == MKV_DTYPE_F32 ? D / 16 : D / 32;
   u32x4 w[kOps];
-  // row `j` of q (j < 0: zeros); kg: the lane's share of the contraction
-  MKV_DEV void load(const char* row, bool ok, int kg) {
+  // kg: the lane's share of the contraction
+  MKV_DEV void load(const char* row, int kg) {
 #pragma unroll
     for (int s = 0; s < kOps; ++s) {
       const int d = KV == MKV_DTYPE_F32 ? 16 * s + 4 * kg
                     : DTypeInfo<KV>::kBytes == 2 ? 32 * s + 8 * kg : 64 * (s >> 1) + 16 * kg + 8 * (s & 1);
-      w[s] = u32x4{0, 0, 0, 0};
-      if (ok) w[s] = ld16(row + d * (KV == MKV_DTYPE_F32 ? 4 : 2));
+      w[s] = ld16(row + d * (KV == MKV_DTYPE_F32 ? 4 : 2));
     }
+  }
+  MKV_DEV void keep(bool ok) {
+#pragma unroll
+    for (int s = 0; s < kOps; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[s][e] = ok ? w[s][e] : 0u;
   }
 };
 
@@ -210,35 +215,92 @@ MKV_DEV f32x4 decode_scores(const DecodeQ<KV, CT, D>& q, const DecodeTile<KV, CT
   return s;
 }
 
-// The tiles of a wave, four at a time: their weights from e(tile, i), all of the
-// wave's lanes writing (lane row kg the kg-th tile's keys).
-template <int NI, class E>
-MKV_DEV void write_tiles(const WeightArgs& a, const Seq& sq, int seq, int h, int k0, int k1, int tiles, int wave, E e) {
-  const int lane = threadIdx.x & 63, c = lane & 15, kg = lane >> 4;
-  for (int i0 = 0; i0 * kWaves + wave < tiles; i0 += 4) {
-    const int t = k0 + 16 * ((i0 + kg) * kWaves + wave) + c;
-    const int slot = t < k1 ? slot_of(a, seq, t) : -1;
+// The tiles of a wave: tile n holds keys k0 + 16 (n kWaves + wave) on.  Their block
+// entries come by one load, a lane a tile (64 of them at most).
+struct WaveTiles {
+  const WeightArgs& a;
+  int k0, k1, num, wave, entry;
+  MKV_DEV WaveTiles(const WeightArgs& args, int seq, int k0_, int k1_, int wave_)
+      : a(args), k0(k0_), k1(k1_), num(((k1_ - k0_ + 15) / 16 - wave_ + kWaves - 1) / kWaves), wave(wave_) {
+    const int t = min(key(threadIdx.x & 63), k1 - 1);
+    entry = a.idx.block_tables[(int64_t)seq * a.idx.bt_stride + (t >> a.idx.bs_log2)];
+  }
+  MKV_DEV int key(int n) const { return k0 + 16 * (n * kWaves + wave); }
+  MKV_DEV bool is_there(int e) const { return e >= 0 && e < a.idx.num_blocks; }
+  MKV_DEV int slot(int e, int t) const { return (e << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)); }
+};
+
+// Their weights, four tiles a round, all of the wave's lanes writing (lane row kg the
+// kg-th tile's keys).  The old weights of the first kHeld rounds come ahead, under the
+// scores' loads.
+template <int NI>
+struct TileWeights {
+  static constexpr int kHeld = 4;
+  const WeightArgs& a;
+  const WaveTiles& w;
+  int64_t fresh;  // tokens from here on came with these rows and start from 0
+  int h, lane;
+  int slot[kHeld];
+  float old[kHeld];
+
+  MKV_DEV int key(int round) const { return w.key(4 * round + (lane >> 4)) + (lane & 15); }
+  MKV_DEV int slot_at(int round) const {
+    const int e = __shfl(w.entry, 4 * round + (lane >> 4)), t = key(round);
+    return t < w.k1 && w.is_there(e) ? w.slot(e, t) : -1;
+  }
+  MKV_DEV float load(int s) const { return a.weights[(int64_t)max(s, 0) * a.num_kv_heads + h]; }
+  MKV_DEV TileWeights(const WeightArgs& args, const WaveTiles& tiles, int64_t first, int h_, bool used = true)
+      : a(args), w(tiles), fresh(first), h(h_), lane(threadIdx.x & 63) {
+    if (!used) return;
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) slot[r] = slot_at(r);
+    if (a.decay != 0.0f) {
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r) old[r] = load(slot[r]);
+    }
+  }
+  template <class E>
+  MKV_DEV void round(int r, int s, float was, E e) const {
     float mine = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float w = 0.0f;
-      if ((i0 + j) * kWaves + wave < tiles) {
+      float x = 0.0f;
+      if (4 * r + j < w.num) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) w += e((i0 + j) * kWaves + wave, i);
+        for (int i = 0; i < NI; ++i) x += e(4 * r + j, i);
       }
-      w = sum_of_rows(w);
-      mine = kg == j ? w : mine;
+      x = sum_of_rows(x);
+      mine = lane >> 4 == j ? x : mine;
     }
-    if (slot >= 0) add_weight(a, sq, slot, h, t, mine);
+    if (a.decay != 0.0f && key(r) < fresh) mine = __builtin_fmaf(a.decay, was, mine);
+    if (s >= 0) a.weights[(int64_t)s * a.num_kv_heads + h] = mine;
   }
-}
+  // e(n, i): the weight of this lane's key and i-th query in tile n
+  template <bool MORE, class E>
+  MKV_DEV void write(E e) const {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+      if (4 * r < w.num) round(r, slot[r], old[r], e);
+    if constexpr (MORE) {
+      for (int r = kHeld; 4 * r < w.num; ++r) {
+        const int s = slot_at(r);
+        round(r, s, a.decay != 0.0f ? load(s) : 0.0f, e);
+      }
+    }
+  }
+};
 
-template <int KV, int CT, int D, int NI>
+constexpr int kSplitKeys = 1024;  // of a unit: 16 tiles a wave
+
+// One workgroup a (sequence, KV head) where its scores fit the LDS; else (SPLIT) a
+// workgroup a unit of the keys, whose scores go to memory with their running maximum
+// and sum, and weights_finish_kernel.
+template <int KV, int CT, int D, int NI, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) {
   using Tile = DecodeTile<KV, CT, D>;
   constexpr int kAhead = KV == MKV_DTYPE_F32 ? 2 : 4;  // tiles of a wave in a batch; two batches in flight
   extern __shared__ float scores[];                    // (tile, i, lane)
-  __shared__ float part[2][kWaves][4 * NI];
+  __shared__ float part_m[kWaves][4 * NI], part_l[kWaves][4 * NI];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int c = lane & 15, kg = lane >> 4;
   const int pair = blockIdx.x / a.grid_units, x = blockIdx.x % a.grid_units;
@@ -250,28 +312,31 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
   const int query = 4 * (c & 3) + (c >> 2);
   constexpr int kQBytes = D * (KV == MKV_DTYPE_F32 ? 4 : 2);
   DecodeQ<KV, CT, D> q;
-  q.load(a.q + (sq.q0 * a.num_heads + h * a.group + min(query, a.group - 1)) * kQBytes, query < a.group, kg);
+  q.load(a.q + (sq.q0 * a.num_heads + h * a.group + min(query, a.group - 1)) * kQBytes, kg);
   const int64_t row_bytes = (int64_t)a.num_kv_heads * D * Tile::kEb;
   const char* const kbase = a.k + (int64_t)h * D * Tile::kEb + 16 * kg;
   float mul = a.mul;
   if (a.scale_mode == 1) mul *= load_uniform_f32(a.k_scale);
-  const bool split = units > 1;
+  bool begun = false;
   for (int u = x; u < units; u += a.grid_units) {
     const int k0 = u * a.unit, k1 = min(sq.keys, k0 + a.unit);
-    const int tiles = (k1 - k0 + 15) / 16;
-    float m[NI];
+    const WaveTiles w(a, seq, k0, k1, wave);
+    float* const kept = SPLIT ? a.ws_t + ((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI * 64 + lane : nullptr;
+    float m[NI], l[NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) m[i] = kNegBig;
-    auto load = [&](Tile (&t)[kAhead], uint32_t& here, int i0) {
+    for (int i = 0; i < NI; ++i) {
+      m[i] = kNegBig;
+      l[i] = 0.0f;
+    }
+    auto load = [&](Tile (&t)[kAhead], uint32_t& here, int n0) MKV_INLINE {
       here = 0;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const int tile = (i0 + j) * kWaves + wave, key = k0 + 16 * tile;
-        if (tile < tiles) {
-          const int64_t phys = a.idx.physical_block(seq, key >> a.idx.bs_log2);
-          here |= phys >= 0 ? 1u << j : 0u;
+        if (n0 + j < w.num) {
+          const int key = w.key(n0 + j), e = __builtin_amdgcn_readlane(w.entry, n0 + j);
+          here |= w.is_there(e) ? 1u << j : 0u;
           // (keys past the last: the tile's first, which is there)
-          const int64_t slot = (max(phys, (int64_t)0) << a.idx.bs_log2) + (key & ((1 << a.idx.bs_log2) - 1)) + (key + c < k1 ? c : 0);
+          const int64_t slot = w.slot(w.is_there(e) ? e : 0, key) + (key + c < k1 ? c : 0);
           const char* p = kbase + slot * row_bytes;
 #pragma unroll
           for (int i = 0; i < Tile::kLoads; ++i) t[j].w[i] = ld16(p + 64 * i);
@@ -279,83 +344,81 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
         }
       }
     };
-    auto take = [&](const Tile (&t)[kAhead], uint32_t here, int i0) {
+    auto take = [&](const Tile (&t)[kAhead], uint32_t here, int n0) MKV_INLINE {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const int tile = (i0 + j) * kWaves + wave;
-        if (tile < tiles) {
+        if (n0 + j < w.num) {
           const f32x4 s = decode_scores<KV, CT, D>(q, t[j]);
-          const bool sees = (here >> j & 1) && k0 + 16 * tile + c < k1;
+          const bool sees = (here >> j & 1) && w.key(n0 + j) + c < k1;
           const float f = mul * t[j].scale;
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
             const float v = sees ? s[i] * f : kNegInf;
-            m[i] = fmaxf(m[i], v);
-            scores[(tile * NI + i) * 64 + lane] = v;
+            if constexpr (SPLIT) {
+              kept[(((n0 + j) * kWaves + wave) * NI + i) * 64] = v;
+              const float top = fmaxf(m[i], v);
+              l[i] = __builtin_fmaf(l[i], __builtin_amdgcn_exp2f(m[i] - top), __builtin_amdgcn_exp2f(v - top));
+              m[i] = top;
+            } else {
+              scores[(((n0 + j) * kWaves + wave) * NI + i) * 64 + lane] = v;
+              m[i] = fmaxf(m[i], v);
+            }
           }
         }
       }
     };
-    {
-      Tile t0[kAhead], t1[kAhead];
-      uint32_t h0, h1;
-      load(t0, h0, 0);
-      for (int i0 = 0; i0 * kWaves + wave < tiles; i0 += 2 * kAhead) {
-        load(t1, h1, i0 + kAhead);
-        take(t0, h0, i0);
-        load(t0, h0, i0 + 2 * kAhead);
-        take(t1, h1, i0 + kAhead);
-      }
+    Tile t0[kAhead], t1[kAhead];
+    uint32_t h0, h1;
+    load(t0, h0, 0);
+    load(t1, h1, kAhead);
+    if (!begun) q.keep(query < a.group);
+    begun = true;
+    const TileWeights<NI> out(a, w, sq.first, h, !SPLIT);
+    for (int n0 = 0; n0 < w.num; n0 += 2 * kAhead) {
+      take(t0, h0, n0);
+      load(t0, h0, n0 + 2 * kAhead);
+      take(t1, h1, n0 + kAhead);
+      load(t1, h1, n0 + 3 * kAhead);
     }
-    // ---- the queries' maxima and sums ----
-#pragma unroll
-    for (int i = 0; i < NI; ++i) m[i] = row_all(m[i], [](float u, float v) { return fmaxf(u, v); });
-    if (c == 0) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) part[0][wave][4 * i + kg] = m[i];
-    }
-    __syncthreads();
-    float l[NI];
+    // ---- the queries' maxima and sums, of the wave and of all ----
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      for (int v = 0; v < kWaves; ++v) m[i] = fmaxf(m[i], part[0][v][4 * i + kg]);
-      l[i] = 0.0f;
-    }
-    for (int tile = wave; tile < tiles; tile += kWaves)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        float* const at = scores + (tile * NI + i) * 64 + lane;
-        const float e = __builtin_amdgcn_exp2f(*at - m[i]);
-        l[i] += e;
-        if (split)
-          a.ws_t[(((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI + tile * NI + i) * 64 + lane] = *at;
-        else
+      const float top = row_all(m[i], [](float v, float w) { return fmaxf(v, w); });
+      if constexpr (SPLIT) {
+        l[i] *= __builtin_amdgcn_exp2f(m[i] - top);
+      } else {
+        for (int n = 0; n < w.num; ++n) {
+          float* const at = scores + ((n * kWaves + wave) * NI + i) * 64 + lane;
+          const float e = __builtin_amdgcn_exp2f(*at - top);
+          l[i] += e;
           *at = e;
+        }
       }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) l[i] = row_all(l[i], [](float u, float v) { return u + v; });
-    if (c == 0) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) part[1][wave][4 * i + kg] = l[i];
+      m[i] = top;
+      l[i] = row_all(l[i], [](float v, float w) { return v + w; });
+      if (c == 0) {
+        part_m[wave][4 * i + kg] = m[i];
+        part_l[wave][4 * i + kg] = l[i];
+      }
     }
     __syncthreads();
+    float f[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      l[i] = 0.0f;
-      for (int v = 0; v < kWaves; ++v) l[i] += part[1][v][4 * i + kg];
+      float top = part_m[0][4 * i + kg], sum = 0.0f;
+#pragma unroll
+      for (int v = 1; v < kWaves; ++v) top = fmaxf(top, part_m[v][4 * i + kg]);
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) sum += part_l[v][4 * i + kg] * __builtin_amdgcn_exp2f(part_m[v][4 * i + kg] - top);
+      if (SPLIT && wave == 0 && c == 0) a.ws_ml[((int64_t)pair * a.max_units + u) * 4 * NI + 4 * i + kg] = f32x2{top, sum};
+      f[i] = 4 * i + kg < a.group ? inverse(sum) * __builtin_amdgcn_exp2f(m[i] - top) : 0.0f;
     }
-    if (split) {
-      if (wave == 0 && c == 0) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          a.ws_ml[((int64_t)pair * a.max_units + u) * 4 * NI + 4 * i + kg] = f32x2{m[i], l[i]};
-      }
+    if constexpr (SPLIT) {
+      __syncthreads();  // (the parts are read)
     } else {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) l[i] = 4 * i + kg < a.group ? inverse(l[i]) : 0.0f;
-      write_tiles<NI>(a, sq, seq, h, k0, k1, tiles, wave, [&](int tile, int i) {
-        // (a query that is none: its factor is 0, its score finite or NaN alone)
-        return 4 * i + kg < a.group ? scores[(tile * NI + i) * 64 + lane] * l[i] : 0.0f;
+      // (a lane row without a query: its factor would meet no finite score)
+      out.template write<true>([&](int n, int i) {
+        return 4 * i + kg < a.group ? scores[((n * kWaves + wave) * NI + i) * 64 + lane] * f[i] : 0.0f;
       });
     }
   }
@@ -365,36 +428,50 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
 template <int NI>
 __global__ __launch_bounds__(kThreads) void weights_finish_kernel(WeightArgs a) {
   constexpr int Q = 4 * NI;  // queries
+  constexpr int kHeld = 4 * TileWeights<NI>::kHeld;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), kg = lane >> 4;
   const int pair = blockIdx.x / a.grid_units, x = blockIdx.x % a.grid_units;
   const int seq = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
   const Seq sq = seq_of(a, seq);
   const int units = (int)(((int64_t)sq.keys + a.unit - 1) / a.unit);
-  if (x >= units || units <= 1) return;
-  // a lane's query is lane % Q, its units every 64 / Q-th
+  if (x >= units) return;
   const f32x2* ml = a.ws_ml + (int64_t)pair * a.max_units * Q + lane % Q;
-  float m = kNegBig, l = 0.0f;
-  for (int u = lane / Q; u < units; u += 64 / Q) m = fmaxf(m, ml[(int64_t)u * Q][0]);
-#pragma unroll
-  for (int o = Q; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-  for (int u = lane / Q; u < units; u += 64 / Q) {
-    const f32x2 v = ml[(int64_t)u * Q];
-    l += v[1] * __builtin_amdgcn_exp2f(v[0] - m);
-  }
-#pragma unroll
-  for (int o = Q; o < 64; o <<= 1) l += __shfl_xor(l, o);
-  l = inverse(l);
   float mi[NI], li[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    mi[i] = __shfl(m, 4 * i + kg);
-    li[i] = __shfl(l, 4 * i + kg);
-  }
   for (int u = x; u < units; u += a.grid_units) {
-    const int k0 = u * a.unit, k1 = min(sq.keys, k0 + a.unit), tiles = (k1 - k0 + 15) / 16;
-    const float* t = a.ws_t + ((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI * 64 + lane;
-    write_tiles<NI>(a, sq, seq, h, k0, k1, tiles, wave, [&](int tile, int i) {
-      return 4 * i + kg < a.group ? __builtin_amdgcn_exp2f(t[(tile * NI + i) * 64] - mi[i]) * li[i] : 0.0f;
+    const int k0 = u * a.unit, k1 = min(sq.keys, k0 + a.unit);
+    const WaveTiles w(a, seq, k0, k1, wave);
+    // the wave's scores (a unit is 1024 keys: all of them)
+    const float* kept = a.ws_t + ((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI * 64 + lane;
+    float t[kHeld][NI];
+#pragma unroll
+    for (int n = 0; n < kHeld; ++n)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) t[n][i] = kept[((min(n, max(w.num - 1, 0)) * kWaves + wave) * NI + i) * 64];
+    const TileWeights<NI> out(a, w, sq.first, h);
+    if (u == x) {
+      // a lane's query is lane % Q, its units every 64 / Q-th
+      float m = kNegBig, l = 0.0f;
+      for (int v = lane / Q; v < units; v += 64 / Q) {
+        const f32x2 part = ml[(int64_t)v * Q];
+        const float top = fmaxf(m, part[0]);
+        l = l * __builtin_amdgcn_exp2f(m - top) + part[1] * __builtin_amdgcn_exp2f(part[0] - top);
+        m = top;
+      }
+#pragma unroll
+      for (int o = Q; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o), top = fmaxf(m, m2);
+        l = l * __builtin_amdgcn_exp2f(m - top) + l2 * __builtin_amdgcn_exp2f(m2 - top);
+        m = top;
+      }
+      l = inverse(l);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        mi[i] = __shfl(m, 4 * i + kg);
+        li[i] = __shfl(l, 4 * i + kg);
+      }
+    }
+    out.template write<false>([&](int n, int i) {
+      return 4 * i + kg < a.group ? __builtin_amdgcn_exp2f(t[n][i] - mi[i]) * li[i] : 0.0f;
     });
   }
 }
@@ -1108,7 +1185,7 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
   if (one_row) {
     p.ni = group <= 4 ? 1 : 4;
     const int most = 4096 / p.ni;  // 64 KB of scores: two workgroups a CU
-    p.unit = capacity <= most ? (int)((capacity + 15) / 16 * 16) : 1024;
+    p.unit = capacity <= most ? (int)((capacity + 15) / 16 * 16) : kSplitKeys;
     p.max_units = (int)((capacity + p.unit - 1) / p.unit);
     const int64_t room = 16384 / pairs;
     p.grid_units = (int)(p.max_units < room ? p.max_units : room < 1 ? 1 : room);
@@ -1139,12 +1216,17 @@ int launch_weights(WeightArgs& a, const Plan& p, hipStream_t s) {
   if (p.decode) {
     const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * p.grid_units));
     const size_t lds = (size_t)p.unit / 16 * p.ni * 64 * 4;
-    if (p.ni == 1)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1>), grid, dim3(kThreads), lds, s, a);
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4>), grid, dim3(kThreads), lds, s, a);
-    if (hipError_t e = hipGetLastError()) return (int)e;
-    if (p.max_units > 1) {
+    if (p.max_units == 1) {
+      if (p.ni == 1)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, false>), grid, dim3(kThreads), lds, s, a);
+      else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, false>), grid, dim3(kThreads), lds, s, a);
+    } else {
+      if (p.ni == 1)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, true>), grid, dim3(kThreads), 0, s, a);
+      else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, true>), grid, dim3(kThreads), 0, s, a);
+      if (hipError_t e = hipGetLastError()) return (int)e;
       if (p.ni == 1)
         hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<1>), grid, dim3(kThreads), 0, s, a);
       else

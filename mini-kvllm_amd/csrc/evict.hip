@@ -18,9 +18,11 @@
 namespace mkv {
 namespace {
 
-constexpr int kMaxTensors = 64;  // a launch's tensors, their addresses in the kernel arguments
+// (lambdas whose arrays have to stay in registers)
+#define MKV_INLINE __attribute__((always_inline))
+
+constexpr int kMaxTensors = 128;  // a launch's tensors, their addresses in the kernel arguments
 constexpr int kBins = 2048;
-constexpr int kLdsKeys = 8192;   // capacities up to this keep their keys in LDS
 
 struct EvictArgs {
   PagedIndex idx;
@@ -59,11 +61,6 @@ MKV_DEV int slot_of(const EvictArgs& a, int b, int t) {
   const int32_t p = a.idx.block_tables[(int64_t)b * a.idx.bt_stride + (t >> a.idx.bs_log2)];
   return p >= 0 && p < a.idx.num_blocks ? (p << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : -1;
 }
-MKV_DEV uint32_t key_at(const EvictArgs& a, const float* w, int b, int h, int t) {
-  const int s = slot_of(a, b, t);
-  return s >= 0 ? order_of(w[(int64_t)s * a.heads + h]) : 0u;
-}
-
 // Workgroups of one (layer, sequence) lie 8 apart, on one XCD: its heads share the
 // weights' cache lines.
 MKV_DEV bool place_of(const EvictArgs& a, int layers, int i, int& layer, int& b, int& h) {
@@ -75,43 +72,96 @@ MKV_DEV bool place_of(const EvictArgs& a, int layers, int i, int& layer, int& b,
   return layer < layers;
 }
 
-// The weights' keys of long tables, transposed to a row a head.
+// The weights' keys of long tables, transposed to a row a head: four heads a load
+// where their number allows it.
 __global__ __launch_bounds__(256) void evict_keys_kernel(EvictArgs a, Weights w, int layer0) {
   const int b = blockIdx.y, layer = blockIdx.z;
   int64_t len;
   const int n = length_of(a, b, len);
   if (n <= a.budget) return;
   uint32_t* const out = a.keys + (int64_t)((layer0 + layer) * a.batch + b) * a.heads * a.key_stride;
+  const bool wide = a.heads % 4 == 0 && (reinterpret_cast<uintptr_t>(w.base[layer]) & 15) == 0;
   for (int t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
     const int s = slot_of(a, b, t);
     const float* row = w.base[layer] + (int64_t)max(s, 0) * a.heads;
-    for (int h = 0; h < a.heads; ++h) out[h * a.key_stride + t] = s >= 0 ? order_of(row[h]) : 0u;
+    if (wide) {
+      for (int h = 0; h < a.heads; h += 4) {
+        const u32x4 v = ld16(row + h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[(h + e) * a.key_stride + t] = s >= 0 ? order_of(__uint_as_float(v[e])) : 0u;
+      }
+    } else {
+      for (int h = 0; h < a.heads; ++h) out[h * a.key_stride + t] = s >= 0 ? order_of(row[h]) : 0u;
+    }
   }
 }
 
-template <int T, bool LDS>
+// The keys of a (layer, sequence, KV head), four tokens a lane at a time: each wave has
+// a run of consecutive tokens, kHeld of its vectors in registers, the rest (of rows
+// longer than they take) in memory.
+template <int T, int HELD>
+struct Keys {
+  static constexpr int kWaves = T / 64;
+  u32x4 held[HELD];
+  const u32x4* more;  // the row in memory
+  int first, num;     // the wave's first token, and its vectors
+  MKV_DEV int token(int j) const { return first + 256 * j + 4 * (threadIdx.x & 63); }
+  MKV_DEV Keys(int n, int wave) {
+    num = (n + 256 * kWaves - 1) / (256 * kWaves);
+    first = wave * num * 256;
+  }
+  // f(vector j's keys, its first token)
+  template <class F>
+  MKV_DEV void each(int n, F f) const {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j)
+      if (j < num && first + 256 * j < n) f(held[j], token(j));
+    for (int j = HELD; j < num && first + 256 * j < n; ++j) f(more[token(j) / 4], token(j));
+  }
+};
+
+// KEYS: from the transposed keys; else from the weights themselves (up to HELD vectors
+// a wave: 256 T / 64 HELD tokens).
+template <int T, int HELD, bool KEYS>
 __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w, int layer0, int layers) {
-  extern __shared__ uint32_t lds_keys[];
+  constexpr int kWaves = T / 64;
   __shared__ int hist[kBins];
-  __shared__ int scan[T / 64], found[2], part_kept[T / 64], part_equal[T / 64];
+  __shared__ int scan[kWaves], found[2], part_kept[kWaves], part_equal[kWaves];
   int layer, b, h;
   if (!place_of(a, layers, blockIdx.x, layer, b, h)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   int64_t len;
   const int n = length_of(a, b, len);
   if (layer0 + layer == 0 && h == 0 && tid == 0) a.new_lens[b] = min(len, (int64_t)a.budget);
   if (n <= a.budget) return;
   const int64_t at = ((int64_t)(layer0 + layer) * a.batch + b) * a.heads + h;
-  const uint32_t* keys = LDS ? lds_keys : a.keys + at * a.key_stride;
-  if constexpr (LDS) {
-    constexpr int kAhead = 4;  // (their loads in one round trip)
-    for (int t0 = tid; t0 < n; t0 += T * kAhead) {
-      uint32_t k[kAhead];
+  Keys<T, HELD> keys(n, wave);
+  if constexpr (KEYS) {
+    // (rows are a multiple of four long; what lies behind the last token is masked)
+    keys.more = reinterpret_cast<const u32x4*>(a.keys + at * a.key_stride);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) k[j] = t0 + j * T < n ? key_at(a, w.base[layer], b, h, t0 + j * T) : 0u;
+    for (int j = 0; j < HELD; ++j) keys.held[j] = j < keys.num && keys.token(j) < n ? keys.more[keys.token(j) / 4] : u32x4{0, 0, 0, 0};
+  } else {
+    keys.more = nullptr;
+    int slot[HELD];  // (four tokens lie in one block)
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (t0 + j * T < n) lds_keys[t0 + j * T] = k[j];
+    for (int j = 0; j < HELD; ++j)
+      if (j < keys.num) slot[j] = a.idx.block_tables[(int64_t)b * a.idx.bt_stride + (min(keys.token(j), n - 1) >> a.idx.bs_log2)];
+    float x[HELD][4];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (j >= keys.num) continue;
+      const bool there = slot[j] >= 0 && slot[j] < a.idx.num_blocks;
+      const int64_t s = ((int64_t)(there ? slot[j] : 0) << a.idx.bs_log2) + (keys.token(j) & ((1 << a.idx.bs_log2) - 1));
+      if (!there) slot[j] = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = w.base[layer][(s + e) * a.heads + h];
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (j >= keys.num) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keys.held[j][e] = slot[j] >= 0 ? order_of(x[j][e]) : 0u;
     }
   }
   const int first = a.sinks, last = n - a.recent;  // the middle: [first, last)
@@ -122,26 +172,30 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
     constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = kShift[pass], bins = 1 << kBits[pass];
-      __syncthreads();
+      constexpr int kNone = 32;
+      const int shift = kShift[pass], bins = 1 << kBits[pass], upper = pass == 0 ? kNone : kShift[pass > 0 ? pass - 1 : 0];
       for (int i = tid; i < kBins; i += T) hist[i] = 0;
       __syncthreads();
-      const uint32_t above = pass == 0 ? 0u : least >> kShift[pass > 0 ? pass - 1 : 0];
-      for (int t0 = first; t0 < last; t0 += T) {
-        const int t = t0 + tid;
-        const uint32_t k = t < last ? keys[t] : 0u;
-        const bool in = t < last && (pass == 0 || k >> kShift[pass > 0 ? pass - 1 : 0] == above);
-        const int d = (int)(k >> shift) & (bins - 1);
-        // (many alike: one addition for the wave)
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(in);
-        if (mine == 0) continue;
-        const int d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(mine));
-        if (__builtin_amdgcn_ballot_w64(in && d == d0) == mine) {
-          if (lane == __builtin_ctzll(mine)) atomicAdd(&hist[d0], __popcll(mine));
-        } else if (in) {
-          atomicAdd(&hist[d], 1);
+      const uint32_t above = pass == 0 ? 0u : least >> upper;
+      keys.each(n, [&](const u32x4& v, int t) MKV_INLINE {
+        // (most vectors lie in the middle whole)
+        const int t0 = uniform(t - 4 * lane);
+        const bool whole = t0 >= first && t0 + 256 <= last;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = (whole || (t + e >= first && t + e < last)) && (pass == 0 || v[e] >> upper == above);
+          const int d = (int)(v[e] >> shift) & (bins - 1);
+          const uint64_t mine = __builtin_amdgcn_ballot_w64(in);
+          if (mine == 0) continue;
+          // (many alike: one addition for the wave)
+          const int one = __builtin_ctzll(mine), d0 = __builtin_amdgcn_readlane(d, one);
+          if (__builtin_amdgcn_ballot_w64(in && d == d0) == mine) {
+            if (lane == one) atomicAdd(&hist[d0], __popcll(mine));
+          } else if (in) {
+            atomicAdd(&hist[d], 1);
+          }
         }
-      }
+      });
       __syncthreads();
       // the bin in which the want-th largest lies; thread tid has bins from the top
       constexpr int kPer = kBins / T;
@@ -175,20 +229,30 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
       least |= (uint32_t)found[0] << shift;
       want -= found[1];
     }
-  } else {
-    __syncthreads();
   }
-  // ---- the kept tokens' places: a run of tokens a wave ----
-  constexpr int kWaves = T / 64;
-  const int run = (n + 64 * kWaves - 1) / (64 * kWaves) * 64;
-  const int t_lo = wave * run, t_hi = min(n, t_lo + run);
-  int kept = 0, equal = 0;
-  for (int t0 = t_lo; t0 < t_hi; t0 += 64) {
-    const int t = t0 + lane;
-    const bool in = t < t_hi, mid = in && t >= first && t < last;
-    const uint32_t k = mid ? keys[t] : 0u;
-    kept += __popcll(__builtin_amdgcn_ballot_w64((in && !mid) || (mid && k > least)));
-    equal += __popcll(__builtin_amdgcn_ballot_w64(mid && k == least));
+  // ---- the kept tokens' places, in order ----
+  int kept = 0, equal = 0;  // of the lane
+  keys.each(n, [&](const u32x4& v, int t) MKV_INLINE {
+    const int t0 = uniform(t - 4 * lane);
+    if (t0 >= first && t0 + 256 <= last) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kept += v[e] > least;
+        equal += v[e] == least;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = t + e < n, mid = in && t + e >= first && t + e < last;
+        kept += (in && !mid) || (mid && v[e] > least);
+        equal += mid && v[e] == least;
+      }
+    }
+  });
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    kept += __shfl_xor(kept, o);
+    equal += __shfl_xor(equal, o);
   }
   if (lane == 0) {
     part_kept[wave] = kept;
@@ -201,65 +265,91 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
     tied += part_equal[v];
   }
   int32_t* const out = a.slots + at * a.budget;
-  for (int t0 = t_lo; t0 < t_hi; t0 += 64) {
-    const int t = t0 + lane;
-    const bool in = t < t_hi, mid = in && t >= first && t < last;
-    const uint32_t k = mid ? keys[t] : 0u;
-    const bool eq = mid && k == least;
-    const uint64_t eqs = __builtin_amdgcn_ballot_w64(eq), below = (1ull << lane) - 1;
-    const bool keep = (in && !mid) || (mid && k > least) || (eq && tied + __popcll(eqs & below) < want);
-    const uint64_t keeps = __builtin_amdgcn_ballot_w64(keep);
-    const int place = to + __popcll(keeps & below);
-    if (keep && place < a.budget) out[place] = slot_of(a, b, t);
-    to += __popcll(keeps);
-    tied += __popcll(eqs);
-  }
+  const uint64_t below = (1ull << lane) - 1;
+  keys.each(n, [&](const u32x4& v, int t) MKV_INLINE {
+    // equal tokens ahead of the lane's, then the kept ones
+    bool eq[4], keep[4];
+    int eq_ahead = tied, eq_all = 0, eq_own = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      eq[e] = t + e < n && t + e >= first && t + e < last && v[e] == least;
+      const uint64_t ball = __builtin_amdgcn_ballot_w64(eq[e]);
+      eq_ahead += __popcll(ball & below);
+      eq_all += __popcll(ball);
+    }
+    int place = to, all = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = t + e < n, mid = in && t + e >= first && t + e < last;
+      keep[e] = (in && !mid) || (mid && v[e] > least) || (eq[e] && eq_ahead + eq_own < want);
+      eq_own += eq[e];
+      const uint64_t ball = __builtin_amdgcn_ballot_w64(keep[e]);
+      place += __popcll(ball & below);
+      all += __popcll(ball);
+    }
+    const int s = slot_of(a, b, min(t, n - 1));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (keep[e] && place < a.budget) out[place] = s >= 0 ? s + e : -1;
+      place += keep[e];
+    }
+    to += all;
+    tied += eq_all;
+  });
 }
 
-// Rows of one head (X a 16- or 4-byte item, `units` of them a row from `col0` on), or
-// of all heads together (heads_together: 4 bytes a head).
+// Rows of one head (X a 16- or 4-byte item, `units` of them a row), or of all heads
+// together (heads_together: 4 bytes a head).  The next batch's slots are on their way
+// while this one's rows are.
 constexpr int kItems = 8;  // a thread's, in registers
 constexpr int kMaxHeadBytes = 64 * kItems * 4;  // (a row of the smallest workgroup's 4-byte items)
 template <typename X, int T>
-MKV_DEV void move_rows(const EvictArgs& a, char* base, int64_t token_bytes, int64_t off, int units, int b,
-                       const int32_t* slots, int64_t head_stride, bool heads_together) {
+MKV_DEV void move_rows(const EvictArgs& a, char* base, int64_t token_bytes, int units, int b, const int32_t* slots,
+                       int64_t head_stride, bool heads_together) {
   const int mask = (1 << a.idx.bs_log2) - 1;
   const int32_t* bt = a.idx.block_tables + (int64_t)b * a.idx.bt_stride;
   const int per = max(T * kItems / units, 1);  // rows of a batch
-  for (int j0 = 0; j0 < a.budget; j0 += per) {
-    const int rows = min(per, a.budget - j0);
-    X v[kItems];
-    char* to[kItems];
+  int row[kItems], col[kItems], from[kItems], to[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int item = i * T + (int)threadIdx.x;
+    row[i] = item / units;
+    col[i] = item - row[i] * units;
+  }
+  auto look_up = [&](int j0) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int item = i * T + (int)threadIdx.x;
-      const int r = item / units, c = item - r * units;
-      to[i] = nullptr;
-      if (r < rows) {
-        const int j = j0 + r;
-        const int s = slots[(heads_together ? c * head_stride : 0) + j];
-        const int p = bt[j >> a.idx.bs_log2];
-        if (s >= 0 && p >= 0 && p < a.idx.num_blocks) {
-          const int d = (p << a.idx.bs_log2) + (j & mask);
-          if (d != s) {
-            to[i] = base + d * token_bytes + off + c * (int64_t)sizeof(X);
-            v[i] = *reinterpret_cast<const X*>(base + s * token_bytes + off + c * (int64_t)sizeof(X));
-          }
-        }
-      }
+      const int j = min(j0 + row[i], a.budget - 1);
+      from[i] = slots[(heads_together ? col[i] * head_stride : 0) + j];
+      to[i] = bt[j >> a.idx.bs_log2];
     }
+  };
+  look_up(0);
+  for (int j0 = 0; j0 < a.budget; j0 += per) {
+    X v[kItems];
+    int d[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int j = j0 + row[i];
+      const bool ok = row[i] < per && j < a.budget && from[i] >= 0 && to[i] >= 0 && to[i] < a.idx.num_blocks;
+      d[i] = ok ? (to[i] << a.idx.bs_log2) + (j & mask) : -1;
+      if (d[i] == from[i]) d[i] = -1;
+      if (d[i] >= 0) v[i] = *reinterpret_cast<const X*>(base + from[i] * token_bytes + col[i] * (int)sizeof(X));
+    }
+    if (j0 + per < a.budget) look_up(j0 + per);
     // every row of the batch has been read before any is written
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (T > 64) __syncthreads();
 #pragma unroll
     for (int i = 0; i < kItems; ++i)
-      if (to[i]) *reinterpret_cast<X*>(to[i]) = v[i];
+      if (d[i] >= 0) *reinterpret_cast<X*>(base + d[i] * token_bytes + col[i] * (int)sizeof(X)) = v[i];
   }
 }
 
 template <int T>
 __global__ __launch_bounds__(T) void evict_move_kernel(EvictArgs a, Moved m, int slices) {
-  const int h = blockIdx.x / slices, slice = blockIdx.x % slices, b = blockIdx.y, t = blockIdx.z;
+  // (the last tensors, of 4 bytes a head, first: theirs are the longest turns)
+  const int h = blockIdx.x / slices, slice = blockIdx.x % slices, b = blockIdx.y, t = gridDim.z - 1 - blockIdx.z;
   int64_t len;
   if (length_of(a, b, len) <= a.budget) return;
   const int64_t bytes = m.head_bytes[t], token = bytes * a.heads;
@@ -267,14 +357,17 @@ __global__ __launch_bounds__(T) void evict_move_kernel(EvictArgs a, Moved m, int
   const int32_t* slots = a.slots + (lists + h) * a.budget;
   char* const base = m.base[t];
   if (bytes == 4) {
-    if (h == 0 && slice == 0) move_rows<uint32_t, T>(a, base, token, 0, a.heads, b, slots, a.budget, true);
+    // (few sequences: two heads a workgroup)
+    const int share = T > 256 ? 2 : a.heads;
+    if (h % share == 0 && slice == 0)
+      move_rows<uint32_t, T>(a, base + 4 * h, token, min(share, a.heads - h), b, slots, a.budget, true);
   } else if (bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
     // a slice: an even share of the row's 16-byte items
     const int units = (int)(bytes / 16), share = (units + slices - 1) / slices, c0 = slice * share;
     if (c0 < units)
-      move_rows<u32x4, T>(a, base, token, h * bytes + 16 * c0, min(share, units - c0), b, slots, 0, false);
+      move_rows<u32x4, T>(a, base + h * bytes + 16 * c0, token, min(share, units - c0), b, slots, 0, false);
   } else if (slice == 0) {
-    move_rows<uint32_t, T>(a, base, token, h * bytes, (int)(bytes / 4), b, slots, 0, false);
+    move_rows<uint32_t, T>(a, base + h * bytes, token, (int)(bytes / 4), b, slots, 0, false);
   }
 }
 
@@ -287,6 +380,13 @@ int log2_exact(int64_t v) {
 
 int64_t capacity_of(int max_blocks, int block_size) { return (int64_t)max_blocks * block_size; }
 
+// The forms of the selection by the table's width: tokens that a workgroup of 256
+// threads holds (8 vectors a wave); wider ones go by transposed keys.
+constexpr int kHeldVectors = 8;
+constexpr int kHeldTokens = 256 * 4 * kHeldVectors;
+bool needs_keys(int64_t cap) { return cap > kHeldTokens; }
+int64_t key_stride_of(int64_t cap) { return (cap + 3) / 4 * 4; }
+
 }  // namespace
 }  // namespace mkv
 
@@ -296,7 +396,7 @@ extern "C" size_t mkv_evict_tokens_workspace_size(int num_layers, int batch, int
                                                   int max_blocks, int budget) {
   if (num_layers <= 0 || batch <= 0 || num_kv_heads <= 0 || max_blocks <= 0 || block_size <= 0 || budget <= 0) return 0;
   const size_t lists = (size_t)num_layers * batch * num_kv_heads, cap = (size_t)capacity_of(max_blocks, block_size);
-  return lists * ((size_t)budget + (cap > kLdsKeys ? cap : 0)) * 4;
+  return ((lists * budget + 3) / 4 * 4 + (needs_keys(cap) ? lists * key_stride_of(cap) : 0)) * 4;
 }
 
 extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_bytes, const int* layer_of,
@@ -309,7 +409,7 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
       num_pages < 0 || max_blocks < 0 || budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
     return MKV_ERR_BAD_SHAPE;
   const int bs_log2 = log2_exact(block_size);
-  if (bs_log2 < 0) return MKV_ERR_BAD_BLOCK_SIZE;
+  if (bs_log2 < 2) return MKV_ERR_BAD_BLOCK_SIZE;
   if (num_pages > (0x7fffffff >> bs_log2) || capacity_of(max_blocks, block_size) > 0x7fff0000) return MKV_ERR_BAD_SHAPE;
   if (seq_lens_dtype != MKV_INDEX_I32 && seq_lens_dtype != MKV_INDEX_I64) return MKV_ERR_UNSUPPORTED_DTYPE;
   if (batch == 0 || num_layers == 0) return MKV_OK;
@@ -327,7 +427,7 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
     if (!weights[l]) return MKV_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(weights[l]) & 3) return MKV_ERR_MISALIGNED;
   }
-  if ((reinterpret_cast<uintptr_t>(workspace) & 3) != 0) return MKV_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return MKV_ERR_MISALIGNED;
   const int64_t cap = capacity_of(max_blocks, block_size);
   const int64_t pairs = ((int64_t)(num_layers < kMaxTensors ? num_layers : kMaxTensors) * batch + 7) / 8 * 8;
   if (pairs * num_kv_heads > 0x3fffff || (int64_t)num_layers * batch * num_kv_heads > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
@@ -344,21 +444,21 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
   a.recent = recent;
   a.new_lens = new_lens;
   a.slots = reinterpret_cast<int32_t*>(workspace);
-  a.keys = reinterpret_cast<uint32_t*>(a.slots + (size_t)num_layers * batch * num_kv_heads * budget);
-  a.key_stride = cap;
+  a.keys = reinterpret_cast<uint32_t*>(a.slots + ((size_t)num_layers * batch * num_kv_heads * budget + 3) / 4 * 4);
+  a.key_stride = key_stride_of(cap);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   for (int l0 = 0; l0 < num_layers; l0 += kMaxTensors) {
     const int layers = num_layers - l0 < kMaxTensors ? num_layers - l0 : kMaxTensors;
     Weights w;
     for (int l = 0; l < layers; ++l) w.base[l] = reinterpret_cast<const float*>(weights[l0 + l]);
     const dim3 grid((unsigned)(((int64_t)layers * batch + 7) / 8 * 8 * num_kv_heads));
-    if (cap > kLdsKeys) {
-      const unsigned x = (unsigned)((cap + 255) / 256 < 256 ? (cap + 255) / 256 : 256);
+    if (needs_keys(cap)) {
+      const unsigned x = (unsigned)((cap + 255) / 256 < 1024 ? (cap + 255) / 256 : 1024);
       hipLaunchKernelGGL(evict_keys_kernel, dim3(x, (unsigned)batch, (unsigned)layers), dim3(256), 0, s, a, w, l0);
       if (hipError_t e = hipGetLastError()) return (int)e;
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, false>), grid, dim3(1024), 0, s, a, w, l0, layers);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, 16, true>), grid, dim3(1024), 0, s, a, w, l0, layers);
     } else {
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, true>), grid, dim3(256), (size_t)cap * 4, s, a, w, l0, layers);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, kHeldVectors, false>), grid, dim3(256), 0, s, a, w, l0, layers);
     }
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
@@ -370,8 +470,19 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
       m.head_bytes[t] = (int32_t)head_bytes[t0 + t];
       m.layer[t] = layer_of[t0 + t];
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_move_kernel<256>), dim3((unsigned)num_kv_heads, (unsigned)batch, (unsigned)n),
-                       dim3(256), 0, s, a, m, 1);
+    // Workgroups: one a (tensor, sequence, head), or of few of them larger ones, a
+    // slice of the row each (64 bytes at least): what is in flight has to cover the
+    // memory's latency, 16 KB a CU and more.
+    const int64_t whole = (int64_t)num_kv_heads * batch * n;
+    auto move = [&](auto threads, int slices) {
+      constexpr int T = decltype(threads)::value;
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_move_kernel<T>), dim3((unsigned)(num_kv_heads * slices), (unsigned)batch, (unsigned)n),
+                         dim3(T), 0, s, a, m, slices);
+    };
+    if (whole >= 2048)
+      move(std::integral_constant<int, 256>{}, 1);
+    else
+      move(std::integral_constant<int, 1024>{}, whole >= 512 ? 1 : 2);
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
   return MKV_OK;

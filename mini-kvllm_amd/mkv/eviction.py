@@ -42,8 +42,8 @@ class CacheEviction:
         if len(shape) != 4 or not all(shape):
             raise ValueError(f"a cache must be (num_blocks, block_size, num_kv_heads, head_dim); got {tuple(shape)}")
         self.num_blocks, self.block_size, self.num_kv_heads = shape[:3]
-        if self.block_size & (self.block_size - 1):
-            raise ValueError(f"block_size must be a power of two; got {self.block_size}")
+        if self.block_size < 4 or self.block_size & (self.block_size - 1):
+            raise ValueError(f"block_size must be a power of two from 4 on; got {self.block_size}")
         if self.num_kv_heads > 1024 or self.num_blocks * self.block_size > 0x7fffffff:
             raise ValueError(f"a cache of {tuple(shape)} has too many heads or tokens")
         rows = self.num_blocks * self.block_size * self.num_kv_heads

@@ -27,7 +27,7 @@ def evict(lib, **over):  # noqa: F811
 
 
 def test_evict_refusals(lib):  # noqa: F811
-    assert evict(lib, bs=24) == -6 and evict(lib, heads=0) == -2 and evict(lib, heads=1025) == -2
+    assert evict(lib, bs=24) == -6 and evict(lib, bs=2) == -6 and evict(lib, heads=0) == -2 and evict(lib, heads=1025) == -2
     assert evict(lib, batch=70000) == -2 and evict(lib, budget=0) == -2 and evict(lib, sinks=-1) == -2
     assert evict(lib, sinks=5, recent=4) == -2 and evict(lib, recent=2 ** 31 - 1) == -2
     assert evict(lib, pages=1 << 28) == -2 and evict(lib, blocks=1 << 28, stride=1 << 28) == -2
