@@ -298,7 +298,9 @@ constexpr int kSplitKeys = 1024;  // of a unit: 16 tiles a wave
 template <int KV, int CT, int D, int NI, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) {
   using Tile = DecodeTile<KV, CT, D>;
-  constexpr int kAhead = KV == MKV_DTYPE_F32 ? 2 : 4;  // tiles of a wave in a batch; two batches in flight
+  // Tiles of a wave in a batch, two batches in flight: twice as many leave half the
+  // workgroups on a CU (contexts of 98k and 131k keys 109 us against 100).
+  constexpr int kAhead = KV == MKV_DTYPE_F32 ? 1 : 2;
   extern __shared__ float scores[];                    // (tile, i, lane)
   __shared__ float part_m[kWaves][4 * NI], part_l[kWaves][4 * NI];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -321,7 +323,6 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
   for (int u = x; u < units; u += a.grid_units) {
     const int k0 = u * a.unit, k1 = min(sq.keys, k0 + a.unit);
     const WaveTiles w(a, seq, k0, k1, wave);
-    float* const kept = SPLIT ? a.ws_t + ((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI * 64 + lane : nullptr;
     float m[NI], l[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -354,13 +355,12 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
             const float v = sees ? s[i] * f : kNegInf;
+            scores[(((n0 + j) * kWaves + wave) * NI + i) * 64 + lane] = v;
             if constexpr (SPLIT) {
-              kept[(((n0 + j) * kWaves + wave) * NI + i) * 64] = v;
               const float top = fmaxf(m[i], v);
               l[i] = __builtin_fmaf(l[i], __builtin_amdgcn_exp2f(m[i] - top), __builtin_amdgcn_exp2f(v - top));
               m[i] = top;
             } else {
-              scores[(((n0 + j) * kWaves + wave) * NI + i) * 64 + lane] = v;
               m[i] = fmaxf(m[i], v);
             }
           }
@@ -379,6 +379,16 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
       load(t0, h0, n0 + 2 * kAhead);
       take(t1, h1, n0 + kAhead);
       load(t1, h1, n0 + 3 * kAhead);
+    }
+    if constexpr (SPLIT) {
+      // (here: stores among the loads would have to end before the loads behind them)
+      float* const kept = a.ws_t + ((int64_t)pair * a.max_units + u) * (a.unit / 16) * NI * 64 + lane;
+      for (int n = 0; n < w.num; ++n)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int at = ((n * kWaves + wave) * NI + i) * 64;
+          kept[at] = scores[at + lane];
+        }
     }
     // ---- the queries' maxima and sums, of the wave and of all ----
 #pragma unroll
@@ -1223,9 +1233,9 @@ int launch_weights(WeightArgs& a, const Plan& p, hipStream_t s) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, false>), grid, dim3(kThreads), lds, s, a);
     } else {
       if (p.ni == 1)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, true>), grid, dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, true>), grid, dim3(kThreads), lds, s, a);
       else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, true>), grid, dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, true>), grid, dim3(kThreads), lds, s, a);
       if (hipError_t e = hipGetLastError()) return (int)e;
       if (p.ni == 1)
         hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<1>), grid, dim3(kThreads), 0, s, a);

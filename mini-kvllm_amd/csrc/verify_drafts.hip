@@ -41,6 +41,7 @@ struct VerifyArgs {
   int64_t row_stride, draft_stride;  // elements
   int64_t total;
   int vocab, chunks;
+  int group;          // lanes of the walk that join a row's chunks: a power of two
   const void* ids;
   const void* parents;  // NULL: chains
   int ids_i64, parents_i64;
@@ -131,16 +132,14 @@ MKV_DEV Nodes nodes_of(const VerifyArgs& a, int s) {
   const int64_t q1 = min(max((int64_t)a.cu[s + 1], q0), a.total);
   return Nodes{q0, (int)min(q1 - q0, (int64_t)a.max_nodes)};
 }
-// log2(e) / T; 0: greedy
+// log2(e) / T, above 0 (an infinite T: all alike but -inf); 0: greedy
 MKV_DEV float slope_of(const VerifyArgs& a, int s) {
   const float t = a.temperatures ? a.temperatures[s] : 1.0f;
-  return t > 1e-30f ? kLog2e / t : 0.0f;
+  return t > 1e-30f ? fmaxf(kLog2e / t, 1e-36f) : 0.0f;
 }
 MKV_DEV bool finite(float x) { return fabsf(x) < __builtin_huge_valf(); }
-// e^((x - m) / T): 0 for -inf at any T
-MKV_DEV float weight(float x, float m, float c) {
-  return x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((x - m) * c);
-}
+// e^((x - m) / T): 0 for -inf (m is finite, c above 0)
+MKV_DEV float weight(float x, float m, float c) { return __builtin_amdgcn_exp2f((x - m) * c); }
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
@@ -221,6 +220,16 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   }
 }
 
+// Maximum, sum and the maximum's place of two parts of a row (a NaN is the largest).
+MKV_DEV void join(float& m, float& s, int& place, float m2, float s2, int place2, float c) {
+  const float top = maximum(m, m2);
+  const bool first = m == top || m != m, second = m2 == top || m2 != m2;
+  place = min(first ? place : 0x7fffffff, second ? place2 : 0x7fffffff);
+  // (a sum without a finite maximum is not looked at)
+  s = (m == top ? s : s * weight(m, top, c)) + (m2 == top ? s2 : s2 * weight(m2, top, c));
+  m = top;
+}
+
 // A node in LDS.
 struct Node {
   float m, s;      // of its row: maximum and sum
@@ -273,24 +282,21 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a)
     nodes[i].parent = p >= 0 && p < i ? (int)p : -1;
     nodes[i].u = a.uniforms[r];
   }
-  for (int i = wave; i < n; i += kWalkThreads / 64) {
-    for (int which = 0; which < (a.draft ? 2 : 1); ++which) {
+  // ---- the rows' maxima and sums: as many lanes a row as it has chunks, up to 64 ----
+  {
+    const int group = min(a.group, 64), in = tid & (group - 1);
+    for (int r0 = tid / group; r0 < (a.draft ? 2 : 1) * n; r0 += kWalkThreads / group) {
+      const int which = r0 >= n ? 1 : 0, i = r0 - which * n;
       const f32x4* st = a.stats + (which * a.total + rows.first + i) * a.chunks;
       float m = kNegInf, s = 0.0f;
       int place = 0x7fffffff;
-      for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-        f32x4 v = f32x4{kNegInf, 0.0f, __int_as_float(0x7fffffff), 0.0f};
-        if (c0 + lane < a.chunks) v = st[c0 + lane];
-        const float top = maximum(m, wave_max(v[0]));
-        const bool ok = finite(top);
-        const float f0 = ok ? weight(m, top, c) : 0.0f, f = ok ? weight(v[0], top, c) : 0.0f;
-        int here = v[0] == top || v[0] != v[0] ? __float_as_int(v[2]) : 0x7fffffff;
-        here = wave_all(here, [](int u, int w) { return min(u, w); });
-        place = m == top || m != m ? min(place, here) : here;
-        s = s * f0 + wave_sum(v[1] * f);
-        m = top;
+      for (int c0 = in; c0 < a.chunks; c0 += group) {
+        const f32x4 v = st[c0];
+        join(m, s, place, v[0], v[1], __float_as_int(v[2]), c);
       }
-      if (lane == 0) {
+      for (int o = 1; o < group; o <<= 1)
+        join(m, s, place, __shfl_xor(m, o), __shfl_xor(s, o), __shfl_xor(place, o), c);
+      if (in == 0) {
         if (which == 0) {
           nodes[i].m = m;
           nodes[i].s = s;
@@ -334,8 +340,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a)
   float fa = 1.0f, fb = 0.0f;  // what is left: fa p - fb q (drafts without q: fa p, but for what was turned down)
   float rest = 1.0f;           // without q: p less what was turned down
   bool behind = false;         // a rejection whose sum is still to be taken
-  for (int i = 1; i < n; ++i) {
-    if (nodes[i].parent != cur) continue;
+  // the first child of the node reached behind node `after`, n: none
+  auto next_child = [&](int after) {
+    for (int i0 = (after + 1) & ~63; i0 < n; i0 += 64) {
+      const int i = i0 + lane;
+      const uint64_t kids = __builtin_amdgcn_ballot_w64(i > after && i < n && nodes[min(i, n - 1)].parent == cur);
+      if (kids) return i0 + __builtin_ctzll(kids);
+    }
+    return n;
+  };
+  for (int i = next_child(0); i < n; i = next_child(i)) {
     bool take;
     const bool with_q = a.draft && nodes[cur].place < 0 && finite(nodes[cur].qm);
     if (nodes[cur].place >= 0) {
@@ -415,40 +429,65 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
   const char* prow = a.logits + st.row * a.row_stride * kSize<DT>;
   const char* qrow = a.draft + (a.draft ? st.row * a.draft_stride * kSize<DT> : 0);
   const char* nrow = reinterpret_cast<const char*>(a.noise + seq * a.noise_stride);
-  unsigned long long best = 0;
+  // the leader's value and place: of what is left, or (fallback) of p itself
+  auto race = [&](bool fallback) -> unsigned long long {
+    float best = 0.0f;
+    int at_best = 0;
 #pragma unroll
-  for (int j = 0; j < kPer / P::kVec; ++j) {
-    const int at = (j * kThreads + tid) * P::kVec;
-    const int64_t i = (int64_t)chunk * kChunk + at;
-    if (i >= a.vocab) continue;
-    float x[P::kVec], y[P::kVec] = {}, e[P::kVec];
-    P::load(prow, i, a.vocab, x);
-    if (st.q_mul > 0.0f) P::load(qrow, i, a.vocab, y);
+    for (int j = 0; j < kPer / P::kVec; ++j) {
+      const int at = (j * kThreads + tid) * P::kVec;
+      const int64_t i = (int64_t)chunk * kChunk + at;
+      if (i >= a.vocab) continue;
+      float x[P::kVec], y[P::kVec], e[P::kVec];
+      P::load(prow, i, a.vocab, x);
+      if (st.q_mul > 0.0f) P::load(qrow, i, a.vocab, y);
 #pragma unroll
-    for (int v = 0; v < P::kVec; v += 4) N::load(nrow, i + v, a.vocab, e + v);
-    const uint32_t gone = out[at >> 5] >> (at & 31);
+      for (int v = 0; v < P::kVec; v += 4) N::load(nrow, i + v, a.vocab, e + v);
+      const uint32_t gone = st.barred && !fallback ? out[at >> 5] >> (at & 31) : 0u;
 #pragma unroll
-    for (int v = 0; v < P::kVec; ++v) {
-      const float p = st.p_mul * weight(x[v], st.p_max, st.c);
-      float w = gone >> v & 1 ? 0.0f : p;
-      if (st.q_mul > 0.0f) w = p - st.q_mul * weight(y[v], st.q_max, st.c);
-      const bool left = w > 0.0f;
-      const float value = (left ? w : weight(x[v], st.p_max, st.c)) / e[v];
-      const unsigned long long key = (unsigned long long)(left ? 1u : 0u) << 63 |
-                                     (unsigned long long)__float_as_uint(value) << 32 | (uint32_t)~(uint32_t)(i + v);
-      if (i + v < a.vocab && value > 0.0f && key > best) best = key;
+      for (int v = 0; v < P::kVec; ++v) {
+        float w = weight(x[v], st.p_max, st.c);
+        if (!fallback) {
+          w *= st.p_mul;
+          if (st.q_mul > 0.0f) w -= st.q_mul * weight(y[v], st.q_max, st.c);
+          w = gone >> v & 1 ? 0.0f : w;
+        }
+        // (past the row's end: x is -inf)
+        const float value = w * __builtin_amdgcn_rcpf(e[v]);
+        const bool ahead = w > 0.0f && value > best;
+        best = ahead ? value : best;
+        at_best = ahead ? at + v : at_best;
+      }
     }
-  }
-  best = wave_all(best, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
-  __shared__ unsigned long long part[kThreads / 64];
-  if (lane == 0) part[tid >> 6] = best;
+    // a lane's places rise, so that its first leader is the lowest
+    unsigned long long key = best > 0.0f ? (unsigned long long)(fallback ? 0u : 1u) << 63 |
+                                               (unsigned long long)__float_as_uint(best) << 32 |
+                                               (uint32_t)~(uint32_t)((int64_t)chunk * kChunk + at_best)
+                                         : 0ull;
+    return wave_all(key, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
+  };
+  __shared__ unsigned long long part[2][kThreads / 64];
+  unsigned long long best = race(false);
+  if (lane == 0) part[0][tid >> 6] = best;
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) best = part[0][w] > best ? part[0][w] : best;
+  if (best == 0) {  // nothing is left in this chunk
+    best = race(true);
+    if (lane == 0) part[1][tid >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) best = part[1][w] > best ? part[1][w] : best;
+  }
   if (tid != 0) return;
-  for (int w = 1; w < kThreads / 64; ++w) best = part[w] > best ? part[w] : best;
-  // (a maximum: the order of the workgroups changes nothing)
-  __hip_atomic_fetch_max(&a.state[seq].best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (__hip_atomic_fetch_add(&a.state[seq].arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)a.chunks) {
-    const unsigned long long won = __hip_atomic_load(&a.state[seq].best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // (a maximum: the order of the workgroups changes nothing.  Both counters are at the
+  // memory's side; the first one's answer is here before the second one goes out)
+  unsigned long long* const leader = &a.state[seq].best;
+  unsigned long long was = __hip_atomic_fetch_max(leader, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" : "+v"(was) : : "memory");
+  if (__hip_atomic_fetch_add(&a.state[seq].arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (unsigned)a.chunks) {
+    asm volatile("" ::: "memory");
+    const unsigned long long won = __hip_atomic_load(leader, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // (no key at all: E is infinite or not a number everywhere)
     a.next[seq] = won ? (int64_t)(uint32_t)~(uint32_t)won : 0;
   }
@@ -519,6 +558,8 @@ extern "C" int mkv_verify_drafts(int64_t* accepted, int64_t* num_accepted, int64
   a.total = total;
   a.vocab = vocab;
   a.chunks = chunks;
+  a.group = 1;
+  while (a.group < chunks && a.group < 64) a.group <<= 1;
   a.ids = token_ids;
   a.parents = parents;
   a.ids_i64 = ids_dtype == MKV_INDEX_I64;

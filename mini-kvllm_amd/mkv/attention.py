@@ -791,6 +791,12 @@ class Attention(nn.Module):
         # explicit one (DECODE_STREAM, n > 0 for n-token split-K,
         # DECODE_WORKGROUP), as for paged_attention_decode
         self.decode_split_tokens = 0
+        # fp32 (num_blocks, block_size, num_kv_heads), injected like the caches:
+        # every step then accumulates the attention weight that each cached token
+        # receives (paged_attention_weights, with this decay), which
+        # mkv.CacheEviction goes by
+        self.attention_weights: torch.Tensor | None = None
+        self.weights_decay = 1.0
 
     def _mode(self) -> str:
         mode = self.kv_cache_dtype
@@ -827,6 +833,15 @@ class Attention(nn.Module):
             k_scale=self.k_scale if quant else None, v_scale=self.v_scale if quant else None,
             kv_cache_dtype=self.kv_cache_dtype)
 
+    def _accumulate(self, q, context, cu_seqlens_q, scale):
+        if context.context_lens is None or context.block_tables is None:
+            raise ValueError("attention weights require context_lens and block_tables")
+        paged_attention_weights(
+            q, self.k_cache, self.attention_weights, context.block_tables, context.context_lens, scale, self.num_heads,
+            self.num_kv_heads, self.head_dim, self.block_size, cu_seqlens_q=cu_seqlens_q,
+            k_scale=self.k_scale if self._mode() != "auto" else None, kv_cache_dtype=self.kv_cache_dtype,
+            decay=self.weights_decay)
+
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                 kv_appended: bool = False) -> torch.Tensor:
         """The reference's forward (store, then attend).  kv_appended=True:
@@ -855,6 +870,10 @@ class Attention(nn.Module):
             cu_seqlens = context.cu_seqlens_q
             if cu_seqlens is None:
                 raise ValueError("cu_seqlens_q must be provided for varlen attention")
+            if self.attention_weights is not None:
+                if getattr(context, "tree_mask", None) is not None:
+                    raise ValueError("attention weights are not accumulated over trees of drafted tokens")
+                self._accumulate(q, context, cu_seqlens, scale)
             if getattr(context, "tree_mask", None) is not None:
                 # drafted tokens: each row sees the prefix and what its mask names
                 if context.context_lens is None or context.block_tables is None:
@@ -906,5 +925,7 @@ class Attention(nn.Module):
             o = self._prefill(q, context.block_tables, context.context_lens, cu_seqlens,
                               context.positions, scale)
             return o.reshape(o.shape[0], self.num_heads * self.head_dim)
+        if self.attention_weights is not None:
+            self._accumulate(q, context, None, scale)
         o = self._decode(q, context.block_tables, context.context_lens, scale)
         return o.reshape(o.shape[0], self.num_heads * self.head_dim)

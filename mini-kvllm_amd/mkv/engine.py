@@ -42,8 +42,9 @@ from torch.utils._device import DeviceContext
 
 from . import _lib
 from . import context as C
-from .attention import DECODE_STREAM, DECODE_WORKGROUP, Attention, _dtype_code, _stream
+from .attention import DECODE_STREAM, DECODE_WORKGROUP, PER_TOKEN_HEAD_MODES, Attention, _dtype_code, _stream
 from .decode_state import DecodeGraphs, DecodeMetadata
+from .eviction import CacheEviction
 from .logprobs import MAX_TOP, token_logprobs
 from .producer import qkv_norm_rope_append, qkv_norm_rope_append_decode
 
@@ -466,6 +467,7 @@ class Qwen3Model(torch.nn.Module):
             att.k_cache = torch.zeros(num_blocks, self.block_size, cfg.num_kv_heads, cfg.head_dim,
                                       dtype=cdt, device=dev)
             att.v_cache = torch.zeros_like(att.k_cache)
+            att.attention_weights = None  # (those of caches before these)
             att.kv_cache_dtype = kv_cache_dtype
             if kv_cache_dtype == "fp8_per_tensor":
                 att.k_scale = torch.ones(1, device=dev)
@@ -473,6 +475,19 @@ class Qwen3Model(torch.nn.Module):
             elif kv_cache_dtype != "auto":
                 att.k_scale = torch.zeros(num_blocks, self.block_size, cfg.num_kv_heads, device=dev)
                 att.v_scale = torch.zeros_like(att.k_scale)
+
+    def attach_attention_weights(self, decay: float = 1.0) -> CacheEviction:
+        """Accumulate, from now on, the attention weight that every cached token
+        receives in each layer and KV head (decay times what it had, a step), beside
+        the caches of :meth:`attach_kv_cache`; returns the eviction that goes by it.
+        Decode steps then run the producer, the weights and the attention as calls of
+        their own."""
+        att = [lay["attn"] for lay in self.layers]
+        for a in att:
+            a.attention_weights = torch.zeros(a.k_cache.shape[:3], dtype=torch.float32, device=a.k_cache.device)
+            a.weights_decay = decay
+        scales = ([a.k_scale for a in att], [a.v_scale for a in att]) if self.kv_cache_dtype in PER_TOKEN_HEAD_MODES else (None, None)
+        return CacheEviction([a.k_cache for a in att], [a.v_cache for a in att], [a.attention_weights for a in att], *scales)
 
     def scales(self) -> list[torch.Tensor]:
         """The per-tensor FP8 scales (what a decode graph's capture must
@@ -504,7 +519,7 @@ class Qwen3Model(torch.nn.Module):
             qkv = normed_linear(x, residual, lay["in_norm"], cfg.eps, lay["qkv"], 0, free)
             att = lay["attn"]
             ctx = C.current_context()
-            if self.fuse_decode_step and not ctx.is_prefill:
+            if self.fuse_decode_step and not ctx.is_prefill and att.attention_weights is None:
                 # a decode step: the producer step and the attention in one
                 # launch where the decode schedule allows it
                 o = qkv_norm_rope_append_decode(
