@@ -520,16 +520,41 @@ MKV_DEV void meet() {
 }
 MKV_DEV int div_group(const WeightArgs& a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.inv_group); }
 
-template <class X>
-MKV_DEV X wave_sum(X x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+// Sums over the wave's lanes up to each, by DPP moves.
+MKV_DEV int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using All = std::integral_constant<int, 0xf>;
+  add(std::integral_constant<int, 0x111>{}, All{});  // row_shr 1, 2, 4, 8
+  add(std::integral_constant<int, 0x112>{}, All{});
+  add(std::integral_constant<int, 0x114>{}, All{});
+  add(std::integral_constant<int, 0x118>{}, All{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15, 31
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return x;
+}
+MKV_DEV double wave_scan(double x) {  // (whole numbers: exact)
+  auto add = [&](auto ctrl, auto rows) {
+    const int64_t b = __builtin_bit_cast(int64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    x += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  using All = std::integral_constant<int, 0xf>;
+  add(std::integral_constant<int, 0x111>{}, All{});
+  add(std::integral_constant<int, 0x112>{}, All{});
+  add(std::integral_constant<int, 0x114>{}, All{});
+  add(std::integral_constant<int, 0x118>{}, All{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
   return x;
 }
 MKV_DEV int64_t lane64(int64_t x, int l) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
                    (uint32_t)__builtin_amdgcn_readlane((int)x, l));
 }
+MKV_DEV double lane64(double x, int l) { return __builtin_bit_cast(double, lane64(__builtin_bit_cast(int64_t, x), l)); }
 // Which of the sequences' parts (sequence q has parts(q)) number i is: the sequence
 // and its place in it; false past the last.  Every wave works it out alike, a lane a
 // sequence, so that workgroups' numbers have no gaps.
@@ -544,14 +569,7 @@ MKV_DEV bool find_part(const WeightArgs& a, int i, Place& p, F parts) {
   int base = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
     const Seq q = seq_of(a, min(s0 + lane, a.num_seqs - 1));
-    const int n = s0 + lane < a.num_seqs ? parts(q) : 0;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o);
-      if (lane >= o) upto += y;
-    }
-    upto += base;
+    const int n = s0 + lane < a.num_seqs ? parts(q) : 0, upto = base + wave_scan(n);
     const uint64_t mine = __builtin_amdgcn_ballot_w64(i >= upto - n && i < upto);
     if (mine) {
       const int l = __builtin_ctzll(mine);
@@ -639,7 +657,7 @@ struct Pieces {
     own = seq_of(a, min(lane, a.num_seqs - 1));
     for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
       const Seq q = lane_seq(s0);
-      total += wave_sum(s0 + lane < a.num_seqs ? cost(q, blocks(q)) : 0.0);
+      total += lane64(wave_scan(s0 + lane < a.num_seqs ? cost(q, blocks(q)) : 0.0), 63);
     }
     const double most = total / ((double)a.group * kMinPiece);
     num = uniform(most < a.shares ? (int)most + 1 : a.shares);
@@ -654,28 +672,18 @@ struct Pieces {
       const bool mine = s0 + lane < a.num_seqs;
       const int n = mine ? blocks(s) : 0;
       const double c = mine ? cost(s, n) : 0.0;
-      double upto = c;
-      int upto_n = n;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(upto, o);
-        const int yn = __shfl_up(upto_n, o);
-        if (lane >= o) {
-          upto += y;
-          upto_n += yn;
-        }
-      }
-      upto += base;
+      const double upto = base + wave_scan(c);
+      const int upto_n = wave_scan(n);
       const uint64_t here = __builtin_amdgcn_ballot_w64(mine && x < upto);
       if (here || s0 + 64 >= a.num_seqs) {
         const int l = here ? __builtin_ctzll(here) : 63;
         seq = min(s0 + l, a.num_seqs - 1);
         q = Seq{lane64(s.q0, l), lane64(s.n, l), lane64(s.first, l), __builtin_amdgcn_readlane(s.keys, l)};
-        base = __builtin_bit_cast(double, lane64(__builtin_bit_cast(int64_t, upto - c), l));
+        base = lane64(upto - c, l);
         base_blocks += __builtin_amdgcn_readlane(upto_n - n, l);
         return;
       }
-      base = __builtin_bit_cast(double, lane64(__builtin_bit_cast(int64_t, upto), 63));
+      base = lane64(upto, 63);
       base_blocks += __builtin_amdgcn_readlane(upto_n, 63);
     }
   }
@@ -976,7 +984,7 @@ __global__ __launch_bounds__(kThreads) void weights_join_kernel(WeightArgs a) {
   double base = 0.0;
   for (int s0 = 0; s0 <= p.seq; s0 += 64) {
     const Seq q = work.lane_seq(s0);
-    base += wave_sum(s0 + (int)(threadIdx.x & 63) < p.seq ? work.cost(q, work.blocks(q)) : 0.0);
+    base += lane64(wave_scan(s0 + (int)(threadIdx.x & 63) < p.seq ? work.cost(q, work.blocks(q)) : 0.0), 63);
   }
   const double c0 = base + work.cost(p.q, p.at), c1 = base + work.cost(p.q, p.at + 1);
   // the pieces from `lo` to `hi` have a part of it
