@@ -18,7 +18,7 @@
 // Read bound: the logits' rows, once, for their maxima and sums
 // (verify_stats_kernel); the walk reads a few words a node (verify_walk_kernel, a
 // workgroup a sequence), and the last row, its draft's and E are read once more
-// (verify_draw_kernel).  Only siblings of a rejected token in a tree with draft
+// (verify_draw_kernel; the walk's own for up to 8192 logits).  Only siblings of a rejected token in a tree with draft
 // distributions cost more: a pass over the two rows for the sum of what is left.
 // Sums are fp32 within a workgroup's 8192 logits.
 #include <type_traits>
@@ -265,11 +265,70 @@ MKV_DEV double left_over(const VerifyArgs& a, int64_t row, float c, float pm, fl
   return sum;
 }
 
+// The race p / E over what is left of p in a chunk (over p itself where rounding leaves
+// nothing): the leader's value and place, by the whole workgroup.
+// out: a bit a logit that is left out.
+template <int DT, int THREADS>
+MKV_DEV unsigned long long race(const VerifyArgs& a, const DrawState& st, int seq, int chunk, const uint32_t* out,
+                                unsigned long long (*part)[THREADS / 64]) {
+  using P = Piece<DT>;
+  using N = Piece<MKV_DTYPE_F32>;
+  const int tid = threadIdx.x;
+  const char* prow = a.logits + st.row * a.row_stride * kSize<DT>;
+  const char* qrow = a.draft + (a.draft ? st.row * a.draft_stride * kSize<DT> : 0);
+  const char* nrow = reinterpret_cast<const char*>(a.noise + seq * a.noise_stride);
+  auto run = [&](bool fallback) -> unsigned long long {
+    float best = 0.0f;
+    int at_best = 0;
+#pragma unroll
+    for (int j = 0; j < kChunk / THREADS / P::kVec; ++j) {
+      const int at = (j * THREADS + tid) * P::kVec;
+      const int64_t i = (int64_t)chunk * kChunk + at;
+      if (i >= a.vocab) continue;
+      float x[P::kVec], y[P::kVec], e[P::kVec];
+      P::load(prow, i, a.vocab, x);
+      if (st.q_mul > 0.0f) P::load(qrow, i, a.vocab, y);
+#pragma unroll
+      for (int v = 0; v < P::kVec; v += 4) N::load(nrow, i + v, a.vocab, e + v);
+      const uint32_t gone = st.barred && !fallback ? out[at >> 5] >> (at & 31) : 0u;
+#pragma unroll
+      for (int v = 0; v < P::kVec; ++v) {
+        float w = weight(x[v], st.p_max, st.c);
+        if (!fallback) {
+          w *= st.p_mul;
+          if (st.q_mul > 0.0f) w -= st.q_mul * weight(y[v], st.q_max, st.c);
+          w = gone >> v & 1 ? 0.0f : w;
+        }
+        // (past the row's end: x is -inf)
+        const float value = w * __builtin_amdgcn_rcpf(e[v]);
+        const bool ahead = w > 0.0f && value > best;
+        best = ahead ? value : best;
+        at_best = ahead ? at + v : at_best;
+      }
+    }
+    // a lane's places rise, so that its first leader is the lowest
+    unsigned long long key = best > 0.0f ? (unsigned long long)(fallback ? 0u : 1u) << 63 |
+                                               (unsigned long long)__float_as_uint(best) << 32 |
+                                               (uint32_t)~(uint32_t)((int64_t)chunk * kChunk + at_best)
+                                         : 0ull;
+    key = wave_all(key, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
+    if ((tid & 63) == 0) part[fallback][tid >> 6] = key;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) key = part[fallback][w] > key ? part[fallback][w] : key;
+    return key;
+  };
+  const unsigned long long best = run(false);
+  return best ? best : run(true);  // nothing is left in this chunk
+}
+
 template <int DT>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a) {
   extern __shared__ __align__(16) char lds[];
   Node* const nodes = reinterpret_cast<Node*>(lds);
   __shared__ double sums[kWalkThreads / 64];
+  __shared__ uint32_t out_bits[kChunk / 32];
+  __shared__ unsigned long long part[2][kWalkThreads / 64];
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Nodes rows = nodes_of(a, seq);
   const int n = rows.n;
@@ -384,41 +443,55 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a)
     }
   }
   for (int i = taken + tid; i < a.max_nodes; i += kWalkThreads) out[i] = -1;
-  if (tid != 0) return;
-  a.num_accepted[seq] = taken;
-  DrawState st{};
-  if (n == 0) {
-    a.next[seq] = -1;
-  } else if (nodes[cur].place >= 0) {
-    a.next[seq] = nodes[cur].place;
-  } else {
-    st.draws = 1;
-    st.row = rows.first + cur;
-    st.c = c;
-    st.p_max = nodes[cur].m;
-    st.p_mul = fa / nodes[cur].s;
-    if (a.draft && finite(nodes[cur].qm) && fb > 0.0f) {
-      st.q_max = nodes[cur].qm;
-      st.q_mul = fb / nodes[cur].qs;
-    } else {
-      for (int j = cur + 1; j < n; ++j)
-        if (nodes[j].parent == cur) a.barred[(int64_t)seq * a.max_nodes + st.barred++] = nodes[j].token;
+  if (tid == 0) a.num_accepted[seq] = taken;
+  if (n == 0 || nodes[cur].place >= 0) {
+    if (tid == 0) {
+      a.next[seq] = n == 0 ? -1 : nodes[cur].place;
+      a.state[seq] = DrawState{};
     }
+    return;
   }
-  a.state[seq] = st;
+  DrawState st{};
+  st.draws = 1;
+  st.row = rows.first + cur;
+  st.c = c;
+  st.p_max = nodes[cur].m;
+  st.p_mul = fa / nodes[cur].s;
+  const bool with_q = a.draft && finite(nodes[cur].qm) && fb > 0.0f;
+  if (with_q) {
+    st.q_max = nodes[cur].qm;
+    st.q_mul = fb / nodes[cur].qs;
+  }
+  if (a.chunks > 1) {
+    if (tid != 0) return;
+    for (int j = cur + 1; j < n; ++j)
+      if (!with_q && nodes[j].parent == cur) a.barred[(int64_t)seq * a.max_nodes + st.barred++] = nodes[j].token;
+    a.state[seq] = st;
+    return;
+  }
+  // A vocabulary of one chunk: the draw is here, and its launch not made (64 sequences
+  // of 3-24 nodes over 8000 logits: 32 us in three launches, 27 in two).
+  for (int i = tid; i < kChunk / 32; i += kWalkThreads) out_bits[i] = 0;
+  __syncthreads();
+  st.barred = !with_q && cur + 1 < n;
+  for (int j = cur + 1 + tid; j < n; j += kWalkThreads) {
+    const int x = nodes[j].token;
+    if (nodes[j].parent == cur && x >= 0) atomicOr(&out_bits[x >> 5], 1u << (x & 31));
+  }
+  __syncthreads();
+  const unsigned long long won = race<DT, kWalkThreads>(a, st, seq, 0, out_bits, part);
+  // (no key at all: E is infinite or not a number everywhere)
+  if (tid == 0) a.next[seq] = won ? (int64_t)(uint32_t)~(uint32_t)won : 0;
 }
 
-// The next token where the walk ended: the race p / E over what is left of p (over p
-// itself where rounding leaves nothing), a workgroup a chunk; the sequence's last one
-// to arrive writes the winner.
+// The next token where the walk ended, a workgroup a chunk; the sequence's last one to
+// arrive writes the race's winner.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
-  using P = Piece<DT>;
-  using N = Piece<MKV_DTYPE_F32>;
-  const int chunk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int chunk = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
   const DrawState st = a.state[seq];
   if (!st.draws) return;
-  __shared__ uint32_t out[kChunk / 32];  // a bit a logit that is left out
+  __shared__ uint32_t out[kChunk / 32];
   for (int i = tid; i < kChunk / 32; i += kThreads) out[i] = 0;
   __syncthreads();
   for (int i = tid; i < st.barred; i += kThreads) {
@@ -426,59 +499,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     if (x >= 0 && x < kChunk) atomicOr(&out[x >> 5], 1u << (x & 31));
   }
   __syncthreads();
-  const char* prow = a.logits + st.row * a.row_stride * kSize<DT>;
-  const char* qrow = a.draft + (a.draft ? st.row * a.draft_stride * kSize<DT> : 0);
-  const char* nrow = reinterpret_cast<const char*>(a.noise + seq * a.noise_stride);
-  // the leader's value and place: of what is left, or (fallback) of p itself
-  auto race = [&](bool fallback) -> unsigned long long {
-    float best = 0.0f;
-    int at_best = 0;
-#pragma unroll
-    for (int j = 0; j < kPer / P::kVec; ++j) {
-      const int at = (j * kThreads + tid) * P::kVec;
-      const int64_t i = (int64_t)chunk * kChunk + at;
-      if (i >= a.vocab) continue;
-      float x[P::kVec], y[P::kVec], e[P::kVec];
-      P::load(prow, i, a.vocab, x);
-      if (st.q_mul > 0.0f) P::load(qrow, i, a.vocab, y);
-#pragma unroll
-      for (int v = 0; v < P::kVec; v += 4) N::load(nrow, i + v, a.vocab, e + v);
-      const uint32_t gone = st.barred && !fallback ? out[at >> 5] >> (at & 31) : 0u;
-#pragma unroll
-      for (int v = 0; v < P::kVec; ++v) {
-        float w = weight(x[v], st.p_max, st.c);
-        if (!fallback) {
-          w *= st.p_mul;
-          if (st.q_mul > 0.0f) w -= st.q_mul * weight(y[v], st.q_max, st.c);
-          w = gone >> v & 1 ? 0.0f : w;
-        }
-        // (past the row's end: x is -inf)
-        const float value = w * __builtin_amdgcn_rcpf(e[v]);
-        const bool ahead = w > 0.0f && value > best;
-        best = ahead ? value : best;
-        at_best = ahead ? at + v : at_best;
-      }
-    }
-    // a lane's places rise, so that its first leader is the lowest
-    unsigned long long key = best > 0.0f ? (unsigned long long)(fallback ? 0u : 1u) << 63 |
-                                               (unsigned long long)__float_as_uint(best) << 32 |
-                                               (uint32_t)~(uint32_t)((int64_t)chunk * kChunk + at_best)
-                                         : 0ull;
-    return wave_all(key, [](unsigned long long u, unsigned long long v) { return u > v ? u : v; });
-  };
   __shared__ unsigned long long part[2][kThreads / 64];
-  unsigned long long best = race(false);
-  if (lane == 0) part[0][tid >> 6] = best;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) best = part[0][w] > best ? part[0][w] : best;
-  if (best == 0) {  // nothing is left in this chunk
-    best = race(true);
-    if (lane == 0) part[1][tid >> 6] = best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) best = part[1][w] > best ? part[1][w] : best;
-  }
+  const unsigned long long best = race<DT, kThreads>(a, st, seq, chunk, out, part);
   if (tid != 0) return;
   // (a maximum: the order of the workgroups changes nothing.  Both counters are at the
   // memory's side; the first one's answer is here before the second one goes out)
@@ -507,6 +529,7 @@ int launch_verify(const VerifyArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(HIP_KERNEL_NAME(verify_walk_kernel<DT>), dim3(a.num_seqs), dim3(kWalkThreads),
                      (size_t)a.max_nodes * sizeof(Node), s, a);
   if (hipError_t e = hipGetLastError()) return (int)e;
+  if (a.chunks == 1) return MKV_OK;
   hipLaunchKernelGGL(HIP_KERNEL_NAME(verify_draw_kernel<DT>), dim3(a.chunks, a.num_seqs), dim3(kThreads), 0, s, a);
   return (int)hipGetLastError();
 }
