@@ -116,7 +116,8 @@ struct Keys {
 #pragma unroll
     for (int j = 0; j < HELD; ++j)
       if (j < num && first + 256 * j < n) f(held[j], token(j));
-    for (int j = HELD; j < num && first + 256 * j < n; ++j) f(more[token(j) / 4], token(j));
+    // (lanes behind the row's end: its last vector, masked)
+    for (int j = HELD; j < num && first + 256 * j < n; ++j) f(more[min(token(j), n - 1) / 4], token(j));
   }
 };
 

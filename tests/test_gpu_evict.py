@@ -142,6 +142,18 @@ def test_long_tables_and_many_layers(dev):
     same(d, c)
 
 
+def test_rows_longer_than_the_registers_hold(dev):
+    """Past 65536 tokens the rest of a row's keys are read again and again; lengths
+    that end within a vector of 256, in the table's last page."""
+    announce("evict: 66500 and 131073 tokens")
+    c, bt, ctx = make([66500, 131073], 1, 2, 4, 16, seed=9)
+    for budget, sinks, recent in ((1200, 4, 64), (66400, 0, 1)):
+        d, want = on(dev, c), {n: [x.clone() for x in xs] for n, xs in c.items()}
+        oracle(want, bt, ctx, budget, sinks, recent)
+        assert handle(d).evict(bt.to(dev), ctx.to(dev), budget, sinks=sinks, recent=recent).tolist() == [budget] * 2
+        same(d, want)
+
+
 def test_absent_pages_are_left_out(dev):
     """An entry outside the pool: its tokens' weights count as lowest, and no row
     is read from there or written there."""
