@@ -123,10 +123,13 @@ struct Keys {
 
 // KEYS: from the transposed keys; else from the weights themselves (up to HELD vectors
 // a wave: 256 T / 64 HELD tokens).
-template <int T, int HELD, bool KEYS>
+// COPIES of the histograms, lanes by turns, lessen what meets at one address: long rows
+// 74 us with one and a wave's common key counted ahead, 61 with four and plain atomics
+// (1, 8, 16: 64, 63, 68); short ones 35 and, with one and plain atomics, 32 (2: 34).
+template <int T, int HELD, bool KEYS, int COPIES>
 __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w, int layer0, int layers) {
   constexpr int kWaves = T / 64;
-  __shared__ int hist[kBins];
+  __shared__ __align__(16) int hist[kBins * COPIES];
   __shared__ int scan[kWaves], found[2], part_kept[kWaves], part_equal[kWaves];
   int layer, b, h;
   if (!place_of(a, layers, blockIdx.x, layer, b, h)) return;
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
     for (int pass = 0; pass < 3; ++pass) {
       constexpr int kNone = 32;
       const int shift = kShift[pass], bins = 1 << kBits[pass], upper = pass == 0 ? kNone : kShift[pass > 0 ? pass - 1 : 0];
-      for (int i = tid; i < kBins; i += T) hist[i] = 0;
+      for (int i = tid; i < kBins * COPIES; i += T) hist[i] = 0;
       __syncthreads();
       const uint32_t above = pass == 0 ? 0u : least >> upper;
       keys.each(n, [&](const u32x4& v, int t) MKV_INLINE {
@@ -186,15 +189,7 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
         for (int e = 0; e < 4; ++e) {
           const bool in = (whole || (t + e >= first && t + e < last)) && (pass == 0 || v[e] >> upper == above);
           const int d = (int)(v[e] >> shift) & (bins - 1);
-          const uint64_t mine = __builtin_amdgcn_ballot_w64(in);
-          if (mine == 0) continue;
-          // (many alike: one addition for the wave)
-          const int one = __builtin_ctzll(mine), d0 = __builtin_amdgcn_readlane(d, one);
-          if (__builtin_amdgcn_ballot_w64(in && d == d0) == mine) {
-            if (lane == one) atomicAdd(&hist[d0], __popcll(mine));
-          } else if (in) {
-            atomicAdd(&hist[d], 1);
-          }
+          if (in) atomicAdd(&hist[d * COPIES + lane % COPIES], 1);
         }
       });
       __syncthreads();
@@ -203,7 +198,9 @@ __global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w,
       int c[kPer], own = 0;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        c[j] = hist[kBins - 1 - (tid * kPer + j)];
+        c[j] = 0;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) c[j] += hist[(kBins - 1 - (tid * kPer + j)) * COPIES + i];
         own += c[j];
       }
       int upto = own;
@@ -457,9 +454,9 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
       const unsigned x = (unsigned)((cap + 255) / 256 < 1024 ? (cap + 255) / 256 : 1024);
       hipLaunchKernelGGL(evict_keys_kernel, dim3(x, (unsigned)batch, (unsigned)layers), dim3(256), 0, s, a, w, l0);
       if (hipError_t e = hipGetLastError()) return (int)e;
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, 16, true>), grid, dim3(1024), 0, s, a, w, l0, layers);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, 16, true, 4>), grid, dim3(1024), 0, s, a, w, l0, layers);
     } else {
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, kHeldVectors, false>), grid, dim3(256), 0, s, a, w, l0, layers);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, kHeldVectors, false, 1>), grid, dim3(256), 0, s, a, w, l0, layers);
     }
     if (hipError_t e = hipGetLastError()) return (int)e;
   }
