@@ -63,6 +63,7 @@ struct WeightArgs {
   // chunks
   int shares;          // pieces of the normalisers' work, at most
   f32x2* part_ml;      // (piece + block, KV head, row of the block): maximum and sum
+  int64_t row_units;   // blocks at most
   float* lse;          // (row) log2 of the normaliser, +inf for a row that sees nothing;
                        // rows by KV head, sequence, token and head of the group
 };
@@ -968,7 +969,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R == 1
       if (r >= rows) continue;
       if (whole)
         a.lse[(h * a.total_q + sq.q0) * a.group + r] = l[b] == 0.0f ? -kNegInf : m[b] + __builtin_amdgcn_logf(l[b]);
-      else  // (pieces and blocks rise together: their sum is a place of its own)
+      else if (base_blocks + block < a.row_units)  // (more of them: cu_seqlens_q falls)
+        // (pieces and blocks rise together: their sum is a place of its own)
         a.part_ml[((int64_t)(piece + base_blocks + block) * a.num_kv_heads + h) * kRows + r - block * kRows] = f32x2{m[b], l[b]};
     }
   }
@@ -1368,6 +1370,7 @@ extern "C" int mkv_paged_weights(float* weights, float decay, const void* q, int
   a.ws_ml = reinterpret_cast<f32x2*>(workspace);
   a.ws_t = reinterpret_cast<float*>(a.ws_ml + (p.decode ? (size_t)num_seqs * num_kv_heads * p.max_units * 4 * p.ni : 0));
   a.shares = p.shares;
+  a.row_units = p.row_units;
   a.part_ml = reinterpret_cast<f32x2*>(workspace);
   a.lse = reinterpret_cast<float*>(a.part_ml + (p.decode ? 0 : (size_t)(p.row_units + p.shares) * num_kv_heads * p.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -30,6 +30,8 @@ workspace has been allocated by a warm-up call.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 
@@ -667,6 +669,8 @@ def paged_attention_weights(query: torch.Tensor, k_cache: torch.Tensor, weights:
     The caches' formats, query types and scales are :func:`paged_attention_tree`'s
     (K alone); head_dim 64 or 128.  Sequences of one call must not share pages.
     Captured in a graph, a call accumulates anew at every replay."""
+    if not math.isfinite(decay):
+        raise ValueError(f"decay must be finite; got {decay}")
     dev = _require_gpu(query, k_cache, weights, block_tables, context_lens,
                        *(t for t in (cu_seqlens_q, k_scale) if t is not None))
     if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:

@@ -480,6 +480,7 @@ class Qwen3Model(torch.nn.Module):
         """Accumulate, from now on, the attention weight that every cached token
         receives in each layer and KV head (decay times what it had, a step), beside
         the caches of :meth:`attach_kv_cache`; returns the eviction that goes by it.
+        Before decode steps are captured: a graph replays what it was captured with.
         Decode steps then run the producer, the weights and the attention as calls of
         their own."""
         att = [lay["attn"] for lay in self.layers]

@@ -49,3 +49,6 @@ def test_the_wrapper_s_checks():
     bt, cl = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int64)
     with pytest.raises(ValueError, match="no CPU fallback"):
         mkv.paged_attention_weights(q, k, w, bt, cl, 0.1, 8, 8, 128, 16)
+    for decay in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="decay must be finite"):
+            mkv.paged_attention_weights(q, k, w, bt, cl, 0.1, 8, 8, 128, 16, decay=decay)
