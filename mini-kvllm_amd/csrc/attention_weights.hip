@@ -586,6 +586,17 @@ MKV_DEV bool find_part(const WeightArgs& a, int i, Place& p, F parts) {
   return false;
 }
 
+template <class F>
+MKV_DEV int count_parts(const WeightArgs& a, F parts) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    const Seq q = seq_of(a, min(s0 + lane, a.num_seqs - 1));
+    total += __builtin_amdgcn_readlane(wave_scan(s0 + lane < a.num_seqs ? parts(q) : 0), 63);
+  }
+  return total;
+}
+
 template <int KV, int CT, int D>
 struct Formats {
   static constexpr bool kF32 = KV == MKV_DTYPE_F32, kCodes = DTypeInfo<KV>::kBytes == 1;
@@ -1020,7 +1031,11 @@ __global__ __launch_bounds__(kThreads) void weights_join_kernel(WeightArgs a) {
   }
 }
 
-// The keys' weights.
+// The keys' weights.  A workgroup takes an even run of the units of 256 keys (fp32: 128)
+// of all sequences, one after another: 4 windows of 32 rows over 8-32k keys 48 us, 3.5
+// TB/s, by a workgroup a unit 59 (it finds its sequence, and its pages, first); 8 chunks
+// of 512 rows, bound by products and exponentials, 82 and 84.  Runs that end within a
+// unit need a kernel more to join them: 86.
 template <int KV, int CT, int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weights_columns_kernel(WeightArgs a) {
   using F = Formats<KV, CT, D>;
@@ -1034,25 +1049,38 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, hf = lane >> 5;
   float mul0 = a.mul;
   if (a.scale_mode == 1) mul0 *= load_uniform_f32(a.k_scale);
-  for (int64_t at = blockIdx.x;; at += gridDim.x) {
-    const int h = (int)(at % a.num_kv_heads);
-    Place place;
-    if (at / a.num_kv_heads > 0x7fffffff ||
-        !find_part(a, (int)(at / a.num_kv_heads), place, [&](const Seq& q) { return (q.keys + kUnit - 1) / kUnit; }))
-      return;
-    const int seq = place.seq;
-    const Seq sq = place.q;
+  auto units_of = [&](const Seq& q) { return (q.keys + kUnit - 1) / kUnit; };
+  const int h = blockIdx.x % a.num_kv_heads, i = blockIdx.x / a.num_kv_heads, shares = gridDim.x / a.num_kv_heads;
+  const int64_t total = count_parts(a, units_of);
+  const int begin = (int)(total * i / shares), end = (int)(total * (i + 1) / shares);
+  Place place;
+  if (begin == end || !find_part(a, begin, place, units_of)) return;
+  int seq = place.seq, unit = place.at, units = place.parts;
+  Seq sq = place.q;
+  for (int left = end - begin; left; --left, ++unit) {
+    if (unit >= units) {  // on to the next sequence with any
+      do {
+        sq = seq_of(a, ++seq);
+        units = units_of(sq);
+      } while (units == 0 && seq + 1 < a.num_seqs);
+      unit = 0;
+    }
     const int rows = (int)sq.n * a.group;
-    const int unit0 = place.at * kUnit, key0 = unit0 + wave * 32 * NK;  // this wave's first key
+    const int unit0 = unit * kUnit, key0 = unit0 + wave * 32 * NK;  // this wave's first key
     // ---- this lane's keys ----
     u32x4 k[NK][F::kOps];
-    float mul[NK], sum[NK];
+    float mul[NK], sum[NK], old[NK];
     int slot[NK];
+#pragma unroll
+    for (int b = 0; b < NK; ++b)
+      slot[b] = a.idx.block_tables[(int64_t)seq * a.idx.bt_stride + (min(key0 + 32 * b + c, sq.keys - 1) >> a.idx.bs_log2)];
 #pragma unroll
     for (int b = 0; b < NK; ++b) {
       const int t = key0 + 32 * b + c;
-      slot[b] = t < sq.keys ? slot_of(a, seq, t) : -1;
-      const char* p = a.k + ((int64_t)max(slot[b], 0) * a.num_kv_heads + h) * (int64_t)(D * F::kEb);
+      slot[b] = t < sq.keys && slot[b] >= 0 && slot[b] < a.idx.num_blocks
+                    ? (slot[b] << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : -1;
+      const int64_t row = (int64_t)max(slot[b], 0) * a.num_kv_heads + h;
+      const char* p = a.k + row * (int64_t)(D * F::kEb);
 #pragma unroll
       for (int s = 0; s < F::kOps; ++s) {
         if constexpr (F::kEb >= 2) {
@@ -1062,8 +1090,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           k[b][s] = codes_to_16<KV, CT>(w[0], w[1]);
         }
       }
-      mul[b] = mul0;
-      if (a.scale_mode == 2) mul[b] *= a.k_scale[(int64_t)max(slot[b], 0) * a.num_kv_heads + h];
+      mul[b] = a.scale_mode == 2 ? mul0 * a.k_scale[row] : mul0;
+      old[b] = a.decay != 0.0f ? a.weights[row] : 0.0f;
       sum[b] = 0.0f;
     }
     // ---- key t is seen by the rows from (t - first) group on: those that see any of
@@ -1170,7 +1198,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
     for (int b = 0; b < NK; ++b) {
       const float w = sum[b] + other_half(sum[b]);
-      if (hf == 0 && slot[b] >= 0) add_weight(a, sq, slot[b], h, key0 + 32 * b + c, w);
+      // (tokens that came with these rows start here, whatever lay there)
+      if (hf == 0 && slot[b] >= 0)
+        a.weights[(int64_t)slot[b] * a.num_kv_heads + h] =
+            a.decay != 0.0f && key0 + 32 * b + c < sq.first ? __builtin_fmaf(a.decay, old[b], w) : w;
     }
   }
 }
@@ -1224,8 +1255,8 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
   // pieces for two workgroups a CU, which run at once
   p.shares = (int)(512 / kv_heads > 0 ? 512 / kv_heads : 1);
   const int unit = f32 ? 128 : 256;
-  const int64_t units = (int64_t)num_seqs * ((capacity + unit - 1) / unit) * kv_heads;
-  p.column_grid = (int)(units < 8192 ? units : 8192);
+  const int64_t units = (int64_t)num_seqs * ((capacity + unit - 1) / unit);
+  p.column_grid = (int)(units < p.shares ? units : p.shares) * kv_heads;
   p.bytes = (size_t)total_q * heads * 4 + (size_t)(p.row_units + p.shares) * kv_heads * p.rows * 8;
   p.bytes = (p.bytes + 15) / 16 * 16;
   return p;
