@@ -140,6 +140,24 @@ def test_many_sequences(dev):
     check(dev, make("bf16", rows, [n + r for n, r in zip(ctx, rows)], 4, 2, 128, 16, seed=6))
 
 
+@pytest.mark.parametrize("fmt", ["fp32", "bf16", "int8_token"])
+def test_runs_of_units_cross_sequences(dev, fmt):
+    """More units of keys than workgroups: each takes several, of several sequences,
+    some of them empty."""
+    announce(f"weights: 140 sequences of 16 KV heads, {fmt}")
+    ctx = [0 if i % 5 == 3 else 1 + 61 * i % 700 for i in range(140)]
+    rows = [min(n, 1 + i % 7) if i % 4 else 0 for i, n in enumerate(ctx)]
+    check(dev, make(fmt, rows, ctx, 32, 16, 64, 16, seed=17), 0.5)
+
+
+@pytest.mark.parametrize("fmt", ["fp32", "bf16", "fp8"])
+@pytest.mark.parametrize("width", [1008, 1024, 1040, 4080, 4096, 4112])
+def test_widths_at_which_a_context_is_split(dev, fmt, width):
+    announce(f"weights: a table of {width} tokens, {fmt}")
+    for Hq in (4, 10):  # (a group of up to four, and more)
+        check(dev, make(fmt, None, [width, width - 15, 3], Hq, 2, 128, 16, seed=width), 0.5)
+
+
 @pytest.mark.parametrize("fmt", ["fp32", "bf16", "fp8_token"])
 def test_a_prompt_s_rows(dev, fmt):
     """Hundreds of rows of each sequence: every form of the row blocks."""
