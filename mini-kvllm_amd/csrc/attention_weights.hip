@@ -8,14 +8,21 @@
 //
 // Decode (one row a sequence): K is read once.  A workgroup takes one KV head's keys,
 // the scores go to LDS, and once their maximum and sum are known the weights follow;
-// long contexts are split, their scores kept in memory for a second kernel.
+// long contexts are split, their scores kept in memory for a second kernel.  HBM bound
+// (98k and 131k keys: K and the kept scores 97 us, 4.9 TB/s, the weights 16), latency
+// bound for short contexts (700 keys 10 us, 60 of 300-800 in fp8 14).
 //
 // Chunks: the normaliser of a row takes all of its keys and the weight of a key all
 // of its rows, so scores are computed twice rather than kept: weights_lse_kernel holds
 // 64 rows of q a wave in registers and streams K through LDS (S^T = K Q^T, a row's
 // maximum and sum in its column's lanes), weights_columns_kernel holds 64 keys a wave
 // and streams q (S = Q K^T, a key's sum in its column's lanes).  Neither product's
-// result leaves the registers and no sum is shared, so the result is one only.
+// result leaves the registers and no sum is shared, so the result is one only.  Kept
+// scores would be 4 bytes a pair, written and read (the windows below 131 us, reading K
+// again 48).  Few rows a sequence are bound by reading K twice (4 windows of 32 rows over 8-32k keys 48
+// and 48 us, 3.5 TB/s); many by the matrix and vector units, which run one after another
+// more than beside each other (8 chunks of 512 rows over 1.5-4.6k keys 86 and 82 us: the
+// MFMA is busy 26% of the first, vector instructions issue in 53%).
 //
 // Products are exact (1-byte codes as 16-bit operands of q's type, fp32 on the fp32
 // MFMA), their sums, the softmax and the weights fp32.
@@ -645,8 +652,8 @@ constexpr int kMinPiece = 256;  // keys
 
 // The normalisers' work is (block of ROWS rows, its keys) after (block, its keys), in
 // the sequences' order, dealt out in even pieces: a piece may end one block and begin
-// the next (8 chunks of 512 rows over 1.5-4.6k keys, whole blocks in shares of their
-// own: 88 us).  Block b of a sequence costs what its last row sees, in keys x group,
+// the next.  Pieces are as many as run at once; twice, three and four times that many
+// took longer.  Block b of a sequence costs what its last row sees, in keys x group,
 //   E(b) = first group + (b + 1) ROWS,   C(b) = E(0) + .. + E(b - 1),
 // whole numbers that doubles hold exactly.
 template <int ROWS, int TILE>
