@@ -19,10 +19,10 @@
 // and streams q (S = Q K^T, a key's sum in its column's lanes).  Neither product's
 // result leaves the registers and no sum is shared, so the result is one only.  Kept
 // scores would be 4 bytes a pair, written and read (the windows below 131 us, reading K
-// again 48).  Few rows a sequence are bound by reading K twice (4 windows of 32 rows over 8-32k keys 48
-// and 48 us, 3.5 TB/s); many by the matrix and vector units, which run one after another
-// more than beside each other (8 chunks of 512 rows over 1.5-4.6k keys 86 and 82 us: the
-// MFMA is busy 26% of the first, vector instructions issue in 53%).
+// again 48).  4 windows of 32 rows over 8-32k keys take 48 and 48 us, 3.5 TB/s of K with
+// vector instructions issuing in 44% of the first (a fourth tile's room: 51); 8 chunks of
+// 512 rows over 1.5-4.6k keys 86 and 82 us, where the matrix and the vector units run
+// one after another more than beside each other: 26% and 53% of the first.
 //
 // Products are exact (1-byte codes as 16-bit operands of q's type, fp32 on the fp32
 // MFMA), their sums, the softmax and the weights fp32.
