@@ -150,6 +150,15 @@ def test_runs_of_units_cross_sequences(dev, fmt):
     check(dev, make(fmt, rows, ctx, 32, 16, 64, 16, seed=17), 0.5)
 
 
+@pytest.mark.parametrize("fmt", ["fp32", "bf16", "fp8_token"])
+def test_short_sequences(dev, fmt):
+    """A few tokens each: pieces of the rows' work that hold none of a block's keys."""
+    announce(f"weights: 64 sequences of 3 to 80 tokens, {fmt}")
+    for Hq, Hkv in ((6, 2), (16, 16)):
+        rows = [3 + i % 2 for i in range(64)]
+        check(dev, make(fmt, rows, [n + i * 7 % 78 for i, n in enumerate(rows)], Hq, Hkv, 64, 16, seed=18), 0.5)
+
+
 @pytest.mark.parametrize("fmt", ["fp32", "bf16", "fp8"])
 @pytest.mark.parametrize("width", [1008, 1024, 1040, 4080, 4096, 4112])
 def test_widths_at_which_a_context_is_split(dev, fmt, width):
