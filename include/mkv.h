@@ -699,7 +699,10 @@ int mkv_trim_pages(int32_t* block_tables, int64_t bt_stride, int max_blocks, con
  * positions below budget.
  * new_lens[b] = min(seq_lens[b], budget).  What lies at positions from budget on stays
  * as it was; positions outside the block table or the pool are left out (their weights
- * count as lowest). */
+ * count as lowest).
+ * workspace: 4 bytes a (layer, sequence, KV head, token of the budget), and for tables
+ * of more than 8192 tokens 4 a (KV head, token of the table) of as many layers and
+ * sequences as 256 MiB hold (of one sequence at least). */
 size_t mkv_evict_tokens_workspace_size(int num_layers, int batch, int num_kv_heads, int block_size, int max_blocks,
                                        int budget);
 int mkv_evict_tokens(const void* const* tensors, const int64_t* head_bytes, const int* layer_of, int num_tensors,

@@ -26,6 +26,12 @@ namespace {
 
 constexpr int kMaxTensors = 128;  // a launch's tensors, their addresses in the kernel arguments
 constexpr int kBins = 2048;
+// Keys of long tables in the workspace: those of as many layers (of one layer's sequences,
+// if need be) as this many bytes hold, of one sequence at least.  The table's width, which
+// may be far past the lengths, sets their size: 28 layers of 60 sequences and 8 heads under
+// tables of 131,072 tokens would be 6.6 GiB together (300-800 tokens cut to 256: 1.46 ms
+// with all of that, 1.63 a layer at a time; under tables of 1024 tokens 0.83).
+constexpr size_t kMaxKeyBytes = (size_t)256 << 20;
 
 struct EvictArgs {
   PagedIndex idx;
@@ -35,7 +41,7 @@ struct EvictArgs {
   int budget, sinks, recent;
   int64_t* new_lens;
   int32_t* slots;   // workspace: (layers, batch, heads, budget), the kept tokens' slots in order
-  uint32_t* keys;   // workspace: (layers, batch, heads, key_stride), for long tables
+  uint32_t* keys;   // workspace: (layers, sequences, heads, key_stride) of a launch, for long tables
   int64_t key_stride;
 };
 struct Weights {
@@ -64,25 +70,29 @@ MKV_DEV int slot_of(const EvictArgs& a, int b, int t) {
   const int32_t p = a.idx.block_tables[(int64_t)b * a.idx.bt_stride + (t >> a.idx.bs_log2)];
   return p >= 0 && p < a.idx.num_blocks ? (p << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : -1;
 }
+// A launch's layers from `layer` on and sequences from `seq` on.
+struct Slice {
+  int layer, layers, seq, seqs;
+};
 // Workgroups of one (layer, sequence) lie 8 apart, on one XCD: its heads share the
-// weights' cache lines.
-MKV_DEV bool place_of(const EvictArgs& a, int layers, int i, int& layer, int& b, int& h) {
+// weights' cache lines.  (layer and b: within the slice)
+MKV_DEV bool place_of(const EvictArgs& a, const Slice& s, int i, int& layer, int& b, int& h) {
   const int group = i / (8 * a.heads), in = i % (8 * a.heads);
   const int pair = group * 8 + in % 8;
   h = in / 8;
-  layer = pair / a.batch;
-  b = pair % a.batch;
-  return layer < layers;
+  layer = pair / s.seqs;
+  b = pair % s.seqs;
+  return layer < s.layers;
 }
 
 // The weights' keys of long tables, transposed to a row a head: four heads a load
 // where their number allows it.
-__global__ __launch_bounds__(256) void evict_keys_kernel(EvictArgs a, Weights w, int layer0) {
-  const int b = blockIdx.y, layer = blockIdx.z;
+__global__ __launch_bounds__(256) void evict_keys_kernel(EvictArgs a, Weights w, Slice of) {
+  const int b = of.seq + blockIdx.y, layer = blockIdx.z;
   int64_t len;
   const int n = length_of(a, b, len);
   if (n <= a.budget) return;
-  uint32_t* const out = a.keys + (int64_t)((layer0 + layer) * a.batch + b) * a.heads * a.key_stride;
+  uint32_t* const out = a.keys + ((int64_t)layer * of.seqs + blockIdx.y) * a.heads * a.key_stride;
   const bool wide = a.heads % 4 == 0 && (reinterpret_cast<uintptr_t>(w.base[layer]) & 15) == 0;
   for (int t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
     const int s = slot_of(a, b, t);
@@ -130,22 +140,23 @@ struct Keys {
 // 74 us with one and a wave's common key counted ahead, 61 with four and plain atomics
 // (1, 8, 16: 64, 63, 68); short ones 35 and, with one and plain atomics, 32 (2: 34).
 template <int T, int HELD, bool KEYS, int COPIES>
-__global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w, int layer0, int layers) {
+__global__ __launch_bounds__(T) void evict_select_kernel(EvictArgs a, Weights w, Slice of) {
   constexpr int kWaves = T / 64;
   __shared__ __align__(16) int hist[kBins * COPIES];
   __shared__ int scan[kWaves], found[2], part_kept[kWaves], part_equal[kWaves];
-  int layer, b, h;
-  if (!place_of(a, layers, blockIdx.x, layer, b, h)) return;
+  int layer, in, h;
+  if (!place_of(a, of, blockIdx.x, layer, in, h)) return;
+  const int b = of.seq + in;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   int64_t len;
   const int n = length_of(a, b, len);
-  if (layer0 + layer == 0 && h == 0 && tid == 0) a.new_lens[b] = min(len, (int64_t)a.budget);
+  if (of.layer + layer == 0 && h == 0 && tid == 0) a.new_lens[b] = min(len, (int64_t)a.budget);
   if (n <= a.budget) return;
-  const int64_t at = ((int64_t)(layer0 + layer) * a.batch + b) * a.heads + h;
+  const int64_t at = ((int64_t)(of.layer + layer) * a.batch + b) * a.heads + h;
   Keys<T, HELD> keys(n, wave);
   if constexpr (KEYS) {
     // (rows are a multiple of four long; what lies behind the last token is masked)
-    keys.more = reinterpret_cast<const u32x4*>(a.keys + at * a.key_stride);
+    keys.more = reinterpret_cast<const u32x4*>(a.keys + (((int64_t)layer * of.seqs + in) * a.heads + h) * a.key_stride);
 #pragma unroll
     for (int j = 0; j < HELD; ++j) keys.held[j] = j < keys.num && keys.token(j) < n ? keys.more[keys.token(j) / 4] : u32x4{0, 0, 0, 0};
   } else {
@@ -387,6 +398,25 @@ constexpr int kHeldVectors = 8;
 constexpr int kHeldTokens = 256 * 4 * kHeldVectors;
 bool needs_keys(int64_t cap) { return cap > kHeldTokens; }
 int64_t key_stride_of(int64_t cap) { return (cap + 3) / 4 * 4; }
+// The layers and sequences of a selection's launch, at most: even shares.
+struct Share {
+  int layers, seqs;
+};
+Share share_of(int num_layers, int batch, int heads, int64_t cap) {
+  Share s{num_layers < kMaxTensors ? num_layers : kMaxTensors, batch};
+  if (needs_keys(cap)) {
+    const size_t one = (size_t)heads * key_stride_of(cap) * 4, fit = kMaxKeyBytes > one ? kMaxKeyBytes / one : 1;
+    const size_t layers = fit / batch < (size_t)s.layers ? fit / batch : s.layers;
+    if (layers) {
+      const int turns = (int)((num_layers + layers - 1) / layers);
+      s.layers = (num_layers + turns - 1) / turns;
+    } else {
+      const int turns = (int)((batch + fit - 1) / fit);
+      s = Share{1, (batch + turns - 1) / turns};
+    }
+  }
+  return s;
+}
 
 }  // namespace
 }  // namespace mkv
@@ -397,7 +427,8 @@ extern "C" size_t mkv_evict_tokens_workspace_size(int num_layers, int batch, int
                                                   int max_blocks, int budget) {
   if (num_layers <= 0 || batch <= 0 || num_kv_heads <= 0 || max_blocks <= 0 || block_size <= 0 || budget <= 0) return 0;
   const size_t lists = (size_t)num_layers * batch * num_kv_heads, cap = (size_t)capacity_of(max_blocks, block_size);
-  return ((lists * budget + 3) / 4 * 4 + (needs_keys(cap) ? lists * key_stride_of(cap) : 0)) * 4;
+  const Share s = share_of(num_layers, batch, num_kv_heads, cap);
+  return ((lists * budget + 3) / 4 * 4 + (needs_keys(cap) ? (size_t)s.layers * s.seqs * num_kv_heads * key_stride_of(cap) : 0)) * 4;
 }
 
 extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_bytes, const int* layer_of,
@@ -448,20 +479,24 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
   a.keys = reinterpret_cast<uint32_t*>(a.slots + ((size_t)num_layers * batch * num_kv_heads * budget + 3) / 4 * 4);
   a.key_stride = key_stride_of(cap);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  for (int l0 = 0; l0 < num_layers; l0 += kMaxTensors) {
-    const int layers = num_layers - l0 < kMaxTensors ? num_layers - l0 : kMaxTensors;
+  const Share share = share_of(num_layers, batch, num_kv_heads, cap);
+  for (int l0 = 0; l0 < num_layers; l0 += share.layers) {
+    const int layers = num_layers - l0 < share.layers ? num_layers - l0 : share.layers;
     Weights w;
     for (int l = 0; l < layers; ++l) w.base[l] = reinterpret_cast<const float*>(weights[l0 + l]);
-    const dim3 grid((unsigned)(((int64_t)layers * batch + 7) / 8 * 8 * num_kv_heads));
-    if (needs_keys(cap)) {
-      const unsigned x = (unsigned)((cap + 255) / 256 < 1024 ? (cap + 255) / 256 : 1024);
-      hipLaunchKernelGGL(evict_keys_kernel, dim3(x, (unsigned)batch, (unsigned)layers), dim3(256), 0, s, a, w, l0);
+    for (int b0 = 0; b0 < batch; b0 += share.seqs) {
+      const Slice of{l0, layers, b0, batch - b0 < share.seqs ? batch - b0 : share.seqs};
+      const dim3 grid((unsigned)(((int64_t)layers * of.seqs + 7) / 8 * 8 * num_kv_heads));
+      if (needs_keys(cap)) {
+        const unsigned x = (unsigned)((cap + 255) / 256 < 1024 ? (cap + 255) / 256 : 1024);
+        hipLaunchKernelGGL(evict_keys_kernel, dim3(x, (unsigned)of.seqs, (unsigned)layers), dim3(256), 0, s, a, w, of);
+        if (hipError_t e = hipGetLastError()) return (int)e;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, 16, true, 4>), grid, dim3(1024), 0, s, a, w, of);
+      } else {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, kHeldVectors, false, 1>), grid, dim3(256), 0, s, a, w, of);
+      }
       if (hipError_t e = hipGetLastError()) return (int)e;
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<1024, 16, true, 4>), grid, dim3(1024), 0, s, a, w, l0, layers);
-    } else {
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(evict_select_kernel<256, kHeldVectors, false, 1>), grid, dim3(256), 0, s, a, w, l0, layers);
     }
-    if (hipError_t e = hipGetLastError()) return (int)e;
   }
   for (int t0 = 0; t0 < num_tensors; t0 += kMaxTensors) {
     const int n = num_tensors - t0 < kMaxTensors ? num_tensors - t0 : kMaxTensors;

@@ -47,6 +47,21 @@ def test_evict_refusals(lib):  # noqa: F811
     assert evict(lib, batch=65535, heads=1024, ws_bytes=1 << 62) == -2
 
 
+def test_the_keys_room_is_bounded(lib):  # noqa: F811
+    """What long tables take follows their width: no more than 256 MiB beside the kept
+    tokens' slots, whatever the layers and sequences, or what one sequence of a layer
+    takes."""
+    def keys(layers, batch, heads, blocks, budget=256):
+        return lib.mkv_evict_tokens_workspace_size(layers, batch, heads, 16, blocks, budget) - layers * batch * heads * budget * 4
+
+    assert keys(28, 60, 8, 131072 // 16) <= 256 << 20  # (all of them: 6.6 GiB)
+    assert keys(28, 60, 8, 8192 // 16) == 0
+    assert keys(4, 2, 8, 66000 // 16) == 4 * 2 * 8 * 4 * 66000
+    for layers, batch, heads, blocks in ((1, 1, 8, 1 << 20), (3, 500, 4, 1 << 17), (200, 3, 1, 1 << 18), (300, 7, 2, 4096)):
+        one = heads * blocks * 16 * 4
+        assert one <= keys(layers, batch, heads, blocks) <= max(one, 256 << 20)
+
+
 def test_trim_refusals(lib):  # noqa: F811
     def trim(bt=p, stride=4, blocks=4, lens=p, held=p, refs=p, pages=10, bs=16, rows=3):
         return lib.mkv_trim_pages(bt, stride, blocks, lens, held, refs, pages, bs, rows, None)

@@ -154,6 +154,20 @@ def test_rows_longer_than_the_registers_hold(dev):
         same(d, want)
 
 
+@pytest.mark.parametrize("tokens", [1 << 22, 1 << 24])
+def test_tables_whose_keys_go_in_turns(dev, tokens):
+    """Tables so wide that the room for keys holds some of the layers, or some of a
+    layer's sequences, at a time."""
+    announce(f"evict: three layers of three sequences under tables of {tokens} tokens")
+    c, bt, ctx = make([300, 9000, 77], 3, 2, 8, 16, scales=True, seed=13, width=tokens // 16)
+    for budget, sinks, recent in ((60, 2, 5), (301, 0, 20)):
+        d, want = on(dev, c), {n: [x.clone() for x in xs] for n, xs in c.items()}
+        lens_want = oracle(want, bt, ctx, budget, sinks, recent)
+        new = handle(d).evict(bt.to(dev), ctx.to(dev), budget, sinks=sinks, recent=recent)
+        assert new.tolist() == lens_want.tolist()
+        same(d, want)
+
+
 def test_absent_pages_are_left_out(dev):
     """An entry outside the pool: its tokens' weights count as lowest, and no row
     is read from there or written there."""
