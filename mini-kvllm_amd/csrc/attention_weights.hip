@@ -300,6 +300,16 @@ struct TileWeights {
 
 constexpr int kSplitKeys = 1024;  // of a unit: 16 tiles a wave
 
+// The workgroup's pair and first unit.  Workgroups go to the XCDs by turns.  A unit's
+// heads share the weights' cache lines and stay together where the units are a multiple of
+// 8, and then the sequences' first units, the only ones with keys under a wide table, are
+// on unlike XCDs (60 sequences of 300-800 tokens under tables of 32,768: 49 us; all first
+// units on one XCD: 181).
+MKV_DEV void place_of(const WeightArgs& a, int& pair, int& x) {
+  pair = blockIdx.x / a.grid_units;
+  x = (int)(blockIdx.x % a.grid_units + pair / a.num_kv_heads) % a.grid_units;
+}
+
 // One workgroup a (sequence, KV head) where its scores fit the LDS; else (SPLIT) a
 // workgroup a unit of the keys, whose scores go to memory with their running maximum
 // and sum, and weights_finish_kernel.
@@ -313,7 +323,8 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
   __shared__ float part_m[kWaves][4 * NI], part_l[kWaves][4 * NI];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int c = lane & 15, kg = lane >> 4;
-  const int pair = blockIdx.x / a.grid_units, x = blockIdx.x % a.grid_units;
+  int pair, x;
+  place_of(a, pair, x);
   const int seq = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
   const Seq sq = seq_of(a, seq);
   const int units = (int)(((int64_t)sq.keys + a.unit - 1) / a.unit);
@@ -448,7 +459,8 @@ __global__ __launch_bounds__(kThreads) void weights_finish_kernel(WeightArgs a) 
   constexpr int Q = 4 * NI;  // queries
   constexpr int kHeld = 4 * TileWeights<NI>::kHeld;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), kg = lane >> 4;
-  const int pair = blockIdx.x / a.grid_units, x = blockIdx.x % a.grid_units;
+  int pair, x;
+  place_of(a, pair, x);
   const int seq = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
   const Seq sq = seq_of(a, seq);
   const int units = (int)(((int64_t)sq.keys + a.unit - 1) / a.unit);
