@@ -65,8 +65,9 @@ struct WeightArgs {
   int unit;            // keys of a workgroup's turn
   int grid_units;      // workgroups of a (sequence, KV head)
   int max_units;
-  float* ws_t;         // scores of split contexts
-  f32x2* ws_ml;        // (sequence, KV head, unit, query): maximum and sum
+  int pair0;           // the launch's first (sequence, KV head)
+  float* ws_t;         // scores of split contexts, of the launch's pairs
+  f32x2* ws_ml;        // (pair, unit, query): maximum and sum
   // chunks
   int shares;          // pieces of the normalisers' work, at most
   f32x2* part_ml;      // (piece + block, KV head, row of the block): maximum and sum
@@ -307,7 +308,7 @@ constexpr int kSplitKeys = 1024;  // of a unit: 16 tiles a wave
 // units on one XCD: 181).
 MKV_DEV void place_of(const WeightArgs& a, int& pair, int& x) {
   pair = blockIdx.x / a.grid_units;
-  x = (int)(blockIdx.x % a.grid_units + pair / a.num_kv_heads) % a.grid_units;
+  x = (int)(blockIdx.x % a.grid_units + (a.pair0 + pair) / a.num_kv_heads) % a.grid_units;
 }
 
 // One workgroup a (sequence, KV head) where its scores fit the LDS; else (SPLIT) a
@@ -325,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void weights_decode_kernel(WeightArgs a) 
   const int c = lane & 15, kg = lane >> 4;
   int pair, x;
   place_of(a, pair, x);
-  const int seq = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
+  const int seq = (a.pair0 + pair) / a.num_kv_heads, h = (a.pair0 + pair) % a.num_kv_heads;
   const Seq sq = seq_of(a, seq);
   const int units = (int)(((int64_t)sq.keys + a.unit - 1) / a.unit);
   if (x >= units) return;
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(kThreads) void weights_finish_kernel(WeightArgs a) 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), kg = lane >> 4;
   int pair, x;
   place_of(a, pair, x);
-  const int seq = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
+  const int seq = (a.pair0 + pair) / a.num_kv_heads, h = (a.pair0 + pair) % a.num_kv_heads;
   const Seq sq = seq_of(a, seq);
   const int units = (int)(((int64_t)sq.keys + a.unit - 1) / a.unit);
   if (x >= units) return;
@@ -1242,6 +1243,7 @@ struct Plan {
   bool decode;
   // decode
   int ni, unit, max_units, grid_units;
+  int pairs;                     // (sequence, KV head) pairs of a launch
   // chunks
   int row_groups, rows, shares;  // rows: of a block
   int64_t row_units;             // blocks at most
@@ -1249,7 +1251,13 @@ struct Plan {
   size_t bytes;
 };
 
-constexpr size_t kMaxScores = (size_t)1 << 30;  // bytes of kept scores
+// Bytes of kept scores at a time.  Their room follows the table's width, which may be far
+// past the contexts, so that pairs whose scores do not fit go in up to four turns (60
+// sequences of 300-800 tokens, 16/8 heads, fp8, under tables of 131,072: 87 us, and 53 in
+// one turn with 0.94 GiB; of 30k tokens 940 and 917).  Past those, one-row sequences go
+// the chunks' way, which keeps no scores.
+constexpr size_t kMaxScores = (size_t)256 << 20;
+constexpr int kMaxTurns = 4;
 
 Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t capacity, bool one_row, bool f32) {
   Plan p{};
@@ -1262,9 +1270,11 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
     p.max_units = (int)((capacity + p.unit - 1) / p.unit);
     const int64_t room = 16384 / pairs;
     p.grid_units = (int)(p.max_units < room ? p.max_units : room < 1 ? 1 : room);
-    if (p.max_units > 1)
-      p.bytes = (size_t)pairs * p.max_units * 4 * p.ni * (8 + (size_t)p.unit * 4);
-    if (p.bytes <= kMaxScores) {
+    const size_t each = p.max_units > 1 ? (size_t)p.max_units * 4 * p.ni * (8 + (size_t)p.unit * 4) : 0;
+    if (each <= kMaxScores && (size_t)pairs * each <= kMaxTurns * kMaxScores) {
+      const int64_t fit = each ? (int64_t)(kMaxScores / each) : pairs, turns = (pairs + fit - 1) / fit;
+      p.pairs = (int)((pairs + turns - 1) / turns);
+      p.bytes = (size_t)p.pairs * each;
       p.decode = true;
       return p;
     }
@@ -1287,25 +1297,30 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
 template <int KV, int CT, int D>
 int launch_weights(WeightArgs& a, const Plan& p, hipStream_t s) {
   if (p.decode) {
-    const dim3 grid((unsigned)((int64_t)a.num_seqs * a.num_kv_heads * p.grid_units));
     const size_t lds = (size_t)p.unit / 16 * p.ni * 64 * 4;
-    if (p.max_units == 1) {
-      if (p.ni == 1)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, false>), grid, dim3(kThreads), lds, s, a);
-      else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, false>), grid, dim3(kThreads), lds, s, a);
-    } else {
-      if (p.ni == 1)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, true>), grid, dim3(kThreads), lds, s, a);
-      else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, true>), grid, dim3(kThreads), lds, s, a);
+    const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
+    for (int64_t pair0 = 0; pair0 < pairs; pair0 += p.pairs) {
+      const dim3 grid((unsigned)((pairs - pair0 < p.pairs ? pairs - pair0 : p.pairs) * p.grid_units));
+      a.pair0 = (int)pair0;
+      if (p.max_units == 1) {
+        if (p.ni == 1)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, false>), grid, dim3(kThreads), lds, s, a);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, false>), grid, dim3(kThreads), lds, s, a);
+      } else {
+        if (p.ni == 1)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 1, true>), grid, dim3(kThreads), lds, s, a);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_decode_kernel<KV, CT, D, 4, true>), grid, dim3(kThreads), lds, s, a);
+        if (hipError_t e = hipGetLastError()) return (int)e;
+        if (p.ni == 1)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<1>), grid, dim3(kThreads), 0, s, a);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<4>), grid, dim3(kThreads), 0, s, a);
+      }
       if (hipError_t e = hipGetLastError()) return (int)e;
-      if (p.ni == 1)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<1>), grid, dim3(kThreads), 0, s, a);
-      else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(weights_finish_kernel<4>), grid, dim3(kThreads), 0, s, a);
     }
-    return (int)hipGetLastError();
+    return MKV_OK;
   }
   auto normalisers = [&](auto groups) {
     constexpr int R = decltype(groups)::value, kRows = 32 * Formats<KV, CT, D>::kBlocks * R;
@@ -1396,8 +1411,7 @@ extern "C" int mkv_paged_weights(float* weights, float decay, const void* q, int
   const Plan p = make_plan(num_seqs, total_q, num_heads, num_kv_heads, (int64_t)max_blocks * block_size, one_row != 0,
                            kv_dtype == MKV_DTYPE_F32);
   if (p.bytes > workspace_bytes || (p.bytes && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
-  if (p.decode ? (int64_t)num_seqs * num_kv_heads * p.grid_units > kMaxGrid : p.row_units * num_kv_heads > kMaxGrid)
-    return MKV_ERR_BAD_SHAPE;
+  if (p.decode ? (int64_t)p.pairs * p.grid_units > kMaxGrid : p.row_units * num_kv_heads > kMaxGrid) return MKV_ERR_BAD_SHAPE;
   WeightArgs a;
   a.q = reinterpret_cast<const char*>(q);
   a.k = reinterpret_cast<const char*>(k_cache);
@@ -1420,8 +1434,9 @@ extern "C" int mkv_paged_weights(float* weights, float decay, const void* q, int
   a.unit = p.unit;
   a.grid_units = p.grid_units;
   a.max_units = p.max_units;
+  a.pair0 = 0;
   a.ws_ml = reinterpret_cast<f32x2*>(workspace);
-  a.ws_t = reinterpret_cast<float*>(a.ws_ml + (p.decode ? (size_t)num_seqs * num_kv_heads * p.max_units * 4 * p.ni : 0));
+  a.ws_t = reinterpret_cast<float*>(a.ws_ml + (p.decode ? (size_t)p.pairs * p.max_units * 4 * p.ni : 0));
   a.shares = p.shares;
   a.row_units = p.row_units;
   a.part_ml = reinterpret_cast<f32x2*>(workspace);

@@ -198,6 +198,17 @@ def test_tables_with_holes_and_wide_ones(dev, rows):
                         context_lens=torch.tensor([4, 0, 25])))
 
 
+@pytest.mark.parametrize("fmt", ["fp32", "bf16", "fp8_token"])
+@pytest.mark.parametrize("Hq,Hkv,tokens", [(8, 4, 1 << 20), (10, 2, 1 << 20), (10, 2, 4300000), (2, 1, 17000000)])
+def test_scores_that_are_kept_in_turns(dev, fmt, Hq, Hkv, tokens):
+    """Tables so wide that the scores of some (sequence, KV head) pairs are kept at a
+    time, and ones under which a single pair's are not kept at all."""
+    announce(f"weights: decode, {fmt}, {Hq}/{Hkv} heads, tables of {tokens} tokens")
+    c = make(fmt, None, [2900, 1, 0, 1025, 64], Hq, Hkv, 64, 16, seed=19)
+    pad = torch.full((5, tokens // 16 - c["block_tables"].shape[1]), -1, dtype=torch.int32)
+    check(dev, dict(c, block_tables=torch.cat([c["block_tables"], pad], 1)), 0.5)
+
+
 def test_values_that_are_not_finite(dev):
     """A NaN key reaches what the rows that see it see, and nothing else; tokens
     that no row sees change nothing; the entries of new tokens may hold anything."""

@@ -44,6 +44,20 @@ def test_refusals(lib):  # noqa: F811
     assert weights(lib, seqs=1 << 23, total=1 << 23, ws_bytes=1 << 62) == -2
 
 
+def test_the_scores_room_is_bounded(lib):  # noqa: F811
+    """Decode's kept scores follow the table's width: no more than 256 MiB of them,
+    whatever the sequences and heads."""
+    def room(seqs, hq, hkv, tokens):
+        return lib.mkv_paged_weights_workspace_size(seqs, seqs, hq, hkv, 128, 16, tokens // 16, _lib.DTYPE_BF16, 1)
+
+    # (of all pairs at once: 0.94 GiB, just over 1 GiB, 4 GiB)
+    for seqs, hq, hkv, tokens in ((60, 16, 8, 131072), (64, 64, 8, 32768), (64, 64, 8, 131072), (1, 8, 1, 1 << 19)):
+        assert 0 < room(seqs, hq, hkv, tokens) <= 256 << 20
+    assert room(2, 32, 8, 131072) == 2 * 8 * 128 * 4 * (8 + 1024 * 4)
+    # (one pair's would not fit: none are kept)
+    assert 0 < room(1, 8, 1, 1 << 25) <= 1 << 22 and 0 < room(3, 4, 1, 1 << 25) <= 1 << 22
+
+
 def test_the_wrapper_s_checks():
     q, k, w = torch.zeros(2, 8, 128), torch.zeros(4, 16, 8, 128), torch.zeros(4, 16, 8)
     bt, cl = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int64)
