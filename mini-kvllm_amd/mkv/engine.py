@@ -443,6 +443,7 @@ class Qwen3Model(torch.nn.Module):
         self.final_norm = torch.ones(H, dtype=dtype, device=device)
         self.cos_sin = rope_cos_sin(cfg.rope_base, D, cfg.max_position, device)
         self.kv_cache_dtype = "auto"
+        self._captured = False  # a graph holds a step over the caches attached now
 
     def attach_kv_cache(self, num_blocks: int, kv_cache_dtype: str = "fp8_per_tensor",
                         cache_dtype: torch.dtype | None = None) -> None:
@@ -462,6 +463,7 @@ class Qwen3Model(torch.nn.Module):
             raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: the engine runs 'auto', 'fp8_per_tensor', "
                              "'fp8_per_token_head' or 'int8_per_token_head'")
         self.kv_cache_dtype = kv_cache_dtype
+        self._captured = False
         for lay in self.layers:
             att = lay["attn"]
             att.k_cache = torch.zeros(num_blocks, self.block_size, cfg.num_kv_heads, cfg.head_dim,
@@ -480,9 +482,12 @@ class Qwen3Model(torch.nn.Module):
         """Accumulate, from now on, the attention weight that every cached token
         receives in each layer and KV head (decay times what it had, a step), beside
         the caches of :meth:`attach_kv_cache`; returns the eviction that goes by it.
-        Before decode steps are captured: a graph replays what it was captured with.
-        Decode steps then run the producer, the weights and the attention as calls of
-        their own."""
+        Before any step is captured (refused after that, until caches are attached
+        anew): a graph replays what it was captured with.  Decode steps then run the
+        producer, the weights and the attention as calls of their own."""
+        if self._captured:
+            raise RuntimeError("a step has been captured already, and its replays would go on as they were captured: "
+                               "attach the weights before the first captured step")
         att = [lay["attn"] for lay in self.layers]
         for a in att:
             a.attention_weights = torch.zeros(a.k_cache.shape[:3], dtype=torch.float32, device=a.k_cache.device)
@@ -516,6 +521,8 @@ class Qwen3Model(torch.nn.Module):
         # part of them (five launches a layer instead of seven).
         x, residual = None, F.embedding(input_ids, self.embed)
         free = _untouched()
+        if free and residual.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured = True
         for li, lay in enumerate(self.layers):
             qkv = normed_linear(x, residual, lay["in_norm"], cfg.eps, lay["qkv"], 0, free)
             att = lay["attn"]

@@ -1,0 +1,58 @@
+"""GPU tests of attention weights attached to the engine's model: when, and what is
+refused before anything changes."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import announce
+from mkv import engine as E
+
+pytestmark = pytest.mark.gpu
+
+CFG = E.ModelConfig(vocab_size=512, hidden_size=256, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=128,
+                    intermediate_size=512, max_position=4096)
+BS = 16
+
+
+def engine(dev, model=None, use_graphs=True, kv="auto"):
+    model = model or E.Qwen3Model(CFG, dev, seed=5, block_size=BS)
+    return model, E.Engine(model, num_blocks=64, max_num_seqs=4, max_num_batched_tokens=64, max_model_len=256,
+                           kv_cache_dtype=kv, use_graphs=use_graphs)
+
+
+def given(model):
+    return [float(lay["attn"].attention_weights.double().sum()) for lay in model.layers]
+
+
+def test_not_behind_captured_steps(dev):
+    """A captured step goes on as it was captured: weights attached behind it would
+    miss every replay, and replays would write weights that were given up."""
+    announce("weights attached: behind captured steps they are refused")
+    prompt = torch.randint(0, CFG.vocab_size, (20,), generator=torch.Generator().manual_seed(1)).tolist()
+    model, eng = engine(dev)
+    eng.generate([prompt], max_tokens=4)
+    with pytest.raises(RuntimeError, match="captured already"):
+        model.attach_attention_weights()
+    assert all(lay["attn"].attention_weights is None for lay in model.layers)
+    # caches of a new engine: no step over them is captured
+    _, eng = engine(dev, model)
+    model.attach_attention_weights()
+    model.attach_attention_weights(decay=0.5)
+    eng.generate([prompt], max_tokens=4)
+    kept = [lay["attn"].attention_weights for lay in model.layers]
+    with pytest.raises(RuntimeError, match="captured already"):
+        model.attach_attention_weights()
+    assert all(lay["attn"].attention_weights is w for lay, w in zip(model.layers, kept))
+    # steps that are not captured take them at any time: four rows of a request's
+    # five decoded tokens follow
+    model, eng = engine(dev, use_graphs=False)
+    req = eng.add_request(prompt, 6)
+    eng.step()
+    eng.step()
+    model.attach_attention_weights()
+    while not eng.sched.done():
+        eng.step()
+    assert len(req.tokens) == 26
+    for w in given(model):
+        assert abs(w - 4 * CFG.num_heads) <= 1e-3
