@@ -837,9 +837,19 @@ class Attention(nn.Module):
             k_scale=self.k_scale if quant else None, v_scale=self.v_scale if quant else None,
             kv_cache_dtype=self.kv_cache_dtype)
 
-    def _accumulate(self, q, context, cu_seqlens_q, scale):
+    def check_accumulates(self, context) -> None:
+        """Refuse a step that a layer with attention_weights cannot accumulate, before
+        anything of it is in the cache."""
+        if self.attention_weights is None:
+            return
+        if context.is_prefill and getattr(context, "tree_mask", None) is not None:
+            raise ValueError("attention weights are not accumulated over trees of drafted tokens")
         if context.context_lens is None or context.block_tables is None:
             raise ValueError("attention weights require context_lens and block_tables")
+        if not math.isfinite(self.weights_decay):
+            raise ValueError(f"weights_decay must be finite; got {self.weights_decay}")
+
+    def _accumulate(self, q, context, cu_seqlens_q, scale):
         paged_attention_weights(
             q, self.k_cache, self.attention_weights, context.block_tables, context.context_lens, scale, self.num_heads,
             self.num_kv_heads, self.head_dim, self.block_size, cu_seqlens_q=cu_seqlens_q,
@@ -854,6 +864,7 @@ class Attention(nn.Module):
         used by a full prefill."""
         context = current_context()
         mode = self._mode()
+        self.check_accumulates(context)
         if (not kv_appended and self.k_cache.numel() > 0 and self.v_cache.numel() > 0
                 and context.slot_mapping is not None):
             if k.dim() == 4:
@@ -875,8 +886,6 @@ class Attention(nn.Module):
             if cu_seqlens is None:
                 raise ValueError("cu_seqlens_q must be provided for varlen attention")
             if self.attention_weights is not None:
-                if getattr(context, "tree_mask", None) is not None:
-                    raise ValueError("attention weights are not accumulated over trees of drafted tokens")
                 self._accumulate(q, context, cu_seqlens, scale)
             if getattr(context, "tree_mask", None) is not None:
                 # drafted tokens: each row sees the prefix and what its mask names

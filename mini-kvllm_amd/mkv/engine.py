@@ -30,6 +30,7 @@ tokens per second; it is not a port of the reference's runner.  The pieces:
 from __future__ import annotations
 
 import functools
+import math
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -488,12 +489,17 @@ class Qwen3Model(torch.nn.Module):
         if self._captured:
             raise RuntimeError("a step has been captured already, and its replays would go on as they were captured: "
                                "attach the weights before the first captured step")
+        if not math.isfinite(decay):
+            raise ValueError(f"decay must be finite; got {decay}")
         att = [lay["attn"] for lay in self.layers]
-        for a in att:
-            a.attention_weights = torch.zeros(a.k_cache.shape[:3], dtype=torch.float32, device=a.k_cache.device)
-            a.weights_decay = decay
+        if any(a.k_cache.dim() != 4 for a in att):
+            raise RuntimeError("attach_kv_cache comes first")
+        weights = [torch.zeros(a.k_cache.shape[:3], dtype=torch.float32, device=a.k_cache.device) for a in att]
         scales = ([a.k_scale for a in att], [a.v_scale for a in att]) if self.kv_cache_dtype in PER_TOKEN_HEAD_MODES else (None, None)
-        return CacheEviction([a.k_cache for a in att], [a.v_cache for a in att], [a.attention_weights for a in att], *scales)
+        eviction = CacheEviction([a.k_cache for a in att], [a.v_cache for a in att], weights, *scales)
+        for a, w in zip(att, weights):
+            a.attention_weights, a.weights_decay = w, decay
+        return eviction
 
     def scales(self) -> list[torch.Tensor]:
         """The per-tensor FP8 scales (what a decode graph's capture must
@@ -523,6 +529,8 @@ class Qwen3Model(torch.nn.Module):
         free = _untouched()
         if free and residual.is_cuda and torch.cuda.is_current_stream_capturing():
             self._captured = True
+        for lay in self.layers:
+            lay["attn"].check_accumulates(C.current_context())
         for li, lay in enumerate(self.layers):
             qkv = normed_linear(x, residual, lay["in_norm"], cfg.eps, lay["qkv"], 0, free)
             att = lay["attn"]

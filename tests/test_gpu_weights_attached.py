@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from conftest import announce
+from mkv import context as C
 from mkv import engine as E
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,37 @@ def test_not_behind_captured_steps(dev):
     assert len(req.tokens) == 26
     for w in given(model):
         assert abs(w - 4 * CFG.num_heads) <= 1e-3
+
+
+@pytest.mark.parametrize("kv", ["auto", "fp8_per_tensor", "int8_per_token_head"])
+def test_a_refused_step_leaves_the_cache_as_it_was(dev, kv):
+    """A tree, or a step without its lengths, over a model that accumulates: no K or V,
+    no scale and no weight has changed."""
+    announce(f"weights attached: refused steps change nothing, {kv} KV")
+    model = E.Qwen3Model(CFG, dev, seed=5, block_size=BS)
+    model.attach_kv_cache(8, kv)
+    model.attach_attention_weights()
+    ids = torch.arange(6, device=dev)
+    step = dict(cu_seqlens_q=torch.tensor([0, 6], dtype=torch.int32, device=dev), slot_mapping=ids, positions=ids,
+                context_lens=torch.tensor([6], device=dev), max_seqlen_q=6,
+                block_tables=torch.tensor([[0]], dtype=torch.int32, device=dev))
+
+    def state():
+        return [t.clone() for lay in model.layers for n in ("k_cache", "v_cache", "k_scale", "v_scale", "attention_weights")
+                if (t := getattr(lay["attn"], n)) is not None]
+
+    before = state()
+    try:
+        for change, what in ((dict(tree_mask=torch.ones(6, 6, dtype=torch.bool, device=dev)), "not accumulated over trees"),
+                             (dict(context_lens=None), "require context_lens"), (dict(block_tables=None), "require context_lens")):
+            C.set_context(True, **dict(step, **change))
+            with pytest.raises(ValueError, match=what):
+                model(ids, ids, ids)
+            for a, b in zip(state(), before):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        C.set_context(True, **step)
+        model(ids, ids, ids)
+    finally:
+        C.reset_context()
+    for w in given(model):
+        assert abs(w - 6 * CFG.num_heads) <= 1e-3

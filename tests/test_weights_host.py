@@ -7,6 +7,8 @@ import torch
 
 import mkv
 from mkv import _lib
+from mkv import context as C
+from mkv import engine as E
 from test_step_operators_host import lib, p  # noqa: F401  (lib: a fixture)
 
 
@@ -66,3 +68,40 @@ def test_the_wrapper_s_checks():
     for decay in (float("nan"), float("inf")):
         with pytest.raises(ValueError, match="decay must be finite"):
             mkv.paged_attention_weights(q, k, w, bt, cl, 0.1, 8, 8, 128, 16, decay=decay)
+
+
+def test_a_layer_refuses_a_step_ahead_of_its_store():
+    """What cannot be accumulated is refused before the step's K and V go anywhere."""
+    att = mkv.Attention(4, 64, 1.0, 2, 16)
+    att.k_cache, att.v_cache = torch.zeros(4, 16, 2, 64), torch.zeros(4, 16, 2, 64)
+    att.attention_weights = torch.zeros(4, 16, 2)
+    q, k, v = torch.zeros(1, 4, 64), torch.zeros(1, 2, 64), torch.zeros(1, 2, 64)
+    step = dict(slot_mapping=torch.zeros(1, dtype=torch.int64), context_lens=torch.ones(1, dtype=torch.int64),
+                block_tables=torch.zeros(1, 1, dtype=torch.int32))
+    chunk = dict(step, cu_seqlens_q=torch.tensor([0, 1], dtype=torch.int32))
+    try:
+        for prefill, c, decay, what in (
+                (True, dict(chunk, tree_mask=torch.ones(1, 1, dtype=torch.bool)), 1.0, "not accumulated over trees"),
+                (True, dict(chunk, context_lens=None), 1.0, "require context_lens"),
+                (False, dict(step, block_tables=None), 1.0, "require context_lens"),
+                (False, step, float("nan"), "must be finite")):
+            att.weights_decay = decay
+            C.set_context(prefill, **c)
+            with pytest.raises(ValueError, match=what):
+                att(q, k, v)
+    finally:
+        C.reset_context()
+
+
+def test_the_model_refuses_weights_before_it_changes():
+    cfg = E.ModelConfig(vocab_size=32, hidden_size=64, num_layers=1, num_heads=2, num_kv_heads=1, head_dim=64,
+                        intermediate_size=64, max_position=64)
+    model = E.Qwen3Model(cfg, "cpu", block_size=16)
+    with pytest.raises(RuntimeError, match="attach_kv_cache comes first"):
+        model.attach_attention_weights()
+    model.attach_kv_cache(2, "auto")
+    with pytest.raises(ValueError, match="must be finite"):
+        model.attach_attention_weights(float("inf"))
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        model.attach_attention_weights()
+    assert model.layers[0]["attn"].attention_weights is None
