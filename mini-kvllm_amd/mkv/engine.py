@@ -445,6 +445,7 @@ class Qwen3Model(torch.nn.Module):
         self.cos_sin = rope_cos_sin(cfg.rope_base, D, cfg.max_position, device)
         self.kv_cache_dtype = "auto"
         self._captured = False  # a graph holds a step over the caches attached now
+        self._engine_tables: torch.Tensor | None = None  # of the Engine that drives the model
 
     def attach_kv_cache(self, num_blocks: int, kv_cache_dtype: str = "fp8_per_tensor",
                         cache_dtype: torch.dtype | None = None) -> None:
@@ -464,7 +465,7 @@ class Qwen3Model(torch.nn.Module):
             raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: the engine runs 'auto', 'fp8_per_tensor', "
                              "'fp8_per_token_head' or 'int8_per_token_head'")
         self.kv_cache_dtype = kv_cache_dtype
-        self._captured = False
+        self._captured, self._engine_tables = False, None
         for lay in self.layers:
             att = lay["attn"]
             att.k_cache = torch.zeros(num_blocks, self.block_size, cfg.num_kv_heads, cfg.head_dim,
@@ -485,7 +486,14 @@ class Qwen3Model(torch.nn.Module):
         the caches of :meth:`attach_kv_cache`; returns the eviction that goes by it.
         Before any step is captured (refused after that, until caches are attached
         anew): a graph replays what it was captured with.  Decode steps then run the
-        producer, the weights and the attention as calls of their own."""
+        producer, the weights and the attention as calls of their own.
+
+        The eviction is for a program that keeps its sequences itself, their lengths
+        in the cache and their positions apart (a cut shortens the one and not the
+        other).  :class:`Engine` has both from its host's token lists and cannot have
+        its sequences cut: the eviction refuses its tables.  Rows of drafted tokens
+        count as any others, accepted or not; sequences of a step must not share
+        pages."""
         if self._captured:
             raise RuntimeError("a step has been captured already, and its replays would go on as they were captured: "
                                "attach the weights before the first captured step")
@@ -497,6 +505,7 @@ class Qwen3Model(torch.nn.Module):
         weights = [torch.zeros(a.k_cache.shape[:3], dtype=torch.float32, device=a.k_cache.device) for a in att]
         scales = ([a.k_scale for a in att], [a.v_scale for a in att]) if self.kv_cache_dtype in PER_TOKEN_HEAD_MODES else (None, None)
         eviction = CacheEviction([a.k_cache for a in att], [a.v_cache for a in att], weights, *scales)
+        eviction.engine_tables = self._engine_tables
         for a, w in zip(att, weights):
             a.attention_weights, a.weights_decay = w, decay
         return eviction
@@ -641,6 +650,7 @@ class Engine:
         self._next_id = 0
         # decode-step state on the device
         self.meta = DecodeMetadata(self.max_rows, self.max_blocks, self.bs, num_blocks, self.dev)
+        model._engine_tables = self.meta.block_tables
         self.ids_buf = torch.zeros(self.max_rows, dtype=torch.int64, device=self.dev)
         self.temp_buf = torch.ones(self.max_rows, dtype=torch.float32, device=self.dev)
         self.logits_buf = None

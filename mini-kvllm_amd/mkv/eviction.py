@@ -23,7 +23,9 @@ class CacheEviction:
     """All layers' K and V pools (num_blocks, block_size, num_kv_heads, head_dim),
     their accumulated weights, fp32 (num_blocks, block_size, num_kv_heads), and, with
     per-token-head formats, their scales of that shape: contiguous, none overlapping
-    another.  The tensors are kept; they must stay where they are."""
+    another.  The tensors are kept; they must stay where they are.  ``tensors``: all of
+    them, what :class:`mkv.CachePages` takes so that page copies and compactions bring
+    a token's weights along."""
 
     def __init__(self, k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor],
                  weights: Sequence[torch.Tensor], k_scales: Sequence[torch.Tensor] | None = None,
@@ -37,6 +39,8 @@ class CacheEviction:
         if not self.num_layers or any(len(x) != self.num_layers for x in groups):
             raise ValueError(f"every layer needs each of its tensors; got {[len(x) for x in groups]}")
         self.tensors = [t for x in groups for t in x]
+        # tables whose sequences' lengths and positions are the host's (mkv.engine.Engine)
+        self.engine_tables: torch.Tensor | None = None
         self.device = _require_gpu(*self.tensors)
         shape = groups[0][0].shape
         if len(shape) != 4 or not all(shape):
@@ -88,6 +92,10 @@ class CacheEviction:
         the host.  Sequences must not share pages of the positions below the budget
         (forks: evict first); the tables' pages must be in the pool."""
         _require_gpu(self.tensors[0], block_tables, seq_lens)
+        if (self.engine_tables is not None
+                and block_tables.untyped_storage().data_ptr() == self.engine_tables.untyped_storage().data_ptr()):
+            raise ValueError("these are an Engine's sequences: it goes by its host's lengths and positions, which a cut "
+                             "does not change")
         if seq_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] < seq_lens.numel():
             raise ValueError(f"block_tables {tuple(block_tables.shape)} must cover seq_lens {tuple(seq_lens.shape)}")
         if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:

@@ -91,3 +91,30 @@ def test_a_refused_step_leaves_the_cache_as_it_was(dev, kv):
         C.reset_context()
     for w in given(model):
         assert abs(w - 6 * CFG.num_heads) <= 1e-3
+
+
+def test_an_engine_s_sequences_are_not_cut(dev):
+    """It takes lengths and rotary positions from its host's token lists, which a cut
+    would leave behind: its tables are refused, and nothing has changed."""
+    announce("weights attached: the eviction refuses the engine's tables")
+    prompt = torch.randint(0, CFG.vocab_size, (40,), generator=torch.Generator().manual_seed(2)).tolist()
+    plain = engine(dev)[1].generate([prompt], max_tokens=6)
+    model, eng = engine(dev)
+    model.fuse_decode_step = False
+    evict = model.attach_attention_weights()
+    req = eng.add_request(prompt, 6)
+    for _ in range(3):
+        eng.step()
+    before = [t.clone() for t in evict.tensors]
+    for tables in (eng.meta.block_tables, eng.meta.block_tables[:2, :4]):
+        with pytest.raises(ValueError, match="an Engine's sequences"):
+            evict.evict(tables, eng.meta.seq_lens[:tables.shape[0]], 16)
+    assert all(torch.equal(a, b) for a, b in zip(evict.tensors, before))
+    while not eng.sched.done():
+        eng.step()
+    assert [req.tokens[40:]] == plain
+    # the model without its engine: tables of the program's own
+    model.attach_kv_cache(8, "auto")
+    new = model.attach_attention_weights().evict(torch.tensor([[3, 1, 2]], dtype=torch.int32, device=dev),
+                                                 torch.tensor([40], device=dev), 16)
+    assert new.tolist() == [16]
