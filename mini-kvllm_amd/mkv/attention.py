@@ -667,7 +667,10 @@ def paged_attention_weights(query: torch.Tensor, k_cache: torch.Tensor, weights:
     their entries held; decay 0 starts every token of the contexts from 0.
 
     The caches' formats, query types and scales are :func:`paged_attention_tree`'s
-    (K alone); head_dim 64 or 128.  Sequences of one call must not share pages.
+    (K alone); head_dim 64 or 128.  Sequences of one call must not share pages (forks
+    that do: a call each, one after another; in one call, one's addition to a shared
+    token is lost).  Rows of drafted tokens count as any others: where the rejected ones
+    shall not, call it behind the compaction, with the accepted rows' queries alone.
     Captured in a graph, a call accumulates anew at every replay."""
     if not math.isfinite(decay):
         raise ValueError(f"decay must be finite; got {decay}")
@@ -798,7 +801,9 @@ class Attention(nn.Module):
         # fp32 (num_blocks, block_size, num_kv_heads), injected like the caches:
         # every step then accumulates the attention weight that each cached token
         # receives (paged_attention_weights, with this decay), which
-        # mkv.CacheEviction goes by
+        # mkv.CacheEviction goes by.  The sequences of a step must not share
+        # pages then: of two that do (rows of mkv.PagePool that forked), one's
+        # addition to a shared token's entry is lost, and nothing checks it
         self.attention_weights: torch.Tensor | None = None
         self.weights_decay = 1.0
 
