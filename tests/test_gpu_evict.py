@@ -191,6 +191,62 @@ def test_absent_pages_are_left_out(dev):
     same(d, want)
 
 
+def test_absent_pages_under_wide_tables(dev):
+    """The same by transposed keys: absent pages within the sequences, of all their
+    tokens, and behind them."""
+    announce("evict: absent pages, tables of 9600 tokens")
+    H, bs, width, budget, sinks, recent = 3, 16, 600, 70, 3, 9
+    c, bt, ctx = make([9000, 300, 90], 2, H, 8, bs, scales=True, seed=14, width=width)
+    g = torch.Generator().manual_seed(3)
+    bt[0, torch.randperm(560, generator=g)[:40]] = -1
+    bt[0, [0, 3, 561]] = 10 ** 6
+    bt[1, 2], bt[1, 18], bt[2] = -1, 2 ** 31 - 1, -1
+    d, want = on(dev, c), {n: [x.clone() for x in xs] for n, xs in c.items()}
+    blocks = c["w"][0].shape[0]
+    for b, n in enumerate(ctx.tolist()):
+        t = torch.arange(n)
+        page = bt[b, t // bs].long()
+        here = torch.where((page >= 0) & (page < blocks), page * bs + t % bs, -1).tolist()
+        for i in range(2):
+            for h in range(H):
+                w = c["w"][i].flatten(0, 1)[:, h].tolist()
+                mid = sorted(range(sinks, n - recent), key=lambda j: (-w[here[j]] if here[j] >= 0 else 1.0, j))
+                keep = list(range(sinks)) + sorted(mid[:budget - sinks - recent]) + list(range(n - recent, n))
+                for name, xs in want.items():
+                    x, src = xs[i].flatten(0, 1), c[name][i].flatten(0, 1)
+                    for j, s in enumerate(keep):
+                        if here[s] >= 0 and here[j] >= 0:
+                            x[here[j], h] = src[here[s], h]
+    new = handle(d).evict(bt.to(dev), ctx.to(dev), budget, sinks=sinks, recent=recent)
+    assert new.tolist() == [70, 70, 70]
+    same(d, want)
+
+
+def test_turns_are_captured(dev):
+    announce("evict: keys in turns, captured and replayed")
+    c, bt, ctx = make([300, 900, 77], 3, 2, 8, 16, seed=15, width=(1 << 24) // 16)
+    d, btd, ctxd = on(dev, c), bt.to(dev), ctx.to(dev)
+    ev = handle(d)
+    ev.evict(btd, ctxd, 60, sinks=2, recent=5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with graph_capture(graph):
+        out = ev.evict(btd, ctxd, 60, sinks=2, recent=5)
+    g = torch.Generator().manual_seed(4)
+    for turn in range(3):
+        for n, xs in c.items():
+            for x, y in zip(xs, d[n]):
+                if x.dtype == torch.float32:
+                    x.copy_(torch.rand(x.shape, generator=g))
+                y.copy_(x)
+        want = {n: [x.clone() for x in xs] for n, xs in c.items()}
+        oracle(want, bt, ctx, 60, 2, 5)
+        graph.replay()
+        torch.cuda.synchronize()
+        same(d, want)
+        assert out.tolist() == [60, 60, 60]
+
+
 def test_captured_replayed_and_on_another_stream(dev):
     announce("evict: captured twice, replayed on new weights, side stream")
     cases = []

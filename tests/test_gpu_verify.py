@@ -185,6 +185,24 @@ def test_a_full_vocabulary_and_many_sequences(dev):
     check(mkv.verify_drafts(**on(dev, c)), c)
 
 
+def test_siblings_over_a_full_vocabulary(dev):
+    """Trees drawn from the draft over 151,936 tokens, their uniforms high: siblings
+    behind one, two and three rejections, each with the sum of what is left."""
+    announce("verify: drawn trees of four children over 151936 tokens")
+    sizes = [5, 13, 5, 9, 5, 21]
+    c = make(torch.bfloat16, sizes, 151936, 4, True, [1.0, 0.8, 1.2, 1.0, 0.7, 1.0], seed=6)
+    for s, n in enumerate(sizes):
+        r = int(c["cu_seqlens_q"][s])
+        g = torch.Generator().manual_seed(s)
+        for i in range(1, n):
+            p = (i - 1) // 4
+            c["parents"][r + i] = p
+            row = torch.softmax(c["draft_logits"][r + p].double() / float(c["temperatures"][s]), -1)
+            c["token_ids"][r + i] = int(torch.multinomial(row, 1, generator=g))
+    c["uniforms"] = 0.7 + 0.3 * c["uniforms"]
+    check(mkv.verify_drafts(**on(dev, c)), c, least=0.5)
+
+
 @pytest.mark.parametrize("drawn", [True, False])
 def test_masked_tokens_ties_and_odd_rows(dev, drawn):
     """A grammar's -inf, rows with NaN, +inf or nothing, equal logits, equal

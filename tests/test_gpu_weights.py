@@ -209,6 +209,37 @@ def test_scores_that_are_kept_in_turns(dev, fmt, Hq, Hkv, tokens):
     check(dev, dict(c, block_tables=torch.cat([c["block_tables"], pad], 1)), 0.5)
 
 
+def test_turns_are_captured(dev):
+    announce("weights: scores kept in turns, captured and replayed")
+    c = make("fp8", None, [2900, 1, 0, 1025, 64], 10, 2, 64, 16, seed=20)
+    pad = torch.full((5, (1 << 20) // 16 - c["block_tables"].shape[1]), -1, dtype=torch.int32)
+    d = on(dev, dict(c, block_tables=torch.cat([c["block_tables"], pad], 1)))
+    mkv.paged_attention_weights(**d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with graph_capture(graph):
+        mkv.paged_attention_weights(**d)
+    for turn in range(3):
+        before = d["weights"].clone()
+        graph.replay()
+        want = mkv.paged_attention_weights(**dict(d, weights=before))
+        torch.cuda.synchronize()
+        assert torch.equal(d["weights"], want), f"replay {turn}"
+
+
+def test_sequences_that_share_pages_take_turns(dev):
+    """Forks over shared pages, a call each: what every one of them gives is there."""
+    announce("weights: two sequences over the same pages, a call each")
+    c = make("bf16", None, [70, 70], 8, 2, 128, 16, seed=21)
+    c["block_tables"][1, :4] = c["block_tables"][0, :4]
+    d, w = on(dev, c), c["weights"]
+    for b in range(2):
+        one = dict(query=c["query"][b:b + 1], block_tables=c["block_tables"][b:b + 1], context_lens=c["context_lens"][b:b + 1])
+        mkv.paged_attention_weights(**dict(d, **on(dev, one)), decay=0.5)
+        w, add = oracle(dict(c, weights=w, **one), 0.5)
+    assert float((d["weights"].cpu().double() - w).abs().max()) <= RTOL * 4 * 2 + 2.0 ** -21
+
+
 def test_values_that_are_not_finite(dev):
     """A NaN key reaches what the rows that see it see, and nothing else; tokens
     that no row sees change nothing; the entries of new tokens may hold anything."""
