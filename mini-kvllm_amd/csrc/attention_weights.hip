@@ -17,9 +17,11 @@
 // 64 rows of q a wave in registers and streams K through LDS (S^T = K Q^T, a row's
 // maximum and sum in its column's lanes), weights_columns_kernel holds 64 keys a wave
 // and streams q (S = Q K^T, a key's sum in its column's lanes).  Neither product's
-// result leaves the registers and no sum is shared, so the result is one only.  Kept
-// scores would be 4 bytes a pair, written and read (the windows below 131 us, reading K
-// again 48).  4 windows of 32 rows over 8-32k keys take 48 and 48 us, 3.5 TB/s of K with
+// result leaves the registers.  A key's sum is one wave's; a row's maximum and sum are
+// joined between the waves that share its keys (short sequences) and, by
+// weights_join_kernel, between the pieces that do, in an order that the lengths set, so
+// that the result is one only.  Kept scores would be 4 bytes a pair, written and read
+// (the windows below 131 us, reading K again 48).  4 windows of 32 rows over 8-32k keys take 48 and 48 us, 3.5 TB/s of K with
 // vector instructions issuing in 44% of the first (a fourth tile's room: 51); 8 chunks of
 // 512 rows over 1.5-4.6k keys 86 and 82 us, where the matrix and the vector units run
 // one after another more than beside each other: 26% and 53% of the first.
@@ -158,12 +160,6 @@ MKV_DEV Seq seq_of(const WeightArgs& a, int s) {
 MKV_DEV int slot_of(const WeightArgs& a, int seq, int t) {
   const int32_t p = a.idx.block_tables[(int64_t)seq * a.idx.bt_stride + (t >> a.idx.bs_log2)];
   return p >= 0 && p < a.idx.num_blocks ? (p << a.idx.bs_log2) + (t & ((1 << a.idx.bs_log2) - 1)) : -1;
-}
-MKV_DEV void add_weight(const WeightArgs& a, const Seq& s, int slot, int h, int t, float w) {
-  float* const at = a.weights + (int64_t)slot * a.num_kv_heads + h;
-  // (tokens that came with these rows start here, whatever lay there)
-  if (a.decay != 0.0f && t < s.first) w = __builtin_fmaf(a.decay, *at, w);
-  *at = w;
 }
 
 // ---------------------------------------------------------------------------
@@ -665,8 +661,10 @@ constexpr int kMinPiece = 256;  // keys
 
 // The normalisers' work is (block of ROWS rows, its keys) after (block, its keys), in
 // the sequences' order, dealt out in even pieces: a piece may end one block and begin
-// the next.  Pieces are as many as run at once; twice, three and four times that many
-// took longer.  Block b of a sequence costs what its last row sees, in keys x group,
+// the next.  Pieces are two workgroups a CU, which run at once (where three tiles take 96 KB
+// of LDS, in two rounds: fp32 heads of 128, and 64 rows a block of 16-bit ones); twice,
+// three and four times that many took longer.  Block b of a sequence costs what its last
+// row sees, in keys x group,
 //   E(b) = first group + (b + 1) ROWS,   C(b) = E(0) + .. + E(b - 1),
 // and the loads ahead of them as much as kMinPiece keys (64 sequences of 6-11 tokens, 3 or
 // 4 rows each: 19 us; without it their blocks share 8 pieces, 46),
@@ -1284,7 +1282,7 @@ Plan make_plan(int num_seqs, int64_t total_q, int heads, int kv_heads, int64_t c
   p.row_groups = mean <= held && !f32 ? 1 : mean <= 2 * held ? 2 : 4;
   p.rows = held * p.row_groups;
   p.row_units = num_seqs + rows / p.rows;
-  // pieces for two workgroups a CU, which run at once
+  // pieces for two workgroups a CU
   p.shares = (int)(512 / kv_heads > 0 ? 512 / kv_heads : 1);
   const int unit = f32 ? 128 : 256;
   const int64_t units = (int64_t)num_seqs * ((capacity + unit - 1) / unit);
