@@ -140,7 +140,7 @@ MKV_DEV float inverse(float l) { return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f :
 
 struct Seq {
   int64_t q0, n;      // rows of q
-  int64_t first;      // position of row 0
+  int64_t first;      // position of row 0, or keys where it is past them
   int keys;           // of the context, within the block table
 };
 MKV_DEV Seq seq_of(const WeightArgs& a, int s) {
@@ -152,8 +152,10 @@ MKV_DEV Seq seq_of(const WeightArgs& a, int s) {
     r.n = min(max((int64_t)a.cu[s + 1], r.q0), a.total_q) - r.q0;
   }
   const int64_t c = max(load_index(a.ctx, s, a.ctx_i64), (int64_t)0);
-  r.first = c - r.n;
   r.keys = (int)min(c, (int64_t)a.idx.max_blocks << a.idx.bs_log2);
+  // (a row past the keys sees all of them; the pieces' work stays within doubles' whole
+  // numbers whatever the length given)
+  r.first = min(c - r.n, (int64_t)r.keys);
   return r;
 }
 // slot of token t, or -1 (a lane's own)
@@ -709,9 +711,10 @@ struct Pieces {
       const int upto_n = wave_scan(n);
       const uint64_t here = __builtin_amdgcn_ballot_w64(mine && x < upto);
       if (here || s0 + 64 >= a.num_seqs) {
+        // (none: cu_seqlens_q falls, and the sequences' work overlaps past 2^53)
         const int l = here ? __builtin_ctzll(here) : 63;
         seq = min(s0 + l, a.num_seqs - 1);
-        q = Seq{lane64(s.q0, l), lane64(s.n, l), lane64(s.first, l), __builtin_amdgcn_readlane(s.keys, l)};
+        q = Seq{here ? lane64(s.q0, l) : 0, lane64(s.n, l), lane64(s.first, l), __builtin_amdgcn_readlane(s.keys, l)};
         base = lane64(upto - c, l);
         base_blocks += __builtin_amdgcn_readlane(upto_n - n, l);
         return;
@@ -783,7 +786,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R == 1
     auto limit = [&](int r) { return (int)min(max(sq.first + div_group(a, r) + 1, (int64_t)0), (int64_t)sq.keys); };
     const int k_end = limit(min(block * kRows + kRows, rows) - 1);
     const int kb0 = min(work.key_of(x - c0), k_end), k1 = end >= c1 ? k_end : min(work.key_of(end - c0), k_end);
-    x = c1;
+    x = c1 > x ? c1 : end;  // (no end of a block ahead: as below)
     const bool active = row0 < rows;
     const int low = active ? limit(row0) : 0, high = active ? limit(min(row0 + 32 * NQ, rows) - 1) : 0;
     u32x4 q[NQ][F::kOps];
@@ -1001,7 +1004,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R == 1
       if (r >= rows) continue;
       if (whole)
         a.lse[(h * a.total_q + sq.q0) * a.group + r] = l[b] == 0.0f ? -kNegInf : m[b] + __builtin_amdgcn_logf(l[b]);
-      else if (base_blocks + block < a.row_units)  // (more of them: cu_seqlens_q falls)
+      else if ((uint32_t)(base_blocks + block) < a.row_units)  // (more of them: cu_seqlens_q falls)
         // (pieces and blocks rise together: their sum is a place of its own)
         a.part_ml[((int64_t)(piece + base_blocks + block) * a.num_kv_heads + h) * kRows + r - block * kRows] = f32x2{m[b], l[b]};
     }
@@ -1410,6 +1413,10 @@ extern "C" int mkv_paged_weights(float* weights, float decay, const void* q, int
                            kv_dtype == MKV_DTYPE_F32);
   if (p.bytes > workspace_bytes || (p.bytes && !workspace)) return MKV_ERR_WORKSPACE_TOO_SMALL;
   if (p.decode ? (int64_t)p.pairs * p.grid_units > kMaxGrid : p.row_units * num_kv_heads > kMaxGrid) return MKV_ERR_BAD_SHAPE;
+  // (the pieces' work, in doubles, is exact)
+  const int64_t group = num_heads / num_kv_heads;
+  if (!p.decode && (double)p.row_units * (double)(((int64_t)max_blocks * block_size + kMinPiece + total_q) * group + p.rows) >= 0x1p52)
+    return MKV_ERR_BAD_SHAPE;
   WeightArgs a;
   a.q = reinterpret_cast<const char*>(q);
   a.k = reinterpret_cast<const char*>(k_cache);

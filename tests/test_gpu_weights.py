@@ -240,6 +240,16 @@ def test_sequences_that_share_pages_take_turns(dev):
     assert float((d["weights"].cpu().double() - w).abs().max()) <= RTOL * 4 * 2 + 2.0 ** -21
 
 
+@pytest.mark.parametrize("rows", [None, [300, 0, 33, 520, 7, 1]])
+@pytest.mark.parametrize("fmt", ["fp32", "bf16"])
+def test_lengths_far_past_the_table(dev, fmt, rows):
+    """A length that no table holds: its rows see what the table has."""
+    announce(f"weights: lengths up to 2^62, {fmt}, rows {rows}")
+    c = make(fmt, rows, [700, 90, 33, 520, 64, 9], 16, 2, 64, 16, seed=22)
+    c["context_lens"] = torch.tensor([2 ** 62, 2 ** 45 + 12345, 33, 2 ** 50 - 1, 2 ** 44, 9])
+    check(dev, c, 0.5)
+
+
 def test_values_that_are_not_finite(dev):
     """A NaN key reaches what the rows that see it see, and nothing else; tokens
     that no row sees change nothing; the entries of new tokens may hold anything."""

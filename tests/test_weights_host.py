@@ -60,6 +60,13 @@ def test_the_scores_room_is_bounded(lib):  # noqa: F811
     assert 0 < room(1, 8, 1, 1 << 25) <= 1 << 22 and 0 < room(3, 4, 1, 1 << 25) <= 1 << 22
 
 
+def test_work_past_whole_numbers_is_refused(lib):  # noqa: F811
+    """The work of chunks is dealt out in doubles, which hold it exactly up to 2^53."""
+    size = dict(seqs=1, hq=16, hkv=1, bs=1 << 20, blocks=8, ws_bytes=1 << 62)
+    assert weights(lib, total=1 << 23, max_blocks=2047, bt_stride=2047, **size) == -2
+    assert weights(lib, total=1 << 23, max_blocks=1, bt_stride=1, ws=None, **size) == -7
+
+
 def test_the_wrapper_s_checks():
     q, k, w = torch.zeros(2, 8, 128), torch.zeros(4, 16, 8, 128), torch.zeros(4, 16, 8)
     bt, cl = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int64)
