@@ -30,8 +30,6 @@ workspace has been allocated by a warm-up call.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 import torch.nn as nn
 
@@ -648,6 +646,11 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
 # ---------------------------------------------------------------------------
 # K12: attention weights beside the cache
 # ---------------------------------------------------------------------------
+def _check_decay(decay: float, name: str = "decay") -> None:
+    if not abs(decay) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"{name} must be finite in float32; got {decay}")
+
+
 def paged_attention_weights(query: torch.Tensor, k_cache: torch.Tensor, weights: torch.Tensor,
                             block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
                             num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, *,
@@ -672,8 +675,7 @@ def paged_attention_weights(query: torch.Tensor, k_cache: torch.Tensor, weights:
     token is lost).  Rows of drafted tokens count as any others: where the rejected ones
     shall not, call it behind the compaction, with the accepted rows' queries alone.
     Captured in a graph, a call accumulates anew at every replay."""
-    if not math.isfinite(decay):
-        raise ValueError(f"decay must be finite; got {decay}")
+    _check_decay(decay)
     dev = _require_gpu(query, k_cache, weights, block_tables, context_lens,
                        *(t for t in (cu_seqlens_q, k_scale) if t is not None))
     if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
@@ -851,8 +853,7 @@ class Attention(nn.Module):
             raise ValueError("attention weights are not accumulated over trees of drafted tokens")
         if context.context_lens is None or context.block_tables is None:
             raise ValueError("attention weights require context_lens and block_tables")
-        if not math.isfinite(self.weights_decay):
-            raise ValueError(f"weights_decay must be finite; got {self.weights_decay}")
+        _check_decay(self.weights_decay, "weights_decay")
 
     def _accumulate(self, q, context, cu_seqlens_q, scale):
         paged_attention_weights(

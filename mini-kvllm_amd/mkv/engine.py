@@ -30,7 +30,6 @@ tokens per second; it is not a port of the reference's runner.  The pieces:
 from __future__ import annotations
 
 import functools
-import math
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -43,7 +42,7 @@ from torch.utils._device import DeviceContext
 
 from . import _lib
 from . import context as C
-from .attention import DECODE_STREAM, DECODE_WORKGROUP, PER_TOKEN_HEAD_MODES, Attention, _dtype_code, _stream
+from .attention import DECODE_STREAM, DECODE_WORKGROUP, PER_TOKEN_HEAD_MODES, Attention, _check_decay, _dtype_code, _stream
 from .decode_state import DecodeGraphs, DecodeMetadata
 from .eviction import CacheEviction
 from .logprobs import MAX_TOP, token_logprobs
@@ -497,8 +496,7 @@ class Qwen3Model(torch.nn.Module):
         if self._captured:
             raise RuntimeError("a step has been captured already, and its replays would go on as they were captured: "
                                "attach the weights before the first captured step")
-        if not math.isfinite(decay):
-            raise ValueError(f"decay must be finite; got {decay}")
+        _check_decay(decay)
         att = [lay["attn"] for lay in self.layers]
         if any(a.k_cache.dim() != 4 for a in att):
             raise RuntimeError("attach_kv_cache comes first")

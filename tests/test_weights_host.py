@@ -112,3 +112,12 @@ def test_the_model_refuses_weights_before_it_changes():
     with pytest.raises(ValueError, match="no CPU fallback"):
         model.attach_attention_weights()
     assert model.layers[0]["attn"].attention_weights is None
+
+
+@pytest.mark.parametrize("decay", [3.5e38, -1e300, float("-inf"), float("nan")])
+def test_a_decay_that_float32_does_not_hold(decay):
+    """It would reach the kernel as an infinity, and 0 times that is NaN."""
+    q, k, w = torch.zeros(2, 8, 128), torch.zeros(4, 16, 8, 128), torch.zeros(4, 16, 8)
+    bt, cl = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="decay must be finite"):
+        mkv.paged_attention_weights(q, k, w, bt, cl, 0.1, 8, 8, 128, 16, decay=decay)
