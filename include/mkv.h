@@ -695,7 +695,7 @@ int mkv_trim_pages(int32_t* block_tables, int64_t bt_stride, int max_blocks, con
  * (the weights among them, if they shall), tensor t of layer layer_of[t], (num_pages,
  * block_size, num_kv_heads, head_bytes[t] bytes), a multiple of 4 up to 2048 (HOST arrays);
  * 16-byte accesses where head_bytes and base are multiples of 16.  block_size a power of
- * two from 4 on.  The tensors do not overlap, and sequences share no page of the
+ * two from 4 on, max_blocks block_size <= 2^31 - 2^20.  The tensors do not overlap, and sequences share no page of the
  * positions below budget.
  * new_lens[b] = min(seq_lens[b], budget).  What lies at positions from budget on stays
  * as it was; positions outside the block table or the pool are left out (their weights

@@ -392,6 +392,8 @@ int log2_exact(int64_t v) {
   return l;
 }
 
+// Of a table: a grid's stride past them, 2^18 (evict_keys_kernel), stays within 32 bits.
+constexpr int64_t kMaxTokens = 0x7ff00000;
 int64_t capacity_of(int max_blocks, int block_size) { return (int64_t)max_blocks * block_size; }
 
 // The forms of the selection by the table's width: tokens that a workgroup of 256
@@ -444,7 +446,7 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
     return MKV_ERR_BAD_SHAPE;
   const int bs_log2 = log2_exact(block_size);
   if (bs_log2 < 2) return MKV_ERR_BAD_BLOCK_SIZE;
-  if (num_pages > (0x7fffffff >> bs_log2) || capacity_of(max_blocks, block_size) > 0x7fff0000) return MKV_ERR_BAD_SHAPE;
+  if (num_pages > (0x7fffffff >> bs_log2) || capacity_of(max_blocks, block_size) > kMaxTokens) return MKV_ERR_BAD_SHAPE;
   if (seq_lens_dtype != MKV_INDEX_I32 && seq_lens_dtype != MKV_INDEX_I64) return MKV_ERR_UNSUPPORTED_DTYPE;
   if (batch == 0 || num_layers == 0) return MKV_OK;
   if ((num_tensors && (!tensors || !head_bytes || !layer_of)) || !weights || !block_tables || !seq_lens || !new_lens ||

@@ -62,6 +62,15 @@ def test_the_keys_room_is_bounded(lib):  # noqa: F811
         assert one <= keys(layers, batch, heads, blocks) <= max(one, 256 << 20)
 
 
+def test_tables_at_the_end_of_32_bits(lib):  # noqa: F811
+    """Token numbers and a grid's stride past them (2^18) are held in 32 bits."""
+    def tokens(n):
+        return evict(lib, bs=16, blocks=n // 16, stride=n // 16, batch=1, ws_bytes=0)
+
+    assert tokens(2 ** 31 - 2 ** 18) == -2 and tokens(2 ** 31 - 2 ** 16) == -2
+    assert tokens(2 ** 31 - 2 ** 20) == -7
+
+
 def test_trim_refusals(lib):  # noqa: F811
     def trim(bt=p, stride=4, blocks=4, lens=p, held=p, refs=p, pages=10, bs=16, rows=3):
         return lib.mkv_trim_pages(bt, stride, blocks, lens, held, refs, pages, bs, rows, None)
