@@ -734,7 +734,7 @@ int mkv_evict_tokens(const void* const* tensors, const int64_t* head_bytes, cons
  * with one of these counts as absent.  Tokens outside the vocabulary and nodes whose
  * parent is no earlier node are never accepted; nodes past max_nodes (<= 1024) are not
  * looked at (acceptance 0); a sequence without nodes has num_accepted 0 and next token
- * -1.  acceptance behind the last sequence is not written.  Sums are fp32. */
+ * -1.  acceptance of rows that are no sequence's is not written.  Sums are fp32. */
 size_t mkv_verify_drafts_workspace_size(int64_t total, int vocab, int num_seqs, int max_nodes, int has_draft);
 int mkv_verify_drafts(int64_t* accepted, int64_t* num_accepted, int64_t* next_tokens, float* acceptance,
                       const void* logits, int64_t row_stride, const void* draft_logits, int64_t draft_stride, int dtype,

@@ -54,7 +54,7 @@ def verify_drafts(logits: torch.Tensor, token_ids: torch.Tensor, cu_seqlens_q: t
     way of sampling.  Ties go to the lowest index.
 
     max_nodes (up to 1024): the most nodes of a sequence; those past it are not looked
-    at.  Rows of acceptance behind the last sequence are not written.  A row with a NaN
+    at.  Rows of acceptance that are no sequence's are not written.  A row with a NaN
     or +inf, or -inf alone, is taken as greedy; tokens outside the vocabulary and nodes
     whose parent is no earlier node are never accepted."""
     dev = _require_gpu(logits, token_ids, cu_seqlens_q, uniforms, noise,
