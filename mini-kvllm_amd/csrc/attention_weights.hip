@@ -302,8 +302,8 @@ constexpr int kSplitKeys = 1024;  // of a unit: 16 tiles a wave
 // The workgroup's pair and first unit.  Workgroups go to the XCDs by turns.  A unit's
 // heads share the weights' cache lines and stay together where the units are a multiple of
 // 8, and then the sequences' first units, the only ones with keys under a wide table, are
-// on unlike XCDs (60 sequences of 300-800 tokens under tables of 32,768: 49 us; all first
-// units on one XCD: 181).
+// on unlike XCDs (60 sequences of 300-800 tokens under tables of 32,768: 38 us; all first
+// units on one XCD: 171).
 MKV_DEV void place_of(const WeightArgs& a, int& pair, int& x) {
   pair = blockIdx.x / a.grid_units;
   x = (int)(blockIdx.x % a.grid_units + (a.pair0 + pair) / a.num_kv_heads) % a.grid_units;
@@ -1254,8 +1254,8 @@ struct Plan {
 
 // Bytes of kept scores at a time.  Their room follows the table's width, which may be far
 // past the contexts, so that pairs whose scores do not fit go in up to four turns (60
-// sequences of 300-800 tokens, 16/8 heads, fp8, under tables of 131,072: 87 us, and 53 in
-// one turn with 0.94 GiB; of 30k tokens 940 and 917).  Past those, one-row sequences go
+// sequences of 300-800 tokens, 16/8 heads, fp8, under tables of 131,072: 75 us, and 42 in
+// one turn with 0.94 GiB; of 30k tokens, 32/8, bf16, 929 and 906).  Past those, one-row sequences go
 // the chunks' way, which keeps no scores.
 constexpr size_t kMaxScores = (size_t)256 << 20;
 constexpr int kMaxTurns = 4;
