@@ -697,7 +697,7 @@ int mkv_trim_pages(int32_t* block_tables, int64_t bt_stride, int max_blocks, con
  * 16-byte accesses where head_bytes and base are multiples of 16.  block_size a power of
  * two from 4 on, max_blocks block_size <= 2^31 - 2^20.  The tensors do not overlap, and sequences share no page of the
  * positions below budget.
- * new_lens[b] = min(seq_lens[b], budget).  What lies at positions from budget on stays
+ * new_lens[b] = min(seq_lens[b], budget), of its own memory, not seq_lens.  What lies at positions from budget on stays
  * as it was; positions outside the block table or the pool are left out (their weights
  * count as lowest).
  * workspace: 4 bytes a (layer, sequence, KV head, token of the budget), and for tables

@@ -469,6 +469,10 @@ extern "C" int mkv_evict_tokens(const void* const* tensors, const int64_t* head_
   if (pairs * num_kv_heads > 0x3fffff || (int64_t)num_layers * batch * num_kv_heads > 0x7fffffff) return MKV_ERR_BAD_SHAPE;
   if (workspace_bytes < mkv_evict_tokens_workspace_size(num_layers, batch, num_kv_heads, block_size, max_blocks, budget))
     return MKV_ERR_WORKSPACE_TOO_SMALL;
+  // (the move reads the old lengths behind the selection's new ones)
+  const char *const old_at = static_cast<const char*>(seq_lens), *const new_at = reinterpret_cast<const char*>(new_lens);
+  if (old_at < new_at + 8 * (int64_t)batch && new_at < old_at + (seq_lens_dtype == MKV_INDEX_I64 ? 8 : 4) * (int64_t)batch)
+    return MKV_ERR_BAD_SHAPE;
   EvictArgs a;
   a.idx = PagedIndex{block_tables, bt_stride, max_blocks, num_pages, bs_log2, 0};
   a.lens = seq_lens;

@@ -62,6 +62,12 @@ def test_the_keys_room_is_bounded(lib):  # noqa: F811
         assert one <= keys(layers, batch, heads, blocks) <= max(one, 256 << 20)
 
 
+def test_new_lengths_over_the_old_ones_are_refused(lib):  # noqa: F811
+    """The rows move by the old lengths, behind the launch that writes the new ones."""
+    assert evict(lib, lens=p, new=p) == -2 and evict(lib, lens=p, new=p + 8) == -2
+    assert evict(lib, lens=p + 12, new=p, lens_dt=0) == -2
+
+
 def test_tables_at_the_end_of_32_bits(lib):  # noqa: F811
     """Token numbers and a grid's stride past them (2^18) are held in 32 bits."""
     def tokens(n):
