@@ -536,8 +536,10 @@ class Qwen3Model(torch.nn.Module):
         free = _untouched()
         if free and residual.is_cuda and torch.cuda.is_current_stream_capturing():
             self._captured = True
+        ctx = C.current_context()
         for lay in self.layers:
-            lay["attn"].check_accumulates(C.current_context())
+            if lay["attn"].attention_weights is not None:
+                lay["attn"].check_accumulates(ctx)
         for li, lay in enumerate(self.layers):
             qkv = normed_linear(x, residual, lay["in_norm"], cfg.eps, lay["qkv"], 0, free)
             att = lay["attn"]
